@@ -56,10 +56,12 @@ typedef struct ihipStream_t* origami_stream_t; /* == hipStream_t */
 #define ORIGAMI_CACHE_KV_FIRST 0
 #define ORIGAMI_CACHE_BLOCKS_FIRST 1
 
-/* element types of dequantize inputs and outputs */
+/* element types of dequantize, append and attention inputs and outputs */
 #define ORIGAMI_DTYPE_FLOAT16 1
 #define ORIGAMI_DTYPE_BFLOAT16 2
 #define ORIGAMI_DTYPE_FLOAT32 3
+/* element type of paged caches read and written by the append and the attention */
+#define ORIGAMI_DTYPE_FLOAT8_E4M3FN 4
 
 /* KIVI symbol packing: LSB-first at `bits` bits (what the reference kernel
  * reads), or KIVI's own container, where 3-bit symbols sit one per nibble
@@ -428,6 +430,93 @@ int origami_kivi_quantize(const void* kv, int64_t dtype, int64_t tokens, int64_t
                           int64_t group_size, int64_t sink_tokens, uint8_t* payload,
                           int64_t payload_bytes, const int64_t* offsets, uint8_t* workspace,
                           int64_t workspace_bytes, origami_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Operators on the paged cache that follow a restore: the tokens after the
+ * restored prefix are appended, and queries attend to both.  No reference
+ * counterpart (there the model's own kernels do this).  For inference: they
+ * have no gradient.
+ * ------------------------------------------------------------------------- */
+
+/*
+ * Appends `tokens` tokens to the paged cache, with the position rotation and,
+ * for models that have them, norms of queries and keys per head on the way;
+ * the queries are rotated in the same launch.
+ *
+ * key and value are [tokens, heads, head_dim], query and query_out [tokens,
+ * query_heads, head_dim] (query_heads 0: neither) of dtype FLOAT16 or BFLOAT16;
+ * channels are contiguous and strides (host, [8]) are the token and head
+ * strides of key, value, query and query_out, in elements.  query_out may be
+ * query itself.  For a row x of query or key, in binary32:
+ *  - query_norm / key_norm (device, [head_dim], of dtype or FLOAT32; null:
+ *    none): x * (1 / sqrt(mean(x^2) + eps)) * weight;
+ *  - cos_sin (device float32, [table_rows, rotary_dim]; null: none): row
+ *    positions[token] holds rotary_dim / 2 cosines, then as many sines; the
+ *    first rotary_dim channels are rotated in pairs (i, i + rotary_dim / 2), or
+ *    (2 i, 2 i + 1) where `interleaved`: (a cos - b sin, b cos + a sin);
+ *  - rounded once, to dtype, or for a cache of FLOAT8_E4M3FN divided by k_scale
+ *    (values by v_scale), limited to +-448 and rounded to e4m3 (scales are 1
+ *    for other caches, which have dtype).
+ * Token t goes to slot slots[t] = block * block_size + offset.  A token whose
+ * slot is outside the cache (such as -1, for padding) is not written; neither is
+ * one whose position is outside the table, and its query row becomes zero.
+ * Slots inside the cache must be distinct: which of two tokens a slot holds
+ * afterwards is not defined.  head_dim is a multiple of 8, at most 256; kv_cache
+ * is 16-byte aligned.
+ */
+int origami_append_kv_cache(
+    const void* key, const void* value, const void* query, void* query_out, int64_t dtype,
+    const int64_t* strides, int64_t tokens, int64_t query_heads, void* kv_cache,
+    int64_t cache_dtype, int64_t cache_layout, int64_t num_blocks, int64_t block_size,
+    int64_t heads, int64_t head_dim, const int64_t* slots, const int64_t* positions,
+    const float* cos_sin, int64_t table_rows, int64_t rotary_dim, int64_t interleaved,
+    const void* query_norm, const void* key_norm, int64_t norm_dtype, double eps,
+    double k_scale, double v_scale, origami_stream_t stream);
+
+/*
+ * Attention of a batch of requests over a paged cache, where all requests share
+ * the first prefix_tokens tokens (in blocks prefix_block_ids): each query row
+ * is softmax(scale * k_scale * q . k) over the prefix and, causally, over its
+ * request's own tokens, times v_scale * v.  The prefix is read once for the whole
+ * batch.
+ *
+ * query and out are [tokens, query_heads, head_dim] of dtype FLOAT16 or
+ * BFLOAT16, channels contiguous; strides (host, [4]) are the token and head
+ * strides of query and out.  Query head h uses cache head
+ * h / (query_heads / heads).  kv_cache has dtype, or FLOAT8_E4M3FN with scales.
+ * Request r has own_tokens[r] tokens in blocks block_tables[r * table_stride ..]
+ * (table_blocks of them), those of its queries included: its query tokens are
+ * rows query_starts[r] .. query_starts[r + 1] - 1 of query (query_starts null:
+ * row r alone) and its last own tokens, so that query i of n sees the prefix and
+ * own tokens 0 .. own_tokens[r] - n + i.  Device arrays are int64.  max_query_tokens
+ * and max_own_tokens bound a request's query and own tokens (they shape the
+ * launch; further tokens are not seen).  Rows that no request has are left as
+ * they were.  Tokens in blocks outside [0, num_blocks) are not seen; what a row
+ * does not see has no influence on it, NaN included.  A row that sees no token,
+ * or only scores of -infinity, becomes zero.
+ * lse (null: none) is a contiguous float32 [tokens, query_heads]: the natural
+ * logarithm of each row's sum of exponentials, -infinity for zero rows.
+ *
+ * The score and output sums, maxima and exponentials are binary32; the
+ * exponentials are rounded to dtype for the product with the values, and the
+ * result once more.  workspace is a 16-byte aligned device buffer of at least
+ * origami_shared_prefix_attention_workspace bytes (0: may be null; -1: invalid
+ * sizes), in use until the call's work is done; calls that can run at the same
+ * time need their own.  Results do not depend on timing.
+ */
+int64_t origami_shared_prefix_attention_workspace(
+    int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_dim, int64_t prefix_tokens,
+    int64_t requests, int64_t max_query_tokens, int64_t max_own_tokens);
+int origami_shared_prefix_attention(
+    const void* query, int64_t dtype, const int64_t* strides, int64_t tokens,
+    int64_t query_heads, const void* kv_cache, int64_t cache_dtype, int64_t cache_layout,
+    int64_t num_blocks, int64_t block_size, int64_t heads, int64_t head_dim,
+    const int64_t* prefix_block_ids, int64_t prefix_block_count, int64_t prefix_tokens,
+    const int64_t* block_tables, int64_t table_stride, int64_t table_blocks,
+    const int64_t* own_tokens, int64_t requests, const int64_t* query_starts,
+    int64_t max_query_tokens, int64_t max_own_tokens, double scale, double k_scale,
+    double v_scale, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+    origami_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -12,7 +12,7 @@ from pathlib import Path
 import numpy as np
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "liborigami_layout.so"
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 ORIGAMI_OK = 0
 ORIGAMI_ERR_INVALID = 1
@@ -25,12 +25,14 @@ CACHE_BLOCKS_FIRST = 1
 DTYPE_FLOAT16 = 1
 DTYPE_BFLOAT16 = 2
 DTYPE_FLOAT32 = 3
+DTYPE_FLOAT8_E4M3FN = 4
 
 KIVI_PACKED_LSB = 0
 KIVI_NIBBLE3 = 1
 
 _i64 = ctypes.c_int64
 _p = ctypes.c_void_p
+_f64 = ctypes.c_double
 
 # name -> argument types (return type is int for all but origami_last_error)
 _SIGNATURES: dict[str, list] = {
@@ -67,6 +69,13 @@ _SIGNATURES: dict[str, list] = {
         _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p],
     "origami_kivi_quantize": [
         _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _i64, _p],
+    "origami_append_kv_cache": [
+        _p, _p, _p, _p, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p,
+        _p, _i64, _i64, _i64, _p, _p, _i64, _f64, _f64, _f64, _p],
+    "origami_shared_prefix_attention_workspace": [_i64] * 8,
+    "origami_shared_prefix_attention": [
+        _p, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p,
+        _i64, _i64, _p, _i64, _p, _i64, _i64, _f64, _f64, _f64, _p, _p, _p, _i64, _p],
 }
 
 EXPORTED_SYMBOLS = ("origami_last_error", "origami_restore_plan_destroy",
@@ -103,6 +112,7 @@ def lib() -> ctypes.CDLL:
                 fn.restype = ctypes.c_int
                 fn.argtypes = args
             L.origami_set_rows_grid_limit.restype = ctypes.c_int64
+            L.origami_shared_prefix_attention_workspace.restype = ctypes.c_int64
             L.origami_restore_plan_destroy.restype = None
             L.origami_restore_plan_destroy.argtypes = [_p]
             L.origami_debug_counters.restype = None

@@ -1,0 +1,53 @@
+// origami_element.h -- 16-bit and 8-bit element types of the operators on the paged cache
+// (origami_append.hip, origami_attention.hip): vectors, loads and conversions.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+namespace origami_element {
+
+using bf16 = __bf16;
+using f16 = _Float16;
+
+template <typename T>
+using Vec2 = T __attribute__((ext_vector_type(2)));
+template <typename T>
+using Vec4 = T __attribute__((ext_vector_type(4)));
+template <typename T>
+using Vec8 = T __attribute__((ext_vector_type(8)));
+using Float4 = float __attribute__((ext_vector_type(4)));
+using U32x2 = uint32_t __attribute__((ext_vector_type(2)));
+using U32x4 = uint32_t __attribute__((ext_vector_type(4)));
+
+// Two e4m3 values, the low (HIGH = false) or high half of `word`, as two T; exact, since T
+// has every value of e4m3.
+template <bool HIGH>
+__device__ __forceinline__ Vec2<bf16> fp8_pair(uint32_t word, bf16) {
+  return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, 1.0f, HIGH);
+}
+template <bool HIGH>
+__device__ __forceinline__ Vec2<f16> fp8_pair(uint32_t word, f16) {
+  return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.0f, HIGH);
+}
+
+// Eight e4m3 values as eight T (16 bytes).
+template <typename T>
+__device__ __forceinline__ U32x4 fp8_expand(U32x2 raw) {
+  U32x4 out;
+  out[0] = __builtin_bit_cast(uint32_t, fp8_pair<false>(raw[0], T()));
+  out[1] = __builtin_bit_cast(uint32_t, fp8_pair<true>(raw[0], T()));
+  out[2] = __builtin_bit_cast(uint32_t, fp8_pair<false>(raw[1], T()));
+  out[3] = __builtin_bit_cast(uint32_t, fp8_pair<true>(raw[1], T()));
+  return out;
+}
+
+// x as it is stored in e4m3: at most 448 in size (the conversion makes NaN of what is larger),
+// NaN kept, rounded to nearest even.
+__device__ __forceinline__ float fp8_clamp(float x) {
+  const float y = fminf(fmaxf(x, -448.0f), 448.0f);
+  return x != x ? x : y;
+}
+
+}  // namespace origami_element

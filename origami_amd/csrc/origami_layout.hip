@@ -2814,7 +2814,7 @@ extern "C" {
 
 const char* origami_last_error(void) { return g_last_error.c_str(); }
 
-int origami_abi_version(void) { return 3; }
+int origami_abi_version(void) { return 4; }
 
 void origami_debug_counters(int64_t* plans_created, int64_t* device_allocations) {
   if (plans_created) *plans_created = g_plans_created.load(std::memory_order_relaxed);

@@ -10,9 +10,12 @@
 // way the reference's TORCH_CHECKs raise.  There is no device code here.
 #include <torch/extension.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <string>
 #include <vector>
@@ -430,6 +433,198 @@ void restore_plan_destroy(int64_t handle) {
   delete reinterpret_cast<PreparedRestore*>(handle);
 }
 
+// ---------------------------------------------------------------------------
+// Operators on the paged cache that follow a restore.  The cache order is that of
+// the layout entry points ([2, NB, bs, H, D] is recognised first).
+// ---------------------------------------------------------------------------
+
+int64_t paged_dtype_code(at::ScalarType t, const char* name) {
+  if (t == at::kFloat8_e4m3fn) return ORIGAMI_DTYPE_FLOAT8_E4M3FN;
+  TORCH_CHECK(t == at::kHalf || t == at::kBFloat16, name,
+              " must be float16 or bfloat16 (a kv_cache may be float8_e4m3fn)");
+  return dtype_code(t, name);
+}
+
+void require_no_grad(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), name,
+              " requires a gradient, which this operator does not have");
+}
+
+// A [tokens, heads, head_dim] tensor whose channels are contiguous.
+void require_rows(const at::Tensor& t, const char* name, const at::Tensor& cache,
+                  at::ScalarType dtype) {
+  TORCH_CHECK(t.is_cuda() && t.device() == cache.device(), name,
+              " must be on the kv_cache device");
+  TORCH_CHECK(t.dim() == 3, name, " must be [tokens, heads, head_dim]");
+  TORCH_CHECK(t.scalar_type() == dtype, name, " must have the same dtype as the other rows");
+  TORCH_CHECK(t.size(2) == cache.size(4), name, " head_dim differs from the kv_cache's");
+  TORCH_CHECK(t.stride(2) == 1 || t.numel() == 0, name, " channels must be contiguous");
+  require_no_grad(t, name);
+}
+
+// A contiguous int64 tensor of at least `count` values; null when it has none.
+const int64_t* require_index(const at::Tensor& t, const char* name, const at::Tensor& cache,
+                             int64_t count) {
+  TORCH_CHECK(t.is_cuda() && t.device() == cache.device(), name,
+              " must be on the kv_cache device");
+  TORCH_CHECK(t.scalar_type() == at::kLong && t.dim() == 1 && t.is_contiguous(), name,
+              " must be a contiguous int64 vector");
+  TORCH_CHECK(t.numel() == count, name, " must have ", count, " values, not ", t.numel());
+  return count > 0 ? t.data_ptr<int64_t>() : nullptr;
+}
+
+// New tokens into the cache; returns the rotated queries (an undefined tensor, None in
+// Python, without queries).
+c10::optional<at::Tensor> append_kv_cache(
+    at::Tensor key, at::Tensor value, at::Tensor kv_cache, at::Tensor slots,
+    c10::optional<at::Tensor> query, c10::optional<at::Tensor> positions,
+    c10::optional<at::Tensor> cos_sin, bool interleaved, c10::optional<at::Tensor> query_norm,
+    c10::optional<at::Tensor> key_norm, double eps, double k_scale, double v_scale,
+    c10::optional<at::Tensor> query_out) {
+  require_device(kv_cache, "kv_cache");
+  const CacheGeom g = layout_cache_geometry(kv_cache);
+  const int64_t dtype = paged_dtype_code(key.scalar_type(), "key");
+  TORCH_CHECK(dtype != ORIGAMI_DTYPE_FLOAT8_E4M3FN, "key must be float16 or bfloat16");
+  require_rows(key, "key", kv_cache, key.scalar_type());
+  require_rows(value, "value", kv_cache, key.scalar_type());
+  const int64_t tokens = key.size(0), D = kv_cache.size(4);
+  TORCH_CHECK(key.size(1) == g.heads && value.size(1) == g.heads,
+              "key and value heads differ from the kv_cache's");
+  TORCH_CHECK(value.size(0) == tokens, "key and value must have the same tokens");
+  const int64_t* const slot = require_index(slots, "slots", kv_cache, tokens);
+  int64_t strides[8] = {key.stride(0), key.stride(1), value.stride(0), value.stride(1), 0, 0, 0, 0};
+  const c10::OptionalDeviceGuard guard(kv_cache.device());
+
+  c10::optional<at::Tensor> out;
+  int64_t query_heads = 0;
+  if (query) {
+    require_rows(*query, "query", kv_cache, key.scalar_type());
+    TORCH_CHECK(query->size(0) == tokens, "query and key must have the same tokens");
+    query_heads = query->size(1);
+    if (query_out) {
+      require_rows(*query_out, "query_out", kv_cache, key.scalar_type());
+      TORCH_CHECK(query_out->sizes() == query->sizes(), "query_out must have the query's shape");
+      at::assert_no_internal_overlap(*query_out);
+    }
+    out = query_out ? *query_out : at::empty({tokens, query_heads, D}, query->options());
+    strides[4] = query->stride(0);
+    strides[5] = query->stride(1);
+    strides[6] = out->stride(0);
+    strides[7] = out->stride(1);
+  } else {
+    TORCH_CHECK(!query_out, "query_out needs a query");
+    TORCH_CHECK(!query_norm, "query_norm needs a query");
+  }
+  const int64_t* position = nullptr;
+  int64_t table_rows = 0, rotary_dim = 0;
+  TORCH_CHECK(positions.has_value() == cos_sin.has_value(),
+              "rotation needs both positions and cos_sin");
+  if (cos_sin) {
+    position = require_index(*positions, "positions", kv_cache, tokens);
+    require_device(*cos_sin, "cos_sin");
+    require_no_grad(*cos_sin, "cos_sin");
+    TORCH_CHECK(cos_sin->device() == kv_cache.device(), "cos_sin must be on the kv_cache device");
+    TORCH_CHECK(cos_sin->scalar_type() == at::kFloat && cos_sin->dim() == 2,
+                "cos_sin must be float32 [positions, rotary_dim]");
+    table_rows = cos_sin->size(0);
+    rotary_dim = cos_sin->size(1);
+  }
+  int64_t norm_dtype = dtype;
+  for (const auto* norm : {&query_norm, &key_norm})
+    if (*norm) {
+      require_device(**norm, "norm weights");
+      require_no_grad(**norm, "norm weights");
+      TORCH_CHECK((*norm)->device() == kv_cache.device(),
+                  "norm weights must be on the kv_cache device");
+      TORCH_CHECK((*norm)->dim() == 1 && (*norm)->numel() == D,
+                  "norm weights must have head_dim values");
+      norm_dtype = dtype_code((*norm)->scalar_type(), "norm weights");
+    }
+  TORCH_CHECK(!query_norm || !key_norm || query_norm->scalar_type() == key_norm->scalar_type(),
+              "norm weights must have the same dtype");
+  check(origami_append_kv_cache(
+      key.data_ptr(), value.data_ptr(), query ? query->data_ptr() : nullptr,
+      out ? out->data_ptr() : nullptr, dtype, strides, tokens, query_heads, kv_cache.data_ptr(),
+      paged_dtype_code(kv_cache.scalar_type(), "kv_cache"), g.layout, g.num_blocks, g.block_size,
+      g.heads, D, slot, position, cos_sin ? cos_sin->data_ptr<float>() : nullptr, table_rows,
+      rotary_dim, interleaved, query_norm ? query_norm->data_ptr() : nullptr,
+      key_norm ? key_norm->data_ptr() : nullptr, norm_dtype, eps, k_scale, v_scale,
+      current_stream(kv_cache)));
+  return out;
+}
+
+// Attention of a batch over a shared prefix and each request's own tokens; fills lse where
+// it is given and returns the output rows.
+at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
+                                   c10::optional<at::Tensor> prefix_block_ids,
+                                   int64_t prefix_tokens, at::Tensor block_tables,
+                                   at::Tensor own_tokens, c10::optional<at::Tensor> query_starts,
+                                   c10::optional<int64_t> max_query_tokens,
+                                   c10::optional<int64_t> max_own_tokens,
+                                   c10::optional<double> scale, double k_scale, double v_scale,
+                                   c10::optional<at::Tensor> out_, c10::optional<at::Tensor> lse) {
+  require_device(kv_cache, "kv_cache");
+  const CacheGeom g = layout_cache_geometry(kv_cache);
+  const int64_t dtype = paged_dtype_code(query.scalar_type(), "query");
+  TORCH_CHECK(dtype != ORIGAMI_DTYPE_FLOAT8_E4M3FN, "query must be float16 or bfloat16");
+  require_rows(query, "query", kv_cache, query.scalar_type());
+  const int64_t tokens = query.size(0), Hq = query.size(1), D = kv_cache.size(4);
+  TORCH_CHECK(block_tables.is_cuda() && block_tables.device() == kv_cache.device(),
+              "block_tables must be on the kv_cache device");
+  TORCH_CHECK(block_tables.scalar_type() == at::kLong && block_tables.dim() == 2 &&
+                  (block_tables.stride(1) == 1 || block_tables.size(1) <= 1),
+              "block_tables must be int64 [requests, blocks] with contiguous rows");
+  const int64_t requests = block_tables.size(0), blocks = block_tables.size(1);
+  const int64_t* const own = require_index(own_tokens, "own_tokens", kv_cache, requests);
+  const int64_t *prefix = nullptr, *starts = nullptr;
+  int64_t prefix_blocks = 0;
+  if (prefix_block_ids) {
+    prefix_blocks = prefix_block_ids->numel();
+    prefix = require_index(*prefix_block_ids, "prefix_block_ids", kv_cache, prefix_blocks);
+  }
+  if (query_starts) starts = require_index(*query_starts, "query_starts", kv_cache, requests + 1);
+  TORCH_CHECK(starts || tokens == requests,
+              "without query_starts every request has one query token");
+  const int64_t most = max_query_tokens ? *max_query_tokens : (starts ? tokens : std::min<int64_t>(tokens, 1));
+  const int64_t most_own = max_own_tokens ? *max_own_tokens : blocks * g.block_size;
+  const c10::OptionalDeviceGuard guard(kv_cache.device());
+
+  at::Tensor out;
+  if (out_) {
+    out = *out_;
+    require_rows(out, "out", kv_cache, query.scalar_type());
+    TORCH_CHECK(out.sizes() == query.sizes(), "out must have the query's shape");
+    at::assert_no_internal_overlap(out);
+    at::assert_no_overlap(out, query);
+  } else {
+    // rows of no request are not written: zero in a new tensor
+    out = starts ? at::zeros({tokens, Hq, D}, query.options())
+                 : at::empty({tokens, Hq, D}, query.options());
+  }
+  if (lse) {
+    require_device(*lse, "lse");
+    TORCH_CHECK(lse->device() == kv_cache.device() && lse->scalar_type() == at::kFloat &&
+                    lse->dim() == 2 && lse->size(0) == tokens && lse->size(1) == Hq,
+                "lse must be float32 [tokens, query heads] on the kv_cache device");
+  }
+  const int64_t bytes = origami_shared_prefix_attention_workspace(
+      tokens, Hq, g.heads, D, prefix_tokens, requests, most, most_own);
+  TORCH_CHECK(bytes >= 0, origami_last_error());
+  at::Tensor work;
+  if (bytes > 0) work = at::empty({bytes}, query.options().dtype(at::kByte));
+  const int64_t strides[4] = {query.stride(0), query.stride(1), out.stride(0), out.stride(1)};
+  check(origami_shared_prefix_attention(
+      query.data_ptr(), dtype, strides, tokens, Hq, kv_cache.data_ptr(),
+      paged_dtype_code(kv_cache.scalar_type(), "kv_cache"), g.layout, g.num_blocks, g.block_size,
+      g.heads, D, prefix, prefix_blocks, prefix_tokens,
+      block_tables.numel() ? block_tables.data_ptr<int64_t>() : nullptr, block_tables.stride(0),
+      blocks, own, requests, starts, most, most_own,
+      scale ? *scale : 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(D, 1))), k_scale,
+      v_scale, out.data_ptr(), lse ? lse->data_ptr<float>() : nullptr,
+      bytes > 0 ? work.data_ptr() : nullptr, bytes, current_stream(kv_cache)));
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -448,5 +643,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("restore_plan_create", &restore_plan_create);
   m.def("restore_plan_launch", &restore_plan_launch);
   m.def("restore_plan_destroy", &restore_plan_destroy);
+  m.def("append_kv_cache", &append_kv_cache);
+  m.def("shared_prefix_attention", &shared_prefix_attention);
   m.def("abi_version", &origami_abi_version);
 }

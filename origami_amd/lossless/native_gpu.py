@@ -3,8 +3,9 @@
 Mirrors lossless/native_gpu.py of the reference (load_bitpack_cuda_extension,
 available, unpack_canonical_storage_chunks, cachegen_unpack_dequantize*,
 kivi_dequantize_to_kv_cache; native_gpu.py:35-261) and adds the pieces the reference lacks: the pack, the
-fused unpack+scatter into the paged KV cache and the fused gather+pack from
-it.
+fused unpack+scatter into the paged KV cache, the fused gather+pack from it,
+and what runs on the cache after a restore: appending new tokens and the
+attention of a batch that shares a prefix.
 
 All work is enqueued on the calling thread's current stream of the tensors'
 device, like the reference (bitpack_layout_cuda.cpp:370).  Chunk metadata stays
@@ -724,6 +725,78 @@ def kivi_quantize(kv: torch.Tensor, *, dims: Sequence[int], strides: Sequence[in
 
 
 # ---------------------------------------------------------------------------
+# Operators on the paged cache that follow a restore (no reference counterpart)
+# ---------------------------------------------------------------------------
+
+def append_kv_cache(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor,
+                    slots: torch.Tensor, *, query: torch.Tensor | None = None,
+                    positions: torch.Tensor | None = None, cos_sin: torch.Tensor | None = None,
+                    interleaved: bool = False, query_norm: torch.Tensor | None = None,
+                    key_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                    k_scale: float = 1.0, v_scale: float = 1.0,
+                    query_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Appends tokens to the paged cache and rotates their queries, in one launch.
+
+    key and value are float16 or bfloat16 [tokens, heads, head_dim], query [tokens,
+    query_heads, head_dim]; views of one projection's output are fine (channels contiguous).
+    Token t goes to slot slots[t] = block id * block size + offset (int64; any slot outside
+    the cache, such as -1, is not written, and no slot may be given twice).  Queries and keys
+    are normalised per head where query_norm / key_norm ([head_dim], the keys' dtype or
+    float32) are given, x / sqrt(mean(x^2) + eps) * weight, and rotated where cos_sin (float32
+    [table positions, rotary_dim]: cosines, then sines, of each pair's angle) and positions
+    (int64 [tokens]) are given: channels (i, i + rotary_dim / 2) are a pair, or (2 i, 2 i + 1)
+    with `interleaved`.  A token whose position is outside the table is not written, and its
+    query becomes zero.  Arithmetic is float32, rounded once.  A float8_e4m3fn kv_cache holds
+    key / k_scale and value / v_scale, limited to +-448.  Returns the queries: query_out
+    (which may be `query`) or a new tensor; None without `query`.  For inference only: inputs
+    that require a gradient are refused."""
+    return _ext.ext().append_kv_cache(key, value, kv_cache, slots, query, positions, cos_sin,
+                                      interleaved, query_norm, key_norm, eps, k_scale, v_scale,
+                                      query_out)
+
+
+def shared_prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor,
+                            prefix_block_ids: torch.Tensor | None, prefix_tokens: int,
+                            block_tables: torch.Tensor, own_tokens: torch.Tensor, *,
+                            query_starts: torch.Tensor | None = None,
+                            max_query_tokens: int | None = None,
+                            max_own_tokens: int | None = None, scale: float | None = None,
+                            k_scale: float = 1.0, v_scale: float = 1.0,
+                            out: torch.Tensor | None = None, return_lse: bool = False):
+    """Attention of a batch over the paged cache, where all requests share the first
+    prefix_tokens tokens (in blocks prefix_block_ids): the prefix is read once for the batch.
+
+    query is float16 or bfloat16 [tokens, query_heads, head_dim]; kv_cache has its dtype or
+    is float8_e4m3fn with k_scale / v_scale; query head h uses cache head
+    h // (query_heads // heads).  Request r has own_tokens[r] tokens of its own in blocks
+    block_tables[r] (int64, rows contiguous), those of its queries included.  Without
+    query_starts, row r of query is request r's newest token; with it (int64
+    [requests + 1]) rows query_starts[r] .. query_starts[r + 1] - 1 are request r's newest
+    tokens.  A row sees the whole prefix and its request's own tokens up to itself; it
+    becomes zero if it sees none.  Rows of no request are left as they were (zero in a new
+    tensor).  All of these are device tensors and nothing is read back, so a call can be
+    captured in a graph and replayed as lengths grow.  max_query_tokens and max_own_tokens
+    bound a request's query and own tokens and shape the launch (defaults: all rows, the
+    whole block table); tokens past them are not seen.  Tokens in blocks outside the cache are
+    not seen.  scale defaults to head_dim ** -0.5.
+
+    Returns the output, and with return_lse also float32 [tokens, query_heads] natural
+    logarithms of the rows' sums of exponentials (-inf for zero rows), with which results over
+    different tokens can be joined.  For inference only: inputs that require a gradient are
+    refused."""
+    lse = None
+    if return_lse:
+        shape = tuple(query.shape[:2])
+        lse = (torch.empty(shape, dtype=torch.float32, device=query.device)
+               if query_starts is None else
+               torch.full(shape, -float("inf"), dtype=torch.float32, device=query.device))
+    result = _ext.ext().shared_prefix_attention(
+        query, kv_cache, prefix_block_ids, prefix_tokens, block_tables, own_tokens, query_starts,
+        max_query_tokens, max_own_tokens, scale, k_scale, v_scale, out, lse)
+    return (result, lse) if return_lse else result
+
+
+# ---------------------------------------------------------------------------
 # Reference extension surface (origami_bitpack_cuda_v6, cpp:894-903)
 # ---------------------------------------------------------------------------
 
@@ -749,5 +822,6 @@ __all__ = [
     "block_ids_tensor", "unpack_to_kv_cache", "pack_from_kv_cache", "scatter_kv_blocks",
     "gather_kv_blocks", "kv_symbol_layout", "CACHE_KV_FIRST", "CACHE_BLOCKS_FIRST",
     "cachegen_unpack_dequantize_to_kv_cache", "cachegen_unpack_dequantize",
-    "kivi_dequantize_to_kv_cache", "dequant_cache_geometry",
+    "kivi_dequantize_to_kv_cache", "dequant_cache_geometry", "append_kv_cache",
+    "shared_prefix_attention",
 ]

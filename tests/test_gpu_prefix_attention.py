@@ -1,0 +1,317 @@
+"""shared_prefix_attention on the GPU against plain 64-bit attention (tests/pagedref.py)."""
+import math
+
+import pytest
+import torch
+
+from origami_amd.lossless import native_gpu
+from tests import pagedref
+
+pytestmark = pytest.mark.gpu
+BF16, F16, FP8 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+class Batch:
+    """A paged cache and a batch on it; every cell that the batch does not hold is NaN."""
+
+    def __init__(self, dev, *, heads=2, group=4, D=128, bs=16, dtype=BF16, cache_dtype=None,
+                 order="kv_first", prefix=100, own=(5, 33), queries=None, seed=0, spare=3,
+                 peak=2.0):
+        gen = torch.Generator().manual_seed(seed)
+        self.heads, self.D, self.bs, self.dtype, self.prefix = heads, D, bs, dtype, prefix
+        cache_dtype = cache_dtype or dtype
+        width = max(-(-max(own, default=0) // bs), 1)
+        shared = -(-prefix // bs)
+        NB = shared + len(own) * width + spare
+        ids = torch.randperm(NB, generator=gen)
+        self.prefix_ids = ids[:shared].to(dev)
+        self.tables = ids[shared:shared + len(own) * width].view(len(own), width).to(dev)
+        kv = torch.randn(2, NB, bs, heads, D, generator=gen)
+        self.k_scale, self.v_scale = (0.5, 0.25) if cache_dtype == FP8 else (1.0, 1.0)
+        live = torch.zeros(NB, bs, dtype=torch.bool)
+        for table, n in [(ids[:shared], prefix)] + [(t.cpu(), n) for t, n in zip(self.tables, own)]:
+            for i in range(n):
+                live[table[i // bs], i % bs] = True
+        kv[:, ~live] = math.nan
+        kv = kv if order == "kv_first" else kv.transpose(0, 1).contiguous()
+        self.cache = kv.to(cache_dtype).to(dev)
+        self.own = torch.tensor(own, dtype=torch.int64, device=dev)
+        self.starts = None
+        n = len(own)
+        if queries is not None:
+            self.starts = torch.tensor([0, *queries]).cumsum(0).to(dev)
+            n = sum(queries)
+        self.query = (peak * torch.randn(n, heads * group, D, generator=gen)).to(dtype).to(dev)
+
+    def run(self, **kw):
+        return native_gpu.shared_prefix_attention(
+            self.query, self.cache, self.prefix_ids, self.prefix, self.tables, self.own,
+            **{"query_starts": self.starts, "k_scale": self.k_scale, "v_scale": self.v_scale,
+               "return_lse": True, **kw})
+
+    def check(self, got, lse, rows=None, scale=None):
+        ref, ref_lse, size, largest = pagedref.attend(
+            self.query, self.cache, self.prefix_ids, self.prefix, self.tables, self.own,
+            self.starts, scale, self.k_scale, self.v_scale)
+        tokens = self.prefix + int(self.own.max()) if self.own.numel() else self.prefix
+        rows = slice(None) if rows is None else rows
+        tol = pagedref.attend_tolerance(self.dtype, self.D, tokens, size, largest, ref)
+        assert torch.equal(got[rows].isnan(), ref[rows].isnan())
+        off = (got.double() - ref).abs() - tol
+        assert not (off[rows] > 0).any(), float(off[rows].nan_to_num(0).max())
+        if lse is not None:
+            same = lse.double() == ref_lse  # infinities
+            off = (lse.double() - ref_lse).abs() - pagedref.lse_tolerance(
+                self.D, tokens, largest, ref_lse)
+            assert (same | (off <= 0) | ref_lse.isnan())[rows].all()
+
+
+@pytest.mark.parametrize("dtype,cache_dtype", [(BF16, BF16), (F16, F16), (BF16, FP8), (F16, FP8)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("order", ["kv_first", "blocks_first"])
+def test_types_and_sizes(cuda_device, dtype, cache_dtype, D, order):
+    b = Batch(cuda_device, D=D, dtype=dtype, cache_dtype=cache_dtype, order=order, prefix=150,
+              own=(1, 40, 16, 77, 33))
+    b.check(*b.run())
+
+
+@pytest.mark.parametrize("heads,group", [(1, 1), (3, 1), (1, 7), (2, 16), (1, 17), (1, 48), (5, 8)])
+@pytest.mark.parametrize("queries", [None, (2, 0, 5, 1)])
+def test_head_groups(cuda_device, heads, group, queries):
+    b = Batch(cuda_device, heads=heads, group=group, D=64, prefix=70, own=(9, 3, 50, 1),
+              queries=queries, seed=heads * group)
+    b.check(*b.run())
+
+
+@pytest.mark.parametrize("D", [8, 16, 24, 40, 72, 80, 96, 120, 136, 192, 248])
+@pytest.mark.parametrize("cache_dtype", [BF16, FP8])
+def test_odd_head_sizes(cuda_device, D, cache_dtype):
+    b = Batch(cuda_device, D=D, cache_dtype=cache_dtype, prefix=45, own=(3, 70), seed=D)
+    b.check(*b.run())
+
+
+@pytest.mark.parametrize("bs", [1, 2, 5, 8, 16, 24, 32, 64, 256])
+@pytest.mark.parametrize("prefix", [0, 1, 31, 32, 33, 257])
+def test_block_sizes(cuda_device, bs, prefix):
+    b = Batch(cuda_device, bs=bs, prefix=prefix, own=(31, 1, 32, 65), D=64, seed=bs + prefix)
+    b.check(*b.run())
+
+
+@pytest.mark.parametrize("own", [(0,), (1,), (130,), (0, 0, 0), (0, 5, 0, 129), (511, 513, 512)])
+@pytest.mark.parametrize("prefix", [0, 1, 700])
+def test_lengths(cuda_device, own, prefix):
+    b = Batch(cuda_device, prefix=prefix, own=own, D=64, seed=prefix + len(own))
+    b.check(*b.run())
+
+
+@pytest.mark.parametrize("prefix,own", [(5000, (1, 900)), (20011, (40,) * 20), (0, (9001, 17)),
+                                        (2500, (2100,))])
+@pytest.mark.parametrize("cache_dtype", [BF16, FP8])
+def test_long(cuda_device, prefix, own, cache_dtype):
+    b = Batch(cuda_device, prefix=prefix, own=own, cache_dtype=cache_dtype, seed=prefix)
+    b.check(*b.run())
+
+
+@pytest.mark.parametrize("queries,own,prefix", [
+    ((1,), (1,), 0), ((5, 5, 5), (5, 90, 33), 300), ((3, 0, 7), (3, 4, 7), 50),
+    ((64, 17), (64, 80), 129), ((130,), (130,), 0), ((200, 1, 77), (233, 9, 77), 400),
+    ((129, 300), (400, 300), 64), ((70,) * 6, (75,) * 6, 1000)])
+@pytest.mark.parametrize("heads,group", [(2, 1), (1, 5), (2, 4)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_several_queries(cuda_device, queries, own, prefix, heads, group, dtype):
+    b = Batch(cuda_device, prefix=prefix, own=own, queries=queries, heads=heads, group=group,
+              D=64 if group == 1 else 128, dtype=dtype, seed=sum(queries))
+    b.check(*b.run())
+    b.check(*b.run(max_query_tokens=max(queries), max_own_tokens=max(own)))
+
+
+def test_queries_beyond_the_own_tokens(cuda_device):
+    """More query rows than own tokens: the first rows see the prefix alone, or nothing."""
+    for prefix in (0, 40):
+        b = Batch(cuda_device, prefix=prefix, own=(2, 0), queries=(6, 3), D=64)
+        b.check(*b.run())
+
+
+def test_masked_values_have_no_influence(cuda_device):
+    """NaN and infinities in later own tokens reach the rows that see them and no others."""
+    for value in (math.nan, math.inf, -math.inf):
+        for half in (0, 1):
+            b = Batch(cuda_device, prefix=20, own=(40, 37), queries=(30, 37), heads=2, group=2)
+            table, bs = b.tables[0].tolist(), b.bs
+            b.cache[half, table[25 // bs], 25 % bs, 1, 7] = value
+            got, lse = b.run()
+            # token 25 is that of query 15 of request 0; heads 2 and 3 read cache head 1
+            sees = torch.zeros(67, 4, dtype=torch.bool, device=cuda_device)
+            sees[15:30, 2:] = True
+            clean = Batch(cuda_device, prefix=20, own=(40, 37), queries=(30, 37), heads=2, group=2)
+            ref, ref_lse = clean.run()
+            assert torch.equal(got[~sees], ref[~sees])
+            assert torch.equal(lse[~sees], ref_lse[~sees])
+            if half == 1:
+                assert not got[sees][:, 7].isfinite().any()
+                keep = [d for d in range(b.D) if d != 7]
+                assert torch.equal(got[sees][:, keep], ref[sees][:, keep])
+            elif math.isnan(value):
+                assert got[sees].isnan().all()
+
+
+def test_blocks_outside_the_cache_are_not_seen(cuda_device):
+    b = Batch(cuda_device, prefix=100, own=(50, 60, 3), D=64)
+    NB = pagedref.halves(b.cache).shape[1]
+    b.prefix_ids[2] = -1
+    b.prefix_ids[6] = NB
+    b.tables[0, 1] = 1 << 40
+    b.tables[2, 0] = -(1 << 50)
+    b.check(*b.run())
+    b.prefix_ids.fill_(-1)
+    b.tables.fill_(NB)
+    got, lse = b.run()
+    assert not got.any() and (lse == -math.inf).all()
+
+
+def test_strided_inputs_and_output(cuda_device):
+    """Queries inside a projection's rows, tables behind the prefix's columns, head-major output."""
+    b = Batch(cuda_device, prefix=96, own=(50, 60, 3))
+    rows = torch.full((3, 13, 128), math.nan, dtype=b.dtype, device=cuda_device)
+    rows[:, 2:10] = b.query
+    wide = torch.full((3, 9), -1, dtype=torch.int64, device=cuda_device)
+    wide[:, 3:3 + b.tables.shape[1]] = b.tables
+    plain, lse = b.run()
+    out = torch.full((8, 3, 128), 7.0, dtype=b.dtype, device=cuda_device).transpose(0, 1)
+    b.query, b.tables = rows[:, 2:10], wide[:, 3:3 + b.tables.shape[1]]
+    got, again = b.run(out=out)
+    assert got.data_ptr() == out.data_ptr()
+    assert torch.equal(out, plain) and torch.equal(lse, again)
+    odd = torch.zeros(3 * 8 * 129 + 1, dtype=b.dtype, device=cuda_device)[1:]
+    odd = odd.as_strided((3, 8, 128), (8 * 129, 129, 1))
+    odd.copy_(b.query)  # rows on two-byte boundaries
+    b.query = odd
+    out = torch.zeros(3 * 8 * 129 + 1, dtype=b.dtype, device=cuda_device)[1:]
+    out = out.as_strided((3, 8, 128), (8 * 129, 129, 1))
+    assert torch.equal(b.run(out=out)[0], plain)
+
+
+def test_rows_of_no_request_stay(cuda_device):
+    b = Batch(cuda_device, prefix=50, own=(9, 20), queries=(2, 3), D=64)
+    b.query = torch.cat((b.query[:1], b.query, b.query[:4]))
+    b.starts = b.starts + 1
+    out = torch.full_like(b.query, 3.0)
+    got, lse = b.run(out=out)
+    rest = [0, 6, 7, 8, 9]
+    assert (out[rest] == 3.0).all() and (lse[rest] == -math.inf).all()
+    b.check(got, lse, rows=slice(1, 6))
+    assert not b.run()[0][rest].any()
+
+
+def test_scale(cuda_device):
+    for scale in (0.0, 1.0, -0.3):
+        b = Batch(cuda_device, prefix=50, own=(9, 20), D=64, peak=0.5)
+        b.check(*b.run(scale=scale), scale=scale)
+
+
+def test_far_blocks_of_a_large_cache(cuda_device):
+    """Rows past 2^31 elements (and past 2^32 bytes) of the cache."""
+    NB, bs, H, D = 40000, 16, 8, 256
+    b = Batch(cuda_device, heads=H, D=D, bs=bs, prefix=40, own=(20, 33), group=1)
+    kv = torch.empty(2, NB, bs, H, D, dtype=BF16, device=cuda_device)
+    small = b.cache.shape[1]
+    kv[:, NB - small:] = b.cache
+    plain = b.run()
+    b.cache, b.prefix_ids, b.tables = kv, b.prefix_ids + NB - small, b.tables + NB - small
+    for x, y in zip(b.run(), plain):
+        assert torch.equal(x, y)
+
+
+def test_same_result_every_time_and_on_another_stream(cuda_device):
+    b = Batch(cuda_device, prefix=3001, own=(900, 20, 400), queries=(4, 1, 9))
+    plain, lse = b.run()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = [b.run() for _ in range(3)]
+    torch.cuda.current_stream().wait_stream(stream)
+    for x, y in got:
+        assert torch.equal(x, plain) and torch.equal(y, lse)
+
+
+def test_captured_steps_follow_the_lengths(cuda_device):
+    """Two captured calls replayed in turn while lengths grow, with eager calls between."""
+    bound = dict(max_own_tokens=208)
+    batches = [Batch(cuda_device, prefix=300, own=(200, 200, 200), seed=s) for s in (1, 2)]
+    graphs = []
+    for b in batches:
+        b.own.fill_(1)
+        b.run(**bound)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            result = b.run(**bound)
+        graphs.append((graph, result))
+    for step in range(4):
+        for b, (graph, result) in zip(batches, graphs):
+            b.own.copy_(torch.tensor([3 + 40 * step, 200 - step, 64 * step]))
+            graph.replay()
+            eager = b.run(**bound)
+            torch.cuda.synchronize()
+            assert torch.equal(result[0], eager[0]) and torch.equal(result[1], eager[1])
+            b.check(*result)
+
+
+def test_parts_join_by_lse(cuda_device):
+    """The results over the prefix alone and the own tokens alone, joined by their lse."""
+    b = Batch(cuda_device, prefix=200, own=(30, 41), dtype=F16)
+    whole, _ = b.run()
+    none = torch.zeros_like(b.own)
+    p, lp = native_gpu.shared_prefix_attention(b.query, b.cache, b.prefix_ids, 200, b.tables, none,
+                                               return_lse=True)
+    o, lo = native_gpu.shared_prefix_attention(b.query, b.cache, None, 0, b.tables, b.own,
+                                               return_lse=True)
+    w = torch.sigmoid(lp - lo)[..., None]
+    joined = w * p.float() + (1 - w) * o.float()
+    assert (joined - whole.float()).abs().max() < 4 * 2.0 ** -11 * 4  # four roundings of |v| < 4
+
+
+def test_empty_calls(cuda_device):
+    b = Batch(cuda_device, prefix=20, own=(5, 6), D=64)
+    got, lse = native_gpu.shared_prefix_attention(
+        b.query[:0], b.cache, b.prefix_ids, 20, b.tables[:0], b.own[:0], return_lse=True)
+    assert got.shape == (0, 8, 64) and lse.shape == (0, 8)
+    starts = torch.zeros(3, dtype=torch.int64, device=cuda_device)
+    got, lse = native_gpu.shared_prefix_attention(
+        b.query, b.cache, b.prefix_ids, 20, b.tables, b.own, query_starts=starts, return_lse=True)
+    assert not got.any() and (lse == -math.inf).all()
+
+
+def test_refusals(cuda_device):
+    b = Batch(cuda_device, prefix=20, own=(5, 6), D=64)
+
+    def refused(match, **kw):
+        args = dict(query=b.query, kv_cache=b.cache, prefix_block_ids=b.prefix_ids,
+                    prefix_tokens=20, block_tables=b.tables, own_tokens=b.own)
+        args.update(kw)
+        with pytest.raises(RuntimeError, match=match):
+            native_gpu.shared_prefix_attention(**args)
+
+    refused("same dtype|queries' dtype", query=b.query.half())
+    refused("float16 or bfloat16", query=b.query.float())
+    refused("head_dim differs", query=b.query[..., :32])
+    refused("channels must be contiguous", query=b.query.transpose(1, 2).contiguous().transpose(1, 2))
+    refused("multiple of the cache's heads", query=b.query[:, :3])
+    refused("kv_cache device", query=b.query.cpu())
+    refused("requires a gradient", query=b.query.clone().requires_grad_())
+    refused("prefix tokens exceed", prefix_tokens=33)
+    refused("prefix tokens exceed", prefix_block_ids=None)
+    refused("must not be negative", prefix_tokens=-1)
+    refused("must be a contiguous int64 vector", own_tokens=b.own.int())
+    refused("must have 2 values", own_tokens=b.own[:1])
+    refused("must have 3 values", query_starts=b.own)
+    refused("int64 .requests, blocks.", block_tables=b.tables.int())
+    refused("one query token", query=b.query[:1])
+    refused("exceeds the block tables", max_own_tokens=1000)
+    refused("exceeds the query tokens", query_starts=torch.zeros(3, dtype=torch.int64,
+                                                                 device=cuda_device),
+            max_query_tokens=3)
+    refused("scales are for float8", k_scale=0.5)
+    refused("out must have", out=b.query[:1].clone())
+    refused("rank 5", kv_cache=b.cache[0])
+    refused("contiguous", kv_cache=b.cache[:, :, :, :1])

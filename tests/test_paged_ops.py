@@ -1,0 +1,100 @@
+"""Refusals of the C entry points of the operators on the paged cache; no GPU is needed, since
+they are checked before anything is launched."""
+import pytest
+
+from origami_amd import _native
+
+BF16, FP8, F32 = _native.DTYPE_BFLOAT16, _native.DTYPE_FLOAT8_E4M3FN, _native.DTYPE_FLOAT32
+
+
+def _append(**kw):
+    a = dict(key=16, value=16, query=16, query_out=16, dtype=BF16, strides=[8] * 8, tokens=4,
+             query_heads=4, kv_cache=16, cache_dtype=BF16, layout=0, num_blocks=4, block_size=16,
+             heads=2, head_dim=64, slots=16, positions=16, cos_sin=16, table_rows=10,
+             rotary_dim=64, interleaved=0, query_norm=None, key_norm=None, norm_dtype=BF16,
+             eps=1e-6, k_scale=1.0, v_scale=1.0, stream=None)
+    a.update(kw)
+    strides = _native.i64_array(a["strides"])
+    a["strides"] = strides.ctypes.data
+    return _native.call("origami_append_kv_cache", *a.values())
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(dtype=F32), "must be float16 or bfloat16"),
+    (dict(cache_dtype=F32), "keys' dtype or be float8_e4m3fn"),
+    (dict(tokens=-1), "must not be negative"),
+    (dict(heads=0), "must not be negative"),
+    (dict(head_dim=60), "multiple of 8"),
+    (dict(head_dim=264), "at most 256"),
+    (dict(block_size=0), "block size must be positive"),
+    (dict(layout=7), "kv_cache must be"),
+    (dict(num_blocks=1 << 40), "too many token slots"),
+    (dict(query_out=None), "need an output"),
+    (dict(rotary_dim=7), "even rotary size"),
+    (dict(rotary_dim=66), "even rotary size"),
+    (dict(positions=None), "needs positions"),
+    (dict(table_rows=0), "needs positions"),
+    (dict(key_norm=16, norm_dtype=_native.DTYPE_FLOAT16), "norm weights"),
+    (dict(eps=-1.0), "eps"),
+    (dict(eps=float("nan")), "eps"),
+    (dict(cache_dtype=FP8, k_scale=0.0), "scales must be positive"),
+    (dict(cache_dtype=FP8, v_scale=float("nan")), "scales must be positive"),
+    (dict(v_scale=2.0), "for float8_e4m3fn"),
+    (dict(kv_cache=24), "16-byte aligned"),
+    (dict(tokens=1 << 29), "too many rows"),
+])
+def test_append_refuses(change, message):
+    with pytest.raises(_native.OrigamiNativeError, match=message) as e:
+        _append(**change)
+    assert e.value.code == _native.ORIGAMI_ERR_INVALID
+
+
+def _attend(**kw):
+    a = dict(query=16, dtype=BF16, strides=[8] * 4, tokens=3, query_heads=4, kv_cache=16,
+             cache_dtype=BF16, layout=0, num_blocks=4, block_size=16, heads=2, head_dim=64,
+             prefix_ids=16, prefix_blocks=2, prefix=32, tables=16, table_stride=2, table_blocks=2,
+             own=16, requests=3, starts=None, max_query=1, max_own=32, scale=1.0, k_scale=1.0,
+             v_scale=1.0, out=16, lse=None, workspace=16, workspace_bytes=1 << 30, stream=None)
+    a.update(kw)
+    strides = _native.i64_array(a["strides"])
+    a["strides"] = strides.ctypes.data
+    return _native.call("origami_shared_prefix_attention", *a.values())
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(dtype=F32), "queries must be float16 or bfloat16"),
+    (dict(cache_dtype=F32), "queries' dtype or be float8_e4m3fn"),
+    (dict(query_heads=3), "multiple of the cache's heads"),
+    (dict(heads=0), "multiple of the cache's heads"),
+    (dict(head_dim=4), "multiple of 8"),
+    (dict(head_dim=512), "at most 256"),
+    (dict(tokens=-1), "must not be negative"),
+    (dict(prefix=-1), "must not be negative"),
+    (dict(max_query=4), "exceeds the query tokens"),
+    (dict(prefix=1 << 30), "too many tokens"),
+    (dict(tokens=1 << 29, starts=16), "too many query rows"),
+    (dict(num_blocks=1 << 28), "too many token slots"),
+    (dict(block_size=0), "block size must be positive"),
+    (dict(layout=3), "kv_cache must be"),
+    (dict(prefix=33), "exceed the prefix blocks"),
+    (dict(max_own=33), "exceeds the block tables"),
+    (dict(tokens=4), "one query token"),
+    (dict(max_query=2), "one query token"),
+    (dict(k_scale=-1.0), "scales must be positive"),
+    (dict(v_scale=0.5), "for float8_e4m3fn"),
+    (dict(kv_cache=17), "16-byte aligned"),
+    (dict(workspace_bytes=8), "workspace is too small"),
+    (dict(workspace=None), "workspace is too small"),
+])
+def test_attention_refuses(change, message):
+    with pytest.raises(_native.OrigamiNativeError, match=message) as e:
+        _attend(**change)
+    assert e.value.code == _native.ORIGAMI_ERR_INVALID
+
+
+def test_workspace_sizes():
+    size = _native.lib().origami_shared_prefix_attention_workspace
+    assert size(3, 4, 2, 64, 32, 3, 1, 32) > 0
+    assert size(0, 4, 2, 64, 32, 3, 0, 32) == 0
+    assert size(3, 3, 2, 64, 32, 3, 1, 32) == -1
+    assert size(1, 4, 2, 64, 0, 1, 1, 16) == 0  # one part: the rows are written at once
