@@ -5,6 +5,7 @@
 // The tokens come in parts (the prefix, the request's own tokens, ranges of either).  A part
 // gives m, the sum l and the unnormalised row O in binary32; parts are joined with the weights
 // exp(m_part - m), so that no part waits for another.
+#include <algorithm>
 #include <type_traits>
 
 #include "origami_element.h"
@@ -26,11 +27,20 @@ constexpr int kStep = 32;  // tokens of one product P V (the depth of its matrix
 // the largest stay far from binary32's limit.
 template <typename T>
 constexpr float kLift = std::is_same<T, f16>::value ? 10.0f : 0.0f;
+// How far (in powers of two) the maximum may rise before what is summed so far is scaled down;
+// 2^(kLift + kSlack) is within half precision.
+template <typename T>
+constexpr float kSlack = std::is_same<T, f16>::value ? 4.0f : 8.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Rows of a workgroup.  The last shape is for up to 128 channels: with 256, results of 32 rows a wave
+// and the tiles on their way would not fit the registers.
+constexpr int kShapeRows[3] = {16, 64, 128};
 
 // The work of one kind: row tiles of every KV head, over ranges of tokens.
 struct Group {
   int32_t units;   // workgroups
+  int32_t shape;   // kShapeRows[shape] rows each
   int32_t tiles;   // row tiles of a request, or of the batch
   int32_t splits;  // ranges of `chunk` tokens
   int32_t chunk;
@@ -43,6 +53,7 @@ struct AttendParams {
   int64_t q_token, q_head;  // strides, in elements
   void* out;
   int64_t o_token, o_head;
+  bool out_vec;  // its rows start on 8 bytes
   float* lse;  // [tokens, query heads], or null
   const uint8_t* cache;
   int64_t blk_stride, half_stride;  // rows of H * D, as cache_geometry
@@ -52,20 +63,30 @@ struct AttendParams {
   int32_t block_size, prefix, max_own, max_query;
   int32_t tokens, requests, Hq, H, G, D;
   float scale, v_scale;  // scale includes log2 e and the keys' scale
-  Group shared, each;    // the prefix with the whole batch's rows; each request's rows
+  Group group[2];        // the prefix with the whole batch's rows; each request's rows
   int32_t slots;
   float *part_o, *part_ml;  // [slots][rows][D], [slots][rows][2]
 };
 
-template <typename T>
-__device__ __forceinline__ Float4 mfma16(Vec8<T> a, Vec8<T> b, Float4 c);
-template <>
-__device__ __forceinline__ Float4 mfma16<bf16>(Vec8<bf16> a, Vec8<bf16> b, Float4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-template <>
-__device__ __forceinline__ Float4 mfma16<f16>(Vec8<f16> a, Vec8<f16> b, Float4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+// MR x MR scores or results: value x of a lane is in column lane % MR and in row
+// 4 (lane / MR) + x % 4 + (256 / MR) (x / 4).
+template <int MR>
+using Tile = float __attribute__((ext_vector_type(MR * MR / 64)));
+
+// c + a b, where a lane has 8 values of row (a) and column (b) lane % MR, from 8 (lane / MR) on.
+template <typename T, int MR>
+__device__ __forceinline__ Tile<MR> mfma(Vec8<T> a, Vec8<T> b, Tile<MR> c) {
+  if constexpr (MR == 16) {
+    if constexpr (std::is_same<T, bf16>::value)
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  } else {
+    if constexpr (std::is_same<T, bf16>::value)
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
 }
 
 typedef short Short4 __attribute__((ext_vector_type(4)));
@@ -77,11 +98,49 @@ __device__ __forceinline__ U32x2 read_column(const uint8_t* p) {
       (__attribute__((address_space(3))) Short4*)p));
 }
 
-// Whether one of the two 16-bit values in `w` is an infinity or NaN.
+// Four channels of a cache row.
+template <typename T, bool FP8>
+__device__ __forceinline__ Float4 four_values(const uint8_t* row, int ch) {
+  Float4 out;
+  if constexpr (FP8) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(row + ch);
+    const Vec2<T> a = fp8_pair<false>(w, T()), b = fp8_pair<true>(w, T());
+    out = Float4{static_cast<float>(a[0]), static_cast<float>(a[1]), static_cast<float>(b[0]),
+                 static_cast<float>(b[1])};
+  } else {
+    const Vec4<T> v = *reinterpret_cast<const Vec4<T>*>(row + 2 * ch);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = static_cast<float>(v[j]);
+  }
+  return out;
+}
+
+// Infinities and NaN among eight values become 0; whether there were any.
 template <typename T>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-  constexpr uint32_t e = std::is_same<T, bf16>::value ? 0x7f80u : 0x7c00u;
-  return (w & e) == e || ((w >> 16) & e) == e;
+__device__ __forceinline__ bool drop_odd(U32x4& w) {
+  constexpr uint32_t low = std::is_same<T, bf16>::value ? 0x7f80u : 0x7c00u, high = low << 16;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool l = (w[i] & low) == low, h = (w[i] & high) == high;
+    odd |= l || h;
+    w[i] = (l ? 0u : w[i] & 0xffffu) | (h ? 0u : w[i] & 0xffff0000u);
+  }
+  return odd;
+}
+
+// Four values rounded to T; `vec`: rows start on 8 bytes.
+template <typename T>
+__device__ __forceinline__ void store4(T* dst, Float4 v, bool vec) {
+  Vec4<T> w;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = static_cast<T>(v[j]);
+  if (vec) {
+    *reinterpret_cast<Vec4<T>*>(dst) = w;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) dst[j] = w[j];
 }
 
 // A request's place in the batch.
@@ -104,19 +163,77 @@ __device__ __forceinline__ Request request_of(const AttendParams& p, int r) {
   return q;
 }
 
-// One workgroup: 16 MT rows of one KV head over a range of tokens, which its four waves take
-// in turn, 32 at a time.  A wave holds its rows' queries and results in registers and its
-// tokens' keys and values in LDS, and needs no other wave until the end.
-template <typename T, bool FP8, int DP, int MT>
-__device__ void attend(const AttendParams& p, const Group& g, int unit, bool batch, uint8_t* lds) {
-  constexpr int KS = DP / 32, DT = DP / 16;    // depth steps of Q K, channel tiles of P V
-  constexpr int NCH = DP / 8;                  // 16-byte pieces of a row in LDS
-  constexpr int RPI = 64 / NCH, IT = kStep / RPI;  // rows of one load, loads of a step
-  constexpr int M = 16 * MT;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, q4 = lane >> 4;
+// Where the 16-byte piece `piece` of token `tok`'s row is in LDS, in pieces of its row.  Keys are
+// read by 16 lanes from the same piece of 16 tokens, values by 32 lanes from pieces next to each
+// other (2 of 8 tokens, or 4 of 4): with the token's low bits in the piece's number these
+// are in different banks (of 256 bytes: two 128-byte rows of 64 channels, one of 128).
+template <int DP>
+__device__ __forceinline__ int key_piece(int tok, int piece) {
+  return piece ^ (DP == 64 ? (tok >> 1) & 7 : tok & 15);
+}
+template <int DP, int MR>
+__device__ __forceinline__ int value_piece(int tok, int piece) {
+  const int t = DP == 64 ? tok >> 1 : tok;
+  if (MR == 16) return piece ^ ((t & (DP == 64 ? 3 : 7)) << 1);
+  return piece ^ ((t & (DP == 64 ? 1 : 3)) << 2);
+}
 
-  // the unit: KV head fastest
+// The values of MR channels (tile d) of 32 tokens' k-th part, as V P takes them: value j is that
+// of token 4 (lane / MR) + j % 4 + (256 / MR) (2 k + j / 4).
+template <typename T, int DP, int MR>
+__device__ __forceinline__ Vec8<T> read_values(const uint8_t* values, int lane, int k, int d) {
+  constexpr int NCH = DP / 8;
+  const int c16 = lane & 15;
+  U32x4 out;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int tok = 256 / MR * (2 * k + j) + 4 * (lane / MR) + (c16 >> 2);
+    const int piece = MR / 8 * d + (MR == 32 ? ((lane >> 4) & 1) * 2 : 0) + ((c16 & 3) >> 1);
+    const U32x2 w =
+        read_column(values + (tok * NCH + value_piece<DP, MR>(tok, piece)) * 16 + (c16 & 1) * 8);
+    out[2 * j] = w[0];
+    out[2 * j + 1] = w[1];
+  }
+  return __builtin_bit_cast(Vec8<T>, out);
+}
+
+// Tokens that a team of waves (the WR waves with the same tokens) has in LDS at a time.
+template <int DP, int WR>
+constexpr int kTeamTokens = WR == 4 && DP < 256 ? 64 : 32;
+
+// One workgroup: WR MR rows of one KV head over a range of tokens.  Its waves are WR row waves
+// by kWaves / WR token waves: a wave takes MR rows, and of every kWaves / WR times kTeamTokens
+// tokens its share.  Rows (queries, results, sums) stay in registers; keys and values go
+// through LDS, where the WR waves of a team share them, and the next ones are on their way
+// to registers meanwhile.  With WR = 1 no wave needs another until the end; else two buffers
+// take turns, so that one barrier a step is enough.
+template <typename T, bool FP8, int DP, int MR, int WR>
+__device__ __forceinline__ void attend(const AttendParams& p, const Group& g, int unit, bool batch,
+                                       uint8_t* lds) {
+  constexpr int WT = kWaves / WR, TT = kTeamTokens<DP, WR>;
+  constexpr int NG = 64 / MR;             // lane groups: the depth of a product is 8 NG
+  constexpr int KS = DP / (8 * NG);       // depth steps of K Q
+  constexpr int DT = DP / MR;             // channel tiles of V P
+  constexpr int X = MR / 2;               // scores of a lane in 32 tokens
+  constexpr int ST = TT / kStep;          // steps of 32 tokens
+  constexpr int ACC = MR * MR / 64;       // values of a lane in a tile
+  constexpr int STRIDE = 4 * NG;          // tokens between a lane's groups of four
+  constexpr int NCH = DP / 8;             // 16-byte pieces of a row in LDS
+  constexpr int RPI = 64 / NCH;           // rows of one load
+  constexpr int IT = TT / (RPI * WR);     // loads of a tile
+  constexpr int kBuffers = WR == 1 ? 1 : 2;
+  constexpr int kTile = TT * DP * 2;      // bytes of a team's keys
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wr = wave % WR, wt = wave / WR;
+  const int c = lane % MR, q4 = lane / MR;
+
+  // The unit: row tiles of the same keys are 8 units apart, so that they run on the same chiplet
+  // at about the same time and its L2 gives the keys to all but the first.
   int u = unit;
+  const int eighth = u & 7;
+  u >>= 3;
+  const int tile = u % g.tiles;
+  u = (u / g.tiles) * 8 + eighth;
   const int h = u % p.H;
   u /= p.H;
   int r = 0;
@@ -126,323 +243,407 @@ __device__ void attend(const AttendParams& p, const Group& g, int unit, bool bat
     u /= p.requests;
     rq = request_of(p, r);
   }
-  const int tile = u % g.tiles, split = u / g.tiles;
-  const int rows = rq.count * p.G, row0 = tile * M;
-  if (row0 >= rows) return;
+  const int split = u;
+  const int rows = rq.count * p.G, row0 = tile * WR * MR;
+  if (split >= g.splits || row0 >= rows) return;
   const int end = batch ? p.prefix : p.prefix + rq.own;  // of the tokens, prefix first
   const int64_t* const table = p.tables + static_cast<int64_t>(r) * p.table_stride;
 
-  // this lane's rows
-  int limit[MT];  // tokens the row sees
-  int64_t at[MT];  // its row of the partial results, -1 past the last
-  Vec8<T> qf[MT][KS];
-  int most = 0, least = INT32_MAX;
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int row = row0 + 16 * m + c;
-    const bool live = row < rows;
-    const int i = live ? row / p.G : 0, head = h * p.G + (live ? row - i * p.G : 0);
-    limit[m] = batch ? p.prefix : p.prefix + min(max(rq.own - rq.count + i + 1, 0), rq.own);
-    const int64_t n = rq.first + i;
-    at[m] = live ? n * p.Hq + head : -1;
+  // this lane's row
+  const int row = row0 + wr * MR + c;
+  const bool live = row < rows;
+  const int qi = live ? row / p.G : 0, head = h * p.G + (live ? row - qi * p.G : 0);
+  const int limit =  // tokens it sees
+      batch ? p.prefix : p.prefix + min(max(rq.own - rq.count + qi + 1, 0), rq.own);
+  const int64_t n = rq.first + qi, at = n * p.Hq + head;
+  // the scale's sign goes with the queries, and so does a scale of zero, so that hidden scores of
+  // -infinity stay what they are
+  const float scale = p.scale == 0.0f ? 1.0f : fabsf(p.scale);
+  Vec8<T> qf[KS];
+  {
     const T* const src = static_cast<const T*>(p.query) + n * p.q_token + head * p.q_head;
+    const bool vec =
+        ((reinterpret_cast<uintptr_t>(p.query) | 2 * p.q_token | 2 * p.q_head) & 15) == 0;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-      const int d = 32 * k + 8 * q4;
-      qf[m][k] = Vec8<T>{};
+      const int d = 8 * (NG * k + q4);
+      qf[k] = Vec8<T>{};
       if (live && d < p.D) {
-        if (((reinterpret_cast<uintptr_t>(p.query) | 2 * p.q_token | 2 * p.q_head) & 15) == 0) {
-          qf[m][k] = *reinterpret_cast<const Vec8<T>*>(src + d);
+        if (vec) {
+          qf[k] = *reinterpret_cast<const Vec8<T>*>(src + d);
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) qf[m][k][j] = src[d + j];
+          for (int j = 0; j < 8; ++j) qf[k][j] = src[d + j];
         }
+        if (p.scale <= 0.0f) qf[k] = p.scale == 0.0f ? Vec8<T>{} : -qf[k];
       }
     }
-    if (live) {
-      most = max(most, limit[m]);
-      least = min(least, limit[m]);
-    }
   }
-#pragma unroll
-  for (int x = 1; x < 16; x <<= 1) {
-    most = max(most, __shfl_xor(most, x));
-    least = min(least, __shfl_xor(least, x));
-  }
+  // The tokens that some row of the workgroup sees, and those that all rows of the wave see;
+  // limits grow along the rows.
+  const int last_row = min(row0 + WR * MR, rows) - 1;
+  const int most = batch ? p.prefix
+                         : p.prefix + min(max(rq.own - rq.count + last_row / p.G + 1, 0), rq.own);
+  const int first_row = min(row0 + wr * MR, rows - 1);
+  const int least =
+      batch ? p.prefix : p.prefix + min(max(rq.own - rq.count + first_row / p.G + 1, 0), rq.own);
+  const int nearest =  // the tokens that all rows of the workgroup see
+      batch ? p.prefix : p.prefix + min(max(rq.own - rq.count + row0 / p.G + 1, 0), rq.own);
   const int t0 = g.first + split * g.chunk;
   const int t1 = min(min(end, most), t0 + g.chunk);
 
-  Float4 o[MT][DT];
-  float top[MT], sum[MT];
+  Tile<MR> o[DT];
+  float base = -INFINITY, sum = 0.0f;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    top[m] = -INFINITY;
-    sum[m] = 0.0f;
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[m][d] = Float4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+    for (int x = 0; x < ACC; ++x) o[d][x] = 0.0f;
 
-  constexpr int kTile = kStep * DP * 2;  // bytes of a wave's keys
-  uint8_t* const ks = lds + wave * 2 * kTile;
-  uint8_t* const vs = ks + kTile;
+  uint8_t* const team = lds + wt * kBuffers * 2 * kTile;
   const int piece = lane % NCH, sub = lane / NCH;
-  const bool has = 8 * piece < p.D;
-  const int64_t cell = FP8 ? 1 : 2;
+  const bool has = 8 * piece < p.D, exact = p.D == DP;
+  constexpr int cell = FP8 ? 1 : 2;
   const int64_t pitch = static_cast<int64_t>(p.H) * p.D * cell;
-  const int64_t col = (static_cast<int64_t>(h) * p.D + 8 * piece) * cell;
-  const int64_t vhalf = p.half_stride * pitch;
+  const uint8_t* const keys =
+      p.cache + (static_cast<int64_t>(h) * p.D + (has ? 8 * piece : 0)) * cell;
+  const uint8_t* const values = keys + p.half_stride * pitch;
 
-  // the cache row of token t, -1 where it has none
-  const auto cache_row = [&](int t) -> int {
+  // the block of token t, and its cache row, -1 where it has none
+  const auto block_of = [&](int t) -> int64_t {
     if (t >= t1) return -1;
     const bool pre = t < p.prefix;
-    const int i = pre ? t : t - p.prefix, b = i / p.block_size;
-    const int64_t id = pre ? p.prefix_ids[b] : table[b];
-    if (id < 0 || id >= p.num_blocks) return -1;
-    return static_cast<int>(id * p.blk_stride + (i - b * p.block_size));
+    const int i = pre ? t : t - p.prefix;
+    return (pre ? p.prefix_ids : table)[i / p.block_size];
   };
-
-  for (int t = t0 + wave * kStep; t < t1; t += kWaves * kStep) {
-    const int mine = cache_row(t + (lane & 31));
-    const uint32_t there = static_cast<uint32_t>(__ballot(mine >= 0));
-    // keys and values of 32 tokens into LDS, zero where there are none
+  const auto row_of = [&](int t, int64_t id) -> int {
+    if (id < 0 || id >= p.num_blocks) return -1;
+    const int i = t < p.prefix ? t : t - p.prefix;
+    return static_cast<int>(id * p.blk_stride + i % p.block_size);
+  };
+  using Raw = typename std::conditional<FP8, U32x2, U32x4>::type;
+  Raw kr[IT], vr[IT];
+  const auto load_tile = [&](int mine) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const int tok = i * RPI + sub;
-      const int at_row = __shfl(mine, tok);
-      U32x4 kv = {}, vv = {};
-      if (at_row >= 0 && has) {
-        const uint8_t* const src = p.cache + at_row * pitch + col;
-        if constexpr (FP8) {
-          kv = fp8_expand<T>(*reinterpret_cast<const U32x2*>(src));
-          vv = fp8_expand<T>(*reinterpret_cast<const U32x2*>(src + vhalf));
-        } else {
-          kv = *reinterpret_cast<const U32x4*>(src);
-          vv = *reinterpret_cast<const U32x4*>(src + vhalf);
-        }
-      }
-      *reinterpret_cast<U32x4*>(ks + (tok * NCH + piece) * 16) = kv;
-      *reinterpret_cast<U32x4*>(vs + (tok * NCH + piece) * 16) = vv;
+      // rows that are not there are read from the cache's first (and made zero below)
+      const int64_t at_row = max(__shfl(mine, (i * WR + wr) * RPI + sub), 0) * pitch;
+      kr[i] = *reinterpret_cast<const Raw*>(keys + at_row);
+      vr[i] = *reinterpret_cast<const Raw*>(values + at_row);
     }
-    __builtin_amdgcn_wave_barrier();
+  };
+  // `partly`: some rows may not see some of the tokens.  A hidden token's weight is 0, but 0
+  // times an infinity or NaN is NaN: such values go in as 0, and reach the rows that see them
+  // at the end.
+  bool odd = false;
+  const auto store_tile = [&](uint8_t* buf, uint64_t there, bool partly) {
+    const bool all = exact && there == ~0ull;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int tok = (i * WR + wr) * RPI + sub;
+      U32x4 kv, vv;
+      if constexpr (FP8) {
+        kv = fp8_expand<T>(kr[i]);
+        vv = fp8_expand<T>(vr[i]);
+      } else {
+        kv = kr[i];
+        vv = vr[i];
+      }
+      if (partly) odd |= drop_odd<T>(vv);
+      if (!all && !(has && ((there >> tok) & 1))) kv = vv = U32x4{0, 0, 0, 0};
+      *reinterpret_cast<U32x4*>(buf + (tok * NCH + key_piece<DP>(tok, piece)) * 16) = kv;
+      *reinterpret_cast<U32x4*>(buf + kTile + (tok * NCH + value_piece<DP, MR>(tok, piece)) * 16) =
+          vv;
+    }
+  };
 
-    // S = K Q: token 16 s + 4 q4 + i against row c
-    Float4 sc[MT][2];
+  constexpr int kRound = WT * TT;  // tokens of a step of the workgroup
+  const int tl = lane % TT;
+  int t = t0 + wt * TT;  // the first of this wave's tokens
+  int mine = row_of(t + tl, block_of(t + tl));
+  if (t0 < t1) load_tile(mine);
+  int64_t ahead = block_of(t + kRound + tl);
+  int turn = 0;
+  // with a barrier in it, the loop is the same for all waves
+  for (int tb = t0; (WR == 1 ? t : tb) < t1; tb += kRound, t += kRound) {
+    uint8_t* const buf = team + turn * 2 * kTile;
+    const uint64_t there = __ballot(mine >= 0);  // twice 32 tokens where TT is 32
+    store_tile(buf, there, t + TT > nearest);
+    if constexpr (WR == 1)
+      __builtin_amdgcn_wave_barrier();
+    else
+      __syncthreads();
+    mine = row_of(t + kRound + tl, ahead);
+    ahead = block_of(t + 2 * kRound + tl);
+    if ((WR == 1 ? t : tb) + kRound < t1) load_tile(mine);
+
+    const bool whole = there == ~0ull && t + TT <= least;
+#pragma unroll 1
+    for (int s = 0; s < ST; ++s) {
+      const uint8_t* const kb = buf + s * kStep * NCH * 16;
+      const uint8_t* const vb = kb + kTile;
+      const int ts = t + s * kStep;  // the step's first token
+      // S = K Q: row c against token STRIDE (i / 4) + 4 q4 + i % 4
+      Tile<MR> sc[X / ACC];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+      for (int m = 0; m < X / ACC; ++m) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m) sc[m][s] = Float4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int x = 0; x < ACC; ++x) sc[m][x] = 0.0f;
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const Vec8<T> kf =
-            *reinterpret_cast<const Vec8<T>*>(ks + ((16 * s + c) * NCH + 4 * k + q4) * 16);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) sc[m][s] = mfma16<T>(kf, qf[m][k], sc[m][s]);
-      }
-    }
-    const bool whole = there == 0xffffffffu && t + kStep <= least;
-    Vec8<T> pf[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      float best = top[m];
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tok = 16 * s + 4 * q4 + i;
-          float v = sc[m][s][i] * p.scale;
-          if (!whole && (t + tok >= limit[m] || !((there >> tok) & 1))) v = -INFINITY;
-          sc[m][s][i] = v;
-          best = fmaxf(best, v);
+        for (int k = 0; k < KS; ++k) {
+          const int tok = MR * m + c;
+          const Vec8<T> kf = *reinterpret_cast<const Vec8<T>*>(
+              kb + (tok * NCH + key_piece<DP>(tok, NG * k + q4)) * 16);
+          sc[m] = mfma<T, MR>(kf, qf[k], sc[m]);
         }
-      best = fmaxf(best, __shfl_xor(best, 16));
-      best = fmaxf(best, __shfl_xor(best, 32));
-      const float keep = __builtin_amdgcn_exp2f(top[m] - (best == -INFINITY ? 0.0f : best));
-      const float base = best == -INFINITY ? 0.0f : best - kLift<T>;
-      top[m] = best;
-      sum[m] *= keep;
+      }
+      if (!whole) {
+        const uint32_t seen = static_cast<uint32_t>(there >> (kStep * s));
 #pragma unroll
-      for (int d = 0; d < DT; ++d) o[m][d] *= keep;
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(sc[m][s][i] - base);
-          sum[m] += e;
-          pf[m][4 * s + i] = static_cast<T>(e);
+        for (int i = 0; i < X; ++i) {
+          const int tok = STRIDE * (i / 4) + 4 * q4 + i % 4;
+          if (ts + tok >= limit || !((seen >> tok) & 1)) sc[i / ACC][i % ACC] = -INFINITY;
         }
-    }
-    // O += V P: channel 16 d + 4 q4 + i of row c
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      U32x4 vf;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int tok = 16 * s + 4 * q4 + (c >> 2);
-        const U32x2 w = read_column(vs + (tok * NCH + 2 * d + ((c & 3) >> 1)) * 16 + (c & 1) * 8);
-        vf[2 * s] = w[0];
-        vf[2 * s + 1] = w[1];
       }
-      if (!whole && __any(not_finite<T>(vf[0]) || not_finite<T>(vf[1]) || not_finite<T>(vf[2]) ||
-                          not_finite<T>(vf[3]))) {
-        // an infinity or NaN reaches only the rows that see its token: row by row, with the
-        // tokens that the row does not see taken as zero
-        for (int m = 0; m < MT; ++m)
-          for (int x = 0; x < 16; ++x) {
-            const int lim = __shfl(limit[m], x);
-            Vec8<T> v = __builtin_bit_cast(Vec8<T>, vf);
+      float best = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (t + 16 * (j >> 2) + 4 * q4 + (j & 3) >= lim) v[j] = static_cast<T>(0.0f);
-            const Float4 add = mfma16<T>(v, pf[m], Float4{0.0f, 0.0f, 0.0f, 0.0f});
-            if (x == c) o[m][d] += add;
-          }
-        continue;
+      for (int i = 0; i < X; ++i) best = fmaxf(best, sc[i / ACC][i % ACC]);
+#pragma unroll
+      for (int x = MR; x < 64; x <<= 1) best = fmaxf(best, __shfl_xor(best, x));
+      best *= scale;
+      const bool rises = best > base + kSlack<T>;
+      if (__any(rises)) {  // each row by itself: no row's rounding depends on another
+        const float next = rises ? best : base;
+        const float keep = __builtin_amdgcn_exp2f(base - (next == -INFINITY ? 0.0f : next));
+        base = next;
+        sum *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= keep;
       }
-      const Vec8<T> v = __builtin_bit_cast(Vec8<T>, vf);
+      const float below = kLift<T> - (base == -INFINITY ? 0.0f : base);
+      Vec8<T> pf[X / 8];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) o[m][d] = mfma16<T>(v, pf[m], o[m][d]);
+      for (int i = 0; i < X; ++i) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(sc[i / ACC][i % ACC], scale, below));
+        sum += e;
+        pf[i / 8][i % 8] = static_cast<T>(e);
+      }
+      // O += V P
+#pragma unroll
+      for (int k = 0; k < X / 8; ++k)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          o[d] = mfma<T, MR>(read_values<T, DP, MR>(vb, lane, k, d), pf[k], o[d]);
     }
-    __builtin_amdgcn_wave_barrier();
+    if constexpr (WR == 1)
+      __builtin_amdgcn_wave_barrier();
+    else
+      turn ^= 1;
   }
 
-  // join the waves: the largest maximum, then the weighted sums
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    sum[m] += __shfl_xor(sum[m], 16);
-    sum[m] += __shfl_xor(sum[m], 32);
-  }
-  __syncthreads();
-  float* const ml = reinterpret_cast<float*>(lds);  // [wave][M][2]
-  float* const ol = ml + kWaves * M * 2;            // [M][DP + 4], one wave after the other
-  constexpr int kPitch = DP + 4;
-  if (q4 == 0)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      ml[(wave * M + 16 * m + c) * 2] = top[m];
-      ml[(wave * M + 16 * m + c) * 2 + 1] = sum[m];
-    }
-  __syncthreads();
-  float best[MT], total[MT], weight[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    best[m] = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) best[m] = fmaxf(best[m], ml[(w * M + 16 * m + c) * 2]);
-    const float base = best[m] == -INFINITY ? 0.0f : best[m];
-    total[m] = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-      total[m] += ml[(w * M + 16 * m + c) * 2 + 1] *
-                  __builtin_amdgcn_exp2f(ml[(w * M + 16 * m + c) * 2] - base);
-    weight[m] = __builtin_amdgcn_exp2f(top[m] - base);
-  }
-  for (int w = 0; w < kWaves; ++w) {
-    if (w == wave)
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          Float4* const dst =
-              reinterpret_cast<Float4*>(ol + (16 * m + c) * kPitch + 16 * d + 4 * q4);
-          o[m][d] *= weight[m];
-          if (w > 0) o[m][d] += *dst;
-          *dst = o[m][d];
-        }
+  for (int x = MR; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+  if (t1 > nearest) odd = __syncthreads_or(odd);
+  if constexpr (WT > 1) {
+    // join the token waves: the largest maximum, then the weighted sums, which end in the last one
+    constexpr int M = WR * MR, kPitch = DP + 4;
     __syncthreads();
+    float* const ml = reinterpret_cast<float*>(lds);  // [WT][M][2]
+    float* const ol = ml + WT * M * 2;                // [M][kPitch]
+    const int mr = wr * MR + c;
+    if (q4 == 0) {
+      ml[(wt * M + mr) * 2] = base;
+      ml[(wt * M + mr) * 2 + 1] = sum;
+    }
+    __syncthreads();
+    const float mine_base = base;
+#pragma unroll
+    for (int w = 0; w < WT; ++w) base = fmaxf(base, ml[(w * M + mr) * 2]);
+    const float zero = base == -INFINITY ? 0.0f : base;
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WT; ++w)
+      sum += ml[(w * M + mr) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * M + mr) * 2] - zero);
+    const float weight = __builtin_amdgcn_exp2f(mine_base - zero);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] *= weight;
+#pragma unroll 1
+    for (int w = 0; w < WT; ++w) {
+      if (w == wt)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int x = 0; x < ACC; x += 4) {
+            Float4* const dst = reinterpret_cast<Float4*>(ol + mr * kPitch + MR * d + 4 * q4 +
+                                                          256 / MR * (x / 4));
+            if (w > 0) {
+              const Float4 v = *dst;
+              o[d][x] += v[0];
+              o[d][x + 1] += v[1];
+              o[d][x + 2] += v[2];
+              o[d][x + 3] += v[3];
+            }
+            if (w < WT - 1)
+              *dst = Float4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]};
+          }
+      if (w < WT - 1) __syncthreads();
+    }
+    if (wt != WT - 1) return;
   }
-  if (wave != 0) return;
+  if (odd) {
+    // the values that store_tile left out, to the rows that see them
+    for (int i = max(t0, nearest); i < min(t1, limit); ++i) {
+      const int at_row = row_of(i, block_of(i));
+      if (at_row < 0) continue;
+      const uint8_t* const src =
+          p.cache + (at_row + p.half_stride) * pitch + static_cast<int64_t>(h) * p.D * cell;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    if (at[m] < 0) continue;
-    if (p.slots > 1) {
-      const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
-      const int64_t slot = (g.slot + split) * all + at[m];
-      if (q4 == 0) {
-        p.part_ml[2 * slot] = best[m] - kLift<T>;
-        p.part_ml[2 * slot + 1] = total[m];
-      }
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const int ch = 16 * d + 4 * q4;
+        for (int x = 0; x < ACC; x += 4) {
+          const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
+          const Float4 v = four_values<T, FP8>(src, min(ch, p.D - 4));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[d][x + j] += fabsf(v[j]) < INFINITY ? 0.0f : v[j];
+        }
+    }
+  }
+  if (!live) return;
+  if (p.slots > 1) {
+    const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
+    const int64_t slot = (g.slot + split) * all + at;
+    if (q4 == 0) {
+      p.part_ml[2 * slot] = base - kLift<T>;
+      p.part_ml[2 * slot + 1] = sum;
+    }
+    if (sum == 0.0f) return;  // no token: the join does not read the rest
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int x = 0; x < ACC; x += 4) {
+        const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
         if (ch < p.D)
           *reinterpret_cast<Float4*>(p.part_o + slot * p.D + ch) =
-              *reinterpret_cast<const Float4*>(ol + (16 * m + c) * kPitch + ch);
+              Float4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]};
       }
-    } else {
-      const float inv = total[m] == 0.0f ? 0.0f : p.v_scale / total[m];
-      const int64_t n = at[m] / p.Hq, head = at[m] - n * p.Hq;
-      T* const dst = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head;
+    return;
+  }
+  const float inv = sum == 0.0f ? 0.0f : p.v_scale / sum;
+  T* const dst = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const int ch = 16 * d + 4 * q4;
-        if (ch < p.D) {
-          const Float4 v = *reinterpret_cast<const Float4*>(ol + (16 * m + c) * kPitch + ch);
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) dst[ch + j] = static_cast<T>(v[j] * inv);
-        }
-      }
-      if (p.lse && q4 == 0)
-        p.lse[at[m]] = total[m] == 0.0f ? -INFINITY : kLn2 * (best[m] - kLift<T> + log2f(total[m]));
+    for (int x = 0; x < ACC; x += 4) {
+      const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
+      if (ch < p.D)
+        store4(dst + ch, Float4{o[d][x] * inv, o[d][x + 1] * inv, o[d][x + 2] * inv,
+                                o[d][x + 3] * inv}, p.out_vec);
+    }
+  if (p.lse && q4 == 0)
+    p.lse[at] = sum == 0.0f ? -INFINITY : kLn2 * (base - kLift<T> + log2f(sum));
+}
+
+template <typename T, bool FP8, int DP, int SHAPE>
+__device__ __forceinline__ void attend_shape(const AttendParams& p, int kind, int unit,
+                                             uint8_t* lds) {
+  constexpr int MR = SHAPE == 0 || DP == 256 ? 16 : 32;
+  attend<T, FP8, DP, MR, kShapeRows[SHAPE] / MR>(p, p.group[kind], unit, kind == 0, lds);
+}
+
+// The prefix in workgroups of shape S0 and the requests in those of S1, in one launch.
+template <typename T, bool FP8, int DP, int S0, int S1>
+__global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(AttendParams p) {
+  __shared__ alignas(16) uint8_t lds[512 * DP];  // of every shape
+  int unit = static_cast<int>(blockIdx.x);
+  const int kind = unit >= p.group[0].units;
+  unit -= kind ? p.group[0].units : 0;
+  if (S0 == S1 || kind == 1)
+    attend_shape<T, FP8, DP, S1>(p, kind, unit, lds);
+  else
+    attend_shape<T, FP8, DP, S0>(p, 0, unit, lds);
+}
+
+// Joins the parts of each row: 4 channels a lane, and for rows of many parts several lane groups
+// (`teams`) that take them in turn.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_kernel(AttendParams p, int lanes, int teams) {
+  __shared__ Float4 part[kThreads];
+  __shared__ float part_sum[kThreads];
+  const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
+  const int per = kThreads / (lanes * teams);  // rows
+  const int lane = threadIdx.x % lanes, team = threadIdx.x / lanes % teams;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / (lanes * teams);
+  const int ch = 4 * lane;
+  bool live = row < all;
+  const int64_t n = live ? row / p.Hq : 0, head = row - n * p.Hq;
+  if (p.starts) live = live && n >= p.starts[0] && n < p.starts[p.requests];
+  float best = -INFINITY, total = 0.0f;
+  Float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (live) {
+    // every lane group finds the largest maximum for itself, its lanes sharing the parts
+    for (int s = lane; s < p.slots; s += lanes)
+      best = fmaxf(best, p.part_ml[2 * (s * all + row)]);
+    for (int x = 1; x < lanes; x <<= 1) best = fmaxf(best, __shfl_xor(best, x));
+    const float zero = best == -INFINITY ? 0.0f : best;
+    for (int s = team; s < p.slots; s += teams) {
+      const int64_t slot = s * all + row;
+      const float l = p.part_ml[2 * slot + 1];
+      if (l == 0.0f) continue;  // no token: nothing was written
+      const float w = __builtin_amdgcn_exp2f(p.part_ml[2 * slot] - zero);
+      total += l * w;
+      if (ch < p.D) o += *reinterpret_cast<const Float4*>(p.part_o + slot * p.D + ch) * w;
     }
   }
+  if (teams > 1) {
+    part[threadIdx.x] = o;
+    part_sum[threadIdx.x] = total;
+    __syncthreads();
+    if (team != 0) return;
+    for (int k = 1; k < teams; ++k) {
+      o += part[threadIdx.x + k * lanes];
+      total += part_sum[threadIdx.x + k * lanes];
+    }
+  }
+  if (!live) return;
+  const float inv = total == 0.0f ? 0.0f : p.v_scale / total;
+  if (ch < p.D)
+    store4(static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + ch, o * inv, p.out_vec);
+  if (p.lse && ch == 0) p.lse[row] = total == 0.0f ? -INFINITY : kLn2 * (best + log2f(total));
 }
 
 template <typename T, bool FP8, int DP>
-__global__ __launch_bounds__(kThreads) void attend_kernel(AttendParams p) {
-  __shared__ alignas(16) uint8_t lds[kWaves * 2 * kStep * DP * 2];
-  const int unit = static_cast<int>(blockIdx.x);
-  if (unit < p.shared.units)
-    attend<T, FP8, DP, 1>(p, p.shared, unit, true, lds);
-  else
-    attend<T, FP8, DP, 1>(p, p.each, unit - p.shared.units, false, lds);
-}
-
-// Joins the parts of each row: 4 channels a lane.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void join_kernel(AttendParams p, int lanes) {
-  const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / lanes) + threadIdx.x / lanes;
-  const int ch = 4 * (threadIdx.x % lanes);
-  if (row >= all) return;
-  const int64_t n = row / p.Hq, head = row - n * p.Hq;
-  if (p.starts && (n < p.starts[0] || n >= p.starts[p.requests])) return;
-  float best = -INFINITY;
-  for (int s = 0; s < p.slots; ++s) best = fmaxf(best, p.part_ml[2 * (s * all + row)]);
-  const float base = best == -INFINITY ? 0.0f : best;
-  float total = 0.0f;
-  Float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < p.slots; ++s) {
-    const int64_t slot = s * all + row;
-    const float l = p.part_ml[2 * slot + 1];
-    if (l == 0.0f) continue;  // no token: nothing was written
-    const float w = __builtin_amdgcn_exp2f(p.part_ml[2 * slot] - base);
-    total += l * w;
-    if (ch < p.D) o += *reinterpret_cast<const Float4*>(p.part_o + slot * p.D + ch) * w;
+int launch_units(const AttendParams& p, hipStream_t stream) {
+  const dim3 grid(p.group[0].units + p.group[1].units), block(kThreads);
+  const int s1 = p.group[1].shape, s0 = p.group[0].units ? p.group[0].shape : s1;
+  if (s0 == 0)  // the batch has at least a request's rows: s0 >= s1
+    hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 0, 0>), grid, block, 0, stream, p);
+  else if (s0 == 1 && s1 == 0)
+    hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 1, 0>), grid, block, 0, stream, p);
+  else if (s0 == 1)
+    hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 1, 1>), grid, block, 0, stream, p);
+  if constexpr (DP < 256) {
+    if (s0 == 2 && s1 == 0)
+      hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 2, 0>), grid, block, 0, stream, p);
+    else if (s0 == 2 && s1 == 1)
+      hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 2, 1>), grid, block, 0, stream, p);
+    else if (s0 == 2)
+      hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 2, 2>), grid, block, 0, stream, p);
   }
-  const float inv = total == 0.0f ? 0.0f : p.v_scale / total;
-  T* const dst = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head;
-  if (ch < p.D)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) dst[ch + j] = static_cast<T>(o[j] * inv);
-  if (p.lse && ch == 0) p.lse[row] = total == 0.0f ? -INFINITY : kLn2 * (best + log2f(total));
+  return check_launch("attend_kernel");
 }
 
 template <typename T, bool FP8>
 int launch_attend(const AttendParams& p, hipStream_t stream) {
-  const dim3 grid(p.shared.units + p.each.units), block(kThreads);
-  if (p.D <= 64)
-    hipLaunchKernelGGL((attend_kernel<T, FP8, 64>), grid, block, 0, stream, p);
-  else if (p.D <= 128)
-    hipLaunchKernelGGL((attend_kernel<T, FP8, 128>), grid, block, 0, stream, p);
-  else
-    hipLaunchKernelGGL((attend_kernel<T, FP8, 256>), grid, block, 0, stream, p);
-  if (int rc = check_launch("attend_kernel")) return rc;
+  const int rc = p.D <= 64    ? launch_units<T, FP8, 64>(p, stream)
+                 : p.D <= 128 ? launch_units<T, FP8, 128>(p, stream)
+                              : launch_units<T, FP8, 256>(p, stream);
+  if (rc) return rc;
+  const dim3 block(kThreads);
   if (p.slots == 1) return ORIGAMI_OK;
   const int lanes = p.D <= 64 ? 16 : (p.D <= 128 ? 32 : 64);
-  const int64_t rows = static_cast<int64_t>(p.tokens) * p.Hq, per = kThreads / lanes;
+  const int teams = p.slots >= 8 ? kThreads / lanes : 1;
+  const int64_t rows = static_cast<int64_t>(p.tokens) * p.Hq, per = kThreads / (lanes * teams);
   hipLaunchKernelGGL(join_kernel<T>, dim3(static_cast<unsigned>((rows + per - 1) / per)), block, 0,
-                     stream, p, lanes);
+                     stream, p, lanes, teams);
   return check_launch("join_kernel");
 }
 
@@ -454,17 +655,30 @@ struct Plan {
   int64_t slots, units;
 };
 
-Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t prefix,
-             int64_t requests, int64_t max_query, int64_t max_own) {
+constexpr int64_t kFill = 512;  // workgroups that fill the GPU: two on each of 256 CUs
+
+Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_dim,
+             int64_t prefix, int64_t requests, int64_t max_query, int64_t max_own) {
   Plan plan{};
-  const int64_t G = query_heads / heads, M = 16;
-  const bool apart = requests > 1 && prefix > 0;
-  const int64_t chunk = 512;
-  int64_t units = 0, slot = 0;
+  const int64_t G = query_heads / heads;
+  const int last = head_dim > 128 ? 1 : 2;
+  // A request whose rows fill workgroups by themselves reads the prefix with its own tokens.
+  const bool apart = requests > 1 && prefix > 0 && max_query * G < kShapeRows[last];
+  int64_t slot = 0;  // of the partial results
   const auto fill = [&](Group& g, int64_t n, int64_t rows, int64_t first, int64_t span) {
-    const int64_t splits = span > 0 ? ceil_div(span, chunk) : 1, tiles = ceil_div(rows, M);
-    units += n * heads * tiles * splits;
-    g.units = static_cast<int32_t>(n * heads * tiles * splits);
+    int shape = 0;
+    while (shape < last && rows > kShapeRows[shape]) ++shape;
+    const int64_t tiles = std::max<int64_t>(ceil_div(rows, kShapeRows[shape]), 1);
+    const int64_t keys = std::max<int64_t>(n * heads, 1);
+    // ranges of 128 tokens or more, as many as fill the GPU
+    const int64_t most = std::max<int64_t>(ceil_div(span, 128), 1);
+    int64_t splits = std::min(most, std::max<int64_t>(kFill / (keys * tiles), 1));
+    const int64_t chunk = std::max<int64_t>(ceil_div(ceil_div(span, splits), 128), 1) * 128;
+    splits = std::max<int64_t>(ceil_div(span, chunk), 1);
+    const int64_t units = ceil_div(keys * splits, 8) * 8 * tiles;
+    plan.units += units;
+    g.units = static_cast<int32_t>(std::min<int64_t>(units, INT32_MAX));
+    g.shape = shape;
     g.tiles = static_cast<int32_t>(tiles);
     g.splits = static_cast<int32_t>(splits);
     g.chunk = static_cast<int32_t>(chunk);
@@ -475,7 +689,6 @@ Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t prefix,
   if (apart) fill(plan.shared, 1, tokens * G, 0, prefix);
   fill(plan.each, requests, max_query * G, apart ? prefix : 0, (apart ? 0 : prefix) + max_own);
   plan.slots = slot;
-  plan.units = units;
   return plan;
 }
 
@@ -511,8 +724,8 @@ int64_t origami_shared_prefix_attention_workspace(int64_t tokens, int64_t query_
   if (check_sizes(tokens, query_heads, heads, head_dim, prefix_tokens, requests, max_query_tokens,
                   max_own_tokens))
     return -1;
-  return workspace_bytes_of(plan_of(tokens, query_heads, heads, prefix_tokens, requests,
-                                    max_query_tokens, max_own_tokens),
+  return workspace_bytes_of(plan_of(tokens, query_heads, heads, head_dim, prefix_tokens,
+                                    requests, max_query_tokens, max_own_tokens),
                             tokens, query_heads, head_dim);
 }
 
@@ -552,8 +765,9 @@ int origami_shared_prefix_attention(
   ORIGAMI_REQUIRE(aligned16(kv_cache), "kv_cache must be 16-byte aligned");
   if (tokens == 0 || requests == 0) return ORIGAMI_OK;
 
-  const Plan plan = plan_of(tokens, query_heads, heads, prefix_tokens, requests, max_query_tokens,
-                            max_own_tokens);
+  if (num_blocks == 0) prefix_tokens = max_own_tokens = 0;  // no token is in the cache
+  const Plan plan = plan_of(tokens, query_heads, heads, head_dim, prefix_tokens, requests,
+                            max_query_tokens, max_own_tokens);
   ORIGAMI_REQUIRE(plan.units <= INT32_MAX, "too many row tiles for one call");
   ORIGAMI_REQUIRE(workspace_bytes >= workspace_bytes_of(plan, tokens, query_heads, head_dim) &&
                       (plan.slots == 1 || workspace != nullptr) && aligned16(workspace),
@@ -564,6 +778,7 @@ int origami_shared_prefix_attention(
   p.out = out;
   p.o_token = strides[2];
   p.o_head = strides[3];
+  p.out_vec = ((reinterpret_cast<uintptr_t>(out) | 2 * strides[2] | 2 * strides[3]) & 7) == 0;
   p.lse = lse;
   p.cache = static_cast<const uint8_t*>(kv_cache);
   p.num_blocks = num_blocks;
@@ -584,8 +799,8 @@ int origami_shared_prefix_attention(
   p.D = static_cast<int32_t>(head_dim);
   p.scale = static_cast<float>(scale * k_scale) * kLog2e;
   p.v_scale = static_cast<float>(v_scale);
-  p.shared = plan.shared;
-  p.each = plan.each;
+  p.group[0] = plan.shared;
+  p.group[1] = plan.each;
   p.slots = static_cast<int32_t>(plan.slots);
   const int64_t parts = plan.slots * tokens * query_heads;
   p.part_o = static_cast<float*>(workspace);
