@@ -33,9 +33,13 @@ template <typename T>
 constexpr float kSlack = std::is_same<T, f16>::value ? 4.0f : 8.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+constexpr int64_t kFill = 512;  // workgroups that fill the GPU: two on each of 256 CUs
+constexpr int kFewParts = 4;
+constexpr int kMaxParts = 1024;  // of a row: kFill at most of either kind
+
 // Rows of a workgroup.  The last shape is for up to 128 channels: with 256, results of 32 rows a wave
 // and the tiles on their way would not fit the registers.
-constexpr int kShapeRows[3] = {16, 64, 128};
+constexpr int kShapeRows[4] = {16, 64, 128, 256};
 
 // The work of one kind: row tiles of every KV head, over ranges of tokens.
 struct Group {
@@ -163,6 +167,22 @@ __device__ __forceinline__ Request request_of(const AttendParams& p, int r) {
   return q;
 }
 
+__device__ __forceinline__ uint32_t as_u32(float x) { return __builtin_bit_cast(uint32_t, x); }
+__device__ __forceinline__ float as_float(uint32_t x) { return __builtin_bit_cast(float, x); }
+
+// The largest of the values of lanes c, c + MR, ..., without a trip through LDS.
+template <int MR>
+__device__ __forceinline__ float max_over_groups(float x) {
+  if constexpr (MR == 16) {
+    const auto pair = __builtin_amdgcn_permlane16_swap(as_u32(x), as_u32(x), false, false);
+    const uint32_t one = pair[0], other = pair[1];
+    x = fmaxf(as_float(one), as_float(other));
+  }
+  const auto pair = __builtin_amdgcn_permlane32_swap(as_u32(x), as_u32(x), false, false);
+  const uint32_t one = pair[0], other = pair[1];
+  return fmaxf(as_float(one), as_float(other));
+}
+
 // Where the 16-byte piece `piece` of token `tok`'s row is in LDS, in pieces of its row.  Keys are
 // read by 16 lanes from the same piece of 16 tokens, values by 32 lanes from pieces next to each
 // other (2 of 8 tokens, or 4 of 4): with the token's low bits in the piece's number these
@@ -201,13 +221,13 @@ __device__ __forceinline__ Vec8<T> read_values(const uint8_t* values, int lane, 
 template <int DP, int WR>
 constexpr int kTeamTokens = WR == 4 && DP < 256 ? 64 : 32;
 
-// One workgroup: WR MR rows of one KV head over a range of tokens.  Its waves are WR row waves
-// by kWaves / WR token waves: a wave takes MR rows, and of every kWaves / WR times kTeamTokens
-// tokens its share.  Rows (queries, results, sums) stay in registers; keys and values go
+// One workgroup: WR RB MR rows of one KV head over a range of tokens.  Its waves are WR row
+// waves by kWaves / WR token waves: a wave takes RB times MR rows, and of every kWaves / WR times
+// kTeamTokens tokens its share.  Rows (queries, results, sums) stay in registers; keys and values go
 // through LDS, where the WR waves of a team share them, and the next ones are on their way
 // to registers meanwhile.  With WR = 1 no wave needs another until the end; else two buffers
 // take turns, so that one barrier a step is enough.
-template <typename T, bool FP8, int DP, int MR, int WR>
+template <typename T, bool FP8, int DP, int MR, int RB, int WR>
 __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, int unit, bool batch,
                                        uint8_t* lds) {
   constexpr int WT = kWaves / WR, TT = kTeamTokens<DP, WR>;
@@ -223,7 +243,8 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
   constexpr int IT = TT / (RPI * WR);     // loads of a tile
   constexpr int kBuffers = WR == 1 ? 1 : 2;
   constexpr int kTile = TT * DP * 2;      // bytes of a team's keys
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  // one value for the wave, so that what follows from it is scalar and its conditions are branches
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wr = wave % WR, wt = wave / WR;
   const int c = lane % MR, q4 = lane / MR;
 
@@ -244,60 +265,63 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
     rq = request_of(p, r);
   }
   const int split = u;
-  const int rows = rq.count * p.G, row0 = tile * WR * MR;
+  const int rows = rq.count * p.G, row0 = tile * WR * RB * MR;
   if (split >= g.splits || row0 >= rows) return;
   const int end = batch ? p.prefix : p.prefix + rq.own;  // of the tokens, prefix first
   const int64_t* const table = p.tables + static_cast<int64_t>(r) * p.table_stride;
 
-  // this lane's row
-  const int row = row0 + wr * MR + c;
-  const bool live = row < rows;
-  const int qi = live ? row / p.G : 0, head = h * p.G + (live ? row - qi * p.G : 0);
-  const int limit =  // tokens it sees
-      batch ? p.prefix : p.prefix + min(max(rq.own - rq.count + qi + 1, 0), rq.own);
-  const int64_t n = rq.first + qi, at = n * p.Hq + head;
+  // this lane's rows
+  const auto row_at = [&](int b) { return row0 + (wr * RB + b) * MR + c; };
+  const auto seen_by = [&](int row) -> int {  // tokens that a row sees
+    return batch ? p.prefix : p.prefix + min(max(rq.own - rq.count + row / p.G + 1, 0), rq.own);
+  };
+  int limit[RB];
   // the scale's sign goes with the queries, and so does a scale of zero, so that hidden scores of
   // -infinity stay what they are
   const float scale = p.scale == 0.0f ? 1.0f : fabsf(p.scale);
-  Vec8<T> qf[KS];
-  {
-    const T* const src = static_cast<const T*>(p.query) + n * p.q_token + head * p.q_head;
+  Vec8<T> qf[RB][KS];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int row = row_at(b), qi = row / p.G;
+    limit[b] = seen_by(row);
+    const T* const src = static_cast<const T*>(p.query) + (rq.first + qi) * p.q_token +
+                         (h * p.G + row - qi * p.G) * p.q_head;
     const bool vec =
         ((reinterpret_cast<uintptr_t>(p.query) | 2 * p.q_token | 2 * p.q_head) & 15) == 0;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       const int d = 8 * (NG * k + q4);
-      qf[k] = Vec8<T>{};
-      if (live && d < p.D) {
+      qf[b][k] = Vec8<T>{};
+      if (row < rows && d < p.D) {
         if (vec) {
-          qf[k] = *reinterpret_cast<const Vec8<T>*>(src + d);
+          qf[b][k] = *reinterpret_cast<const Vec8<T>*>(src + d);
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) qf[k][j] = src[d + j];
+          for (int j = 0; j < 8; ++j) qf[b][k][j] = src[d + j];
         }
-        if (p.scale <= 0.0f) qf[k] = p.scale == 0.0f ? Vec8<T>{} : -qf[k];
+        if (p.scale <= 0.0f) qf[b][k] = p.scale == 0.0f ? Vec8<T>{} : -qf[b][k];
       }
     }
   }
   // The tokens that some row of the workgroup sees, and those that all rows of the wave see;
   // limits grow along the rows.
-  const int last_row = min(row0 + WR * MR, rows) - 1;
-  const int most = batch ? p.prefix
-                         : p.prefix + min(max(rq.own - rq.count + last_row / p.G + 1, 0), rq.own);
-  const int first_row = min(row0 + wr * MR, rows - 1);
-  const int least =
-      batch ? p.prefix : p.prefix + min(max(rq.own - rq.count + first_row / p.G + 1, 0), rq.own);
-  const int nearest =  // the tokens that all rows of the workgroup see
-      batch ? p.prefix : p.prefix + min(max(rq.own - rq.count + row0 / p.G + 1, 0), rq.own);
+  const int most = seen_by(min(row0 + WR * RB * MR, rows) - 1);
+  const int least = seen_by(min(row0 + wr * RB * MR, rows - 1));
+  const int nearest = seen_by(row0);  // the tokens that all rows of the workgroup see
   const int t0 = g.first + split * g.chunk;
   const int t1 = min(min(end, most), t0 + g.chunk);
 
-  Tile<MR> o[DT];
-  float base = -INFINITY, sum = 0.0f;
+  Tile<MR> o[RB][DT];
+  float base[RB], sum[RB];
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
+  for (int b = 0; b < RB; ++b) {
+    base[b] = -INFINITY;
+    sum[b] = 0.0f;
 #pragma unroll
-    for (int x = 0; x < ACC; ++x) o[d][x] = 0.0f;
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int x = 0; x < ACC; ++x) o[b][d][x] = 0.0f;
+  }
 
   uint8_t* const team = lds + wt * kBuffers * 2 * kTile;
   const int piece = lane % NCH, sub = lane / NCH;
@@ -383,56 +407,63 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
       const uint8_t* const vb = kb + kTile;
       const int ts = t + s * kStep;  // the step's first token
       // S = K Q: row c against token STRIDE (i / 4) + 4 q4 + i % 4
-      Tile<MR> sc[X / ACC];
+      Tile<MR> sc[RB][X / ACC];
 #pragma unroll
       for (int m = 0; m < X / ACC; ++m) {
 #pragma unroll
-        for (int x = 0; x < ACC; ++x) sc[m][x] = 0.0f;
+        for (int b = 0; b < RB; ++b)
+#pragma unroll
+          for (int x = 0; x < ACC; ++x) sc[b][m][x] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           const int tok = MR * m + c;
           const Vec8<T> kf = *reinterpret_cast<const Vec8<T>*>(
               kb + (tok * NCH + key_piece<DP>(tok, NG * k + q4)) * 16);
-          sc[m] = mfma<T, MR>(kf, qf[k], sc[m]);
+#pragma unroll
+          for (int b = 0; b < RB; ++b) sc[b][m] = mfma<T, MR>(kf, qf[b][k], sc[b][m]);
         }
       }
-      if (!whole) {
-        const uint32_t seen = static_cast<uint32_t>(there >> (kStep * s));
+      Vec8<T> pf[RB][X / 8];
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        if (!whole) {
+          const uint32_t seen = static_cast<uint32_t>(there >> (kStep * s));
+#pragma unroll
+          for (int i = 0; i < X; ++i) {
+            const int tok = STRIDE * (i / 4) + 4 * q4 + i % 4;
+            if (ts + tok >= limit[b] || !((seen >> tok) & 1)) sc[b][i / ACC][i % ACC] = -INFINITY;
+          }
+        }
+        float best = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < X; ++i) best = fmaxf(best, sc[b][i / ACC][i % ACC]);
+        best = max_over_groups<MR>(best) * scale;
+        const bool rises = best > base[b] + kSlack<T>;
+        if (__any(rises)) {  // each row by itself: no row's rounding depends on another
+          const float next = rises ? best : base[b];
+          const float keep = __builtin_amdgcn_exp2f(base[b] - (next == -INFINITY ? 0.0f : next));
+          base[b] = next;
+          sum[b] *= keep;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[b][d] *= keep;
+        }
+        const float below = kLift<T> - (base[b] == -INFINITY ? 0.0f : base[b]);
 #pragma unroll
         for (int i = 0; i < X; ++i) {
-          const int tok = STRIDE * (i / 4) + 4 * q4 + i % 4;
-          if (ts + tok >= limit || !((seen >> tok) & 1)) sc[i / ACC][i % ACC] = -INFINITY;
+          const float e = __builtin_amdgcn_exp2f(fmaf(sc[b][i / ACC][i % ACC], scale, below));
+          sum[b] += e;
+          pf[b][i / 8][i % 8] = static_cast<T>(e);
         }
-      }
-      float best = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < X; ++i) best = fmaxf(best, sc[i / ACC][i % ACC]);
-#pragma unroll
-      for (int x = MR; x < 64; x <<= 1) best = fmaxf(best, __shfl_xor(best, x));
-      best *= scale;
-      const bool rises = best > base + kSlack<T>;
-      if (__any(rises)) {  // each row by itself: no row's rounding depends on another
-        const float next = rises ? best : base;
-        const float keep = __builtin_amdgcn_exp2f(base - (next == -INFINITY ? 0.0f : next));
-        base = next;
-        sum *= keep;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] *= keep;
-      }
-      const float below = kLift<T> - (base == -INFINITY ? 0.0f : base);
-      Vec8<T> pf[X / 8];
-#pragma unroll
-      for (int i = 0; i < X; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(sc[i / ACC][i % ACC], scale, below));
-        sum += e;
-        pf[i / 8][i % 8] = static_cast<T>(e);
       }
       // O += V P
 #pragma unroll
       for (int k = 0; k < X / 8; ++k)
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-          o[d] = mfma<T, MR>(read_values<T, DP, MR>(vb, lane, k, d), pf[k], o[d]);
+        for (int d = 0; d < DT; ++d) {
+          const Vec8<T> v = read_values<T, DP, MR>(vb, lane, k, d);
+#pragma unroll
+          for (int b = 0; b < RB; ++b) o[b][d] = mfma<T, MR>(v, pf[b][k], o[b][d]);
+        }
     }
     if constexpr (WR == 1)
       __builtin_amdgcn_wave_barrier();
@@ -441,31 +472,34 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
   }
 
 #pragma unroll
-  for (int x = MR; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int x = MR; x < 64; x <<= 1) sum[b] += __shfl_xor(sum[b], x);
   if (t1 > nearest) odd = __syncthreads_or(odd);
   if constexpr (WT > 1) {
     // join the token waves: the largest maximum, then the weighted sums, which end in the last one
+    static_assert(RB == 1, "token waves have one block of rows");
     constexpr int M = WR * MR, kPitch = DP + 4;
     __syncthreads();
     float* const ml = reinterpret_cast<float*>(lds);  // [WT][M][2]
     float* const ol = ml + WT * M * 2;                // [M][kPitch]
     const int mr = wr * MR + c;
     if (q4 == 0) {
-      ml[(wt * M + mr) * 2] = base;
-      ml[(wt * M + mr) * 2 + 1] = sum;
+      ml[(wt * M + mr) * 2] = base[0];
+      ml[(wt * M + mr) * 2 + 1] = sum[0];
     }
     __syncthreads();
-    const float mine_base = base;
+    const float mine_base = base[0];
 #pragma unroll
-    for (int w = 0; w < WT; ++w) base = fmaxf(base, ml[(w * M + mr) * 2]);
-    const float zero = base == -INFINITY ? 0.0f : base;
-    sum = 0.0f;
+    for (int w = 0; w < WT; ++w) base[0] = fmaxf(base[0], ml[(w * M + mr) * 2]);
+    const float zero = base[0] == -INFINITY ? 0.0f : base[0];
+    sum[0] = 0.0f;
 #pragma unroll
     for (int w = 0; w < WT; ++w)
-      sum += ml[(w * M + mr) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * M + mr) * 2] - zero);
+      sum[0] += ml[(w * M + mr) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * M + mr) * 2] - zero);
     const float weight = __builtin_amdgcn_exp2f(mine_base - zero);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[d] *= weight;
+    for (int d = 0; d < DT; ++d) o[0][d] *= weight;
 #pragma unroll 1
     for (int w = 0; w < WT; ++w) {
       if (w == wt)
@@ -477,81 +511,89 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
                                                           256 / MR * (x / 4));
             if (w > 0) {
               const Float4 v = *dst;
-              o[d][x] += v[0];
-              o[d][x + 1] += v[1];
-              o[d][x + 2] += v[2];
-              o[d][x + 3] += v[3];
+              o[0][d][x] += v[0];
+              o[0][d][x + 1] += v[1];
+              o[0][d][x + 2] += v[2];
+              o[0][d][x + 3] += v[3];
             }
             if (w < WT - 1)
-              *dst = Float4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]};
+              *dst = Float4{o[0][d][x], o[0][d][x + 1], o[0][d][x + 2], o[0][d][x + 3]};
           }
       if (w < WT - 1) __syncthreads();
     }
     if (wt != WT - 1) return;
   }
-  if (odd) {
-    // the values that store_tile left out, to the rows that see them
-    for (int i = max(t0, nearest); i < min(t1, limit); ++i) {
-      const int at_row = row_of(i, block_of(i));
-      if (at_row < 0) continue;
-      const uint8_t* const src =
-          p.cache + (at_row + p.half_stride) * pitch + static_cast<int64_t>(h) * p.D * cell;
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int row = row_at(b);
+    if (odd) {
+      // the values that store_tile left out, to the rows that see them; those of the tokens
+      // before them were added already, and an infinity or NaN twice is the same
+      for (int i = max(t0, nearest - TT); i < min(t1, limit[b]); ++i) {
+        const int at_row = row_of(i, block_of(i));
+        if (at_row < 0) continue;
+        const uint8_t* const src =
+            p.cache + (at_row + p.half_stride) * pitch + static_cast<int64_t>(h) * p.D * cell;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int x = 0; x < ACC; x += 4) {
+            const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
+            const Float4 v = four_values<T, FP8>(src, min(ch, p.D - 4));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[b][d][x + j] += fabsf(v[j]) < INFINITY ? 0.0f : v[j];
+          }
+      }
+    }
+    if (row >= rows) continue;
+    const int qi = row / p.G, head = h * p.G + row - qi * p.G;
+    const int64_t n = rq.first + qi, at = n * p.Hq + head;
+    if (p.slots > 1) {
+      const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
+      const int64_t slot = (g.slot + split) * all + at;
+      if (q4 == 0) {
+        p.part_ml[2 * slot] = base[b] - kLift<T>;
+        p.part_ml[2 * slot + 1] = sum[b];
+      }
+      if (sum[b] == 0.0f) continue;  // no token: the join does not read the rest
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int x = 0; x < ACC; x += 4) {
           const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
-          const Float4 v = four_values<T, FP8>(src, min(ch, p.D - 4));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[d][x + j] += fabsf(v[j]) < INFINITY ? 0.0f : v[j];
+          if (ch < p.D)
+            *reinterpret_cast<Float4*>(p.part_o + slot * p.D + ch) =
+                Float4{o[b][d][x], o[b][d][x + 1], o[b][d][x + 2], o[b][d][x + 3]};
         }
+    } else {
+      const float inv = sum[b] == 0.0f ? 0.0f : p.v_scale / sum[b];
+      T* const dst = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int x = 0; x < ACC; x += 4) {
+          const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
+          if (ch < p.D)
+            store4(dst + ch, Float4{o[b][d][x] * inv, o[b][d][x + 1] * inv, o[b][d][x + 2] * inv,
+                                    o[b][d][x + 3] * inv}, p.out_vec);
+        }
+      if (p.lse && q4 == 0)
+        p.lse[at] = sum[b] == 0.0f ? -INFINITY : kLn2 * (base[b] - kLift<T> + log2f(sum[b]));
     }
   }
-  if (!live) return;
-  if (p.slots > 1) {
-    const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
-    const int64_t slot = (g.slot + split) * all + at;
-    if (q4 == 0) {
-      p.part_ml[2 * slot] = base - kLift<T>;
-      p.part_ml[2 * slot + 1] = sum;
-    }
-    if (sum == 0.0f) return;  // no token: the join does not read the rest
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int x = 0; x < ACC; x += 4) {
-        const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
-        if (ch < p.D)
-          *reinterpret_cast<Float4*>(p.part_o + slot * p.D + ch) =
-              Float4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]};
-      }
-    return;
-  }
-  const float inv = sum == 0.0f ? 0.0f : p.v_scale / sum;
-  T* const dst = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head;
-#pragma unroll
-  for (int d = 0; d < DT; ++d)
-#pragma unroll
-    for (int x = 0; x < ACC; x += 4) {
-      const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
-      if (ch < p.D)
-        store4(dst + ch, Float4{o[d][x] * inv, o[d][x + 1] * inv, o[d][x + 2] * inv,
-                                o[d][x + 3] * inv}, p.out_vec);
-    }
-  if (p.lse && q4 == 0)
-    p.lse[at] = sum == 0.0f ? -INFINITY : kLn2 * (base - kLift<T> + log2f(sum));
 }
 
 template <typename T, bool FP8, int DP, int SHAPE>
 __device__ __forceinline__ void attend_shape(const AttendParams& p, int kind, int unit,
                                              uint8_t* lds) {
-  constexpr int MR = SHAPE == 0 || DP == 256 ? 16 : 32;
-  attend<T, FP8, DP, MR, kShapeRows[SHAPE] / MR>(p, p.group[kind], unit, kind == 0, lds);
+  constexpr int MR = SHAPE == 0 || DP == 256 ? 16 : 32, RB = SHAPE == 3 ? 2 : 1;
+  attend<T, FP8, DP, MR, RB, kShapeRows[SHAPE] / (MR * RB)>(p, p.group[kind], unit, kind == 0,
+                                                           lds);
 }
 
 // The prefix in workgroups of shape S0 and the requests in those of S1, in one launch.
 template <typename T, bool FP8, int DP, int S0, int S1>
-__global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(AttendParams p) {
+__global__ __launch_bounds__(kThreads, DP == 256 || S0 == 3 ? 1 : 2) void attend_kernel(AttendParams p) {
   __shared__ alignas(16) uint8_t lds[512 * DP];  // of every shape
   int unit = static_cast<int>(blockIdx.x);
   const int kind = unit >= p.group[0].units;
@@ -562,51 +604,123 @@ __global__ __launch_bounds__(kThreads, DP == 256 ? 1 : 2) void attend_kernel(Att
     attend_shape<T, FP8, DP, S0>(p, 0, unit, lds);
 }
 
-// Joins the parts of each row: 4 channels a lane, and for rows of many parts several lane groups
-// (`teams`) that take them in turn.
+// Joins the parts of each row: out = v_scale sum_s w_s O_s / sum_s w_s l_s with
+// w_s = 2^(m_s - max m).  For few parts: 4 channels a lane, `lanes` lanes a row.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void join_kernel(AttendParams p, int lanes, int teams) {
-  __shared__ Float4 part[kThreads];
-  __shared__ float part_sum[kThreads];
+__global__ __launch_bounds__(kThreads) void join_few_kernel(AttendParams p, int lanes) {
   const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
-  const int per = kThreads / (lanes * teams);  // rows
-  const int lane = threadIdx.x % lanes, team = threadIdx.x / lanes % teams;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / (lanes * teams);
-  const int ch = 4 * lane;
-  bool live = row < all;
-  const int64_t n = live ? row / p.Hq : 0, head = row - n * p.Hq;
-  if (p.starts) live = live && n >= p.starts[0] && n < p.starts[p.requests];
-  float best = -INFINITY, total = 0.0f;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / lanes) + threadIdx.x / lanes;
+  const int ch = 4 * (threadIdx.x % lanes);
+  if (row >= all || ch >= p.D) return;
+  const int64_t n = row / p.Hq, head = row - n * p.Hq;
+  if (p.starts && (n < p.starts[0] || n >= p.starts[p.requests])) return;
+  float m[kFewParts], l[kFewParts], best = -INFINITY, total = 0.0f;
+#pragma unroll
+  for (int s = 0; s < kFewParts; ++s) {
+    const int64_t slot = min(s, p.slots - 1) * all + row;
+    m[s] = p.part_ml[2 * slot];
+    l[s] = s < p.slots ? p.part_ml[2 * slot + 1] : 0.0f;
+    best = fmaxf(best, m[s]);
+  }
+  const float zero = best == -INFINITY ? 0.0f : best;
   Float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (live) {
-    // every lane group finds the largest maximum for itself, its lanes sharing the parts
-    for (int s = lane; s < p.slots; s += lanes)
-      best = fmaxf(best, p.part_ml[2 * (s * all + row)]);
-    for (int x = 1; x < lanes; x <<= 1) best = fmaxf(best, __shfl_xor(best, x));
-    const float zero = best == -INFINITY ? 0.0f : best;
-    for (int s = team; s < p.slots; s += teams) {
-      const int64_t slot = s * all + row;
-      const float l = p.part_ml[2 * slot + 1];
-      if (l == 0.0f) continue;  // no token: nothing was written
-      const float w = __builtin_amdgcn_exp2f(p.part_ml[2 * slot] - zero);
-      total += l * w;
-      if (ch < p.D) o += *reinterpret_cast<const Float4*>(p.part_o + slot * p.D + ch) * w;
+#pragma unroll
+  for (int s = 0; s < kFewParts; ++s)
+    if (l[s] != 0.0f) {  // else no token: nothing was written
+      const float w = __builtin_amdgcn_exp2f(m[s] - zero);
+      total += l[s] * w;
+      o += *reinterpret_cast<const Float4*>(p.part_o + (s * all + row) * p.D + ch) * w;
     }
-  }
-  if (teams > 1) {
-    part[threadIdx.x] = o;
-    part_sum[threadIdx.x] = total;
-    __syncthreads();
-    if (team != 0) return;
-    for (int k = 1; k < teams; ++k) {
-      o += part[threadIdx.x + k * lanes];
-      total += part_sum[threadIdx.x + k * lanes];
-    }
-  }
-  if (!live) return;
   const float inv = total == 0.0f ? 0.0f : p.v_scale / total;
-  if (ch < p.D)
-    store4(static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + ch, o * inv, p.out_vec);
+  store4(static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + ch, o * inv, p.out_vec);
+  if (p.lse && ch == 0) p.lse[row] = total == 0.0f ? -INFINITY : kLn2 * (best + log2f(total));
+}
+
+// For many parts: a workgroup takes `4 lanes` channels of one row.  It first lists the parts that
+// have tokens with their weights, then its lane groups add them up in turn, several loads each
+// on their way: a row's parts are one after the other for nobody.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_kernel(AttendParams p, int lanes, int blocks) {
+  __shared__ float weight[kMaxParts];
+  __shared__ int which[kMaxParts];
+  __shared__ float wave_best[kWaves], wave_sum[kWaves];
+  __shared__ int counts[kMaxParts / kThreads][kWaves];
+  __shared__ Float4 part[kThreads];
+  const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
+  const int64_t row = blockIdx.x / blocks;
+  const int ch = 4 * (static_cast<int>(blockIdx.x % blocks) * lanes + threadIdx.x % lanes);
+  const int team = threadIdx.x / lanes, teams = kThreads / lanes;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t n = row / p.Hq, head = row - n * p.Hq;
+  if (p.starts && (n < p.starts[0] || n >= p.starts[p.requests])) return;
+
+  constexpr int kEach = kMaxParts / kThreads;
+  float m[kEach], l[kEach], best = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int s = i * kThreads + threadIdx.x;
+    m[i] = -INFINITY;
+    l[i] = 0.0f;
+    if (s < p.slots) {
+      m[i] = p.part_ml[2 * (s * all + row)];
+      l[i] = p.part_ml[2 * (s * all + row) + 1];
+    }
+    best = fmaxf(best, m[i]);
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) best = fmaxf(best, __shfl_xor(best, x));
+  uint64_t has[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) has[i] = __ballot(l[i] != 0.0f);
+  if (lane == 0) {
+    wave_best[wave] = best;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) counts[i][wave] = __popcll(has[i]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) best = fmaxf(best, wave_best[w]);
+  const float zero = best == -INFINITY ? 0.0f : best;
+  float sum = 0.0f;
+  int parts = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    int at = parts + __popcll(has[i] & ((1ull << lane) - 1));
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      at += w < wave ? counts[i][w] : 0;
+      parts += counts[i][w];
+    }
+    if (l[i] != 0.0f) {
+      const float w = __builtin_amdgcn_exp2f(m[i] - zero);
+      sum += l[i] * w;
+      weight[at] = w;
+      which[at] = i * kThreads + threadIdx.x;
+    }
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+  if (lane == 0) wave_sum[wave] = sum;
+  __syncthreads();
+
+  const float* const src = p.part_o + row * p.D + min(ch, p.D - 4);
+  Float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int s = team; s < parts; s += teams)
+    o += *reinterpret_cast<const Float4*>(src + which[s] * all * p.D) * weight[s];
+  part[threadIdx.x] = o;
+  __syncthreads();
+  for (int k = teams / 2; k > 0; k /= 2) {
+    if (team < k) part[threadIdx.x] += part[threadIdx.x + k * lanes];
+    __syncthreads();
+  }
+  if (team != 0 || ch >= p.D) return;
+  float total = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) total += wave_sum[w];
+  const float inv = total == 0.0f ? 0.0f : p.v_scale / total;
+  store4(static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + ch, part[threadIdx.x] * inv,
+         p.out_vec);
   if (p.lse && ch == 0) p.lse[row] = total == 0.0f ? -INFINITY : kLn2 * (best + log2f(total));
 }
 
@@ -627,6 +741,14 @@ int launch_units(const AttendParams& p, hipStream_t stream) {
       hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 2, 1>), grid, block, 0, stream, p);
     else if (s0 == 2)
       hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 2, 2>), grid, block, 0, stream, p);
+    else if (s0 == 3 && s1 == 0)
+      hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 3, 0>), grid, block, 0, stream, p);
+    else if (s0 == 3 && s1 == 1)
+      hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 3, 1>), grid, block, 0, stream, p);
+    else if (s0 == 3 && s1 == 2)
+      hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 3, 2>), grid, block, 0, stream, p);
+    else if (s0 == 3)
+      hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 3, 3>), grid, block, 0, stream, p);
   }
   return check_launch("attend_kernel");
 }
@@ -639,11 +761,18 @@ int launch_attend(const AttendParams& p, hipStream_t stream) {
   if (rc) return rc;
   const dim3 block(kThreads);
   if (p.slots == 1) return ORIGAMI_OK;
-  const int lanes = p.D <= 64 ? 16 : (p.D <= 128 ? 32 : 64);
-  const int teams = p.slots >= 8 ? kThreads / lanes : 1;
-  const int64_t rows = static_cast<int64_t>(p.tokens) * p.Hq, per = kThreads / (lanes * teams);
-  hipLaunchKernelGGL(join_kernel<T>, dim3(static_cast<unsigned>((rows + per - 1) / per)), block, 0,
-                     stream, p, lanes, teams);
+  const int lanes = p.D <= 64 ? 16 : (p.D <= 128 ? 32 : 64);  // of a whole row
+  const int64_t rows = static_cast<int64_t>(p.tokens) * p.Hq, per = kThreads / lanes;
+  if (p.slots <= kFewParts) {
+    const dim3 joins(static_cast<unsigned>((rows + per - 1) / per));
+    hipLaunchKernelGGL(join_few_kernel<T>, joins, block, 0, stream, p, lanes);
+  } else {
+    // with few rows, workgroups of 32 channels, so that the GPU has enough of them
+    const int some = rows < kFill ? 8 : lanes;
+    const int blocks = (p.D + 4 * some - 1) / (4 * some);
+    const dim3 joins(static_cast<unsigned>(rows * blocks));
+    hipLaunchKernelGGL(join_kernel<T>, joins, block, 0, stream, p, some, blocks);
+  }
   return check_launch("join_kernel");
 }
 
@@ -654,8 +783,6 @@ struct Plan {
   Group shared, each;
   int64_t slots, units;
 };
-
-constexpr int64_t kFill = 512;  // workgroups that fill the GPU: two on each of 256 CUs
 
 Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_dim,
              int64_t prefix, int64_t requests, int64_t max_query, int64_t max_own) {
@@ -670,10 +797,24 @@ Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_di
     while (shape < last && rows > kShapeRows[shape]) ++shape;
     const int64_t tiles = std::max<int64_t>(ceil_div(rows, kShapeRows[shape]), 1);
     const int64_t keys = std::max<int64_t>(n * heads, 1);
-    // ranges of 128 tokens or more, as many as fill the GPU
-    const int64_t most = std::max<int64_t>(ceil_div(span, 128), 1);
-    int64_t splits = std::min(most, std::max<int64_t>(kFill / (keys * tiles), 1));
-    const int64_t chunk = std::max<int64_t>(ceil_div(ceil_div(span, splits), 128), 1) * 128;
+    // Ranges of 128 tokens or more.  A workgroup's time is taken as its steps of 128 tokens and two
+    // more for its start and end, that of the call as the rounds of workgroups that the GPU
+    // takes (at the size of an average request), and a part more to join as 1 / 16 step for every
+    // workgroup's rows in a round.
+    const int64_t steps = std::max<int64_t>(ceil_div(span, 128), 1);
+    const int64_t live = std::max<int64_t>(
+        std::min(keys * tiles, heads * (ceil_div(tokens * G, kShapeRows[shape]) + n / 2)), 1);
+    int64_t splits = 1;
+    double least = 0.0;
+    for (int64_t s = 1; s <= std::min<int64_t>(steps, kFill); ++s) {
+      const double rounds = static_cast<double>(ceil_div(live * s, kFill));
+      const double cost = rounds * (ceil_div(steps, s) + 2) + (s > 1 ? live * s / 16.0 / kFill : 0);
+      if (s == 1 || cost < least) {
+        least = cost;
+        splits = s;
+      }
+    }
+    const int64_t chunk = ceil_div(steps, splits) * 128;
     splits = std::max<int64_t>(ceil_div(span, chunk), 1);
     const int64_t units = ceil_div(keys * splits, 8) * 8 * tiles;
     plan.units += units;
@@ -768,7 +909,8 @@ int origami_shared_prefix_attention(
   if (num_blocks == 0) prefix_tokens = max_own_tokens = 0;  // no token is in the cache
   const Plan plan = plan_of(tokens, query_heads, heads, head_dim, prefix_tokens, requests,
                             max_query_tokens, max_own_tokens);
-  ORIGAMI_REQUIRE(plan.units <= INT32_MAX, "too many row tiles for one call");
+  ORIGAMI_REQUIRE(plan.units <= INT32_MAX && tokens * query_heads <= INT32_MAX / 32,
+                  "too many row tiles for one call");
   ORIGAMI_REQUIRE(workspace_bytes >= workspace_bytes_of(plan, tokens, query_heads, head_dim) &&
                       (plan.slots == 1 || workspace != nullptr) && aligned16(workspace),
                   "attention workspace is too small");
