@@ -19,8 +19,11 @@ using origami_internal::cache_geometry;
 using origami_internal::check_launch;
 using origami_internal::fail;
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
+// Waves of a workgroup, of which one is on each CU: its tiles fill LDS and registers.  With 256
+// channels results alone take half the registers of a wave, so there are four.
+template <int DP>
+constexpr int kWaves = DP == 256 ? 4 : 8;
+constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64;
 constexpr int kStep = 32;  // tokens of one product P V (the depth of its matrix instruction)
 // Exponentials are taken 2^kLift times as large for half precision, so that those of tokens far
 // below the maximum keep their precision (down to 2^-24 of the largest) and sums of 2^30 of
@@ -33,18 +36,19 @@ template <typename T>
 constexpr float kSlack = std::is_same<T, f16>::value ? 4.0f : 8.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-constexpr int64_t kFill = 512;  // workgroups that fill the GPU: two on each of 256 CUs
+constexpr int64_t kFill = 256;  // workgroups that fill the GPU: one on each CU
 constexpr int kFewParts = 4;
-constexpr int kMaxParts = 1024;  // of a row: kFill at most of either kind
+constexpr int kMaxParts = 512;  // of a row: kFill at most of either kind
 
-// Rows of a workgroup.  The last shape is for up to 128 channels: with 256, results of 32 rows a wave
-// and the tiles on their way would not fit the registers.
+// Rows of a workgroup.  Waves take 16 or 32 rows; in the larger shapes more of them have rows of
+// their own, in the smaller ones more have tokens of their own.  With 256 channels there are
+// the first two shapes.
 constexpr int kShapeRows[4] = {16, 64, 128, 256};
 
 // The work of one kind: row tiles of every KV head, over ranges of tokens.
 struct Group {
   int32_t units;   // workgroups
-  int32_t shape;   // kShapeRows[shape] rows each
+  int32_t shape;   // kShapeRows[shape] rows each, at most
   int32_t tiles;   // row tiles of a request, or of the batch
   int32_t splits;  // ranges of `chunk` tokens
   int32_t chunk;
@@ -219,18 +223,17 @@ __device__ __forceinline__ Vec8<T> read_values(const uint8_t* values, int lane, 
 
 // Tokens that a team of waves (the WR waves with the same tokens) has in LDS at a time.
 template <int DP, int WR>
-constexpr int kTeamTokens = WR == 4 && DP < 256 ? 64 : 32;
+constexpr int kTeamTokens = WR >= 4 && DP < 256 ? 64 : 32;
 
-// One workgroup: WR RB MR rows of one KV head over a range of tokens.  Its waves are WR row
-// waves by kWaves / WR token waves: a wave takes RB times MR rows, and of every kWaves / WR times
-// kTeamTokens tokens its share.  Rows (queries, results, sums) stay in registers; keys and values go
+// One workgroup: WR MR rows of one KV head over a range of tokens.  Its waves are WR row waves by
+// WT token waves: a wave takes MR rows, and of every WT kTeamTokens tokens its share.  Rows (queries, results, sums) stay in registers; keys and values go
 // through LDS, where the WR waves of a team share them, and the next ones are on their way
 // to registers meanwhile.  With WR = 1 no wave needs another until the end; else two buffers
 // take turns, so that one barrier a step is enough.
-template <typename T, bool FP8, int DP, int MR, int RB, int WR>
+template <typename T, bool FP8, int DP, int MR, int WR>
 __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, int unit, bool batch,
                                        uint8_t* lds) {
-  constexpr int WT = kWaves / WR, TT = kTeamTokens<DP, WR>;
+  constexpr int WT = kWaves<DP> / WR, TT = kTeamTokens<DP, WR>;
   constexpr int NG = 64 / MR;             // lane groups: the depth of a product is 8 NG
   constexpr int KS = DP / (8 * NG);       // depth steps of K Q
   constexpr int DT = DP / MR;             // channel tiles of V P
@@ -265,63 +268,56 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
     rq = request_of(p, r);
   }
   const int split = u;
-  const int rows = rq.count * p.G, row0 = tile * WR * RB * MR;
+  const int rows = rq.count * p.G, row0 = tile * WR * MR;
   if (split >= g.splits || row0 >= rows) return;
   const int end = batch ? p.prefix : p.prefix + rq.own;  // of the tokens, prefix first
   const int64_t* const table = p.tables + static_cast<int64_t>(r) * p.table_stride;
 
-  // this lane's rows
-  const auto row_at = [&](int b) { return row0 + (wr * RB + b) * MR + c; };
-  const auto seen_by = [&](int row) -> int {  // tokens that a row sees
-    return batch ? p.prefix : p.prefix + min(max(rq.own - rq.count + row / p.G + 1, 0), rq.own);
+  // this lane's row
+  const int row = row0 + wr * MR + c;
+  const auto seen_by = [&](int i) -> int {  // tokens that row i sees
+    return batch ? p.prefix : p.prefix + min(max(rq.own - rq.count + i / p.G + 1, 0), rq.own);
   };
-  int limit[RB];
+  const int limit = seen_by(row);
   // the scale's sign goes with the queries, and so does a scale of zero, so that hidden scores of
   // -infinity stay what they are
   const float scale = p.scale == 0.0f ? 1.0f : fabsf(p.scale);
-  Vec8<T> qf[RB][KS];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const int row = row_at(b), qi = row / p.G;
-    limit[b] = seen_by(row);
-    const T* const src = static_cast<const T*>(p.query) + (rq.first + qi) * p.q_token +
-                         (h * p.G + row - qi * p.G) * p.q_head;
+  const int qi = row / p.G, head = h * p.G + row - qi * p.G;
+  Vec8<T> qf[KS];
+  {
+    const T* const src =
+        static_cast<const T*>(p.query) + (rq.first + qi) * p.q_token + head * p.q_head;
     const bool vec =
         ((reinterpret_cast<uintptr_t>(p.query) | 2 * p.q_token | 2 * p.q_head) & 15) == 0;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       const int d = 8 * (NG * k + q4);
-      qf[b][k] = Vec8<T>{};
+      qf[k] = Vec8<T>{};
       if (row < rows && d < p.D) {
         if (vec) {
-          qf[b][k] = *reinterpret_cast<const Vec8<T>*>(src + d);
+          qf[k] = *reinterpret_cast<const Vec8<T>*>(src + d);
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) qf[b][k][j] = src[d + j];
+          for (int j = 0; j < 8; ++j) qf[k][j] = src[d + j];
         }
-        if (p.scale <= 0.0f) qf[b][k] = p.scale == 0.0f ? Vec8<T>{} : -qf[b][k];
+        if (p.scale <= 0.0f) qf[k] = p.scale == 0.0f ? Vec8<T>{} : -qf[k];
       }
     }
   }
   // The tokens that some row of the workgroup sees, and those that all rows of the wave see;
   // limits grow along the rows.
-  const int most = seen_by(min(row0 + WR * RB * MR, rows) - 1);
-  const int least = seen_by(min(row0 + wr * RB * MR, rows - 1));
+  const int most = seen_by(min(row0 + WR * MR, rows) - 1);
+  const int least = seen_by(min(row0 + wr * MR, rows - 1));
   const int nearest = seen_by(row0);  // the tokens that all rows of the workgroup see
   const int t0 = g.first + split * g.chunk;
   const int t1 = min(min(end, most), t0 + g.chunk);
 
-  Tile<MR> o[RB][DT];
-  float base[RB], sum[RB];
+  Tile<MR> o[DT];
+  float base = -INFINITY, sum = 0.0f;
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    base[b] = -INFINITY;
-    sum[b] = 0.0f;
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int x = 0; x < ACC; ++x) o[b][d][x] = 0.0f;
-  }
+    for (int x = 0; x < ACC; ++x) o[d][x] = 0.0f;
 
   uint8_t* const team = lds + wt * kBuffers * 2 * kTile;
   const int piece = lane % NCH, sub = lane / NCH;
@@ -407,63 +403,54 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
       const uint8_t* const vb = kb + kTile;
       const int ts = t + s * kStep;  // the step's first token
       // S = K Q: row c against token STRIDE (i / 4) + 4 q4 + i % 4
-      Tile<MR> sc[RB][X / ACC];
+      Tile<MR> sc[X / ACC];
 #pragma unroll
       for (int m = 0; m < X / ACC; ++m) {
 #pragma unroll
-        for (int b = 0; b < RB; ++b)
-#pragma unroll
-          for (int x = 0; x < ACC; ++x) sc[b][m][x] = 0.0f;
+        for (int x = 0; x < ACC; ++x) sc[m][x] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           const int tok = MR * m + c;
           const Vec8<T> kf = *reinterpret_cast<const Vec8<T>*>(
               kb + (tok * NCH + key_piece<DP>(tok, NG * k + q4)) * 16);
-#pragma unroll
-          for (int b = 0; b < RB; ++b) sc[b][m] = mfma<T, MR>(kf, qf[b][k], sc[b][m]);
+          sc[m] = mfma<T, MR>(kf, qf[k], sc[m]);
         }
       }
-      Vec8<T> pf[RB][X / 8];
-#pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        if (!whole) {
-          const uint32_t seen = static_cast<uint32_t>(there >> (kStep * s));
-#pragma unroll
-          for (int i = 0; i < X; ++i) {
-            const int tok = STRIDE * (i / 4) + 4 * q4 + i % 4;
-            if (ts + tok >= limit[b] || !((seen >> tok) & 1)) sc[b][i / ACC][i % ACC] = -INFINITY;
-          }
-        }
-        float best = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < X; ++i) best = fmaxf(best, sc[b][i / ACC][i % ACC]);
-        best = max_over_groups<MR>(best) * scale;
-        const bool rises = best > base[b] + kSlack<T>;
-        if (__any(rises)) {  // each row by itself: no row's rounding depends on another
-          const float next = rises ? best : base[b];
-          const float keep = __builtin_amdgcn_exp2f(base[b] - (next == -INFINITY ? 0.0f : next));
-          base[b] = next;
-          sum[b] *= keep;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) o[b][d] *= keep;
-        }
-        const float below = kLift<T> - (base[b] == -INFINITY ? 0.0f : base[b]);
+      if (!whole) {
+        const uint32_t seen = static_cast<uint32_t>(there >> (kStep * s));
 #pragma unroll
         for (int i = 0; i < X; ++i) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(sc[b][i / ACC][i % ACC], scale, below));
-          sum[b] += e;
-          pf[b][i / 8][i % 8] = static_cast<T>(e);
+          const int tok = STRIDE * (i / 4) + 4 * q4 + i % 4;
+          if (ts + tok >= limit || !((seen >> tok) & 1)) sc[i / ACC][i % ACC] = -INFINITY;
         }
+      }
+      float best = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < X; ++i) best = fmaxf(best, sc[i / ACC][i % ACC]);
+      best = max_over_groups<MR>(best) * scale;
+      const bool rises = best > base + kSlack<T>;
+      if (__any(rises)) {  // each row by itself: no row's rounding depends on another
+        const float next = rises ? best : base;
+        const float keep = __builtin_amdgcn_exp2f(base - (next == -INFINITY ? 0.0f : next));
+        base = next;
+        sum *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= keep;
+      }
+      const float below = kLift<T> - (base == -INFINITY ? 0.0f : base);
+      Vec8<T> pf[X / 8];
+#pragma unroll
+      for (int i = 0; i < X; ++i) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(sc[i / ACC][i % ACC], scale, below));
+        sum += e;
+        pf[i / 8][i % 8] = static_cast<T>(e);
       }
       // O += V P
 #pragma unroll
       for (int k = 0; k < X / 8; ++k)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const Vec8<T> v = read_values<T, DP, MR>(vb, lane, k, d);
-#pragma unroll
-          for (int b = 0; b < RB; ++b) o[b][d] = mfma<T, MR>(v, pf[b][k], o[b][d]);
-        }
+        for (int d = 0; d < DT; ++d)
+          o[d] = mfma<T, MR>(read_values<T, DP, MR>(vb, lane, k, d), pf[k], o[d]);
     }
     if constexpr (WR == 1)
       __builtin_amdgcn_wave_barrier();
@@ -472,129 +459,125 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
   }
 
 #pragma unroll
-  for (int b = 0; b < RB; ++b)
-#pragma unroll
-    for (int x = MR; x < 64; x <<= 1) sum[b] += __shfl_xor(sum[b], x);
+  for (int x = MR; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
   if (t1 > nearest) odd = __syncthreads_or(odd);
   if constexpr (WT > 1) {
-    // join the token waves: the largest maximum, then the weighted sums, which end in the last one
-    static_assert(RB == 1, "token waves have one block of rows");
+    // join the token waves: the largest maximum, then the weighted sums, half of the waves
+    // adding the other half's, until the first ones have them
     constexpr int M = WR * MR, kPitch = DP + 4;
+    static_assert((WT * M * 2 + WT / 2 * M * kPitch) * 4 <= 128 * DP * kWaves<DP>, "LDS");
     __syncthreads();
     float* const ml = reinterpret_cast<float*>(lds);  // [WT][M][2]
-    float* const ol = ml + WT * M * 2;                // [M][kPitch]
+    float* const ol = ml + WT * M * 2;                // [WT / 2][M][kPitch]
     const int mr = wr * MR + c;
     if (q4 == 0) {
-      ml[(wt * M + mr) * 2] = base[0];
-      ml[(wt * M + mr) * 2 + 1] = sum[0];
+      ml[(wt * M + mr) * 2] = base;
+      ml[(wt * M + mr) * 2 + 1] = sum;
     }
     __syncthreads();
-    const float mine_base = base[0];
+    const float mine_base = base;
 #pragma unroll
-    for (int w = 0; w < WT; ++w) base[0] = fmaxf(base[0], ml[(w * M + mr) * 2]);
-    const float zero = base[0] == -INFINITY ? 0.0f : base[0];
-    sum[0] = 0.0f;
+    for (int w = 0; w < WT; ++w) base = fmaxf(base, ml[(w * M + mr) * 2]);
+    const float zero = base == -INFINITY ? 0.0f : base;
+    sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < WT; ++w)
-      sum[0] += ml[(w * M + mr) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * M + mr) * 2] - zero);
+      sum += ml[(w * M + mr) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * M + mr) * 2] - zero);
     const float weight = __builtin_amdgcn_exp2f(mine_base - zero);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) o[0][d] *= weight;
+    for (int d = 0; d < DT; ++d) o[d] *= weight;
 #pragma unroll 1
-    for (int w = 0; w < WT; ++w) {
-      if (w == wt)
+    for (int half = WT / 2; half > 0; half /= 2) {
+      float* const rowl = ol + ((wt % half) * M + mr) * kPitch + 4 * q4;
+      if (wt >= half && wt < 2 * half)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int x = 0; x < ACC; x += 4)
+            *reinterpret_cast<Float4*>(rowl + MR * d + 256 / MR * (x / 4)) =
+                Float4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]};
+      __syncthreads();
+      if (wt < half)
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int x = 0; x < ACC; x += 4) {
-            Float4* const dst = reinterpret_cast<Float4*>(ol + mr * kPitch + MR * d + 4 * q4 +
-                                                          256 / MR * (x / 4));
-            if (w > 0) {
-              const Float4 v = *dst;
-              o[0][d][x] += v[0];
-              o[0][d][x + 1] += v[1];
-              o[0][d][x + 2] += v[2];
-              o[0][d][x + 3] += v[3];
-            }
-            if (w < WT - 1)
-              *dst = Float4{o[0][d][x], o[0][d][x + 1], o[0][d][x + 2], o[0][d][x + 3]};
+            const Float4 v = *reinterpret_cast<const Float4*>(rowl + MR * d + 256 / MR * (x / 4));
+            o[d][x] += v[0];
+            o[d][x + 1] += v[1];
+            o[d][x + 2] += v[2];
+            o[d][x + 3] += v[3];
           }
-      if (w < WT - 1) __syncthreads();
+      if (half > 1) __syncthreads();
     }
-    if (wt != WT - 1) return;
+    if (wt != 0) return;
   }
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const int row = row_at(b);
-    if (odd) {
-      // the values that store_tile left out, to the rows that see them; those of the tokens
-      // before them were added already, and an infinity or NaN twice is the same
-      for (int i = max(t0, nearest - TT); i < min(t1, limit[b]); ++i) {
-        const int at_row = row_of(i, block_of(i));
-        if (at_row < 0) continue;
-        const uint8_t* const src =
-            p.cache + (at_row + p.half_stride) * pitch + static_cast<int64_t>(h) * p.D * cell;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int x = 0; x < ACC; x += 4) {
-            const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
-            const Float4 v = four_values<T, FP8>(src, min(ch, p.D - 4));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[b][d][x + j] += fabsf(v[j]) < INFINITY ? 0.0f : v[j];
-          }
-      }
-    }
-    if (row >= rows) continue;
-    const int qi = row / p.G, head = h * p.G + row - qi * p.G;
-    const int64_t n = rq.first + qi, at = n * p.Hq + head;
-    if (p.slots > 1) {
-      const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
-      const int64_t slot = (g.slot + split) * all + at;
-      if (q4 == 0) {
-        p.part_ml[2 * slot] = base[b] - kLift<T>;
-        p.part_ml[2 * slot + 1] = sum[b];
-      }
-      if (sum[b] == 0.0f) continue;  // no token: the join does not read the rest
+  if (odd) {
+    // the values that store_tile left out, to the rows that see them; those of the tokens
+    // before them were added already, and an infinity or NaN twice is the same
+    for (int i = max(t0, nearest - TT); i < min(t1, limit); ++i) {
+      const int at_row = row_of(i, block_of(i));
+      if (at_row < 0) continue;
+      const uint8_t* const src =
+          p.cache + (at_row + p.half_stride) * pitch + static_cast<int64_t>(h) * p.D * cell;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int x = 0; x < ACC; x += 4) {
           const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
-          if (ch < p.D)
-            *reinterpret_cast<Float4*>(p.part_o + slot * p.D + ch) =
-                Float4{o[b][d][x], o[b][d][x + 1], o[b][d][x + 2], o[b][d][x + 3]};
-        }
-    } else {
-      const float inv = sum[b] == 0.0f ? 0.0f : p.v_scale / sum[b];
-      T* const dst = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head;
+          const Float4 v = four_values<T, FP8>(src, min(ch, p.D - 4));
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int x = 0; x < ACC; x += 4) {
-          const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
-          if (ch < p.D)
-            store4(dst + ch, Float4{o[b][d][x] * inv, o[b][d][x + 1] * inv, o[b][d][x + 2] * inv,
-                                    o[b][d][x + 3] * inv}, p.out_vec);
+          for (int j = 0; j < 4; ++j) o[d][x + j] += fabsf(v[j]) < INFINITY ? 0.0f : v[j];
         }
-      if (p.lse && q4 == 0)
-        p.lse[at] = sum[b] == 0.0f ? -INFINITY : kLn2 * (base[b] - kLift<T> + log2f(sum[b]));
     }
   }
+  if (row >= rows) return;
+  const int64_t n = rq.first + qi, at = n * p.Hq + head;
+  if (p.slots > 1) {
+    const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
+    const int64_t slot = (g.slot + split) * all + at;
+    if (q4 == 0) {
+      p.part_ml[2 * slot] = base - kLift<T>;
+      p.part_ml[2 * slot + 1] = sum;
+    }
+    if (sum == 0.0f) return;  // no token: the join does not read the rest
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int x = 0; x < ACC; x += 4) {
+        const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
+        if (ch < p.D)
+          *reinterpret_cast<Float4*>(p.part_o + slot * p.D + ch) =
+              Float4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]};
+      }
+    return;
+  }
+  const float inv = sum == 0.0f ? 0.0f : p.v_scale / sum;
+  T* const dst = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int x = 0; x < ACC; x += 4) {
+      const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
+      if (ch < p.D)
+        store4(dst + ch, Float4{o[d][x] * inv, o[d][x + 1] * inv, o[d][x + 2] * inv,
+                                o[d][x + 3] * inv}, p.out_vec);
+    }
+  if (p.lse && q4 == 0)
+    p.lse[at] = sum == 0.0f ? -INFINITY : kLn2 * (base - kLift<T> + log2f(sum));
 }
 
 template <typename T, bool FP8, int DP, int SHAPE>
 __device__ __forceinline__ void attend_shape(const AttendParams& p, int kind, int unit,
                                              uint8_t* lds) {
-  constexpr int MR = SHAPE == 0 || DP == 256 ? 16 : 32, RB = SHAPE == 3 ? 2 : 1;
-  attend<T, FP8, DP, MR, RB, kShapeRows[SHAPE] / (MR * RB)>(p, p.group[kind], unit, kind == 0,
-                                                           lds);
+  constexpr int MR = SHAPE == 0 || DP == 256 ? 16 : 32;
+  attend<T, FP8, DP, MR, kShapeRows[SHAPE] / MR>(p, p.group[kind], unit, kind == 0, lds);
 }
 
 // The prefix in workgroups of shape S0 and the requests in those of S1, in one launch.
 template <typename T, bool FP8, int DP, int S0, int S1>
-__global__ __launch_bounds__(kThreads, DP == 256 || S0 == 3 ? 1 : 2) void attend_kernel(AttendParams p) {
-  __shared__ alignas(16) uint8_t lds[512 * DP];  // of every shape
+__global__ __launch_bounds__(64 * kWaves<DP>) void attend_kernel(AttendParams p) {
+  __shared__ alignas(16) uint8_t lds[128 * DP * kWaves<DP>];  // of every shape
   int unit = static_cast<int>(blockIdx.x);
   const int kind = unit >= p.group[0].units;
   unit -= kind ? p.group[0].units : 0;
@@ -607,9 +590,9 @@ __global__ __launch_bounds__(kThreads, DP == 256 || S0 == 3 ? 1 : 2) void attend
 // Joins the parts of each row: out = v_scale sum_s w_s O_s / sum_s w_s l_s with
 // w_s = 2^(m_s - max m).  For few parts: 4 channels a lane, `lanes` lanes a row.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void join_few_kernel(AttendParams p, int lanes) {
+__global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams p, int lanes) {
   const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / lanes) + threadIdx.x / lanes;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / lanes) + threadIdx.x / lanes;
   const int ch = 4 * (threadIdx.x % lanes);
   if (row >= all || ch >= p.D) return;
   const int64_t n = row / p.Hq, head = row - n * p.Hq;
@@ -640,25 +623,25 @@ __global__ __launch_bounds__(kThreads) void join_few_kernel(AttendParams p, int 
 // have tokens with their weights, then its lane groups add them up in turn, several loads each
 // on their way: a row's parts are one after the other for nobody.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void join_kernel(AttendParams p, int lanes, int blocks) {
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendParams p, int lanes, int blocks) {
   __shared__ float weight[kMaxParts];
   __shared__ int which[kMaxParts];
-  __shared__ float wave_best[kWaves], wave_sum[kWaves];
-  __shared__ int counts[kMaxParts / kThreads][kWaves];
-  __shared__ Float4 part[kThreads];
+  __shared__ float wave_best[kJoinWaves], wave_sum[kJoinWaves];
+  __shared__ int counts[kMaxParts / kJoinThreads][kJoinWaves];
+  __shared__ Float4 part[kJoinThreads];
   const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
   const int64_t row = blockIdx.x / blocks;
   const int ch = 4 * (static_cast<int>(blockIdx.x % blocks) * lanes + threadIdx.x % lanes);
-  const int team = threadIdx.x / lanes, teams = kThreads / lanes;
+  const int team = threadIdx.x / lanes, teams = kJoinThreads / lanes;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int64_t n = row / p.Hq, head = row - n * p.Hq;
   if (p.starts && (n < p.starts[0] || n >= p.starts[p.requests])) return;
 
-  constexpr int kEach = kMaxParts / kThreads;
+  constexpr int kEach = kMaxParts / kJoinThreads;
   float m[kEach], l[kEach], best = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    const int s = i * kThreads + threadIdx.x;
+    const int s = i * kJoinThreads + threadIdx.x;
     m[i] = -INFINITY;
     l[i] = 0.0f;
     if (s < p.slots) {
@@ -679,7 +662,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttendParams p, int lane
   }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) best = fmaxf(best, wave_best[w]);
+  for (int w = 0; w < kJoinWaves; ++w) best = fmaxf(best, wave_best[w]);
   const float zero = best == -INFINITY ? 0.0f : best;
   float sum = 0.0f;
   int parts = 0;
@@ -687,7 +670,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttendParams p, int lane
   for (int i = 0; i < kEach; ++i) {
     int at = parts + __popcll(has[i] & ((1ull << lane) - 1));
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kJoinWaves; ++w) {
       at += w < wave ? counts[i][w] : 0;
       parts += counts[i][w];
     }
@@ -695,7 +678,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttendParams p, int lane
       const float w = __builtin_amdgcn_exp2f(m[i] - zero);
       sum += l[i] * w;
       weight[at] = w;
-      which[at] = i * kThreads + threadIdx.x;
+      which[at] = i * kJoinThreads + threadIdx.x;
     }
   }
 #pragma unroll
@@ -717,7 +700,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttendParams p, int lane
   if (team != 0 || ch >= p.D) return;
   float total = 0.0f;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) total += wave_sum[w];
+  for (int w = 0; w < kJoinWaves; ++w) total += wave_sum[w];
   const float inv = total == 0.0f ? 0.0f : p.v_scale / total;
   store4(static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + ch, part[threadIdx.x] * inv,
          p.out_vec);
@@ -726,7 +709,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AttendParams p, int lane
 
 template <typename T, bool FP8, int DP>
 int launch_units(const AttendParams& p, hipStream_t stream) {
-  const dim3 grid(p.group[0].units + p.group[1].units), block(kThreads);
+  const dim3 grid(p.group[0].units + p.group[1].units), block(64 * kWaves<DP>);
   const int s1 = p.group[1].shape, s0 = p.group[0].units ? p.group[0].shape : s1;
   if (s0 == 0)  // the batch has at least a request's rows: s0 >= s1
     hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 0, 0>), grid, block, 0, stream, p);
@@ -759,16 +742,16 @@ int launch_attend(const AttendParams& p, hipStream_t stream) {
                  : p.D <= 128 ? launch_units<T, FP8, 128>(p, stream)
                               : launch_units<T, FP8, 256>(p, stream);
   if (rc) return rc;
-  const dim3 block(kThreads);
+  const dim3 block(kJoinThreads);
   if (p.slots == 1) return ORIGAMI_OK;
   const int lanes = p.D <= 64 ? 16 : (p.D <= 128 ? 32 : 64);  // of a whole row
-  const int64_t rows = static_cast<int64_t>(p.tokens) * p.Hq, per = kThreads / lanes;
+  const int64_t rows = static_cast<int64_t>(p.tokens) * p.Hq, per = kJoinThreads / lanes;
   if (p.slots <= kFewParts) {
     const dim3 joins(static_cast<unsigned>((rows + per - 1) / per));
     hipLaunchKernelGGL(join_few_kernel<T>, joins, block, 0, stream, p, lanes);
   } else {
     // with few rows, workgroups of 32 channels, so that the GPU has enough of them
-    const int some = rows < kFill ? 8 : lanes;
+    const int some = rows < 2 * kFill ? 8 : lanes;
     const int blocks = (p.D + 4 * some - 1) / (4 * some);
     const dim3 joins(static_cast<unsigned>(rows * blocks));
     hipLaunchKernelGGL(join_kernel<T>, joins, block, 0, stream, p, some, blocks);
@@ -788,7 +771,7 @@ Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_di
              int64_t prefix, int64_t requests, int64_t max_query, int64_t max_own) {
   Plan plan{};
   const int64_t G = query_heads / heads;
-  const int last = head_dim > 128 ? 1 : 2;
+  const int last = head_dim > 128 ? 1 : 3;
   // A request whose rows fill workgroups by themselves reads the prefix with its own tokens.
   const bool apart = requests > 1 && prefix > 0 && max_query * G < kShapeRows[last];
   int64_t slot = 0;  // of the partial results
@@ -797,24 +780,24 @@ Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_di
     while (shape < last && rows > kShapeRows[shape]) ++shape;
     const int64_t tiles = std::max<int64_t>(ceil_div(rows, kShapeRows[shape]), 1);
     const int64_t keys = std::max<int64_t>(n * heads, 1);
-    // Ranges of 128 tokens or more.  A workgroup's time is taken as its steps of 128 tokens and two
+    // Ranges of 256 tokens or more.  A workgroup's time is taken as its steps of 256 tokens and two
     // more for its start and end, that of the call as the rounds of workgroups that the GPU
-    // takes (at the size of an average request), and a part more to join as 1 / 16 step for every
+    // takes (at the size of an average request), and a part more to join as 1 / 8 step for every
     // workgroup's rows in a round.
-    const int64_t steps = std::max<int64_t>(ceil_div(span, 128), 1);
+    const int64_t steps = std::max<int64_t>(ceil_div(span, 256), 1);
     const int64_t live = std::max<int64_t>(
         std::min(keys * tiles, heads * (ceil_div(tokens * G, kShapeRows[shape]) + n / 2)), 1);
     int64_t splits = 1;
     double least = 0.0;
     for (int64_t s = 1; s <= std::min<int64_t>(steps, kFill); ++s) {
       const double rounds = static_cast<double>(ceil_div(live * s, kFill));
-      const double cost = rounds * (ceil_div(steps, s) + 2) + (s > 1 ? live * s / 16.0 / kFill : 0);
+      const double cost = rounds * (ceil_div(steps, s) + 2) + (s > 1 ? live * s / 8.0 / kFill : 0);
       if (s == 1 || cost < least) {
         least = cost;
         splits = s;
       }
     }
-    const int64_t chunk = ceil_div(steps, splits) * 128;
+    const int64_t chunk = ceil_div(steps, splits) * 256;
     splits = std::max<int64_t>(ceil_div(span, chunk), 1);
     const int64_t units = ceil_div(keys * splits, 8) * 8 * tiles;
     plan.units += units;
