@@ -506,7 +506,7 @@ int origami_append_kv_cache(
  */
 int64_t origami_shared_prefix_attention_workspace(
     int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_dim, int64_t prefix_tokens,
-    int64_t requests, int64_t max_query_tokens, int64_t max_own_tokens);
+    int64_t requests, int64_t max_query_tokens, int64_t max_own_tokens, int64_t cache_dtype);
 int origami_shared_prefix_attention(
     const void* query, int64_t dtype, const int64_t* strides, int64_t tokens,
     int64_t query_heads, const void* kv_cache, int64_t cache_dtype, int64_t cache_layout,

@@ -72,7 +72,7 @@ _SIGNATURES: dict[str, list] = {
     "origami_append_kv_cache": [
         _p, _p, _p, _p, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p,
         _p, _i64, _i64, _i64, _p, _p, _i64, _f64, _f64, _f64, _p],
-    "origami_shared_prefix_attention_workspace": [_i64] * 8,
+    "origami_shared_prefix_attention_workspace": [_i64] * 9,
     "origami_shared_prefix_attention": [
         _p, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p,
         _i64, _i64, _p, _i64, _p, _i64, _i64, _f64, _f64, _f64, _p, _p, _p, _i64, _p],

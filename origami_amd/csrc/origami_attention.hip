@@ -19,12 +19,12 @@ using origami_internal::cache_geometry;
 using origami_internal::check_launch;
 using origami_internal::fail;
 
-// Waves of a workgroup, of which one is on each CU: its tiles fill LDS and registers.  With 256
-// channels results alone take half the registers of a wave, so there are four.
+// Waves of a workgroup.  With 128 channels a workgroup of eight takes a CU's LDS and registers; with
+// 64, two of four do (faster there than one of eight: 19 us against 26 for 24 requests of 12
+// heads), and with 256, where results take half of a wave's registers, one of four.
 template <int DP>
-constexpr int kWaves = DP == 256 ? 4 : 8;
+constexpr int kWaves = DP == 128 ? 8 : 4;
 constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64;
-constexpr int kStep = 32;  // tokens of one product P V (the depth of its matrix instruction)
 // Exponentials are taken 2^kLift times as large for half precision, so that those of tokens far
 // below the maximum keep their precision (down to 2^-24 of the largest) and sums of 2^30 of
 // the largest stay far from binary32's limit.
@@ -36,20 +36,31 @@ template <typename T>
 constexpr float kSlack = std::is_same<T, f16>::value ? 4.0f : 8.0f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-constexpr int64_t kFill = 256;  // workgroups that fill the GPU: one on each CU
-constexpr int kFewParts = 4;
-constexpr int kMaxParts = 512;  // of a row: kFill at most of either kind
+constexpr int64_t kCus = 256;
+constexpr int kFewParts = 8;
+constexpr int kMaxParts = 1024;  // of a row: twice kCus at most of either kind
 
 // Rows of a workgroup.  Waves take 16 or 32 rows; in the larger shapes more of them have rows of
-// their own, in the smaller ones more have tokens of their own.  With 256 channels there are
-// the first two shapes.
+// their own, in the smaller ones more have tokens of their own.  Up to 64 channels there are the
+// first three shapes, up to 128 all, up to 256 the first two.
 constexpr int kShapeRows[4] = {16, 64, 128, 256};
+
+// Division of 0 <= x < 2^31 by a divisor that the host knows: x / d = mulhi(x, mul) >> shift, with
+// mul the ceiling of 2^(32 + shift) / d and 2^shift < d <= 2^(shift + 1) (d = 1: shift -1).
+struct Divisor {
+  uint32_t mul;
+  int32_t d, shift;
+};
+
+__device__ __forceinline__ int divide(int x, const Divisor& by) {
+  return by.shift < 0 ? x : static_cast<int>(__umulhi(x, by.mul) >> by.shift);
+}
 
 // The work of one kind: row tiles of every KV head, over ranges of tokens.
 struct Group {
   int32_t units;   // workgroups
   int32_t shape;   // kShapeRows[shape] rows each, at most
-  int32_t tiles;   // row tiles of a request, or of the batch
+  Divisor tiles;   // row tiles of a request, or of the batch
   int32_t splits;  // ranges of `chunk` tokens
   int32_t chunk;
   int32_t slot;    // the partial results' first slot
@@ -68,13 +79,23 @@ struct AttendParams {
   int64_t num_blocks;
   const int64_t *prefix_ids, *tables, *own_tokens, *starts;
   int64_t table_stride;
-  int32_t block_size, prefix, max_own, max_query;
-  int32_t tokens, requests, Hq, H, G, D;
+  Divisor block_size, requests, H, G;
+  int32_t prefix, max_own, max_query;
+  int32_t tokens, Hq, D;
   float scale, v_scale;  // scale includes log2 e and the keys' scale
   Group group[2];        // the prefix with the whole batch's rows; each request's rows
   int32_t slots;
   float *part_o, *part_ml;  // [slots][rows][D], [slots][rows][2]
 };
+
+// A load that is known to be from memory and not from LDS (whose waits it would share).
+template <typename V>
+__device__ __forceinline__ V load_global(const uint8_t* p) {
+  return *(const __attribute__((address_space(1))) V*)(reinterpret_cast<uintptr_t>(p));
+}
+
+// What a lane reads of a row that is not in the cache, and of channels past the last.
+__device__ const U32x4 kZeros = {0, 0, 0, 0};
 
 // MR x MR scores or results: value x of a lane is in column lane % MR and in row
 // 4 (lane / MR) + x % 4 + (256 / MR) (x / 4).
@@ -134,6 +155,20 @@ __device__ __forceinline__ bool drop_odd(U32x4& w) {
     odd |= l || h;
     w[i] = (l ? 0u : w[i] & 0xffffu) | (h ? 0u : w[i] & 0xffff0000u);
   }
+  return odd;
+}
+// The same for e4m3, whose NaN is all ones but the sign.
+template <typename T>
+__device__ __forceinline__ bool drop_odd(U32x2& w) {
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 32; j += 8)
+      if (((w[i] >> j) & 0x7fu) == 0x7fu) {
+        odd = true;
+        w[i] &= ~(0xffu << j);
+      }
   return odd;
 }
 
@@ -202,7 +237,7 @@ __device__ __forceinline__ int value_piece(int tok, int piece) {
   return piece ^ ((t & (DP == 64 ? 1 : 3)) << 2);
 }
 
-// The values of MR channels (tile d) of 32 tokens' k-th part, as V P takes them: value j is that
+// The values of MR channels (tile d) of a tile's k-th part, as V P takes them: value j is that
 // of token 4 (lane / MR) + j % 4 + (256 / MR) (2 k + j / 4).
 template <typename T, int DP, int MR>
 __device__ __forceinline__ Vec8<T> read_values(const uint8_t* values, int lane, int k, int d) {
@@ -221,9 +256,12 @@ __device__ __forceinline__ Vec8<T> read_values(const uint8_t* values, int lane, 
   return __builtin_bit_cast(Vec8<T>, out);
 }
 
+template <int N>
+using Int = std::integral_constant<int, N>;
+
 // Tokens that a team of waves (the WR waves with the same tokens) has in LDS at a time.
 template <int DP, int WR>
-constexpr int kTeamTokens = WR >= 4 && DP < 256 ? 64 : 32;
+constexpr int kTeamTokens = WR == 8 || (WR == 4 && DP == 64) ? 64 : 32;
 
 // One workgroup: WR MR rows of one KV head over a range of tokens.  Its waves are WR row waves by
 // WT token waves: a wave takes MR rows, and of every WT kTeamTokens tokens its share.  Rows (queries, results, sums) stay in registers; keys and values go
@@ -232,19 +270,19 @@ constexpr int kTeamTokens = WR >= 4 && DP < 256 ? 64 : 32;
 // take turns, so that one barrier a step is enough.
 template <typename T, bool FP8, int DP, int MR, int WR>
 __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, int unit, bool batch,
-                                       uint8_t* lds) {
+                                       uint8_t* lds, float* ml) {
   constexpr int WT = kWaves<DP> / WR, TT = kTeamTokens<DP, WR>;
   constexpr int NG = 64 / MR;             // lane groups: the depth of a product is 8 NG
   constexpr int KS = DP / (8 * NG);       // depth steps of K Q
   constexpr int DT = DP / MR;             // channel tiles of V P
-  constexpr int X = MR / 2;               // scores of a lane in 32 tokens
-  constexpr int ST = TT / kStep;          // steps of 32 tokens
+  constexpr int X = TT / NG;              // scores of a lane in a tile
   constexpr int ACC = MR * MR / 64;       // values of a lane in a tile
   constexpr int STRIDE = 4 * NG;          // tokens between a lane's groups of four
   constexpr int NCH = DP / 8;             // 16-byte pieces of a row in LDS
   constexpr int RPI = 64 / NCH;           // rows of one load
   constexpr int IT = TT / (RPI * WR);     // loads of a tile
-  constexpr int kBuffers = WR == 1 ? 1 : 2;
+  constexpr bool kAhead = WR == 8;        // scores are a step ahead: see below
+  constexpr int kBuffers = WR == 1 ? 1 : (kAhead ? 3 : 2);
   constexpr int kTile = TT * DP * 2;      // bytes of a team's keys
   // one value for the wave, so that what follows from it is scalar and its conditions are branches
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -253,38 +291,50 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
 
   // The unit: row tiles of the same keys are 8 units apart, so that they run on the same chiplet
   // at about the same time and its L2 gives the keys to all but the first.
-  int u = unit;
-  const int eighth = u & 7;
-  u >>= 3;
-  const int tile = u % g.tiles;
-  u = (u / g.tiles) * 8 + eighth;
-  const int h = u % p.H;
-  u /= p.H;
-  int r = 0;
-  Request rq{0, p.tokens, 0};
+  const int eight = unit >> 3, eighth = unit & 7;
+  int u = divide(eight, g.tiles);
+  const int tile = eight - u * g.tiles.d;
+  u = u * 8 + eighth;
+  const int uh = divide(u, p.H), h = u - uh * p.H.d;
+  int r = 0, split = uh;
   if (!batch) {
-    r = u % p.requests;
-    u /= p.requests;
-    rq = request_of(p, r);
+    split = divide(uh, p.requests);
+    r = uh - split * p.requests.d;
   }
-  const int split = u;
-  const int rows = rq.count * p.G, row0 = tile * WR * MR;
-  if (split >= g.splits || row0 >= rows) return;
-  const int end = batch ? p.prefix : p.prefix + rq.own;  // of the tokens, prefix first
+  if (split >= g.splits) return;
+  const int t0 = g.first + split * g.chunk;
   const int64_t* const table = p.tables + static_cast<int64_t>(r) * p.table_stride;
+  // The block of token t.  Blocks of the first tokens are asked for before the request's length is
+  // known: up to the bounds that the host has, the tables can be read.
+  const int bound = batch ? p.prefix : p.prefix + p.max_own;
+  const auto block_of = [&](int t, int before) -> int64_t {
+    if (t >= before) return -1;
+    const bool pre = t < p.prefix;
+    return (pre ? p.prefix_ids : table)[divide(pre ? t : t - p.prefix, p.block_size)];
+  };
+  constexpr int kRound = WT * TT;  // tokens of a step of the workgroup
+  const int tl = lane % TT;
+  int t = t0 + wt * TT;  // the first of this wave's tokens
+  const int64_t first = block_of(t + tl, bound);
+  int64_t ahead = block_of(t + kRound + tl, bound);
+
+  const Request rq = batch ? Request{0, p.tokens, 0} : request_of(p, r);
+  const int rows = rq.count * p.G.d, row0 = tile * WR * MR;
+  if (row0 >= rows) return;
+  const int end = batch ? p.prefix : p.prefix + rq.own;  // of the tokens, prefix first
 
   // this lane's row
   const int row = row0 + wr * MR + c;
   const auto seen_by = [&](int i) -> int {  // tokens that row i sees
-    return batch ? p.prefix : p.prefix + min(max(rq.own - rq.count + i / p.G + 1, 0), rq.own);
+    return batch ? p.prefix : p.prefix + min(max(rq.own - rq.count + divide(i, p.G) + 1, 0), rq.own);
   };
   const int limit = seen_by(row);
   // the scale's sign goes with the queries, and so does a scale of zero, so that hidden scores of
   // -infinity stay what they are
   const float scale = p.scale == 0.0f ? 1.0f : fabsf(p.scale);
-  const int qi = row / p.G, head = h * p.G + row - qi * p.G;
   Vec8<T> qf[KS];
   {
+    const int qi = divide(row, p.G), head = h * p.G.d + row - qi * p.G.d;
     const T* const src =
         static_cast<const T*>(p.query) + (rq.first + qi) * p.q_token + head * p.q_head;
     const bool vec =
@@ -309,7 +359,6 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
   const int most = seen_by(min(row0 + WR * MR, rows) - 1);
   const int least = seen_by(min(row0 + wr * MR, rows - 1));
   const int nearest = seen_by(row0);  // the tokens that all rows of the workgroup see
-  const int t0 = g.first + split * g.chunk;
   const int t1 = min(min(end, most), t0 + g.chunk);
 
   Tile<MR> o[DT];
@@ -321,42 +370,42 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
 
   uint8_t* const team = lds + wt * kBuffers * 2 * kTile;
   const int piece = lane % NCH, sub = lane / NCH;
-  const bool has = 8 * piece < p.D, exact = p.D == DP;
+  const bool has = 8 * piece < p.D;
   constexpr int cell = FP8 ? 1 : 2;
-  const int64_t pitch = static_cast<int64_t>(p.H) * p.D * cell;
+  const int64_t pitch = static_cast<int64_t>(p.H.d) * p.D * cell;
   const uint8_t* const keys =
       p.cache + (static_cast<int64_t>(h) * p.D + (has ? 8 * piece : 0)) * cell;
-  const uint8_t* const values = keys + p.half_stride * pitch;
+  const int64_t to_values = p.half_stride * pitch;
 
-  // the block of token t, and its cache row, -1 where it has none
-  const auto block_of = [&](int t) -> int64_t {
-    if (t >= t1) return -1;
-    const bool pre = t < p.prefix;
-    const int i = pre ? t : t - p.prefix;
-    return (pre ? p.prefix_ids : table)[i / p.block_size];
-  };
+  // the cache row of token t, -1 where it has none
   const auto row_of = [&](int t, int64_t id) -> int {
-    if (id < 0 || id >= p.num_blocks) return -1;
+    if (t >= t1 || id < 0 || id >= p.num_blocks) return -1;
     const int i = t < p.prefix ? t : t - p.prefix;
-    return static_cast<int>(id * p.blk_stride + i % p.block_size);
+    return static_cast<int>(id * p.blk_stride + i - divide(i, p.block_size) * p.block_size.d);
   };
   using Raw = typename std::conditional<FP8, U32x2, U32x4>::type;
   Raw kr[IT], vr[IT];
   const auto load_tile = [&](int mine) {
+    const uint8_t* const zeros = reinterpret_cast<const uint8_t*>(&kZeros);
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      // rows that are not there are read from the cache's first (and made zero below)
-      const int64_t at_row = max(__shfl(mine, (i * WR + wr) * RPI + sub), 0) * pitch;
-      kr[i] = *reinterpret_cast<const Raw*>(keys + at_row);
-      vr[i] = *reinterpret_cast<const Raw*>(values + at_row);
+      const int r = __shfl(mine, (i * WR + wr) * RPI + sub);
+      const bool in = r >= 0 && has;
+      const uint8_t* const src = keys + r * pitch;
+      kr[i] = load_global<Raw>(in ? src : zeros);
+      vr[i] = load_global<Raw>(in ? src + to_values : zeros);
     }
   };
-  // `partly`: some rows may not see some of the tokens.  A hidden token's weight is 0, but 0
-  // times an infinity or NaN is NaN: such values go in as 0, and reach the rows that see them
-  // at the end.
+  // Where some rows may not see some of a tile's tokens: a hidden token's weight is 0, but 0 times
+  // an infinity or NaN is NaN.  Such values go in as 0, and reach the rows that see them at the
+  // end.
   bool odd = false;
-  const auto store_tile = [&](uint8_t* buf, uint64_t there, bool partly) {
-    const bool all = exact && there == ~0ull;
+  const auto drop_odd_values = [&](int t) {
+    if (t + TT > nearest)
+#pragma unroll
+      for (int i = 0; i < IT; ++i) odd |= drop_odd<T>(vr[i]);
+  };
+  const auto store_tile = [&](uint8_t* buf) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int tok = (i * WR + wr) * RPI + sub;
@@ -368,223 +417,295 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
         kv = kr[i];
         vv = vr[i];
       }
-      if (partly) odd |= drop_odd<T>(vv);
-      if (!all && !(has && ((there >> tok) & 1))) kv = vv = U32x4{0, 0, 0, 0};
       *reinterpret_cast<U32x4*>(buf + (tok * NCH + key_piece<DP>(tok, piece)) * 16) = kv;
       *reinterpret_cast<U32x4*>(buf + kTile + (tok * NCH + value_piece<DP, MR>(tok, piece)) * 16) =
           vv;
     }
   };
 
-  constexpr int kRound = WT * TT;  // tokens of a step of the workgroup
-  const int tl = lane % TT;
-  int t = t0 + wt * TT;  // the first of this wave's tokens
-  int mine = row_of(t + tl, block_of(t + tl));
-  if (t0 < t1) load_tile(mine);
-  int64_t ahead = block_of(t + kRound + tl);
-  int turn = 0;
-  // with a barrier in it, the loop is the same for all waves
-  for (int tb = t0; (WR == 1 ? t : tb) < t1; tb += kRound, t += kRound) {
-    uint8_t* const buf = team + turn * 2 * kTile;
-    const uint64_t there = __ballot(mine >= 0);  // twice 32 tokens where TT is 32
-    store_tile(buf, there, t + TT > nearest);
-    if constexpr (WR == 1)
-      __builtin_amdgcn_wave_barrier();
-    else
-      __syncthreads();
+  // With one buffer a wave's tile goes to LDS before its products, and the next one is on its way
+  // to registers.  With two, the next tile goes to LDS in the middle of a tile's products, and
+  // the one after it is on its way.
+  int mine = row_of(t + tl, first), turn = 0;
+  uint64_t there = __ballot(mine >= 0), next_there = 0;  // twice 32 tokens where TT is 32
+  if (t0 < t1) {
+    load_tile(mine);
     mine = row_of(t + kRound + tl, ahead);
-    ahead = block_of(t + 2 * kRound + tl);
-    if ((WR == 1 ? t : tb) + kRound < t1) load_tile(mine);
-
-    const bool whole = there == ~0ull && t + TT <= least;
-#pragma unroll 1
-    for (int s = 0; s < ST; ++s) {
-      const uint8_t* const kb = buf + s * kStep * NCH * 16;
-      const uint8_t* const vb = kb + kTile;
-      const int ts = t + s * kStep;  // the step's first token
-      // S = K Q: row c against token STRIDE (i / 4) + 4 q4 + i % 4
-      Tile<MR> sc[X / ACC];
-#pragma unroll
-      for (int m = 0; m < X / ACC; ++m) {
-#pragma unroll
-        for (int x = 0; x < ACC; ++x) sc[m][x] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const int tok = MR * m + c;
-          const Vec8<T> kf = *reinterpret_cast<const Vec8<T>*>(
-              kb + (tok * NCH + key_piece<DP>(tok, NG * k + q4)) * 16);
-          sc[m] = mfma<T, MR>(kf, qf[k], sc[m]);
-        }
-      }
-      if (!whole) {
-        const uint32_t seen = static_cast<uint32_t>(there >> (kStep * s));
-#pragma unroll
-        for (int i = 0; i < X; ++i) {
-          const int tok = STRIDE * (i / 4) + 4 * q4 + i % 4;
-          if (ts + tok >= limit || !((seen >> tok) & 1)) sc[i / ACC][i % ACC] = -INFINITY;
-        }
-      }
-      float best = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < X; ++i) best = fmaxf(best, sc[i / ACC][i % ACC]);
-      best = max_over_groups<MR>(best) * scale;
-      const bool rises = best > base + kSlack<T>;
-      if (__any(rises)) {  // each row by itself: no row's rounding depends on another
-        const float next = rises ? best : base;
-        const float keep = __builtin_amdgcn_exp2f(base - (next == -INFINITY ? 0.0f : next));
-        base = next;
-        sum *= keep;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] *= keep;
-      }
-      const float below = kLift<T> - (base == -INFINITY ? 0.0f : base);
-      Vec8<T> pf[X / 8];
-#pragma unroll
-      for (int i = 0; i < X; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(sc[i / ACC][i % ACC], scale, below));
-        sum += e;
-        pf[i / 8][i % 8] = static_cast<T>(e);
-      }
-      // O += V P
-#pragma unroll
-      for (int k = 0; k < X / 8; ++k)
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-          o[d] = mfma<T, MR>(read_values<T, DP, MR>(vb, lane, k, d), pf[k], o[d]);
+    ahead = block_of(t + 2 * kRound + tl, t1);
+    if constexpr (kBuffers > 1) {
+      drop_odd_values(t);
+      store_tile(team);
+      load_tile(mine);
+      next_there = __ballot(mine >= 0);
+      mine = row_of(t + 2 * kRound + tl, ahead);
+      ahead = block_of(t + 3 * kRound + tl, t1);
+      __syncthreads();
     }
-    if constexpr (WR == 1)
-      __builtin_amdgcn_wave_barrier();
-    else
-      turn ^= 1;
+  }
+  // A step: the maxima and sums with `count` scores a lane of the tokens from `ts` on, with the
+  // instructions of `between` among those of the exponentials; then O += V P.
+  const auto soften = [&](auto& sc, auto count, int ts, uint64_t seen, bool whole, auto between,
+                          const uint8_t* vb) {
+    constexpr int N = decltype(count)::value;
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int tok = STRIDE * (i / 4) + 4 * q4 + i % 4;
+        if (ts + tok >= limit || !((seen >> tok) & 1)) sc[i / ACC][i % ACC] = -INFINITY;
+      }
+    }
+    float best = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) best = fmaxf(best, sc[i / ACC][i % ACC]);
+    best = max_over_groups<MR>(best) * scale;
+    const bool rises = best > base + kSlack<T>;
+    if (__any(rises)) {  // each row by itself: no row's rounding depends on another
+      const float next = rises ? best : base;
+      const float keep = __builtin_amdgcn_exp2f(base - (next == -INFINITY ? 0.0f : next));
+      base = next;
+      sum *= keep;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= keep;
+    }
+    between();
+    const float below = kLift<T> - (base == -INFINITY ? 0.0f : base);
+    Vec8<T> pf[N / 8];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float e = __builtin_amdgcn_exp2f(fmaf(sc[i / ACC][i % ACC], scale, below));
+      sum += e;
+      pf[i / 8][i % 8] = static_cast<T>(e);
+    }
+    // O += V P
+#pragma unroll
+    for (int k = 0; k < N / 8; ++k)
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        o[d] = mfma<T, MR>(read_values<T, DP, MR>(vb, lane, k, d), pf[k], o[d]);
+  };
+  // S = K Q: row c against token STRIDE (i / 4) + 4 q4 + i % 4, all tiles of 16 or 32 tokens
+  // together, so that no product waits for the one before it
+  const auto score = [&](auto& sc, auto tiles, const uint8_t* kb) {
+    constexpr int N = decltype(tiles)::value;
+#pragma unroll
+    for (int m = 0; m < N; ++m)
+#pragma unroll
+      for (int x = 0; x < ACC; ++x) sc[m][x] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int m = 0; m < N; ++m) {
+        const int tok = MR * m + c;
+        const Vec8<T> kf = *reinterpret_cast<const Vec8<T>*>(
+            kb + (tok * NCH + key_piece<DP>(tok, NG * k + q4)) * 16);
+        sc[m] = mfma<T, MR>(kf, qf[k], sc[m]);
+      }
+  };
+  // with a barrier in it, the loop is the same for all waves
+  if constexpr (kAhead) {
+    // A tile is two steps, and the products K Q of a step run under the exponentials of the one
+    // before: the vector unit has as much to do for a step as the matrix unit.  The first step of
+    // the next tile comes before the last one's values are done with, hence three buffers.
+    static_assert(TT == 64 && MR == 32 && WT == 1, "two steps of 32 tokens");
+    constexpr int kHalf = TT / 2 * DP * 2;  // bytes of a step's keys
+    Tile<MR> sa[1], sb[1];
+    int next = 1;
+    if (t0 < t1) score(sa, Int<1>{}, team);
+    for (; t < t1; t += kRound) {
+      uint8_t* const buf = team + turn * 2 * kTile;
+      uint8_t* const other = team + next * 2 * kTile;
+      const bool whole = there == ~0ull && t + TT <= least;
+      drop_odd_values(t + kRound);
+      soften(sa, Int<X / 2>{}, t, there, whole, [&] { score(sb, Int<1>{}, buf + kHalf); },
+             buf + kTile);
+      store_tile(other);
+      load_tile(mine);
+      __syncthreads();
+      soften(sb, Int<X / 2>{}, t + TT / 2, there >> 32, whole,
+             [&] { score(sa, Int<1>{}, other); }, buf + kTile + kHalf);
+      there = next_there;
+      next_there = __ballot(mine >= 0);
+      mine = row_of(t + 3 * kRound + tl, ahead);
+      ahead = block_of(min(t + 4 * kRound + tl, t1 - 1), t1);
+      turn = next;
+      next = next == 2 ? 0 : next + 1;
+    }
+  } else {
+    for (int tb = t0; (WR == 1 ? t : tb) < t1; tb += kRound, t += kRound) {
+      uint8_t* const buf = team + turn * 2 * kTile;
+      if constexpr (kBuffers == 1) {
+        drop_odd_values(t);
+        store_tile(buf);
+        __builtin_amdgcn_wave_barrier();
+        load_tile(mine);
+        next_there = __ballot(mine >= 0);
+        mine = row_of(t + 2 * kRound + tl, ahead);
+        ahead = block_of(min(t + 3 * kRound + tl, t1 - 1), t1);
+      } else {
+        drop_odd_values(t + kRound);
+      }
+      const bool whole = there == ~0ull && t + TT <= least;
+      Tile<MR> sc[X / ACC];
+      score(sc, Int<X / ACC>{}, buf);
+      if constexpr (kBuffers == 2) {
+        store_tile(team + (turn ^ 1) * 2 * kTile);
+        load_tile(mine);
+      }
+      soften(sc, Int<X>{}, t, there, whole, [] {}, buf + kTile);
+      there = next_there;
+      if constexpr (kBuffers == 1) {
+        __builtin_amdgcn_wave_barrier();
+      } else {
+        next_there = __ballot(mine >= 0);
+        mine = row_of(t + 3 * kRound + tl, ahead);
+        ahead = block_of(min(t + 4 * kRound + tl, t1 - 1), t1);
+        __syncthreads();
+        turn ^= 1;
+      }
+    }
   }
 
 #pragma unroll
   for (int x = MR; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
   if (t1 > nearest) odd = __syncthreads_or(odd);
+
+  // The infinities and NaN that drop_odd_values left out, for four channels of a row that sees
+  // them.  Tokens before theirs have been added already, and an infinity or NaN twice is the same.
+  const auto odd_values = [&](int ch, int before) -> Float4 {
+    Float4 out = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = max(t0, nearest - TT); i < min(t1, before); ++i) {
+      const int at_row = row_of(i, block_of(i, t1));
+      if (at_row < 0) continue;
+      const Float4 v = four_values<T, FP8>(
+          p.cache + (at_row + p.half_stride) * pitch + static_cast<int64_t>(h) * p.D * cell, ch);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[j] += fabsf(v[j]) < INFINITY ? 0.0f : v[j];
+    }
+    return out;
+  };
+  // Four channels of a row's result, and with the first ones its maximum and sum.
+  const auto put = [&](int row, int ch, Float4 v, float base, float sum) {
+    if (row >= rows || ch >= p.D) return;
+    const int qi = divide(row, p.G), head = h * p.G.d + row - qi * p.G.d;
+    const int64_t n = rq.first + qi, at = n * p.Hq + head;
+    if (odd) v += odd_values(ch, seen_by(row));
+    if (p.slots > 1) {
+      const int64_t slot =
+          (g.slot + split) * (static_cast<int64_t>(p.tokens) * p.Hq) + at;
+      if (ch == 0) {
+        p.part_ml[2 * slot] = base - kLift<T>;
+        p.part_ml[2 * slot + 1] = sum;
+      }
+      // without a token the join does not read the rest
+      if (sum != 0.0f) *reinterpret_cast<Float4*>(p.part_o + slot * p.D + ch) = v;
+    } else {
+      const float inv = sum == 0.0f ? 0.0f : p.v_scale / sum;
+      store4(static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + ch, v * inv, p.out_vec);
+      if (p.lse && ch == 0)
+        p.lse[at] = sum == 0.0f ? -INFINITY : kLn2 * (base - kLift<T> + log2f(sum));
+    }
+  };
+
   if constexpr (WT > 1) {
-    // join the token waves: the largest maximum, then the weighted sums, half of the waves
-    // adding the other half's, until the first ones have them
-    constexpr int M = WR * MR, kPitch = DP + 4;
-    static_assert((WT * M * 2 + WT / 2 * M * kPitch) * 4 <= 128 * DP * kWaves<DP>, "LDS");
-    __syncthreads();
-    float* const ml = reinterpret_cast<float*>(lds);  // [WT][M][2]
-    float* const ol = ml + WT * M * 2;                // [WT / 2][M][kPitch]
+    // Join the token waves through LDS.  With one row wave each leaves its part in its own tiles,
+    // which no other wave reads, and all waves add up a share of the rows; else all but the
+    // first token wave leave theirs, which that one adds to its own.
+    constexpr int M = WR * MR, kPitch = DP + 4, kPart = WR == 1 ? 2 * kTile : M * kPitch * 4;
+    static_assert((WR > 1 || MR * kPitch * 4 <= 2 * kTile) &&
+                      (WT - 1) * kPart <= 128 * DP * kWaves<DP>, "LDS");
+    if constexpr (WR > 1) __syncthreads();
     const int mr = wr * MR + c;
-    if (q4 == 0) {
-      ml[(wt * M + mr) * 2] = base;
-      ml[(wt * M + mr) * 2 + 1] = sum;
+    const auto part_row = [&](int w, int r) {
+      return reinterpret_cast<float*>(lds + (WR == 1 ? w : w - 1) * kPart) + r * kPitch;
+    };
+    if (WR == 1 || wt != 0) {
+      if (q4 == 0) {
+        ml[(wt * M + mr) * 2] = base;
+        ml[(wt * M + mr) * 2 + 1] = sum;
+      }
+      float* const dst = part_row(wt, mr) + 4 * q4;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int x = 0; x < ACC; x += 4)
+          *reinterpret_cast<Float4*>(dst + MR * d + 256 / MR * (x / 4)) =
+              Float4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]};
     }
     __syncthreads();
-    const float mine_base = base;
+    if constexpr (WR == 1) {
+      for (int i = threadIdx.x; i < M * (DP / 4); i += 64 * kWaves<DP>) {
+        const int r = i / (DP / 4), ch = 4 * (i % (DP / 4));
+        float most = -INFINITY, total = 0.0f;
 #pragma unroll
-    for (int w = 0; w < WT; ++w) base = fmaxf(base, ml[(w * M + mr) * 2]);
-    const float zero = base == -INFINITY ? 0.0f : base;
-    sum = 0.0f;
+        for (int w = 0; w < WT; ++w) most = fmaxf(most, ml[(w * M + r) * 2]);
+        const float zero = most == -INFINITY ? 0.0f : most;
+        Float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 0; w < WT; ++w)
-      sum += ml[(w * M + mr) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * M + mr) * 2] - zero);
-    const float weight = __builtin_amdgcn_exp2f(mine_base - zero);
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[d] *= weight;
-#pragma unroll 1
-    for (int half = WT / 2; half > 0; half /= 2) {
-      float* const rowl = ol + ((wt % half) * M + mr) * kPitch + 4 * q4;
-      if (wt >= half && wt < 2 * half)
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int x = 0; x < ACC; x += 4)
-            *reinterpret_cast<Float4*>(rowl + MR * d + 256 / MR * (x / 4)) =
-                Float4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]};
-      __syncthreads();
-      if (wt < half)
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int x = 0; x < ACC; x += 4) {
-            const Float4 v = *reinterpret_cast<const Float4*>(rowl + MR * d + 256 / MR * (x / 4));
-            o[d][x] += v[0];
-            o[d][x + 1] += v[1];
-            o[d][x + 2] += v[2];
-            o[d][x + 3] += v[3];
-          }
-      if (half > 1) __syncthreads();
+        for (int w = 0; w < WT; ++w) {
+          const float weight = __builtin_amdgcn_exp2f(ml[(w * M + r) * 2] - zero);
+          total += ml[(w * M + r) * 2 + 1] * weight;
+          v += *reinterpret_cast<const Float4*>(part_row(w, r) + ch) * weight;
+        }
+        put(row0 + r, ch, v, most, total);
+      }
+      return;
     }
     if (wt != 0) return;
-  }
-  if (odd) {
-    // the values that store_tile left out, to the rows that see them; those of the tokens
-    // before them were added already, and an infinity or NaN twice is the same
-    for (int i = max(t0, nearest - TT); i < min(t1, limit); ++i) {
-      const int at_row = row_of(i, block_of(i));
-      if (at_row < 0) continue;
-      const uint8_t* const src =
-          p.cache + (at_row + p.half_stride) * pitch + static_cast<int64_t>(h) * p.D * cell;
+    const float mine_base = base;
+#pragma unroll
+    for (int w = 1; w < WT; ++w) base = fmaxf(base, ml[(w * M + mr) * 2]);
+    const float zero = base == -INFINITY ? 0.0f : base;
+    const float own_weight = __builtin_amdgcn_exp2f(mine_base - zero);
+    sum *= own_weight;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[d] *= own_weight;
+#pragma unroll 1
+    for (int w = 1; w < WT; ++w) {
+      const float weight = __builtin_amdgcn_exp2f(ml[(w * M + mr) * 2] - zero);
+      sum += ml[(w * M + mr) * 2 + 1] * weight;
+      const float* const src = part_row(w, mr) + 4 * q4;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int x = 0; x < ACC; x += 4) {
-          const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
-          const Float4 v = four_values<T, FP8>(src, min(ch, p.D - 4));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[d][x + j] += fabsf(v[j]) < INFINITY ? 0.0f : v[j];
+          const Float4 v = *reinterpret_cast<const Float4*>(src + MR * d + 256 / MR * (x / 4));
+          o[d][x] += v[0] * weight;
+          o[d][x + 1] += v[1] * weight;
+          o[d][x + 2] += v[2] * weight;
+          o[d][x + 3] += v[3] * weight;
         }
     }
   }
-  if (row >= rows) return;
-  const int64_t n = rq.first + qi, at = n * p.Hq + head;
-  if (p.slots > 1) {
-    const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
-    const int64_t slot = (g.slot + split) * all + at;
-    if (q4 == 0) {
-      p.part_ml[2 * slot] = base - kLift<T>;
-      p.part_ml[2 * slot + 1] = sum;
-    }
-    if (sum == 0.0f) return;  // no token: the join does not read the rest
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int x = 0; x < ACC; x += 4) {
-        const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
-        if (ch < p.D)
-          *reinterpret_cast<Float4*>(p.part_o + slot * p.D + ch) =
-              Float4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]};
-      }
-    return;
-  }
-  const float inv = sum == 0.0f ? 0.0f : p.v_scale / sum;
-  T* const dst = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head;
+  int again = row;  // where the row is, anew: there are no registers to keep it through the loop
+  asm volatile("" : "+v"(again));
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int x = 0; x < ACC; x += 4) {
-      const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
-      if (ch < p.D)
-        store4(dst + ch, Float4{o[d][x] * inv, o[d][x + 1] * inv, o[d][x + 2] * inv,
-                                o[d][x + 3] * inv}, p.out_vec);
-    }
-  if (p.lse && q4 == 0)
-    p.lse[at] = sum == 0.0f ? -INFINITY : kLn2 * (base - kLift<T> + log2f(sum));
+    for (int x = 0; x < ACC; x += 4)
+      put(again, MR * d + 4 * q4 + 256 / MR * (x / 4),
+          Float4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]}, base, sum);
 }
 
 template <typename T, bool FP8, int DP, int SHAPE>
 __device__ __forceinline__ void attend_shape(const AttendParams& p, int kind, int unit,
-                                             uint8_t* lds) {
+                                             uint8_t* lds, float* ml) {
   constexpr int MR = SHAPE == 0 || DP == 256 ? 16 : 32;
-  attend<T, FP8, DP, MR, kShapeRows[SHAPE] / MR>(p, p.group[kind], unit, kind == 0, lds);
+  attend<T, FP8, DP, MR, kShapeRows[SHAPE] / MR>(p, p.group[kind], unit, kind == 0, lds,
+                                                       ml);
 }
 
 // The prefix in workgroups of shape S0 and the requests in those of S1, in one launch.
 template <typename T, bool FP8, int DP, int S0, int S1>
-__global__ __launch_bounds__(64 * kWaves<DP>) void attend_kernel(AttendParams p) {
+__global__ __launch_bounds__(64 * kWaves<DP>, DP == 256 ? 1 : 2) void attend_kernel(AttendParams p) {
   __shared__ alignas(16) uint8_t lds[128 * DP * kWaves<DP>];  // of every shape
+  __shared__ float ml[512];  // maxima and sums of the token waves' rows
   int unit = static_cast<int>(blockIdx.x);
   const int kind = unit >= p.group[0].units;
   unit -= kind ? p.group[0].units : 0;
   if (S0 == S1 || kind == 1)
-    attend_shape<T, FP8, DP, S1>(p, kind, unit, lds);
+    attend_shape<T, FP8, DP, S1>(p, kind, unit, lds, ml);
   else
-    attend_shape<T, FP8, DP, S0>(p, 0, unit, lds);
+    attend_shape<T, FP8, DP, S0>(p, 0, unit, lds, ml);
 }
 
 // Joins the parts of each row: out = v_scale sum_s w_s O_s / sum_s w_s l_s with
@@ -596,7 +717,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams p, 
   const int ch = 4 * (threadIdx.x % lanes);
   if (row >= all || ch >= p.D) return;
   const int64_t n = row / p.Hq, head = row - n * p.Hq;
-  if (p.starts && (n < p.starts[0] || n >= p.starts[p.requests])) return;
+  if (p.starts && (n < p.starts[0] || n >= p.starts[p.requests.d])) return;
   float m[kFewParts], l[kFewParts], best = -INFINITY, total = 0.0f;
 #pragma unroll
   for (int s = 0; s < kFewParts; ++s) {
@@ -635,7 +756,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendParams p, int 
   const int team = threadIdx.x / lanes, teams = kJoinThreads / lanes;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int64_t n = row / p.Hq, head = row - n * p.Hq;
-  if (p.starts && (n < p.starts[0] || n >= p.starts[p.requests])) return;
+  if (p.starts && (n < p.starts[0] || n >= p.starts[p.requests.d])) return;
 
   constexpr int kEach = kMaxParts / kJoinThreads;
   float m[kEach], l[kEach], best = -INFINITY;
@@ -717,14 +838,16 @@ int launch_units(const AttendParams& p, hipStream_t stream) {
     hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 1, 0>), grid, block, 0, stream, p);
   else if (s0 == 1)
     hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 1, 1>), grid, block, 0, stream, p);
-  if constexpr (DP < 256) {
+  if constexpr (DP <= 128) {
     if (s0 == 2 && s1 == 0)
       hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 2, 0>), grid, block, 0, stream, p);
     else if (s0 == 2 && s1 == 1)
       hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 2, 1>), grid, block, 0, stream, p);
     else if (s0 == 2)
       hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 2, 2>), grid, block, 0, stream, p);
-    else if (s0 == 3 && s1 == 0)
+  }
+  if constexpr (DP == 128) {
+    if (s0 == 3 && s1 == 0)
       hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 3, 0>), grid, block, 0, stream, p);
     else if (s0 == 3 && s1 == 1)
       hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 3, 1>), grid, block, 0, stream, p);
@@ -751,7 +874,7 @@ int launch_attend(const AttendParams& p, hipStream_t stream) {
     hipLaunchKernelGGL(join_few_kernel<T>, joins, block, 0, stream, p, lanes);
   } else {
     // with few rows, workgroups of 32 channels, so that the GPU has enough of them
-    const int some = rows < 2 * kFill ? 8 : lanes;
+    const int some = rows < 2 * kCus ? 8 : lanes;
     const int blocks = (p.D + 4 * some - 1) / (4 * some);
     const dim3 joins(static_cast<unsigned>(rows * blocks));
     hipLaunchKernelGGL(join_kernel<T>, joins, block, 0, stream, p, some, blocks);
@@ -761,58 +884,112 @@ int launch_attend(const AttendParams& p, hipStream_t stream) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+Divisor divisor(int64_t d) {
+  int shift = -1;
+  while ((int64_t(1) << (shift + 1)) < d) ++shift;
+  const uint64_t mul = d == 1 ? 0 : ((uint64_t(1) << (32 + shift)) + d - 1) / d;
+  return Divisor{static_cast<uint32_t>(mul), static_cast<int32_t>(d), shift};
+}
+
 // The split of a call into units, from sizes that the host has.
 struct Plan {
-  Group shared, each;
+  Group group[2];
   int64_t slots, units;
 };
 
+// Units of one kind, before they are split: `count` of them, `live` with rows if the requests are
+// of one size, over `span` tokens; microseconds of a unit's start and end, and of a token.
+struct Kind {
+  int shape = 0;
+  int64_t tiles = 0, count = 0, live = 0, span = 0, fill = kCus;
+  double token = 0.0;
+
+  int64_t chunk(int64_t splits) const { return ceil_div(ceil_div(span, splits), 64) * 64; }
+  int64_t splits(int64_t wanted) const {
+    const int64_t most = std::min<int64_t>(std::max<int64_t>(span / 128, 1), 2 * kCus);
+    const int64_t s = std::min(std::max<int64_t>(wanted, 1), most);
+    return span > 0 ? ceil_div(span, chunk(s)) : 1;
+  }
+};
+
+// Measured on MI355X: what a workgroup takes besides its tokens, bytes and operations of one
+// CU in a microsecond while all of them work.
+constexpr double kUnitTime = 6.0, kCuBytes = 20e3, kCuFlops = 3.2e6;
+
+// Microseconds of a call whose kinds are split in s0 and s1 ranges: workgroups of the first kind go
+// to the CUs in order, then those of the second; and joining the parts of `rows` rows.
+double call_time(const Kind& k0, int64_t s0, const Kind& k1, int64_t s1, int64_t rows,
+                 int64_t head_dim) {
+  const int64_t n0 = k0.live * s0, n1 = k1.live * s1;
+  const double t0 = n0 ? kUnitTime + k0.token * k0.chunk(s0) : 0.0;
+  const double t1 = kUnitTime + k1.token * k1.chunk(s1);
+  const int64_t full = n0 / k1.fill, rest = n0 % k1.fill, early = k1.fill - rest;
+  double end = (rest ? full + 1 : full) * t0;
+  const int64_t beside = rest ? early * static_cast<int64_t>(t0 / t1) : 0;
+  if (rest && n1 <= early)
+    end = std::max(end, full * t0 + t1);
+  else if (n1 > beside)
+    end += ceil_div(n1 - beside, k1.fill) * t1;
+  const int64_t slots = s1 + (n0 ? s0 : 0);
+  return end + (slots > 1 ? 4.0 + slots * rows * head_dim * 8 / (kCus * kCuBytes) : 0.0);
+}
+
 Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_dim,
-             int64_t prefix, int64_t requests, int64_t max_query, int64_t max_own) {
-  Plan plan{};
-  const int64_t G = query_heads / heads;
-  const int last = head_dim > 128 ? 1 : 3;
+             int64_t prefix, int64_t requests, int64_t max_query, int64_t max_own, int64_t cell) {
+  const int64_t G = query_heads / heads, last = head_dim <= 64 ? 2 : (head_dim <= 128 ? 3 : 1);
+  const int64_t fill = head_dim <= 64 ? 2 * kCus : kCus;  // workgroups that the CUs hold
   // A request whose rows fill workgroups by themselves reads the prefix with its own tokens.
   const bool apart = requests > 1 && prefix > 0 && max_query * G < kShapeRows[last];
-  int64_t slot = 0;  // of the partial results
-  const auto fill = [&](Group& g, int64_t n, int64_t rows, int64_t first, int64_t span) {
-    int shape = 0;
-    while (shape < last && rows > kShapeRows[shape]) ++shape;
-    const int64_t tiles = std::max<int64_t>(ceil_div(rows, kShapeRows[shape]), 1);
-    const int64_t keys = std::max<int64_t>(n * heads, 1);
-    // Ranges of 256 tokens or more.  A workgroup's time is taken as its steps of 256 tokens and two
-    // more for its start and end, that of the call as the rounds of workgroups that the GPU
-    // takes (at the size of an average request), and a part more to join as 1 / 8 step for every
-    // workgroup's rows in a round.
-    const int64_t steps = std::max<int64_t>(ceil_div(span, 256), 1);
-    const int64_t live = std::max<int64_t>(
-        std::min(keys * tiles, heads * (ceil_div(tokens * G, kShapeRows[shape]) + n / 2)), 1);
-    int64_t splits = 1;
-    double least = 0.0;
-    for (int64_t s = 1; s <= std::min<int64_t>(steps, kFill); ++s) {
-      const double rounds = static_cast<double>(ceil_div(live * s, kFill));
-      const double cost = rounds * (ceil_div(steps, s) + 2) + (s > 1 ? live * s / 8.0 / kFill : 0);
-      if (s == 1 || cost < least) {
-        least = cost;
-        splits = s;
+  const auto kind_of = [&](int64_t n, int64_t rows, int64_t all_rows, int64_t span) {
+    Kind k;
+    while (k.shape < last && rows > kShapeRows[k.shape]) ++k.shape;
+    const int64_t unit_rows = kShapeRows[k.shape];
+    k.tiles = std::max<int64_t>(ceil_div(rows, unit_rows), 1);
+    k.count = n * heads * k.tiles;
+    k.live = std::max<int64_t>(
+        std::min(k.count, heads * (ceil_div(all_rows, unit_rows) + n / 2)), 1);
+    k.span = span;
+    k.fill = fill;
+    k.token = fill / kCus * std::max(2.0 * head_dim * cell / kCuBytes,
+                                     4.0 * head_dim * unit_rows / kCuFlops);
+    return k;
+  };
+  Kind k0;
+  if (apart) k0 = kind_of(1, tokens * G, tokens * G, prefix);
+  const Kind k1 = kind_of(requests, max_query * G, tokens * G, (apart ? 0 : prefix) + max_own);
+  // The requests' ranges are tried in a few sizes, the prefix's so that all workgroups are one to four
+  // rounds on the CUs.
+  int64_t best0 = 1, best1 = 1;
+  double least = 0.0;
+  for (const int64_t want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64, 128, 256}) {
+    const int64_t s1 = k1.splits(want);
+    for (int round = 1; round <= 4; ++round) {
+      const int64_t s0 = apart ? k0.splits((fill * round - k1.live * s1) / k0.live) : 1;
+      const double time = call_time(k0, s0, k1, s1, tokens * query_heads, head_dim);
+      if (least == 0.0 || time < least) {
+        least = time;
+        best0 = s0;
+        best1 = s1;
       }
+      if (!apart) break;
     }
-    const int64_t chunk = ceil_div(steps, splits) * 256;
-    splits = std::max<int64_t>(ceil_div(span, chunk), 1);
-    const int64_t units = ceil_div(keys * splits, 8) * 8 * tiles;
+    if (s1 < want) break;
+  }
+  Plan plan{};
+  const auto put = [&](Group& g, const Kind& k, int64_t splits, int64_t first) {
+    const int64_t units = ceil_div(k.count / k.tiles * splits, 8) * 8 * k.tiles;
     plan.units += units;
     g.units = static_cast<int32_t>(std::min<int64_t>(units, INT32_MAX));
-    g.shape = shape;
-    g.tiles = static_cast<int32_t>(tiles);
+    g.shape = k.shape;
+    g.tiles = divisor(k.tiles);
     g.splits = static_cast<int32_t>(splits);
-    g.chunk = static_cast<int32_t>(chunk);
-    g.slot = static_cast<int32_t>(slot);
+    g.chunk = static_cast<int32_t>(k.chunk(splits));
+    g.slot = static_cast<int32_t>(plan.slots);  // of the partial results
     g.first = static_cast<int32_t>(first);
-    slot += splits;
+    plan.slots += splits;
   };
-  if (apart) fill(plan.shared, 1, tokens * G, 0, prefix);
-  fill(plan.each, requests, max_query * G, apart ? prefix : 0, (apart ? 0 : prefix) + max_own);
-  plan.slots = slot;
+  if (apart) put(plan.group[0], k0, best0, 0);
+  put(plan.group[1], k1, best1, apart ? prefix : 0);
   return plan;
 }
 
@@ -844,12 +1021,13 @@ int64_t origami_shared_prefix_attention_workspace(int64_t tokens, int64_t query_
                                                   int64_t heads, int64_t head_dim,
                                                   int64_t prefix_tokens, int64_t requests,
                                                   int64_t max_query_tokens,
-                                                  int64_t max_own_tokens) {
+                                                  int64_t max_own_tokens, int64_t cache_dtype) {
+  const int64_t cell_bytes = cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN ? 1 : 2;
   if (check_sizes(tokens, query_heads, heads, head_dim, prefix_tokens, requests, max_query_tokens,
                   max_own_tokens))
     return -1;
   return workspace_bytes_of(plan_of(tokens, query_heads, heads, head_dim, prefix_tokens,
-                                    requests, max_query_tokens, max_own_tokens),
+                                    requests, max_query_tokens, max_own_tokens, cell_bytes),
                             tokens, query_heads, head_dim);
 }
 
@@ -889,9 +1067,9 @@ int origami_shared_prefix_attention(
   ORIGAMI_REQUIRE(aligned16(kv_cache), "kv_cache must be 16-byte aligned");
   if (tokens == 0 || requests == 0) return ORIGAMI_OK;
 
-  if (num_blocks == 0) prefix_tokens = max_own_tokens = 0;  // no token is in the cache
+  const bool fp8 = cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN;
   const Plan plan = plan_of(tokens, query_heads, heads, head_dim, prefix_tokens, requests,
-                            max_query_tokens, max_own_tokens);
+                            max_query_tokens, max_own_tokens, fp8 ? 1 : 2);
   ORIGAMI_REQUIRE(plan.units <= INT32_MAX && tokens * query_heads <= INT32_MAX / 32,
                   "too many row tiles for one call");
   ORIGAMI_REQUIRE(workspace_bytes >= workspace_bytes_of(plan, tokens, query_heads, head_dim) &&
@@ -912,26 +1090,25 @@ int origami_shared_prefix_attention(
   p.table_stride = table_stride;
   p.own_tokens = own_tokens;
   p.starts = query_starts;
-  p.block_size = static_cast<int32_t>(block_size);
+  p.block_size = divisor(block_size);
   p.prefix = static_cast<int32_t>(prefix_tokens);
   p.max_own = static_cast<int32_t>(max_own_tokens);
   p.max_query = static_cast<int32_t>(max_query_tokens);
   p.tokens = static_cast<int32_t>(tokens);
-  p.requests = static_cast<int32_t>(requests);
+  p.requests = divisor(requests);
   p.Hq = static_cast<int32_t>(query_heads);
-  p.H = static_cast<int32_t>(heads);
-  p.G = static_cast<int32_t>(query_heads / heads);
+  p.H = divisor(heads);
+  p.G = divisor(query_heads / heads);
   p.D = static_cast<int32_t>(head_dim);
   p.scale = static_cast<float>(scale * k_scale) * kLog2e;
   p.v_scale = static_cast<float>(v_scale);
-  p.group[0] = plan.shared;
-  p.group[1] = plan.each;
+  p.group[0] = plan.group[0];
+  p.group[1] = plan.group[1];
   p.slots = static_cast<int32_t>(plan.slots);
   const int64_t parts = plan.slots * tokens * query_heads;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + parts * head_dim;
   const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-  const bool fp8 = cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN;
   if (dtype == ORIGAMI_DTYPE_BFLOAT16)
     return fp8 ? launch_attend<bf16, true>(p, stream) : launch_attend<bf16, false>(p, stream);
   return fp8 ? launch_attend<f16, true>(p, stream) : launch_attend<f16, false>(p, stream);

@@ -607,15 +607,15 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
                     lse->dim() == 2 && lse->size(0) == tokens && lse->size(1) == Hq,
                 "lse must be float32 [tokens, query heads] on the kv_cache device");
   }
+  const int64_t cache_dtype = paged_dtype_code(kv_cache.scalar_type(), "kv_cache");
   const int64_t bytes = origami_shared_prefix_attention_workspace(
-      tokens, Hq, g.heads, D, prefix_tokens, requests, most, most_own);
+      tokens, Hq, g.heads, D, prefix_tokens, requests, most, most_own, cache_dtype);
   TORCH_CHECK(bytes >= 0, origami_last_error());
   at::Tensor work;
   if (bytes > 0) work = at::empty({bytes}, query.options().dtype(at::kByte));
   const int64_t strides[4] = {query.stride(0), query.stride(1), out.stride(0), out.stride(1)};
   check(origami_shared_prefix_attention(
-      query.data_ptr(), dtype, strides, tokens, Hq, kv_cache.data_ptr(),
-      paged_dtype_code(kv_cache.scalar_type(), "kv_cache"), g.layout, g.num_blocks, g.block_size,
+      query.data_ptr(), dtype, strides, tokens, Hq, kv_cache.data_ptr(), cache_dtype, g.layout, g.num_blocks, g.block_size,
       g.heads, D, prefix, prefix_blocks, prefix_tokens,
       block_tables.numel() ? block_tables.data_ptr<int64_t>() : nullptr, block_tables.stride(0),
       blocks, own, requests, starts, most, most_own,

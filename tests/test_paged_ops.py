@@ -94,7 +94,7 @@ def test_attention_refuses(change, message):
 
 def test_workspace_sizes():
     size = _native.lib().origami_shared_prefix_attention_workspace
-    assert size(3, 4, 2, 64, 32, 3, 1, 32) > 0
-    assert size(0, 4, 2, 64, 32, 3, 0, 32) == 0
-    assert size(3, 3, 2, 64, 32, 3, 1, 32) == -1
-    assert size(1, 4, 2, 64, 0, 1, 1, 16) == 0  # one part: the rows are written at once
+    assert size(3, 4, 2, 64, 32, 3, 1, 32, BF16) > 0
+    assert size(0, 4, 2, 64, 32, 3, 0, 32, BF16) == 0
+    assert size(3, 3, 2, 64, 32, 3, 1, 32, BF16) == -1
+    assert size(1, 4, 2, 64, 0, 1, 1, 16, FP8) == 0  # one part: the rows are written at once
