@@ -19,11 +19,16 @@ using origami_internal::cache_geometry;
 using origami_internal::check_launch;
 using origami_internal::fail;
 
-// Waves of a workgroup.  With 128 channels a workgroup of eight takes a CU's LDS and registers; with
-// 64, two of four do (faster there than one of eight: 19 us against 26 for 24 requests of 12
-// heads), and with 256, where results take half of a wave's registers, one of four.
-template <int DP>
-constexpr int kWaves = DP == 128 ? 8 : 4;
+// Rows of a workgroup, and its waves.  Waves take 16 or 32 rows; in the larger shapes more of them have
+// rows of their own, in the smaller ones more have tokens of their own.  Four waves are half of a
+// CU's LDS and registers with up to 128 channels, so that one workgroup's start and end are
+// beside another's products (against eight waves: 93 us for 103 for 64 requests over 32768
+// tokens, 34 for 40 with e4m3).  The last shape, for requests of many rows and 65 to 128
+// channels, shares tiles among eight waves: 536 us for 616 for prompts of up to 1024 tokens after
+// 8192.  With more channels there are the first two shapes, and a workgroup to a CU.
+constexpr int kShapeRows[4] = {16, 64, 128, 256};
+constexpr int kShapeWaves[4] = {4, 4, 4, 8};
+
 constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / 64;
 // Exponentials are taken 2^kLift times as large for half precision, so that those of tokens far
 // below the maximum keep their precision (down to 2^-24 of the largest) and sums of 2^30 of
@@ -39,11 +44,6 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int64_t kCus = 256;
 constexpr int kFewParts = 8;
 constexpr int kMaxParts = 1024;  // of a row: twice kCus at most of either kind
-
-// Rows of a workgroup.  Waves take 16 or 32 rows; in the larger shapes more of them have rows of
-// their own, in the smaller ones more have tokens of their own.  Up to 64 channels there are the
-// first three shapes, up to 128 all, up to 256 the first two.
-constexpr int kShapeRows[4] = {16, 64, 128, 256};
 
 // Division of 0 <= x < 2^31 by a divisor that the host knows: x / d = mulhi(x, mul) >> shift, with
 // mul the ceiling of 2^(32 + shift) / d and 2^shift < d <= 2^(shift + 1) (d = 1: shift -1).
@@ -268,10 +268,10 @@ constexpr int kTeamTokens = WR == 8 || (WR == 4 && DP == 64) ? 64 : 32;
 // through LDS, where the WR waves of a team share them, and the next ones are on their way
 // to registers meanwhile.  With WR = 1 no wave needs another until the end; else two buffers
 // take turns, so that one barrier a step is enough.
-template <typename T, bool FP8, int DP, int MR, int WR>
+template <typename T, bool FP8, int DP, int MR, int WR, int NW>
 __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, int unit, bool batch,
                                        uint8_t* lds, float* ml) {
-  constexpr int WT = kWaves<DP> / WR, TT = kTeamTokens<DP, WR>;
+  constexpr int WT = NW / WR, TT = kTeamTokens<DP, WR>;
   constexpr int NG = 64 / MR;             // lane groups: the depth of a product is 8 NG
   constexpr int KS = DP / (8 * NG);       // depth steps of K Q
   constexpr int DT = DP / MR;             // channel tiles of V P
@@ -612,7 +612,7 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
     // first token wave leave theirs, which that one adds to its own.
     constexpr int M = WR * MR, kPitch = DP + 4, kPart = WR == 1 ? 2 * kTile : M * kPitch * 4;
     static_assert((WR > 1 || MR * kPitch * 4 <= 2 * kTile) &&
-                      (WT - 1) * kPart <= 128 * DP * kWaves<DP>, "LDS");
+                      (WT - 1) * kPart <= 512 * DP, "LDS");
     if constexpr (WR > 1) __syncthreads();
     const int mr = wr * MR + c;
     const auto part_row = [&](int w, int r) {
@@ -633,7 +633,7 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
     }
     __syncthreads();
     if constexpr (WR == 1) {
-      for (int i = threadIdx.x; i < M * (DP / 4); i += 64 * kWaves<DP>) {
+      for (int i = threadIdx.x; i < M * (DP / 4); i += 64 * NW) {
         const int r = i / (DP / 4), ch = 4 * (i % (DP / 4));
         float most = -INFINITY, total = 0.0f;
 #pragma unroll
@@ -690,14 +690,15 @@ template <typename T, bool FP8, int DP, int SHAPE>
 __device__ __forceinline__ void attend_shape(const AttendParams& p, int kind, int unit,
                                              uint8_t* lds, float* ml) {
   constexpr int MR = SHAPE == 0 || DP == 256 ? 16 : 32;
-  attend<T, FP8, DP, MR, kShapeRows[SHAPE] / MR>(p, p.group[kind], unit, kind == 0, lds,
-                                                       ml);
+  attend<T, FP8, DP, MR, kShapeRows[SHAPE] / MR, kShapeWaves[SHAPE]>(p, p.group[kind], unit,
+                                                                    kind == 0, lds, ml);
 }
 
 // The prefix in workgroups of shape S0 and the requests in those of S1, in one launch.
 template <typename T, bool FP8, int DP, int S0, int S1>
-__global__ __launch_bounds__(64 * kWaves<DP>, DP == 256 ? 1 : 2) void attend_kernel(AttendParams p) {
-  __shared__ alignas(16) uint8_t lds[128 * DP * kWaves<DP>];  // of every shape
+__global__ __launch_bounds__(64 * kShapeWaves[S0], DP == 256 ? 1 : 2)
+    void attend_kernel(AttendParams p) {
+  __shared__ alignas(16) uint8_t lds[(S0 == 3 ? 768 : 512) * DP];
   __shared__ float ml[512];  // maxima and sums of the token waves' rows
   int unit = static_cast<int>(blockIdx.x);
   const int kind = unit >= p.group[0].units;
@@ -828,35 +829,28 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendParams p, int 
   if (p.lse && ch == 0) p.lse[row] = total == 0.0f ? -INFINITY : kLn2 * (best + log2f(total));
 }
 
+template <typename T, bool FP8, int DP, int S0, int S1>
+int launch_shapes(const AttendParams& p, hipStream_t stream) {
+  const dim3 grid(p.group[0].units + p.group[1].units), block(64 * kShapeWaves[S0]);
+  hipLaunchKernelGGL((attend_kernel<T, FP8, DP, S0, S1>), grid, block, 0, stream, p);
+  return check_launch("attend_kernel");
+}
+
 template <typename T, bool FP8, int DP>
 int launch_units(const AttendParams& p, hipStream_t stream) {
-  const dim3 grid(p.group[0].units + p.group[1].units), block(64 * kWaves<DP>);
+  // the batch has at least a request's rows: s0 >= s1
   const int s1 = p.group[1].shape, s0 = p.group[0].units ? p.group[0].shape : s1;
-  if (s0 == 0)  // the batch has at least a request's rows: s0 >= s1
-    hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 0, 0>), grid, block, 0, stream, p);
-  else if (s0 == 1 && s1 == 0)
-    hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 1, 0>), grid, block, 0, stream, p);
-  else if (s0 == 1)
-    hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 1, 1>), grid, block, 0, stream, p);
-  if constexpr (DP <= 128) {
-    if (s0 == 2 && s1 == 0)
-      hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 2, 0>), grid, block, 0, stream, p);
-    else if (s0 == 2 && s1 == 1)
-      hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 2, 1>), grid, block, 0, stream, p);
-    else if (s0 == 2)
-      hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 2, 2>), grid, block, 0, stream, p);
-  }
-  if constexpr (DP == 128) {
-    if (s0 == 3 && s1 == 0)
-      hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 3, 0>), grid, block, 0, stream, p);
-    else if (s0 == 3 && s1 == 1)
-      hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 3, 1>), grid, block, 0, stream, p);
-    else if (s0 == 3 && s1 == 2)
-      hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 3, 2>), grid, block, 0, stream, p);
-    else if (s0 == 3)
-      hipLaunchKernelGGL((attend_kernel<T, FP8, DP, 3, 3>), grid, block, 0, stream, p);
-  }
-  return check_launch("attend_kernel");
+  if constexpr (DP == 128)
+    if (s0 == 3) return launch_shapes<T, FP8, DP, 3, 3>(p, stream);
+  if constexpr (DP <= 128)
+    if (s0 == 2)
+      return s1 == 0   ? launch_shapes<T, FP8, DP, 2, 0>(p, stream)
+             : s1 == 1 ? launch_shapes<T, FP8, DP, 2, 1>(p, stream)
+                       : launch_shapes<T, FP8, DP, 2, 2>(p, stream);
+  if constexpr (DP <= 128)
+    if (s0 == 1 && s1 == 0) return launch_shapes<T, FP8, DP, 1, 0>(p, stream);
+  if (s0 == 1) return launch_shapes<T, FP8, DP, 1, 1>(p, stream);
+  return launch_shapes<T, FP8, DP, 0, 0>(p, stream);
 }
 
 template <typename T, bool FP8>
@@ -936,27 +930,30 @@ double call_time(const Kind& k0, int64_t s0, const Kind& k1, int64_t s1, int64_t
 
 Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_dim,
              int64_t prefix, int64_t requests, int64_t max_query, int64_t max_own, int64_t cell) {
-  const int64_t G = query_heads / heads, last = head_dim <= 64 ? 2 : (head_dim <= 128 ? 3 : 1);
-  const int64_t fill = head_dim <= 64 ? 2 * kCus : kCus;  // workgroups that the CUs hold
+  const int64_t G = query_heads / heads, last = head_dim <= 128 ? 2 : 1;
   // A request whose rows fill workgroups by themselves reads the prefix with its own tokens.
   const bool apart = requests > 1 && prefix > 0 && max_query * G < kShapeRows[last];
-  const auto kind_of = [&](int64_t n, int64_t rows, int64_t all_rows, int64_t span) {
+  const auto kind_of = [&](int shape, int64_t n, int64_t rows, int64_t all_rows, int64_t span) {
     Kind k;
+    k.shape = shape;
     while (k.shape < last && rows > kShapeRows[k.shape]) ++k.shape;
+    if (!apart && k.shape == 2 && rows > kShapeRows[2] && head_dim > 64) k.shape = 3;
     const int64_t unit_rows = kShapeRows[k.shape];
     k.tiles = std::max<int64_t>(ceil_div(rows, unit_rows), 1);
     k.count = n * heads * k.tiles;
     k.live = std::max<int64_t>(
         std::min(k.count, heads * (ceil_div(all_rows, unit_rows) + n / 2)), 1);
     k.span = span;
-    k.fill = fill;
-    k.token = fill / kCus * std::max(2.0 * head_dim * cell / kCuBytes,
+    k.fill = head_dim <= 128 && k.shape < 3 ? 2 * kCus : kCus;  // workgroups that the CUs hold
+    k.token = k.fill / kCus * std::max(2.0 * head_dim * cell / kCuBytes,
                                      4.0 * head_dim * unit_rows / kCuFlops);
     return k;
   };
   Kind k0;
-  if (apart) k0 = kind_of(1, tokens * G, tokens * G, prefix);
-  const Kind k1 = kind_of(requests, max_query * G, tokens * G, (apart ? 0 : prefix) + max_own);
+  if (apart) k0 = kind_of(0, 1, tokens * G, tokens * G, prefix);
+  // past 128 channels the kinds have one shape: two there do not fit the scalar registers
+  const Kind k1 = kind_of(head_dim > 128 ? k0.shape : 0, requests, max_query * G, tokens * G,
+                          (apart ? 0 : prefix) + max_own);
   // The requests' ranges are tried in a few sizes, the prefix's so that all workgroups are one to four
   // rounds on the CUs.
   int64_t best0 = 1, best1 = 1;
@@ -964,7 +961,7 @@ Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_di
   for (const int64_t want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64, 128, 256}) {
     const int64_t s1 = k1.splits(want);
     for (int round = 1; round <= 4; ++round) {
-      const int64_t s0 = apart ? k0.splits((fill * round - k1.live * s1) / k0.live) : 1;
+      const int64_t s0 = apart ? k0.splits((k1.fill * round - k1.live * s1) / k0.live) : 1;
       const double time = call_time(k0, s0, k1, s1, tokens * query_heads, head_dim);
       if (least == 0.0 || time < least) {
         least = time;
