@@ -401,7 +401,7 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
   // end.
   bool odd = false;
   const auto drop_odd_values = [&](int t) {
-    if (t + TT > nearest)
+    if (min(t + TT, t1) > nearest)
 #pragma unroll
       for (int i = 0; i < IT; ++i) odd |= drop_odd<T>(vr[i]);
   };
@@ -569,26 +569,26 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
   for (int x = MR; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
   if (t1 > nearest) odd = __syncthreads_or(odd);
 
-  // The infinities and NaN that drop_odd_values left out, for four channels of a row that sees
-  // them.  Tokens before theirs have been added already, and an infinity or NaN twice is the same.
-  const auto odd_values = [&](int ch, int before) -> Float4 {
-    Float4 out = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = max(t0, nearest - TT); i < min(t1, before); ++i) {
+  // Calls add(row of the cache's values) for the tokens among which drop_odd_values left out
+  // infinities and NaN, as far as a row sees them.  The first ones may be tokens before those,
+  // whose values have been added already, and an infinity or NaN twice is the same.
+  const auto each_odd_token = [&](int row, auto add) {
+    for (int i = max(t0, nearest - TT); i < min(t1, seen_by(row)); ++i) {
       const int at_row = row_of(i, block_of(i, t1));
-      if (at_row < 0) continue;
-      const Float4 v = four_values<T, FP8>(
-          p.cache + (at_row + p.half_stride) * pitch + static_cast<int64_t>(h) * p.D * cell, ch);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) out[j] += fabsf(v[j]) < INFINITY ? 0.0f : v[j];
+      if (at_row >= 0)
+        add(p.cache + (at_row + p.half_stride) * pitch + static_cast<int64_t>(h) * p.D * cell);
     }
-    return out;
+  };
+  const auto odd_part = [](Float4 v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = fabsf(v[j]) < INFINITY ? 0.0f : v[j];
+    return v;
   };
   // Four channels of a row's result, and with the first ones its maximum and sum.
   const auto put = [&](int row, int ch, Float4 v, float base, float sum) {
     if (row >= rows || ch >= p.D) return;
     const int qi = divide(row, p.G), head = h * p.G.d + row - qi * p.G.d;
     const int64_t n = rq.first + qi, at = n * p.Hq + head;
-    if (odd) v += odd_values(ch, seen_by(row));
     if (p.slots > 1) {
       const int64_t slot =
           (g.slot + split) * (static_cast<int64_t>(p.tokens) * p.Hq) + at;
@@ -646,6 +646,10 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
           total += ml[(w * M + r) * 2 + 1] * weight;
           v += *reinterpret_cast<const Float4*>(part_row(w, r) + ch) * weight;
         }
+        if (odd)
+          each_odd_token(row0 + r, [&](const uint8_t* values) {
+            v += odd_part(four_values<T, FP8>(values, min(ch, p.D - 4)));
+          });
         put(row0 + r, ch, v, most, total);
       }
       return;
@@ -678,6 +682,18 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
   }
   int again = row;  // where the row is, anew: there are no registers to keep it through the loop
   asm volatile("" : "+v"(again));
+  if (odd)
+    each_odd_token(again, [&](const uint8_t* values) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int x = 0; x < ACC; x += 4) {
+          const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
+          const Float4 v = odd_part(four_values<T, FP8>(values, min(ch, p.D - 4)));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[d][x + j] += v[j];
+        }
+    });
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -704,7 +720,7 @@ __global__ __launch_bounds__(64 * kShapeWaves[S0], DP == 256 ? 1 : 2)
   const int kind = unit >= p.group[0].units;
   unit -= kind ? p.group[0].units : 0;
   if (S0 == S1 || kind == 1)
-    attend_shape<T, FP8, DP, S1>(p, kind, unit, lds, ml);
+    attend_shape<T, FP8, DP, S1>(p, S0 == S1 ? kind : 1, unit, lds, ml);
   else
     attend_shape<T, FP8, DP, S0>(p, 0, unit, lds, ml);
 }

@@ -155,6 +155,60 @@ def test_masked_values_have_no_influence(cuda_device):
                 assert got[sees].isnan().all()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("group", [1, 8, 40])
+def test_odd_values_reach_the_rows_that_see_them(cuda_device, D, group):
+    """Values of infinity and NaN anywhere in the tokens, in workgroups of every shape: the same
+    channels are not finite as in the plain form, and all others are right."""
+    for own, queries in (((40, 97), (30, 97)), ((300,), (257,)), ((64, 9), (1, 2))):
+        b = Batch(cuda_device, prefix=75, own=own, queries=queries, heads=2, group=group, D=D,
+                  seed=D + group)
+        marks = [(b.prefix_ids, 3, 0, 5, math.nan), (b.prefix_ids, 74, 1, 6, math.inf),
+                 (b.tables[0], 2, 0, 9, math.inf), (b.tables[0], own[0] - 3, 1, D - 1, -math.inf),
+                 (b.tables[-1], own[-1] - 1, 0, 0, math.nan), (b.tables[-1], 0, 1, 1, -math.inf)]
+        clean = b.cache.clone()
+        for table, t, h, d, value in marks:
+            b.cache[1, int(table[t // b.bs]), t % b.bs, h, d] = value
+        got, lse = b.run()
+        ref = pagedref.attend(b.query, b.cache, b.prefix_ids, b.prefix, b.tables, b.own,
+                              b.starts)[0]
+        fine = ref.isfinite()  # the plain form has no hidden tokens, so no 0 times infinity
+        assert torch.equal(got.isfinite(), fine)
+        b.cache = clean
+        whole, whole_lse = b.run()
+        assert torch.equal(got[fine], whole[fine]) and torch.equal(lse, whole_lse)
+
+
+@pytest.mark.parametrize("peak", [0.0, 30.0])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_flat_and_steep_scores(cuda_device, peak, dtype):
+    """Equal weights, and weights of one token: maxima that rise late in a long row."""
+    b = Batch(cuda_device, prefix=3000, own=(700, 5), dtype=dtype, D=64, peak=peak, seed=3)
+    b.check(*b.run())
+
+
+@pytest.mark.parametrize("B,prefix,D", [(3, 1000, 128), (40, 600, 128), (70, 333, 64),
+                                        (40, 600, 192)])
+@pytest.mark.parametrize("queries", [1, 3, 11])
+def test_batches_in_every_shape(cuda_device, B, prefix, D, queries):
+    own = [(37 * i) % 150 + queries for i in range(B)]
+    b = Batch(cuda_device, prefix=prefix, own=own, queries=[queries] * B, heads=1, group=5, D=D,
+              seed=B + queries)
+    b.check(*b.run())
+
+
+def test_bounds_far_above_the_lengths(cuda_device):
+    """Tables for much longer requests: ranges without a token are joined as nothing."""
+    b = Batch(cuda_device, prefix=200, own=(3, 90, 41))
+    plain = b.run()
+    wide = torch.full((3, 4000), -1, dtype=torch.int64, device=cuda_device)
+    wide[:, :b.tables.shape[1]] = b.tables
+    b.tables = wide
+    got = b.run()
+    b.check(*got)
+    assert (got[0].float() - plain[0].float()).abs().max() < 0.05
+
+
 def test_blocks_outside_the_cache_are_not_seen(cuda_device):
     b = Batch(cuda_device, prefix=100, own=(50, 60, 3), D=64)
     NB = pagedref.halves(b.cache).shape[1]

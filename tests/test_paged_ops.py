@@ -41,7 +41,8 @@ def _append(**kw):
     (dict(cache_dtype=FP8, v_scale=float("nan")), "scales must be positive"),
     (dict(v_scale=2.0), "for float8_e4m3fn"),
     (dict(kv_cache=24), "16-byte aligned"),
-    (dict(tokens=1 << 29), "too many rows"),
+    (dict(tokens=1 << 25), "too many rows"),
+    (dict(query_heads=1 << 16), "too many rows"),
 ])
 def test_append_refuses(change, message):
     with pytest.raises(_native.OrigamiNativeError, match=message) as e:
