@@ -489,9 +489,10 @@ int origami_append_kv_cache(
  * rows query_starts[r] .. query_starts[r + 1] - 1 of query (query_starts null:
  * row r alone) and its last own tokens, so that query i of n sees the prefix and
  * own tokens 0 .. own_tokens[r] - n + i.  Device arrays are int64.  max_query_tokens
- * and max_own_tokens bound a request's query and own tokens (they shape the
- * launch; further tokens are not seen).  Rows that no request has are left as
- * they were.  Tokens in blocks outside [0, num_blocks) are not seen; what a row
+ * and max_own_tokens bound a request's query and own tokens and shape the
+ * launch: own tokens past the bound are not seen, and the rows of a request
+ * with more query tokens than the bound have no defined values.  Rows that no
+ * request has are left as they were.  Tokens in blocks outside [0, num_blocks) are not seen; what a row
  * does not see has no influence on it, NaN included.  A row that sees no token,
  * or only scores of -infinity, becomes zero.
  * lse (null: none) is a contiguous float32 [tokens, query_heads]: the natural

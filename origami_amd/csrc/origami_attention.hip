@@ -1020,9 +1020,9 @@ int check_sizes(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head
   ORIGAMI_REQUIRE(tokens >= 0 && requests >= 0 && prefix_tokens >= 0 && max_query >= 0 &&
                       max_own >= 0,
                   "token counts must not be negative");
-  ORIGAMI_REQUIRE(max_query <= tokens, "max_query_tokens exceeds the query tokens");
   ORIGAMI_REQUIRE(prefix_tokens + max_own <= (int64_t(1) << 30), "too many tokens for one call");
-  ORIGAMI_REQUIRE(tokens <= INT32_MAX / query_heads, "too many query rows for one call");
+  // a launch has at most 2^32 threads in x
+  ORIGAMI_REQUIRE(tokens < (int64_t(1) << 24) / query_heads, "too many query rows for one call");
   return ORIGAMI_OK;
 }
 
@@ -1039,6 +1039,7 @@ int64_t origami_shared_prefix_attention_workspace(int64_t tokens, int64_t query_
   if (check_sizes(tokens, query_heads, heads, head_dim, prefix_tokens, requests, max_query_tokens,
                   max_own_tokens))
     return -1;
+  max_query_tokens = std::min(max_query_tokens, tokens);
   return workspace_bytes_of(plan_of(tokens, query_heads, heads, head_dim, prefix_tokens,
                                     requests, max_query_tokens, max_own_tokens, cell_bytes),
                             tokens, query_heads, head_dim);
@@ -1072,8 +1073,9 @@ int origami_shared_prefix_attention(
                   "prefix tokens exceed the prefix blocks");
   ORIGAMI_REQUIRE(ceil_div(max_own_tokens, block_size) <= table_blocks,
                   "max_own_tokens exceeds the block tables");
-  ORIGAMI_REQUIRE(query_starts != nullptr || (tokens == requests && max_query_tokens <= 1),
+  ORIGAMI_REQUIRE(query_starts != nullptr || tokens == requests,
                   "without query_starts every request has one query token");
+  max_query_tokens = std::min(max_query_tokens, tokens);
   ORIGAMI_REQUIRE(k_scale > 0.0 && v_scale > 0.0, "cache scales must be positive");
   ORIGAMI_REQUIRE(cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN || (k_scale == 1.0 && v_scale == 1.0),
                   "cache scales are for float8_e4m3fn caches");
@@ -1083,8 +1085,7 @@ int origami_shared_prefix_attention(
   const bool fp8 = cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN;
   const Plan plan = plan_of(tokens, query_heads, heads, head_dim, prefix_tokens, requests,
                             max_query_tokens, max_own_tokens, fp8 ? 1 : 2);
-  ORIGAMI_REQUIRE(plan.units <= INT32_MAX && tokens * query_heads <= INT32_MAX / 32,
-                  "too many row tiles for one call");
+  ORIGAMI_REQUIRE(plan.units < (int64_t(1) << 32) / 512, "too many row tiles for one call");
   ORIGAMI_REQUIRE(workspace_bytes >= workspace_bytes_of(plan, tokens, query_heads, head_dim) &&
                       (plan.slots == 1 || workspace != nullptr) && aligned16(workspace),
                   "attention workspace is too small");

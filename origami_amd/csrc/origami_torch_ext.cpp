@@ -482,6 +482,7 @@ c10::optional<at::Tensor> append_kv_cache(
     c10::optional<at::Tensor> key_norm, double eps, double k_scale, double v_scale,
     c10::optional<at::Tensor> query_out) {
   require_device(kv_cache, "kv_cache");
+  require_no_grad(kv_cache, "kv_cache");
   const CacheGeom g = layout_cache_geometry(kv_cache);
   const int64_t dtype = paged_dtype_code(key.scalar_type(), "key");
   TORCH_CHECK(dtype != ORIGAMI_DTYPE_FLOAT8_E4M3FN, "key must be float16 or bfloat16");
@@ -564,6 +565,7 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
                                    c10::optional<double> scale, double k_scale, double v_scale,
                                    c10::optional<at::Tensor> out_, c10::optional<at::Tensor> lse) {
   require_device(kv_cache, "kv_cache");
+  require_no_grad(kv_cache, "kv_cache");
   const CacheGeom g = layout_cache_geometry(kv_cache);
   const int64_t dtype = paged_dtype_code(query.scalar_type(), "query");
   TORCH_CHECK(dtype != ORIGAMI_DTYPE_FLOAT8_E4M3FN, "query must be float16 or bfloat16");

@@ -777,7 +777,8 @@ def shared_prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor,
     tensor).  All of these are device tensors and nothing is read back, so a call can be
     captured in a graph and replayed as lengths grow.  max_query_tokens and max_own_tokens
     bound a request's query and own tokens and shape the launch (defaults: all rows, the
-    whole block table); tokens past them are not seen.  Tokens in blocks outside the cache are
+    whole block table); own tokens past the bound are not seen, and a request with more query
+    tokens than the bound gets no defined rows.  Tokens in blocks outside the cache are
     not seen.  scale defaults to head_dim ** -0.5.
 
     Returns the output, and with return_lse also float32 [tokens, query_heads] natural

@@ -71,16 +71,14 @@ def _attend(**kw):
     (dict(head_dim=512), "at most 256"),
     (dict(tokens=-1), "must not be negative"),
     (dict(prefix=-1), "must not be negative"),
-    (dict(max_query=4), "exceeds the query tokens"),
     (dict(prefix=1 << 30), "too many tokens"),
-    (dict(tokens=1 << 29, starts=16), "too many query rows"),
+    (dict(tokens=1 << 22, starts=16), "too many query rows"),
     (dict(num_blocks=1 << 28), "too many token slots"),
     (dict(block_size=0), "block size must be positive"),
     (dict(layout=3), "kv_cache must be"),
     (dict(prefix=33), "exceed the prefix blocks"),
     (dict(max_own=33), "exceeds the block tables"),
     (dict(tokens=4), "one query token"),
-    (dict(max_query=2), "one query token"),
     (dict(k_scale=-1.0), "scales must be positive"),
     (dict(v_scale=0.5), "for float8_e4m3fn"),
     (dict(kv_cache=17), "16-byte aligned"),
