@@ -11,10 +11,10 @@
 // each (16 bytes of a 16-bit row), so that the mean and a pair's partner are exchanged between
 // lanes of one wave and nothing goes through LDS; the query, key and value rows of all tokens
 // are one launch, since a decode step has far too few rows to fill one with each.  A workgroup's
-// rows are of one token, whose slot, position and angles are then scalar: 48.6 us (4.2 TB/s) for 8192
-// tokens of 32 + 8 + 8 heads of 128 with norms, where rows numbered through took 55 and 256
-// threads 51.5; three rows a lane group with their loads together took 58 and non-temporal loads 63.
-// One token takes 2.8 us, which is a launch.
+// rows are of one token, whose slot, position and angles are then scalar: 48.6 us (4.2 TB/s) for
+// 8192 tokens of 32 + 8 + 8 heads of 128 with norms, where rows numbered through took 55 and 256
+// threads 51.5; three rows a lane group with their loads together took 58, and non-temporal loads
+// 63.  One token takes 2.8 us, which is a launch.
 #include "origami_element.h"
 #include "origami_internal.h"
 

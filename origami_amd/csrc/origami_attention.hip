@@ -4,7 +4,18 @@
 //   s_t = scale * (q . k_t),  out = sum_t exp(s_t - m) v_t / sum_t exp(s_t - m),  m = max_t s_t
 // The tokens come in parts (the prefix, the request's own tokens, ranges of either).  A part
 // gives m, the sum l and the unnormalised row O in binary32; parts are joined with the weights
-// exp(m_part - m), so that no part waits for another.
+// exp(m_part - m), so that no part waits for another.  Scores, maxima, sums and O are binary32;
+// the exponentials are rounded to the queries' type for the matrix instruction, which adds half a
+// step of the weighted mean of |v|, about what rounding the result does.
+//
+// The rows of all requests that share the prefix are one matrix against each tile of it, so its
+// keys and values are read once (64 requests over 32768 tokens and 33 thousand of their own: 282 MB
+// from memory of 281 that there are).  With few rows a call is bound by memory and, below some
+// tens of microseconds, by the chain of loads at a workgroup's start (lengths, block ids, rows);
+// with rows by the hundred by the vector instructions of the softmax, which are as many cycles as
+// the products' matrix instructions and run beside them only in part: 815 TFLOP/s for prompts of
+// up to 1024 tokens after 8192, at about 40% of the matrix cycles, where a large library
+// product reaches 1150.
 #include <algorithm>
 #include <type_traits>
 
@@ -19,13 +30,13 @@ using origami_internal::cache_geometry;
 using origami_internal::check_launch;
 using origami_internal::fail;
 
-// Rows of a workgroup, and its waves.  Waves take 16 or 32 rows; in the larger shapes more of them have
-// rows of their own, in the smaller ones more have tokens of their own.  Four waves are half of a
-// CU's LDS and registers with up to 128 channels, so that one workgroup's start and end are
+// Rows of a workgroup, and its waves.  Waves take 16 or 32 rows; in the larger shapes more of them
+// have rows of their own, in the smaller ones more have tokens of their own.  Four waves are half
+// of a CU's LDS and registers with up to 128 channels, so that one workgroup's start and end are
 // beside another's products (against eight waves: 93 us for 103 for 64 requests over 32768
-// tokens, 34 for 40 with e4m3).  The last shape, for requests of many rows and 65 to 128
-// channels, shares tiles among eight waves: 536 us for 616 for prompts of up to 1024 tokens after
-// 8192.  With more channels there are the first two shapes, and a workgroup to a CU.
+// tokens, 34 for 40 for 16 over 16384 in e4m3).  The last shape, for requests of many rows and 65
+// to 128 channels, shares tiles among eight waves: 536 us for 616 for prompts of up to 1024 tokens
+// after 8192.  With more channels there are the first two shapes, and a workgroup to a CU.
 constexpr int kShapeRows[4] = {16, 64, 128, 256};
 constexpr int kShapeWaves[4] = {4, 4, 4, 8};
 
@@ -263,11 +274,13 @@ using Int = std::integral_constant<int, N>;
 template <int DP, int WR>
 constexpr int kTeamTokens = WR == 8 || (WR == 4 && DP == 64) ? 64 : 32;
 
-// One workgroup: WR MR rows of one KV head over a range of tokens.  Its waves are WR row waves by
-// WT token waves: a wave takes MR rows, and of every WT kTeamTokens tokens its share.  Rows (queries, results, sums) stay in registers; keys and values go
-// through LDS, where the WR waves of a team share them, and the next ones are on their way
-// to registers meanwhile.  With WR = 1 no wave needs another until the end; else two buffers
-// take turns, so that one barrier a step is enough.
+// One workgroup: WR MR rows of one KV head over a range of tokens.  Its NW waves are WR row waves
+// by WT token waves: a wave takes MR rows, and of every WT kTeamTokens tokens its share.  Rows
+// (queries, results, sums) stay in registers; keys and values go through LDS, where the WR waves
+// of a team share them, and the next ones are on their way to registers meanwhile.  They do not go
+// from memory to LDS directly: e4m3 is widened and odd values are dropped in between.  With
+// WR = 1 no wave needs another until the end; else buffers take turns, so that one barrier a
+// tile is enough.
 template <typename T, bool FP8, int DP, int MR, int WR, int NW>
 __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, int unit, bool batch,
                                        uint8_t* lds, float* ml) {
@@ -326,7 +339,8 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
   // this lane's row
   const int row = row0 + wr * MR + c;
   const auto seen_by = [&](int i) -> int {  // tokens that row i sees
-    return batch ? p.prefix : p.prefix + min(max(rq.own - rq.count + divide(i, p.G) + 1, 0), rq.own);
+    return p.prefix +
+           (batch ? 0 : min(max(rq.own - rq.count + divide(i, p.G) + 1, 0), rq.own));
   };
   const int limit = seen_by(row);
   // the scale's sign goes with the queries, and so does a scale of zero, so that hidden scores of
@@ -730,7 +744,8 @@ __global__ __launch_bounds__(64 * kShapeWaves[S0], DP == 256 ? 1 : 2)
 template <typename T>
 __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams p, int lanes) {
   const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / lanes) + threadIdx.x / lanes;
+  const int64_t row =
+      static_cast<int64_t>(blockIdx.x) * (kJoinThreads / lanes) + threadIdx.x / lanes;
   const int ch = 4 * (threadIdx.x % lanes);
   if (row >= all || ch >= p.D) return;
   const int64_t n = row / p.Hq, head = row - n * p.Hq;
@@ -758,8 +773,8 @@ __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams p, 
 }
 
 // For many parts: a workgroup takes `4 lanes` channels of one row.  It first lists the parts that
-// have tokens with their weights, then its lane groups add them up in turn, several loads each
-// on their way: a row's parts are one after the other for nobody.
+// have tokens with their weights, then its lane groups add them up in turn, several loads each on
+// their way: 7 us for 128 rows of 411 parts, where one wave a row after the other took 55.
 template <typename T>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendParams p, int lanes, int blocks) {
   __shared__ float weight[kMaxParts];
@@ -922,8 +937,9 @@ struct Kind {
   }
 };
 
-// Measured on MI355X: what a workgroup takes besides its tokens, bytes and operations of one
-// CU in a microsecond while all of them work.
+// Measured on MI355X: microseconds that a workgroup takes besides its tokens, and bytes and
+// operations of one CU in a microsecond while all of them work.  Times change by 2% at most where
+// any of the three is half or twice as large: the split needs to be near only.
 constexpr double kUnitTime = 6.0, kCuBytes = 20e3, kCuFlops = 3.2e6;
 
 // Microseconds of a call whose kinds are split in s0 and s1 ranges: workgroups of the first kind go
@@ -970,8 +986,8 @@ Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_di
   // past 128 channels the kinds have one shape: two there do not fit the scalar registers
   const Kind k1 = kind_of(head_dim > 128 ? k0.shape : 0, requests, max_query * G, tokens * G,
                           (apart ? 0 : prefix) + max_own);
-  // The requests' ranges are tried in a few sizes, the prefix's so that all workgroups are one to four
-  // rounds on the CUs.
+  // The requests' ranges are tried in a few sizes, the prefix's so that all workgroups are one to
+  // four rounds on the CUs.
   int64_t best0 = 1, best1 = 1;
   double least = 0.0;
   for (const int64_t want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64, 128, 256}) {

@@ -587,7 +587,8 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
   if (query_starts) starts = require_index(*query_starts, "query_starts", kv_cache, requests + 1);
   TORCH_CHECK(starts || tokens == requests,
               "without query_starts every request has one query token");
-  const int64_t most = max_query_tokens ? *max_query_tokens : (starts ? tokens : std::min<int64_t>(tokens, 1));
+  const int64_t most =
+      max_query_tokens ? *max_query_tokens : (starts ? tokens : std::min<int64_t>(tokens, 1));
   const int64_t most_own = max_own_tokens ? *max_own_tokens : blocks * g.block_size;
   const c10::OptionalDeviceGuard guard(kv_cache.device());
 
@@ -617,8 +618,8 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
   if (bytes > 0) work = at::empty({bytes}, query.options().dtype(at::kByte));
   const int64_t strides[4] = {query.stride(0), query.stride(1), out.stride(0), out.stride(1)};
   check(origami_shared_prefix_attention(
-      query.data_ptr(), dtype, strides, tokens, Hq, kv_cache.data_ptr(), cache_dtype, g.layout, g.num_blocks, g.block_size,
-      g.heads, D, prefix, prefix_blocks, prefix_tokens,
+      query.data_ptr(), dtype, strides, tokens, Hq, kv_cache.data_ptr(), cache_dtype, g.layout,
+      g.num_blocks, g.block_size, g.heads, D, prefix, prefix_blocks, prefix_tokens,
       block_tables.numel() ? block_tables.data_ptr<int64_t>() : nullptr, block_tables.stride(0),
       blocks, own, requests, starts, most, most_own,
       scale ? *scale : 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(D, 1))), k_scale,

@@ -95,7 +95,8 @@ def test_types_and_sizes(cuda_device, dtype, cache_dtype, D, norm, interleaved):
 
 
 @pytest.mark.parametrize("D,rot", [(8, 8), (8, 2), (24, 16), (40, 20), (80, 32), (80, 20), (96, 96),
-                                   (128, 64), (128, 6), (136, 136), (192, 64), (248, 248), (256, 2)])
+                                   (128, 64), (128, 6), (136, 136), (192, 64), (248, 248),
+                                   (256, 2)])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("norm_dtype", [None, BF16, torch.float32])
 def test_rotary_sizes(cuda_device, D, rot, interleaved, norm_dtype):

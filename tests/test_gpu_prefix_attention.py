@@ -350,7 +350,8 @@ def test_refusals(cuda_device):
     refused("same dtype|queries' dtype", query=b.query.half())
     refused("float16 or bfloat16", query=b.query.float())
     refused("head_dim differs", query=b.query[..., :32])
-    refused("channels must be contiguous", query=b.query.transpose(1, 2).contiguous().transpose(1, 2))
+    refused("channels must be contiguous",
+            query=b.query.transpose(1, 2).contiguous().transpose(1, 2))
     refused("multiple of the cache's heads", query=b.query[:, :3])
     refused("kv_cache device", query=b.query.cpu())
     refused("requires a gradient", query=b.query.clone().requires_grad_())
