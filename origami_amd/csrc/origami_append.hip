@@ -292,7 +292,12 @@ extern "C" int origami_append_kv_cache(
   // a launch has at most 2^32 threads in x, and 65535 workgroups in y
   ORIGAMI_REQUIRE(row_heads <= 65535 && tokens < (int64_t(1) << 32) / kThreads,
                   "too many rows for one call");
+  for (int i = 0; i < (query_heads > 0 ? 8 : 4); ++i)
+    ORIGAMI_REQUIRE(strides[i] >= 0, "row strides must not be negative");
   if (tokens == 0) return ORIGAMI_OK;
+  ORIGAMI_REQUIRE(key != nullptr && value != nullptr && slots != nullptr &&
+                      (kv_cache != nullptr || num_blocks == 0),
+                  "keys, values, slots and the cache must not be null");
 
   p.key = rows_of(key, strides);
   p.value = rows_of(value, strides + 2);

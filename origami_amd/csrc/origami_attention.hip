@@ -1096,7 +1096,15 @@ int origami_shared_prefix_attention(
   ORIGAMI_REQUIRE(cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN || (k_scale == 1.0 && v_scale == 1.0),
                   "cache scales are for float8_e4m3fn caches");
   ORIGAMI_REQUIRE(aligned16(kv_cache), "kv_cache must be 16-byte aligned");
+  for (int i = 0; i < 4; ++i)
+    ORIGAMI_REQUIRE(strides[i] >= 0, "row strides must not be negative");
+  ORIGAMI_REQUIRE(table_stride >= 0, "the table stride must not be negative");
   if (tokens == 0 || requests == 0) return ORIGAMI_OK;
+  ORIGAMI_REQUIRE(query != nullptr && out != nullptr && own_tokens != nullptr &&
+                      (kv_cache != nullptr || num_blocks == 0) &&
+                      (prefix_block_ids != nullptr || prefix_tokens == 0) &&
+                      (block_tables != nullptr || max_own_tokens == 0),
+                  "queries, output, lengths, tables and the cache must not be null");
 
   const bool fp8 = cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN;
   const Plan plan = plan_of(tokens, query_heads, heads, head_dim, prefix_tokens, requests,

@@ -43,6 +43,10 @@ def _append(**kw):
     (dict(kv_cache=24), "16-byte aligned"),
     (dict(tokens=1 << 25), "too many rows"),
     (dict(query_heads=1 << 16), "too many rows"),
+    (dict(strides=[8, 8, 8, 8, -8, 8, 8, 8]), "must not be negative"),
+    (dict(key=None), "must not be null"),
+    (dict(slots=None), "must not be null"),
+    (dict(kv_cache=None), "must not be null"),
 ])
 def test_append_refuses(change, message):
     with pytest.raises(_native.OrigamiNativeError, match=message) as e:
@@ -84,6 +88,13 @@ def _attend(**kw):
     (dict(kv_cache=17), "16-byte aligned"),
     (dict(workspace_bytes=8), "workspace is too small"),
     (dict(workspace=None), "workspace is too small"),
+    (dict(strides=[8, -8, 8, 8]), "must not be negative"),
+    (dict(table_stride=-2), "must not be negative"),
+    (dict(out=None), "must not be null"),
+    (dict(own=None), "must not be null"),
+    (dict(tables=None), "must not be null"),
+    (dict(prefix_ids=None), "must not be null"),
+    (dict(kv_cache=None), "must not be null"),
 ])
 def test_attention_refuses(change, message):
     with pytest.raises(_native.OrigamiNativeError, match=message) as e:
