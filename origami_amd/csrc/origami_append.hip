@@ -7,14 +7,20 @@
 //   a' = a cos - b sin,  b' = b cos + a sin          (where a table is given)
 // in binary32, rounded once, to the type that is stored.
 //
-// It is bound by memory: every row is read and written once.  L lanes take a row, 8 channels
-// each (16 bytes of a 16-bit row), so that the mean and a pair's partner are exchanged between
-// lanes of one wave and nothing goes through LDS; the query, key and value rows of all tokens
-// are one launch, since a decode step has far too few rows to fill one with each.  A workgroup's
-// rows are of one token, whose slot, position and angles are then scalar: 48.6 us (4.2 TB/s) for
-// 8192 tokens of 32 + 8 + 8 heads of 128 with norms, where rows numbered through took 55 and 256
-// threads 51.5; three rows a lane group with their loads together took 58, and non-temporal loads
-// 63.  One token takes 2.8 us, which is a launch.
+// Every row is read and written once.  L lanes take a row, 8 channels each (16 bytes of a 16-bit
+// row), so that the mean and a pair's partner are exchanged between lanes of one wave and nothing
+// goes through LDS; the query, key and value rows of all tokens are one launch, since a decode
+// step has far too few rows to fill one with each.
+//
+// Instructions bound it before memory does: of the 16 bytes that a lane moves, a hundred or two.
+// So a workgroup is one wave with rows of one kind of one token, whose pointers, strides, slot,
+// position and angles are then scalar, the sum over a row's lanes is made of lane moves within the
+// adds, and the root is the instruction's.  8192 tokens of 32 + 8 + 8 heads of 128 with norms take
+// 38 us (5.4 TB/s) and, with nothing in a cache, 53; with kinds mixed in a wave, exchanges through
+// the LDS crossbar and the exact root and quotient it was 50 and 68.  128 threads take 42 and 52 and
+// leave half of a workgroup idle where a layer has few heads; 256 take 45; a token's workgroups in
+// a row 43; loads of weights and angles ahead of the row's sum 42.  One token takes 2.9 us, which
+// is a launch.
 #include "origami_element.h"
 #include "origami_internal.h"
 
@@ -26,7 +32,7 @@ using origami_internal::cache_geometry;
 using origami_internal::check_launch;
 using origami_internal::fail;
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 64;
 
 // Rows of one of the inputs, or of the rotated queries: element (token, head, channel) is at
 // token * token_stride + head * head_stride + channel.
@@ -49,10 +55,35 @@ struct AppendParams {
   const int64_t *positions, *slots;
   uint8_t* cache;
   int64_t blk_stride, half_stride, num_slots;  // rows of H * D, as cache_geometry
-  uint32_t block_size;
+  Divisor block_size;
   float scale[2];  // an fp8 cache holds key / scale[0] and value / scale[1]
-  int32_t tokens, row_heads, Hq, H, D;
+  int32_t Hq, H, D;
+  float inverse_D;
+  int32_t query_groups, groups;  // workgroups of a token's queries, and of its keys or values
 };
+
+template <int CTRL>
+__device__ __forceinline__ float add_lane(float v) {
+  const int o = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false);
+  return v + __builtin_bit_cast(float, o);
+}
+
+// The sum of v over L neighbouring lanes, the same bits in each of them.
+template <int L>
+__device__ __forceinline__ float sum_lanes(float v) {
+  v = add_lane<0xb1>(v);   // quad_perm 1 0 3 2
+  v = add_lane<0x4e>(v);   // quad_perm 2 3 0 1
+  v = add_lane<0x141>(v);  // the other way round in 8 lanes
+  if constexpr (L >= 16) v = add_lane<0x140>(v);  // and in 16
+  if constexpr (L >= 32) v += __shfl_xor(v, 16);
+  return v;
+}
+
+// 1 / sqrt(v) of v >= 0, to 1 ulp; small v is scaled, since the instruction takes no subnormals.
+__device__ __forceinline__ float inverse_root(float v) {
+  const bool small = v < 0x1p-96f;
+  return __builtin_amdgcn_rsqf(small ? v * 0x1p64f : v) * (small ? 0x1p32f : 1.0f);
+}
 
 template <typename T>
 __device__ __forceinline__ Vec8<T> load8(const T* p, bool vec) {
@@ -92,9 +123,7 @@ __device__ __forceinline__ void norm_rotate(const AppendParams& p, const T* row,
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
-#pragma unroll
-    for (int m = 1; m < L; m <<= 1) sum += __shfl_xor(sum, m);
-    r = 1.0f / sqrtf(sum / static_cast<float>(p.D) + p.eps);
+    r = inverse_root(sum_lanes<L>(sum) * p.inverse_D + p.eps);
     if (8 * c < p.D) {
       if (p.norm_vec && !p.norm_wide) {
         const Vec8<T> wv = *reinterpret_cast<const Vec8<T>*>(static_cast<const T*>(w) + 8 * c);
@@ -164,20 +193,27 @@ __device__ __forceinline__ void norm_rotate(const AppendParams& p, const T* row,
   for (int j = 0; j < 8; ++j) x[j] = y[j];
 }
 
-// One workgroup: kThreads / L rows of one token (blockIdx.x), whose slot, position and angles are
-// the same for all of them.
+// One workgroup: kThreads / L rows of one kind (blockIdx.y) of one token (blockIdx.x), whose
+// strides, slot, position and angles are the same for all of them.
 template <typename T, bool FP8, int L>
 __global__ __launch_bounds__(kThreads) void append_kv_kernel(AppendParams p) {
+  constexpr int kRows = kThreads / L;
   const int64_t token = blockIdx.x;
-  const int c = static_cast<int>(threadIdx.x % L);
-  int h = blockIdx.y * (kThreads / L) + threadIdx.x / L;
-  if (h >= p.row_heads) return;
-  const int kind = h < p.Hq ? 0 : (h < p.Hq + p.H ? 1 : 2);  // of the queries, keys or values
-  h -= kind == 0 ? 0 : (kind == 1 ? p.Hq : p.Hq + p.H);
+  const int c = static_cast<int>(threadIdx.x % L), row = static_cast<int>(threadIdx.x / L);
+  int group = blockIdx.y;
+  int kind = 0;  // of the queries, keys or values
+  if (group >= p.query_groups) {
+    group -= p.query_groups;
+    kind = group < p.groups ? 1 : 2;
+    group -= kind == 1 ? 0 : p.groups;
+  }
+  const int h0 = group * kRows;
+  if (h0 + row >= (kind == 0 ? p.Hq : p.H)) return;
   const bool live = 8 * c < p.D;
 
   const Rows& in = kind == 0 ? p.query : (kind == 1 ? p.key : p.value);
-  const T* const src = static_cast<const T*>(in.data) + token * in.token + h * in.head;
+  const T* const src =
+      static_cast<const T*>(in.data) + token * in.token + h0 * in.head + row * in.head;
   Vec8<T> raw = {};
   if (live) raw = load8(src + 8 * c, in.vec);
 
@@ -188,11 +224,11 @@ __global__ __launch_bounds__(kThreads) void append_kv_kernel(AppendParams p) {
     placed = pos >= 0 && pos < p.table_rows;
     table = p.cos_sin + (placed ? pos : 0) * p.rot;
   }
+  const void* const w = kind == 2 ? nullptr : p.norm[kind];
   float x[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) x[j] = static_cast<float>(raw[j]);
   if (kind != 2) {
-    const void* w = p.norm[kind];
     if (w || table) {
       norm_rotate<T, L>(p, src, w, table, c, x);
 #pragma unroll
@@ -201,17 +237,18 @@ __global__ __launch_bounds__(kThreads) void append_kv_kernel(AppendParams p) {
   }
   if (!live) return;
   if (kind == 0) {
-    store8(static_cast<T*>(p.out.data) + token * p.out.token + h * p.out.head + 8 * c, raw,
-           p.out.vec);
+    store8(static_cast<T*>(p.out.data) + token * p.out.token + h0 * p.out.head +
+               row * p.out.head + 8 * c,
+           raw, p.out.vec);
     return;
   }
   const int64_t slot = p.slots[token];
   if (!placed || slot < 0 || slot >= p.num_slots) return;
-  const uint32_t s = static_cast<uint32_t>(slot);  // num_slots fits 31 bits
-  const uint32_t block = s / p.block_size;
-  const int64_t at =
-      block * p.blk_stride + (s - block * p.block_size) + (kind == 1 ? 0 : p.half_stride);
-  const int64_t e = (at * p.H + h) * p.D + 8 * c;
+  const int at_slot = static_cast<int>(slot);  // num_slots fits 31 bits
+  const int block = divide(at_slot, p.block_size);
+  const int64_t at = block * p.blk_stride + (at_slot - block * p.block_size.d) +
+                     (kind == 1 ? 0 : p.half_stride);
+  const int64_t e = (at * p.H + h0) * p.D + (row * p.D + 8 * c);
   if constexpr (FP8) {
     const float scale = p.scale[kind - 1];
 #pragma unroll
@@ -230,18 +267,20 @@ __global__ __launch_bounds__(kThreads) void append_kv_kernel(AppendParams p) {
 }
 
 template <typename T, bool FP8, int L>
-int launch_rows(const AppendParams& p, hipStream_t stream) {
+int launch_rows(AppendParams p, uint32_t tokens, hipStream_t stream) {
   constexpr int kRows = kThreads / L;
-  const dim3 grid(p.tokens, (p.row_heads + kRows - 1) / kRows), block(kThreads);
+  p.query_groups = (p.Hq + kRows - 1) / kRows;
+  p.groups = (p.H + kRows - 1) / kRows;
+  const dim3 grid(tokens, p.query_groups + 2 * p.groups), block(kThreads);
   hipLaunchKernelGGL((append_kv_kernel<T, FP8, L>), grid, block, 0, stream, p);
   return check_launch("append_kv_kernel");
 }
 
 template <typename T, bool FP8>
-int launch_append(const AppendParams& p, hipStream_t stream) {
-  return p.D <= 64    ? launch_rows<T, FP8, 8>(p, stream)
-         : p.D <= 128 ? launch_rows<T, FP8, 16>(p, stream)
-                      : launch_rows<T, FP8, 32>(p, stream);
+int launch_append(const AppendParams& p, uint32_t tokens, hipStream_t stream) {
+  return p.D <= 64    ? launch_rows<T, FP8, 8>(p, tokens, stream)
+         : p.D <= 128 ? launch_rows<T, FP8, 16>(p, tokens, stream)
+                      : launch_rows<T, FP8, 32>(p, tokens, stream);
 }
 
 Rows rows_of(const void* data, const int64_t* strides) {
@@ -272,7 +311,7 @@ extern "C" int origami_append_kv_cache(
   if (int rc = cache_geometry(cache_layout, num_blocks, block_size, &p.blk_stride,
                               &p.half_stride))
     return rc;
-  ORIGAMI_REQUIRE(num_blocks == 0 || block_size <= INT32_MAX / num_blocks,
+  ORIGAMI_REQUIRE(block_size <= INT32_MAX / (num_blocks > 0 ? num_blocks : 1),
                   "the cache has too many token slots");
   ORIGAMI_REQUIRE(query_heads == 0 || tokens == 0 || (query != nullptr && query_out != nullptr),
                   "rotated queries need an output");
@@ -290,7 +329,7 @@ extern "C" int origami_append_kv_cache(
   ORIGAMI_REQUIRE(aligned16(kv_cache), "kv_cache must be 16-byte aligned");
   const int64_t row_heads = query_heads + 2 * heads;
   // a launch has at most 2^32 threads in x, and 65535 workgroups in y
-  ORIGAMI_REQUIRE(row_heads <= 65535 && tokens < (int64_t(1) << 32) / kThreads,
+  ORIGAMI_REQUIRE(row_heads <= 65535 && tokens < (int64_t(1) << 25),
                   "too many rows for one call");
   for (int i = 0; i < (query_heads > 0 ? 8 : 4); ++i)
     ORIGAMI_REQUIRE(strides[i] >= 0, "row strides must not be negative");
@@ -317,17 +356,17 @@ extern "C" int origami_append_kv_cache(
   p.slots = slots;
   p.cache = static_cast<uint8_t*>(kv_cache);
   p.num_slots = num_blocks * block_size;
-  p.block_size = static_cast<uint32_t>(block_size);
+  p.block_size = divisor(block_size);
   p.scale[0] = static_cast<float>(k_scale);
   p.scale[1] = static_cast<float>(v_scale);
-  p.tokens = static_cast<int32_t>(tokens);
-  p.row_heads = static_cast<int32_t>(row_heads);
   p.Hq = static_cast<int32_t>(query_heads);
   p.H = static_cast<int32_t>(heads);
   p.D = static_cast<int32_t>(head_dim);
+  p.inverse_D = 1.0f / static_cast<float>(head_dim);
   const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  const uint32_t n = static_cast<uint32_t>(tokens);
   const bool fp8 = cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN;
   if (dtype == ORIGAMI_DTYPE_BFLOAT16)
-    return fp8 ? launch_append<bf16, true>(p, stream) : launch_append<bf16, false>(p, stream);
-  return fp8 ? launch_append<f16, true>(p, stream) : launch_append<f16, false>(p, stream);
+    return fp8 ? launch_append<bf16, true>(p, n, stream) : launch_append<bf16, false>(p, n, stream);
+  return fp8 ? launch_append<f16, true>(p, n, stream) : launch_append<f16, false>(p, n, stream);
 }

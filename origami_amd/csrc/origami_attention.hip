@@ -56,17 +56,6 @@ constexpr int64_t kCus = 256;
 constexpr int kFewParts = 8;
 constexpr int kMaxParts = 1024;  // of a row: twice kCus at most of either kind
 
-// Division of 0 <= x < 2^31 by a divisor that the host knows: x / d = mulhi(x, mul) >> shift, with
-// mul the ceiling of 2^(32 + shift) / d and 2^shift < d <= 2^(shift + 1) (d = 1: shift -1).
-struct Divisor {
-  uint32_t mul;
-  int32_t d, shift;
-};
-
-__device__ __forceinline__ int divide(int x, const Divisor& by) {
-  return by.shift < 0 ? x : static_cast<int>(__umulhi(x, by.mul) >> by.shift);
-}
-
 // The work of one kind: row tiles of every KV head, over ranges of tokens.
 struct Group {
   int32_t units;   // workgroups
@@ -908,13 +897,6 @@ int launch_attend(const AttendParams& p, hipStream_t stream) {
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-Divisor divisor(int64_t d) {
-  int shift = -1;
-  while ((int64_t(1) << (shift + 1)) < d) ++shift;
-  const uint64_t mul = d == 1 ? 0 : ((uint64_t(1) << (32 + shift)) + d - 1) / d;
-  return Divisor{static_cast<uint32_t>(mul), static_cast<int32_t>(d), shift};
-}
 
 // The split of a call into units, from sizes that the host has.
 struct Plan {

@@ -50,4 +50,22 @@ __device__ __forceinline__ float fp8_clamp(float x) {
   return x != x ? x : y;
 }
 
+// Division of 0 <= x < 2^31 by a divisor that the host knows: x / d = mulhi(x, mul) >> shift, with
+// mul the ceiling of 2^(32 + shift) / d and 2^shift < d <= 2^(shift + 1) (d = 1: shift -1).
+struct Divisor {
+  uint32_t mul;
+  int32_t d, shift;
+};
+
+__device__ __forceinline__ int divide(int x, const Divisor& by) {
+  return by.shift < 0 ? x : static_cast<int>(__umulhi(x, by.mul) >> by.shift);
+}
+
+inline Divisor divisor(int64_t d) {
+  int shift = -1;
+  while ((int64_t(1) << (shift + 1)) < d) ++shift;
+  const uint64_t mul = d == 1 ? 0 : ((uint64_t(1) << (32 + shift)) + d - 1) / d;
+  return Divisor{static_cast<uint32_t>(mul), static_cast<int32_t>(d), shift};
+}
+
 }  // namespace origami_element

@@ -112,6 +112,25 @@ def test_tokens_and_heads(cuda_device, T, Hq, H):
     t.check()
 
 
+@pytest.mark.parametrize("exponent", [-66, -52, -48, -47, 0, 50])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_norm_without_eps_of_small_and_large_rows(cuda_device, exponent, D):
+    """Mean squares of 2^-132 to 2^100.  In binary32 the least lose at most D 2^-150 of
+    D 2^-132 or so, 2^-19 of their root; sums and products lose (D / 2 + 8) 2^-24.  A row of
+    zeros has no direction: 0 / 0."""
+    t = Tokens(cuda_device, D=D, Hq=5, H=3, norm=True)
+    t.rows.mul_(2.0 ** exponent)
+    t.rows[3, :8] = 0
+    query = t.run(eps=0.0)
+    key = pagedref.cells(t.cache)[0][t.slots // t.bs, t.slots % t.bs]
+    for got, x, w in ((query, t.query, t.kw["query_norm"]), (key, t.key, t.kw["key_norm"])):
+        x = x.double()
+        ref = x / x.square().mean(-1, keepdim=True).sqrt() * w.double()
+        assert ref[3].isnan().all() and got[3].isnan().all()
+        got, ref = got.double()[torch.arange(len(x)) != 3], ref[torch.arange(len(x)) != 3]
+        assert (got - ref).abs().le(2.0 ** -8 * (1 + 2.0 ** -6) * ref.abs()).all()
+
+
 def test_plain_append_is_exact(cuda_device):
     """Without a norm or a rotation rows are copied bit by bit, NaN and subnormals included."""
     for dtype in (BF16, F16):
