@@ -506,6 +506,8 @@ c10::optional<at::Tensor> append_kv_cache(
       require_rows(*query_out, "query_out", kv_cache, key.scalar_type());
       TORCH_CHECK(query_out->sizes() == query->sizes(), "query_out must have the query's shape");
       at::assert_no_internal_overlap(*query_out);
+      at::assert_no_partial_overlap(*query_out, *query);
+      for (const auto* t : {&key, &value, &kv_cache}) at::assert_no_overlap(*query_out, *t);
     }
     out = query_out ? *query_out : at::empty({tokens, query_heads, D}, query->options());
     strides[4] = query->stride(0);

@@ -264,3 +264,21 @@ def test_refusals(cuda_device):
     refused("rank 5", kv_cache=t.cache[0])
     before = t.cache.clone()
     assert torch.equal(before, t.cache)
+
+
+def test_refuses_results_over_inputs(cuda_device):
+    t = Tokens(cuda_device, T=8, Hq=2, H=2, D=64, rot=64)
+    both = torch.zeros(9, 2, 64, dtype=BF16, device=cuda_device)
+    before = t.cache.clone()
+    t.query = both[:8]
+    with pytest.raises(RuntimeError, match="overlap|single memory location"):
+        t.run(query_out=both[1:])
+    t.key = both[1:]
+    with pytest.raises(RuntimeError, match="overlap|single memory location"):
+        t.run(query_out=t.query)
+    t.key = t.value
+    cells = t.cache.view(-1)[:8 * 2 * 64].view(8, 2, 64)
+    with pytest.raises(RuntimeError, match="overlap|single memory location"):
+        t.run(query_out=cells)
+    assert torch.equal(t.cache, before) and not both.any()
+    assert t.run(query_out=t.query) is not None
