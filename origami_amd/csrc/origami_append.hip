@@ -62,20 +62,11 @@ struct AppendParams {
   int32_t query_groups, groups;  // workgroups of a token's queries, and of its keys or values
 };
 
-template <int CTRL>
-__device__ __forceinline__ float add_lane(float v) {
-  const int o = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false);
-  return v + __builtin_bit_cast(float, o);
-}
-
 // The sum of v over L neighbouring lanes, the same bits in each of them.
 template <int L>
 __device__ __forceinline__ float sum_lanes(float v) {
-  v = add_lane<0xb1>(v);   // quad_perm 1 0 3 2
-  v = add_lane<0x4e>(v);   // quad_perm 2 3 0 1
-  v = add_lane<0x141>(v);  // the other way round in 8 lanes
-  if constexpr (L >= 16) v = add_lane<0x140>(v);  // and in 16
-  if constexpr (L >= 32) v += __shfl_xor(v, 16);
+  v = fold_lanes<L == 8 ? 8 : 16>(v, [](float a, float b) { return a + b; });
+  if constexpr (L == 32) v += __shfl_xor(v, 16);
   return v;
 }
 

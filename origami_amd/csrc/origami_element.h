@@ -50,6 +50,23 @@ __device__ __forceinline__ float fp8_clamp(float x) {
   return x != x ? x : y;
 }
 
+// x of another lane of the same 16, moved without LDS.
+template <int CTRL>
+__device__ __forceinline__ float lane_moved(float x) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+}
+
+// x folded over 8 or 16 neighbouring lanes, the same bits in each of them for a commutative fold.
+template <int LANES, typename Fold>
+__device__ __forceinline__ float fold_lanes(float x, Fold fold) {
+  x = fold(x, lane_moved<0xb1>(x));   // quad_perm 1 0 3 2
+  x = fold(x, lane_moved<0x4e>(x));   // quad_perm 2 3 0 1
+  x = fold(x, lane_moved<0x141>(x));  // the other way round in 8 lanes
+  if constexpr (LANES == 16) x = fold(x, lane_moved<0x140>(x));  // and in 16
+  return x;
+}
+
 // Division of 0 <= x < 2^31 by a divisor that the host knows: x / d = mulhi(x, mul) >> shift, with
 // mul the ceiling of 2^(32 + shift) / d and 2^shift < d <= 2^(shift + 1) (d = 1: shift -1).
 struct Divisor {
