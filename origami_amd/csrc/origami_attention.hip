@@ -189,11 +189,12 @@ __device__ __forceinline__ void store4(T* dst, Float4 v, bool vec) {
 // A request's place in the batch.
 struct Request {
   int32_t first, count;  // its query tokens
-  int32_t own;           // its own tokens
+  int32_t own;           // its own tokens, up to the bound
+  int32_t before;        // of all its own tokens, those before its queries (may be negative)
 };
 
 __device__ __forceinline__ Request request_of(const AttendParams& p, int r) {
-  Request q{r, 1, 0};
+  Request q{r, 1, 0, 0};
   if (p.starts) {
     const int64_t n = p.tokens;
     const int64_t a = min(max(p.starts[r], int64_t(0)), n);
@@ -201,8 +202,12 @@ __device__ __forceinline__ Request request_of(const AttendParams& p, int r) {
     q.first = static_cast<int32_t>(a);
     q.count = static_cast<int32_t>(min(b - a, static_cast<int64_t>(p.max_query)));
   }
-  q.own = static_cast<int32_t>(
-      min(max(p.own_tokens[r], int64_t(0)), static_cast<int64_t>(p.max_own)));
+  // The queries' places follow from the whole length; the bound only hides tokens.  Lengths past
+  // any bound (2^30) and any number of queries (2^24) besides are the same.
+  const int32_t length =
+      static_cast<int32_t>(min(max(p.own_tokens[r], int64_t(0)), int64_t(3) << 29));
+  q.own = min(length, p.max_own);
+  q.before = length - q.count;
   return q;
 }
 
@@ -333,7 +338,7 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
   const int64_t first = block_of(t + tl, bound);
   int64_t ahead = block_of(t + kRound + tl, bound);
 
-  const Request rq = batch ? Request{0, p.tokens, 0} : request_of(p, r);
+  const Request rq = batch ? Request{0, p.tokens, 0, 0} : request_of(p, r);
   const int rows = rq.count * p.G.d, row0 = tile * WR * MR;
   if (row0 >= rows) return;
   const int end = batch ? p.prefix : p.prefix + rq.own;  // of the tokens, prefix first
@@ -342,7 +347,7 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
   const int row = row0 + wr * MR + c;
   const auto seen_by = [&](int i) -> int {  // tokens that row i sees
     return p.prefix +
-           (batch ? 0 : min(max(rq.own - rq.count + divide(i, p.G) + 1, 0), rq.own));
+           (batch ? 0 : min(max(rq.before + divide(i, p.G) + 1, 0), rq.own));
   };
   const int limit = seen_by(row);
   // the scale's sign goes with the queries, and so does a scale of zero, so that hidden scores of

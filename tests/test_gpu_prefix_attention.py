@@ -368,3 +368,40 @@ def test_refusals(cuda_device):
     refused("out must have", out=b.query[:1].clone())
     refused("rank 5", kv_cache=b.cache[0])
     refused("contiguous", kv_cache=b.cache[:, :, :, :1])
+
+
+@pytest.mark.parametrize("own,queries,bound", [((20,), (5,), 10), ((20, 7), (5, 7), 10),
+                                               ((300, 41, 3), (40, 1, 9), 200),
+                                               ((600, 90), (200, 90), 450), ((30, 12), (3, 4), 0)])
+@pytest.mark.parametrize("prefix", [0, 75, 900])
+def test_lengths_above_the_bound(cuda_device, own, queries, bound, prefix):
+    """A row's place follows from its request's whole length, and the bound only hides tokens: each
+    row against a request of its own that has the tokens the row sees."""
+    b = Batch(cuda_device, prefix=prefix, own=own, queries=queries, heads=2, group=3, D=64)
+    got = b.run(max_own_tokens=bound)
+    seen = [min(max(n - c + i + 1, 0), bound) for n, c in zip(own, queries) for i in range(c)]
+    count = torch.tensor(queries, device=cuda_device)
+    b.tables = torch.repeat_interleave(b.tables, count, 0)
+    b.own, b.starts = torch.tensor(seen, device=cuda_device), None
+    b.check(*got)
+
+
+def test_lengths_above_the_block_tables(cuda_device):
+    """The same where the bound is what the tables hold."""
+    b = Batch(cuda_device, prefix=50, own=(64, 64), queries=(9, 5), D=64)
+    b.own.copy_(torch.tensor([70, 66]))
+    got = b.run()
+    seen = [min(70 - 9 + i + 1, 64) for i in range(9)] + [min(66 - 5 + i + 1, 64) for i in range(5)]
+    b.tables = torch.repeat_interleave(b.tables, torch.tensor([9, 5], device=cuda_device), 0)
+    b.own, b.starts = torch.tensor(seen, device=cuda_device), None
+    b.check(*got)
+
+
+@pytest.mark.parametrize("far", [1 << 31, (1 << 40) + 7, (1 << 62)])
+def test_lengths_past_32_bits(cuda_device, far):
+    b = Batch(cuda_device, prefix=50, own=(64, 33), queries=(9, 5), D=64)
+    b.own[0] = far
+    got, _ = b.run()
+    b.own[0] = 64 + 9
+    want, _ = b.run()
+    assert torch.equal(got, want)
