@@ -318,9 +318,9 @@ extern "C" int origami_append_kv_cache(
   ORIGAMI_REQUIRE(cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN || (k_scale == 1.0 && v_scale == 1.0),
                   "cache scales are for float8_e4m3fn caches");
   ORIGAMI_REQUIRE(aligned16(kv_cache), "kv_cache must be 16-byte aligned");
-  const int64_t row_heads = query_heads + 2 * heads;
   // a launch has at most 2^32 threads in x, and 65535 workgroups in y
-  ORIGAMI_REQUIRE(row_heads <= 65535 && tokens < (int64_t(1) << 25),
+  ORIGAMI_REQUIRE(heads <= 65535 && query_heads <= 65535 - 2 * heads &&
+                      tokens < (int64_t(1) << 25),
                   "too many rows for one call");
   for (int i = 0; i < (query_heads > 0 ? 8 : 4); ++i)
     ORIGAMI_REQUIRE(strides[i] >= 0, "row strides must not be negative");

@@ -55,6 +55,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int64_t kCus = 256;
 constexpr int kFewParts = 8;
 constexpr int kMaxParts = 1024;  // of a row: twice kCus at most of either kind
+constexpr int64_t kMostUnits = (int64_t(1) << 32) / 512;  // workgroups of 512 threads in a launch
 
 // The work of one kind: row tiles of every KV head, over ranges of tokens.
 struct Group {
@@ -1038,9 +1039,12 @@ int check_sizes(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head
   ORIGAMI_REQUIRE(tokens >= 0 && requests >= 0 && prefix_tokens >= 0 && max_query >= 0 &&
                       max_own >= 0,
                   "token counts must not be negative");
-  ORIGAMI_REQUIRE(prefix_tokens + max_own <= (int64_t(1) << 30), "too many tokens for one call");
-  // a launch has at most 2^32 threads in x
+  constexpr int64_t kMostTokens = int64_t(1) << 30;
+  ORIGAMI_REQUIRE(prefix_tokens <= kMostTokens && max_own <= kMostTokens - prefix_tokens,
+                  "too many tokens for one call");
+  // a launch has at most 2^32 threads in x; every request has a workgroup a head at least
   ORIGAMI_REQUIRE(tokens < (int64_t(1) << 24) / query_heads, "too many query rows for one call");
+  ORIGAMI_REQUIRE(requests < kMostUnits / heads, "too many requests for one call");
   return ORIGAMI_OK;
 }
 
@@ -1084,7 +1088,7 @@ int origami_shared_prefix_attention(
   if (int rc = cache_geometry(cache_layout, num_blocks, block_size, &p.blk_stride,
                               &p.half_stride))
     return rc;
-  ORIGAMI_REQUIRE(num_blocks == 0 || block_size <= INT32_MAX / 2 / num_blocks,
+  ORIGAMI_REQUIRE(block_size <= INT32_MAX / 2 / std::max<int64_t>(num_blocks, 1),
                   "the cache has too many token slots");
   ORIGAMI_REQUIRE(prefix_block_count >= 0 && table_blocks >= 0 &&
                       ceil_div(prefix_tokens, block_size) <= prefix_block_count,
@@ -1111,7 +1115,7 @@ int origami_shared_prefix_attention(
   const bool fp8 = cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN;
   const Plan plan = plan_of(tokens, query_heads, heads, head_dim, prefix_tokens, requests,
                             max_query_tokens, max_own_tokens, fp8 ? 1 : 2);
-  ORIGAMI_REQUIRE(plan.units < (int64_t(1) << 32) / 512, "too many row tiles for one call");
+  ORIGAMI_REQUIRE(plan.units < kMostUnits, "too many row tiles for one call");
   ORIGAMI_REQUIRE(workspace_bytes >= workspace_bytes_of(plan, tokens, query_heads, head_dim) &&
                       (plan.slots == 1 || workspace != nullptr) && aligned16(workspace),
                   "attention workspace is too small");

@@ -591,7 +591,11 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
               "without query_starts every request has one query token");
   const int64_t most =
       max_query_tokens ? *max_query_tokens : (starts ? tokens : std::min<int64_t>(tokens, 1));
-  const int64_t most_own = max_own_tokens ? *max_own_tokens : blocks * g.block_size;
+  int64_t most_own;  // the block tables' slots; what 64 bits do not hold is refused as too many
+  if (max_own_tokens)
+    most_own = *max_own_tokens;
+  else if (__builtin_mul_overflow(blocks, g.block_size, &most_own))
+    most_own = INT64_MAX;
   const c10::OptionalDeviceGuard guard(kv_cache.device());
 
   at::Tensor out;

@@ -108,3 +108,44 @@ def test_workspace_sizes():
     assert size(0, 4, 2, 64, 32, 3, 0, 32, BF16) == 0
     assert size(3, 3, 2, 64, 32, 3, 1, 32, BF16) == -1
     assert size(1, 4, 2, 64, 0, 1, 1, 16, FP8) == 0  # one part: the rows are written at once
+
+
+INF, NAN, BIG = float("inf"), float("nan"), 1 << 62
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(heads=BIG), "too many rows"),
+    (dict(heads=BIG + (1 << 15)), "too many rows"),
+    (dict(query_heads=BIG, heads=BIG), "too many rows"),
+    (dict(num_blocks=0, block_size=1 << 40), "too many token slots"),
+])
+def test_append_refuses_sizes_past_its_integers(change, message):
+    with pytest.raises(_native.OrigamiNativeError, match=message) as e:
+        _append(**change)
+    assert e.value.code == _native.ORIGAMI_ERR_INVALID
+
+
+@pytest.mark.parametrize("change,message", [
+    # a block size that 32 bits do not hold would give block numbers past the tables
+    (dict(num_blocks=0, block_size=1 << 40, prefix_blocks=1, table_blocks=1),
+     "too many token slots"),
+    (dict(num_blocks=0, block_size=(1 << 32) + 1, prefix_blocks=1, table_blocks=1),
+     "too many token slots"),
+    (dict(prefix=BIG, max_own=BIG, prefix_blocks=BIG, table_blocks=BIG), "too many tokens"),
+    (dict(prefix=0, max_own=BIG + BIG - 1, table_blocks=BIG), "too many tokens"),
+    (dict(starts=16, requests=1 << 40), "too many requests"),
+    (dict(starts=16, requests=BIG), "too many requests"),
+    (dict(starts=16, requests=BIG, tokens=0), "too many requests"),
+    (dict(query_heads=BIG, heads=BIG, tokens=0), "too many query rows"),
+])
+def test_attention_refuses_sizes_past_its_integers(change, message):
+    with pytest.raises(_native.OrigamiNativeError, match=message) as e:
+        _attend(**change)
+    assert e.value.code == _native.ORIGAMI_ERR_INVALID
+
+
+def test_workspace_refuses_sizes_past_its_integers():
+    size = _native.lib().origami_shared_prefix_attention_workspace
+    assert size(3, 4, 2, 64, BIG, 3, 1, BIG, BF16) == -1
+    assert size(3, 4, 2, 64, 32, BIG, 1, 32, BF16) == -1
+    assert size(3, 4, 2, 64, 32, 1 << 23, 1, 32, BF16) == -1
