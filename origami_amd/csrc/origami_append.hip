@@ -21,6 +21,8 @@
 // leave half of a workgroup idle where a layer has few heads; 256 take 45; a token's workgroups in
 // a row 43; loads of weights and angles ahead of the row's sum 42.  One token takes 2.9 us, which
 // is a launch.
+#include <cmath>
+
 #include "origami_element.h"
 #include "origami_internal.h"
 
@@ -29,6 +31,7 @@ namespace {
 using namespace origami_element;
 using origami_internal::aligned16;
 using origami_internal::cache_geometry;
+using origami_internal::cache_scale;
 using origami_internal::check_launch;
 using origami_internal::fail;
 
@@ -313,8 +316,10 @@ extern "C" int origami_append_kv_cache(
   ORIGAMI_REQUIRE((query_norm == nullptr && key_norm == nullptr) || norm_dtype == dtype ||
                       norm_dtype == ORIGAMI_DTYPE_FLOAT32,
                   "norm weights must have the keys' dtype or be float32");
-  ORIGAMI_REQUIRE(eps >= 0.0, "eps must not be negative");
-  ORIGAMI_REQUIRE(k_scale > 0.0 && v_scale > 0.0, "cache scales must be positive");
+  ORIGAMI_REQUIRE(eps >= 0.0 && std::isfinite(static_cast<float>(eps)),
+                  "eps must not be negative or infinite");
+  ORIGAMI_REQUIRE(cache_scale(k_scale) && cache_scale(v_scale),
+                  "cache scales must be positive and finite in binary32");
   ORIGAMI_REQUIRE(cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN || (k_scale == 1.0 && v_scale == 1.0),
                   "cache scales are for float8_e4m3fn caches");
   ORIGAMI_REQUIRE(aligned16(kv_cache), "kv_cache must be 16-byte aligned");

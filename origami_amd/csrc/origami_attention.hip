@@ -17,6 +17,7 @@
 // up to 1024 tokens after 8192, at about 40% of the matrix cycles, where a large library
 // product reaches 1150.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "origami_element.h"
@@ -27,6 +28,7 @@ namespace {
 using namespace origami_element;
 using origami_internal::aligned16;
 using origami_internal::cache_geometry;
+using origami_internal::cache_scale;
 using origami_internal::check_launch;
 using origami_internal::fail;
 
@@ -1098,7 +1100,10 @@ int origami_shared_prefix_attention(
   ORIGAMI_REQUIRE(query_starts != nullptr || tokens == requests,
                   "without query_starts every request has one query token");
   max_query_tokens = std::min(max_query_tokens, tokens);
-  ORIGAMI_REQUIRE(k_scale > 0.0 && v_scale > 0.0, "cache scales must be positive");
+  ORIGAMI_REQUIRE(cache_scale(k_scale) && cache_scale(v_scale),
+                  "cache scales must be positive and finite in binary32");
+  const float log2_scale = static_cast<float>(scale * k_scale) * kLog2e;
+  ORIGAMI_REQUIRE(std::isfinite(log2_scale), "scale must be finite in binary32");
   ORIGAMI_REQUIRE(cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN || (k_scale == 1.0 && v_scale == 1.0),
                   "cache scales are for float8_e4m3fn caches");
   ORIGAMI_REQUIRE(aligned16(kv_cache), "kv_cache must be 16-byte aligned");
@@ -1144,7 +1149,7 @@ int origami_shared_prefix_attention(
   p.H = divisor(heads);
   p.G = divisor(query_heads / heads);
   p.D = static_cast<int32_t>(head_dim);
-  p.scale = static_cast<float>(scale * k_scale) * kLog2e;
+  p.scale = log2_scale;
   p.v_scale = static_cast<float>(v_scale);
   p.group[0] = plan.group[0];
   p.group[1] = plan.group[1];

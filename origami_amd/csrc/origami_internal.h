@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <float.h>
 #include <stdint.h>
 
 #include <string>
@@ -25,6 +26,12 @@ int cache_geometry(int64_t cache_layout, int64_t num_blocks, int64_t block_size,
                    int64_t* blk_stride, int64_t* half_stride);
 
 inline bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
+
+// Whether a scale of cache entries is one in binary32 too.
+inline bool cache_scale(double scale) {
+  const float f = static_cast<float>(scale);
+  return f > 0.0f && f <= FLT_MAX;
+}
 
 inline unsigned grid_for(int64_t work, int64_t per_block, int64_t cap) {
   int64_t g = (work + per_block - 1) / per_block;

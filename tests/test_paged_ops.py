@@ -149,3 +149,31 @@ def test_workspace_refuses_sizes_past_its_integers():
     assert size(3, 4, 2, 64, BIG, 3, 1, BIG, BF16) == -1
     assert size(3, 4, 2, 64, 32, BIG, 1, 32, BF16) == -1
     assert size(3, 4, 2, 64, 32, 1 << 23, 1, 32, BF16) == -1
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(eps=INF), "eps must not be negative or infinite"),
+    (dict(eps=1e39), "eps must not be negative or infinite"),
+    (dict(cache_dtype=FP8, k_scale=INF), "scales must be positive"),
+    (dict(cache_dtype=FP8, v_scale=1e39), "scales must be positive"),
+    (dict(cache_dtype=FP8, k_scale=1e-60), "scales must be positive"),
+])
+def test_append_refuses_numbers_that_binary32_does_not_hold(change, message):
+    with pytest.raises(_native.OrigamiNativeError, match=message) as e:
+        _append(**change)
+    assert e.value.code == _native.ORIGAMI_ERR_INVALID
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(scale=NAN), "scale must be finite"),
+    (dict(scale=-INF), "scale must be finite"),
+    (dict(scale=3e38), "scale must be finite"),  # times log2 e
+    (dict(cache_dtype=FP8, scale=1e30, k_scale=1e10), "scale must be finite"),
+    (dict(cache_dtype=FP8, k_scale=INF), "scales must be positive"),
+    (dict(cache_dtype=FP8, v_scale=1e39), "scales must be positive"),
+    (dict(cache_dtype=FP8, v_scale=1e-60), "scales must be positive"),
+])
+def test_attention_refuses_numbers_that_binary32_does_not_hold(change, message):
+    with pytest.raises(_native.OrigamiNativeError, match=message) as e:
+        _attend(**change)
+    assert e.value.code == _native.ORIGAMI_ERR_INVALID
