@@ -1032,6 +1032,12 @@ int64_t workspace_bytes_of(const Plan& plan, int64_t tokens, int64_t query_heads
   return plan.slots > 1 ? plan.slots * tokens * query_heads * (head_dim + 2) * 4 : 0;
 }
 
+// A request's query tokens at most: no more than there are, and one, which each has where no
+// query_starts say otherwise.
+int64_t bound_of_queries(int64_t max_query, int64_t tokens) {
+  return std::max<int64_t>(std::min(max_query, tokens), 1);
+}
+
 int check_sizes(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_dim,
                 int64_t prefix_tokens, int64_t requests, int64_t max_query, int64_t max_own) {
   ORIGAMI_REQUIRE(heads > 0 && query_heads > 0 && query_heads % heads == 0,
@@ -1063,7 +1069,7 @@ int64_t origami_shared_prefix_attention_workspace(int64_t tokens, int64_t query_
   if (check_sizes(tokens, query_heads, heads, head_dim, prefix_tokens, requests, max_query_tokens,
                   max_own_tokens))
     return -1;
-  max_query_tokens = std::min(max_query_tokens, tokens);
+  max_query_tokens = bound_of_queries(max_query_tokens, tokens);
   return workspace_bytes_of(plan_of(tokens, query_heads, heads, head_dim, prefix_tokens,
                                     requests, max_query_tokens, max_own_tokens, cell_bytes),
                             tokens, query_heads, head_dim);
@@ -1099,7 +1105,7 @@ int origami_shared_prefix_attention(
                   "max_own_tokens exceeds the block tables");
   ORIGAMI_REQUIRE(query_starts != nullptr || tokens == requests,
                   "without query_starts every request has one query token");
-  max_query_tokens = std::min(max_query_tokens, tokens);
+  max_query_tokens = bound_of_queries(max_query_tokens, tokens);
   ORIGAMI_REQUIRE(cache_scale(k_scale) && cache_scale(v_scale),
                   "cache scales must be positive and finite in binary32");
   const float log2_scale = static_cast<float>(scale * k_scale) * kLog2e;

@@ -405,3 +405,12 @@ def test_lengths_past_32_bits(cuda_device, far):
     b.own[0] = 64 + 9
     want, _ = b.run()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("group", [1, 16, 17, 40, 200])
+@pytest.mark.parametrize("own", [(20, 3), (2000,)])
+def test_one_query_each_whatever_the_bound(cuda_device, group, own):
+    """Without query_starts every request has one query, and a bound of none says nothing."""
+    b = Batch(cuda_device, prefix=40, own=own, D=64, heads=1, group=group)
+    out = torch.full_like(b.query, math.nan)
+    b.check(*b.run(max_query_tokens=0, out=out))
