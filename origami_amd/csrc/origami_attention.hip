@@ -623,6 +623,8 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
       // without a token the join does not read the rest
       if (sum != 0.0f) *reinterpret_cast<Float4*>(p.part_o + slot * p.D + ch) = v;
     } else {
+      // a row without a weight is zero also where a value is infinite or NaN
+      if (sum == 0.0f) v = Float4{0.0f, 0.0f, 0.0f, 0.0f};
       const float inv = sum == 0.0f ? 0.0f : p.v_scale / sum;
       store4(static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + ch, v * inv, p.out_vec);
       if (p.lse && ch == 0)

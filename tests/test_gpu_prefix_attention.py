@@ -414,3 +414,19 @@ def test_one_query_each_whatever_the_bound(cuda_device, group, own):
     b = Batch(cuda_device, prefix=40, own=own, D=64, heads=1, group=group)
     out = torch.full_like(b.query, math.nan)
     b.check(*b.run(max_query_tokens=0, out=out))
+
+
+@pytest.mark.parametrize("own", [(20,), (20, 3), (3000, 40)])  # one part, and several
+@pytest.mark.parametrize("group", [2, 40])
+@pytest.mark.parametrize("value", [math.inf, math.nan, 1.0])
+def test_rows_of_scores_of_minus_infinity(cuda_device, own, group, value):
+    """Tokens that are seen, with nothing but scores of -infinity: the row is zero, whatever
+    the values are."""
+    b = Batch(cuda_device, prefix=0, own=own, D=64, heads=1, group=group)
+    b.cache[0, :, :, :, 0] = -math.inf
+    b.cache[1, :, :, :, 3] = value
+    b.query[:, ::2, 0] = 1.0
+    b.query[:, 1::2, 0] = -1.0  # the others see scores of infinity: no defined weights
+    got, lse = b.run()
+    assert not got[:, ::2].any() and (lse[:, ::2] == -math.inf).all()
+    assert got[:, 1::2].isnan().all()
