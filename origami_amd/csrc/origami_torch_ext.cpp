@@ -11,8 +11,11 @@
 #include <torch/extension.h>
 
 #include <ATen/MemoryOverlap.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <cmath>
@@ -445,26 +448,49 @@ int64_t paged_dtype_code(at::ScalarType t, const char* name) {
   return dtype_code(t, name);
 }
 
-void require_no_grad(const at::Tensor& t, const char* name) {
+// No record is kept of operations: it would leave a launch on addresses out, and play back what
+// this call gave.
+void require_eager() {
+  using c10::impl::TorchDispatchModeKey;
+  bool recorded = torch::jit::tracer::isTracing();
+  for (const auto mode : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY,
+                          TorchDispatchModeKey::FUNCTIONAL})
+    recorded |= c10::impl::TorchDispatchModeTLS::get_mode(mode).has_value();
+  TORCH_CHECK(!recorded, "this operator cannot be traced");
+}
+
+// A tensor whose memory holds its values, and of which no gradient or tangent is asked.
+void require_plain(const at::Tensor& t, const char* name) {
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet kOdd(
+      {DispatchKey::Python, DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper,
+       DispatchKey::Batched, DispatchKey::Functionalize, DispatchKey::ZeroTensor,
+       DispatchKey::Conjugate, DispatchKey::Negative});
+  TORCH_CHECK(t.layout() == at::kStrided && !t.key_set().has_any(kOdd), name,
+              " must be a plain tensor, not a wrapped, transformed or lazily negated one");
   TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), name,
               " requires a gradient, which this operator does not have");
+  TORCH_CHECK(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+                t._fw_grad(0).defined()),
+              name, " requires a gradient (it has a tangent), which this operator does not have");
 }
 
 // A [tokens, heads, head_dim] tensor whose channels are contiguous.
 void require_rows(const at::Tensor& t, const char* name, const at::Tensor& cache,
                   at::ScalarType dtype) {
+  require_plain(t, name);
   TORCH_CHECK(t.is_cuda() && t.device() == cache.device(), name,
               " must be on the kv_cache device");
   TORCH_CHECK(t.dim() == 3, name, " must be [tokens, heads, head_dim]");
   TORCH_CHECK(t.scalar_type() == dtype, name, " must have the same dtype as the other rows");
   TORCH_CHECK(t.size(2) == cache.size(4), name, " head_dim differs from the kv_cache's");
   TORCH_CHECK(t.stride(2) == 1 || t.numel() == 0, name, " channels must be contiguous");
-  require_no_grad(t, name);
 }
 
 // A contiguous int64 tensor of at least `count` values; null when it has none.
 const int64_t* require_index(const at::Tensor& t, const char* name, const at::Tensor& cache,
                              int64_t count) {
+  require_plain(t, name);
   TORCH_CHECK(t.is_cuda() && t.device() == cache.device(), name,
               " must be on the kv_cache device");
   TORCH_CHECK(t.scalar_type() == at::kLong && t.dim() == 1 && t.is_contiguous(), name,
@@ -481,8 +507,9 @@ c10::optional<at::Tensor> append_kv_cache(
     c10::optional<at::Tensor> cos_sin, bool interleaved, c10::optional<at::Tensor> query_norm,
     c10::optional<at::Tensor> key_norm, double eps, double k_scale, double v_scale,
     c10::optional<at::Tensor> query_out) {
+  require_eager();
+  require_plain(kv_cache, "kv_cache");
   require_device(kv_cache, "kv_cache");
-  require_no_grad(kv_cache, "kv_cache");
   const CacheGeom g = layout_cache_geometry(kv_cache);
   const int64_t dtype = paged_dtype_code(key.scalar_type(), "key");
   TORCH_CHECK(dtype != ORIGAMI_DTYPE_FLOAT8_E4M3FN, "key must be float16 or bfloat16");
@@ -524,8 +551,8 @@ c10::optional<at::Tensor> append_kv_cache(
               "rotation needs both positions and cos_sin");
   if (cos_sin) {
     position = require_index(*positions, "positions", kv_cache, tokens);
+    require_plain(*cos_sin, "cos_sin");
     require_device(*cos_sin, "cos_sin");
-    require_no_grad(*cos_sin, "cos_sin");
     TORCH_CHECK(cos_sin->device() == kv_cache.device(), "cos_sin must be on the kv_cache device");
     TORCH_CHECK(cos_sin->scalar_type() == at::kFloat && cos_sin->dim() == 2,
                 "cos_sin must be float32 [positions, rotary_dim]");
@@ -535,8 +562,8 @@ c10::optional<at::Tensor> append_kv_cache(
   int64_t norm_dtype = dtype;
   for (const auto* norm : {&query_norm, &key_norm})
     if (*norm) {
+      require_plain(**norm, "norm weights");
       require_device(**norm, "norm weights");
-      require_no_grad(**norm, "norm weights");
       TORCH_CHECK((*norm)->device() == kv_cache.device(),
                   "norm weights must be on the kv_cache device");
       TORCH_CHECK((*norm)->dim() == 1 && (*norm)->numel() == D,
@@ -566,13 +593,15 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
                                    c10::optional<int64_t> max_own_tokens,
                                    c10::optional<double> scale, double k_scale, double v_scale,
                                    c10::optional<at::Tensor> out_, c10::optional<at::Tensor> lse) {
+  require_eager();
+  require_plain(kv_cache, "kv_cache");
   require_device(kv_cache, "kv_cache");
-  require_no_grad(kv_cache, "kv_cache");
   const CacheGeom g = layout_cache_geometry(kv_cache);
   const int64_t dtype = paged_dtype_code(query.scalar_type(), "query");
   TORCH_CHECK(dtype != ORIGAMI_DTYPE_FLOAT8_E4M3FN, "query must be float16 or bfloat16");
   require_rows(query, "query", kv_cache, query.scalar_type());
   const int64_t tokens = query.size(0), Hq = query.size(1), D = kv_cache.size(4);
+  require_plain(block_tables, "block_tables");
   TORCH_CHECK(block_tables.is_cuda() && block_tables.device() == kv_cache.device(),
               "block_tables must be on the kv_cache device");
   TORCH_CHECK(block_tables.scalar_type() == at::kLong && block_tables.dim() == 2 &&
@@ -611,6 +640,7 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
                  : at::empty({tokens, Hq, D}, query.options());
   }
   if (lse) {
+    require_plain(*lse, "lse");
     require_device(*lse, "lse");
     TORCH_CHECK(lse->device() == kv_cache.device() && lse->scalar_type() == at::kFloat &&
                     lse->dim() == 2 && lse->size(0) == tokens && lse->size(1) == Hq,
