@@ -462,7 +462,9 @@ int origami_kivi_quantize(const void* kv, int64_t dtype, int64_t tokens, int64_t
  * one whose position is outside the table, and its query row becomes zero.
  * Slots inside the cache must be distinct: which of two tokens a slot holds
  * afterwards is not defined.  head_dim is a multiple of 8, at most 256; kv_cache
- * is 16-byte aligned.
+ * is 16-byte aligned.  The cache and query_out share no memory with each other or
+ * with an input (but query_out with query, if it is all of it), and query_out has no
+ * element twice: workgroups have no order.  The Python module refuses such calls.
  */
 int origami_append_kv_cache(
     const void* key, const void* value, const void* query, void* query_out, int64_t dtype,
@@ -503,7 +505,9 @@ int origami_append_kv_cache(
  * result once more.  workspace is a 16-byte aligned device buffer of at least
  * origami_shared_prefix_attention_workspace bytes (0: may be null; -1: invalid
  * sizes), in use until the call's work is done; calls that can run at the same
- * time need their own.  Results do not depend on timing.
+ * time need their own.  out, lse and workspace share no memory with each other or
+ * with an input, and out has no element twice (the Python module refuses such
+ * calls).  Results do not depend on timing.
  */
 int64_t origami_shared_prefix_attention_workspace(
     int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_dim, int64_t prefix_tokens,

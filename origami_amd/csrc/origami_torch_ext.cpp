@@ -10,7 +10,6 @@
 // way the reference's TORCH_CHECKs raise.  There is no device code here.
 #include <torch/extension.h>
 
-#include <ATen/MemoryOverlap.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -475,6 +474,117 @@ void require_plain(const at::Tensor& t, const char* name) {
               name, " requires a gradient (it has a tangent), which this operator does not have");
 }
 
+// The bytes of a strided tensor: runs at every sum of count[i] multiples of step[i].
+struct Extent {
+  const char* base = nullptr;
+  int64_t run = 0;  // bytes; 0: no elements
+  int dims = 0;
+  int64_t count[8], step[8];
+  bool repeated = false;  // several indices have one address
+};
+
+Extent extent_of(const at::Tensor& t) {
+  Extent e;
+  if (t.numel() == 0) return e;
+  e.base = static_cast<const char*>(t.data_ptr());
+  e.run = t.element_size();
+  TORCH_CHECK(t.dim() <= 8, "tensors of more than 8 dimensions are not compared");
+  for (int64_t d = t.dim() - 1; d >= 0; --d) {
+    const int64_t n = t.size(d), step = t.stride(d) * t.element_size();
+    if (n == 1) continue;
+    if (step == 0) {
+      e.repeated = true;
+    } else if (step == e.run && e.dims == 0) {
+      e.run *= n;
+    } else {
+      e.count[e.dims] = n;
+      e.step[e.dims++] = step;
+    }
+  }
+  return e;
+}
+
+// Multiples first .. last of a step.
+struct Multiples {
+  int64_t step, first, last;
+};
+
+// Whether a sum of one multiple of each of p[0 .. n - 1] is in [low, high].  With the largest steps
+// first, few multiples of each leave the rest a chance.
+bool some_sum_within(const Multiples* p, int n, int64_t low, int64_t high) {
+  if (n == 0) return low <= 0 && high >= 0;
+  int64_t least = 0, most = 0;  // what the others add
+  for (int i = 1; i < n; ++i) {
+    least += p[i].first * p[i].step;
+    most += p[i].last * p[i].step;
+  }
+  const auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+  const int64_t first = std::max(p->first, -floor_div(most - low, p->step));
+  const int64_t last = std::min(p->last, floor_div(high - least, p->step));
+  if (n == 1) return first <= last;
+  for (int64_t i = first; i <= last; ++i)
+    if (some_sum_within(p + 1, n - 1, low - i * p->step, high - i * p->step)) return true;
+  return false;
+}
+
+void largest_first(Multiples* p, int n) {
+  std::sort(p, p + n, [](const Multiples& a, const Multiples& b) { return a.step > b.step; });
+}
+
+bool share_bytes(const Extent& a, const Extent& b) {
+  if (a.run == 0 || b.run == 0) return false;
+  Multiples p[16];
+  int n = 0;
+  int64_t a_end = a.run, b_end = b.run;
+  for (int i = 0; i < a.dims; ++i) {
+    a_end += (a.count[i] - 1) * a.step[i];
+    p[n++] = {a.step[i], 1 - a.count[i], 0};
+  }
+  const int from_a = n;
+  for (int i = 0; i < b.dims; ++i) {
+    b_end += (b.count[i] - 1) * b.step[i];
+    int at = 0;
+    while (at < from_a && p[at].step != b.step[i]) ++at;
+    if (at < from_a)
+      p[at].last += b.count[i] - 1;
+    else
+      p[n++] = {b.step[i], 0, b.count[i] - 1};
+  }
+  const int64_t apart = b.base - a.base;
+  if (apart >= a_end || -apart >= b_end) return false;
+  // a run of b starts less than a.run after one of a, or less than b.run before it
+  largest_first(p, n);
+  return some_sum_within(p, n, -apart - (b.run - 1), -apart + a.run - 1);
+}
+
+// Whether two elements of a tensor share bytes.
+bool shares_with_itself(const Extent& e) {
+  if (e.run == 0) return false;
+  if (e.repeated) return true;
+  Multiples p[8];
+  for (int i = 0; i < e.dims; ++i) p[i] = {e.step[i], 1 - e.count[i], e.count[i] - 1};
+  largest_first(p, e.dims);
+  for (int i = 0; i < e.dims; ++i) {  // pairs that differ in p[i] first
+    p[i].first = 1;
+    if (some_sum_within(p + i, e.dims - i, 1 - e.run, e.run - 1)) return true;
+  }
+  return false;
+}
+
+bool same_elements(const at::Tensor& a, const at::Tensor& b) {
+  if (a.data_ptr() != b.data_ptr() || a.sizes() != b.sizes()) return false;
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+
+// What a call writes may not be what it reads: launches have no order between their workgroups.
+void require_apart(const at::Tensor& result, const char* result_name, const at::Tensor& input,
+                   const char* name) {
+  TORCH_CHECK(!share_bytes(extent_of(result), extent_of(input)), result_name,
+              " must not overlap ", name);
+}
+
 // A [tokens, heads, head_dim] tensor whose channels are contiguous.
 void require_rows(const at::Tensor& t, const char* name, const at::Tensor& cache,
                   at::ScalarType dtype) {
@@ -532,9 +642,9 @@ c10::optional<at::Tensor> append_kv_cache(
     if (query_out) {
       require_rows(*query_out, "query_out", kv_cache, key.scalar_type());
       TORCH_CHECK(query_out->sizes() == query->sizes(), "query_out must have the query's shape");
-      at::assert_no_internal_overlap(*query_out);
-      at::assert_no_partial_overlap(*query_out, *query);
-      for (const auto* t : {&key, &value, &kv_cache}) at::assert_no_overlap(*query_out, *t);
+      TORCH_CHECK(!shares_with_itself(extent_of(*query_out)), "query_out must not overlap itself");
+      if (!same_elements(*query_out, *query))
+        require_apart(*query_out, "query_out", *query, "another row's query");
     }
     out = query_out ? *query_out : at::empty({tokens, query_heads, D}, query->options());
     strides[4] = query->stride(0);
@@ -572,6 +682,21 @@ c10::optional<at::Tensor> append_kv_cache(
     }
   TORCH_CHECK(!query_norm || !key_norm || query_norm->scalar_type() == key_norm->scalar_type(),
               "norm weights must have the same dtype");
+  const auto apart = [&](const at::Tensor& t, const char* name) {
+    require_apart(kv_cache, "kv_cache", t, name);
+    if (query_out) require_apart(*query_out, "query_out", t, name);
+  };
+  apart(key, "key");
+  apart(value, "value");
+  apart(slots, "slots");
+  if (query) require_apart(kv_cache, "kv_cache", *query, "query");
+  if (query_out) require_apart(*query_out, "query_out", kv_cache, "kv_cache");
+  if (cos_sin) {
+    apart(*positions, "positions");
+    apart(*cos_sin, "cos_sin");
+  }
+  if (query_norm) apart(*query_norm, "query_norm");
+  if (key_norm) apart(*key_norm, "key_norm");
   check(origami_append_kv_cache(
       key.data_ptr(), value.data_ptr(), query ? query->data_ptr() : nullptr,
       out ? out->data_ptr() : nullptr, dtype, strides, tokens, query_heads, kv_cache.data_ptr(),
@@ -632,8 +757,7 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
     out = *out_;
     require_rows(out, "out", kv_cache, query.scalar_type());
     TORCH_CHECK(out.sizes() == query.sizes(), "out must have the query's shape");
-    at::assert_no_internal_overlap(out);
-    at::assert_no_overlap(out, query);
+    TORCH_CHECK(!shares_with_itself(extent_of(out)), "out must not overlap itself");
   } else {
     // rows of no request are not written: zero in a new tensor
     out = starts ? at::zeros({tokens, Hq, D}, query.options())
@@ -646,6 +770,17 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
                     lse->dim() == 2 && lse->size(0) == tokens && lse->size(1) == Hq,
                 "lse must be float32 [tokens, query heads] on the kv_cache device");
   }
+  if (out_ && lse) require_apart(out, "out", *lse, "lse");
+  const auto apart = [&](const at::Tensor& t, const char* name) {
+    if (out_) require_apart(out, "out", t, name);
+    if (lse) require_apart(*lse, "lse", t, name);
+  };
+  apart(query, "query");
+  apart(kv_cache, "kv_cache");
+  apart(block_tables, "block_tables");
+  apart(own_tokens, "own_tokens");
+  if (prefix_block_ids) apart(*prefix_block_ids, "prefix_block_ids");
+  if (query_starts) apart(*query_starts, "query_starts");
   const int64_t cache_dtype = paged_dtype_code(kv_cache.scalar_type(), "kv_cache");
   const int64_t bytes = origami_shared_prefix_attention_workspace(
       tokens, Hq, g.heads, D, prefix_tokens, requests, most, most_own, cache_dtype);
@@ -684,5 +819,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("restore_plan_destroy", &restore_plan_destroy);
   m.def("append_kv_cache", &append_kv_cache);
   m.def("shared_prefix_attention", &shared_prefix_attention);
+  // how both find results that overlap inputs, for tests on any device
+  m.def("_tensors_overlap", [](const at::Tensor& a, const at::Tensor& b) {
+    return share_bytes(extent_of(a), extent_of(b));
+  });
+  m.def("_tensor_overlaps_itself",
+        [](const at::Tensor& t) { return shares_with_itself(extent_of(t)); });
   m.def("abi_version", &origami_abi_version);
 }

@@ -749,7 +749,7 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tens
     query becomes zero.  Arithmetic is float32, rounded once.  A float8_e4m3fn kv_cache holds
     key / k_scale and value / v_scale, limited to +-448.  Returns the queries: query_out
     (which may be `query` itself, but must share no element with anything else) or a new tensor;
-    None without `query`.  For inference only: inputs that require a gradient or carry a tangent
+    None without `query`.  No input may lie in the cache.  Overlaps are refused.  For inference only: inputs that require a gradient or carry a tangent
     are refused, and so are traced and transformed calls."""
     return _ext.ext().append_kv_cache(key, value, kv_cache, slots, query, positions, cos_sin,
                                       interleaved, query_norm, key_norm, eps, k_scale, v_scale,
@@ -780,7 +780,8 @@ def shared_prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor,
     bound a request's query and own tokens and shape the launch (defaults: all rows, the
     whole block table); own tokens past the bound are not seen, and a request with more query
     tokens than the bound gets no defined rows.  Tokens in blocks outside the cache are
-    not seen.  scale defaults to head_dim ** -0.5.
+    not seen.  scale defaults to head_dim ** -0.5.  An `out` that shares memory with an input
+    or has an element twice is refused.
 
     Returns the output, and with return_lse also float32 [tokens, query_heads] natural
     logarithms of the rows' sums of exponentials (-inf for zero rows), with which results over

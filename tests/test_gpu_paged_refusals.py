@@ -6,6 +6,7 @@ import torch.autograd.forward_ad as forward_ad
 from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 
+from origami_amd import _ext
 from tests.test_gpu_append import Tokens
 from tests.test_gpu_prefix_attention import Batch
 
@@ -15,8 +16,8 @@ pytestmark = pytest.mark.gpu
 class Append:
     """append_kv_cache as a function of one of its inputs."""
 
-    def __init__(self, dev, name):
-        self.tokens, self.name = Tokens(dev, T=5, D=64, rot=64, norm=True), name
+    def __init__(self, dev, name, tokens=None):
+        self.tokens, self.name = tokens or Tokens(dev, T=5, D=64, rot=64, norm=True), name
         self.before = self.tokens.cache.clone()
 
     @property
@@ -110,3 +111,108 @@ def test_jvp(cuda_device, op, name):
     with pytest.raises(RuntimeError, match="plain tensor|requires a gradient"):
         torch.func.jvp(call, (call.input,), (torch.ones_like(call.input),))
     assert call.untouched()
+
+
+# -- results over inputs.  A refused call launches nothing, so these race on nothing. --------
+
+
+def _inside(t, shape, dtype):
+    """The first bytes of `t` as another tensor."""
+    return t.view(torch.uint8).view(-1)[:1 << 14].view(dtype)[:shape.numel()].view(shape)
+
+
+@pytest.mark.parametrize("name", ["key", "value", "query", "slots", "positions", "cos_sin",
+                                  "query_norm", "key_norm"])
+def test_append_refuses_inputs_in_the_cache(cuda_device, name):
+    """Tokens moved to other slots, say: one workgroup would read what another has written."""
+    t = Tokens(cuda_device, T=5, D=64, rot=64, norm=True, positions=20)
+    call = Append(cuda_device, name, t)
+    inside = _inside(t.cache, call.input.shape, call.input.dtype)
+    inside.copy_(call.input)
+    before = t.cache.view(torch.int16).clone()  # as numbers, some of the bytes are NaN
+    with pytest.raises(RuntimeError, match=f"kv_cache must not overlap {name}"):
+        call(inside)
+    assert torch.equal(t.cache.view(torch.int16), before)
+
+
+def test_append_refuses_strided_queries_over_each_other(cuda_device):
+    """Views of one projection: parts beside each other are apart, shifted heads are not."""
+    t = Tokens(cuda_device, T=6, Hq=4, H=2, D=64, rot=64)
+    rows = t.rows.clone()
+    plain, cache = t.run(), t.cache.clone()
+    t.query = t.rows[:, :4]
+    for out in (t.rows[:, 1:5], t.rows[:, 2:6], t.rows[:, 4:8],
+                t.rows.as_strided((6, 4, 64), (512, 63, 1)),
+                t.rows[:1, :4].expand(6, 4, 64)):
+        with pytest.raises(RuntimeError, match="must not overlap"):
+            t.run(query_out=out)
+    assert torch.equal(t.rows, rows)
+    wide = torch.zeros(6, 12, 64, dtype=t.dtype, device=cuda_device)
+    wide[:, :8] = rows
+    t.query, t.key, t.value = wide[:, :4], wide[:, 4:6], wide[:, 6:8]
+    t.run(query_out=wide[:, 8:])
+    assert torch.equal(wide[:, 8:], plain) and torch.equal(t.cache, cache)
+    t.run(query_out=wide[:, :4])
+    assert torch.equal(wide[:, :4], plain) and torch.equal(t.cache, cache)
+
+
+@pytest.mark.parametrize("name", ["positions", "cos_sin", "query_norm", "key_norm", "slots"])
+def test_append_refuses_queries_over_other_inputs(cuda_device, name):
+    t = Tokens(cuda_device, T=5, D=64, rot=64, norm=True, positions=20)
+    call = Append(cuda_device, name, t)
+    memory = torch.zeros(1 << 14, dtype=torch.uint8, device=cuda_device)
+    shared = _inside(memory, call.input.shape, call.input.dtype)
+    shared.copy_(call.input)
+    if name in t.kw:
+        t.kw[name] = shared
+    else:
+        t.slots = shared
+    out, before = _inside(memory, t.query.shape, t.query.dtype), t.cache.clone()
+    with pytest.raises(RuntimeError, match=f"query_out must not overlap {name}"):
+        t.run(query_out=out)
+    assert torch.equal(t.cache, before)
+
+
+@pytest.mark.parametrize("name", ["query", "cache", "tables", "own", "starts", "prefix_ids"])
+def test_attention_refuses_an_output_over_inputs(cuda_device, name):
+    b = Batch(cuda_device, prefix=20, own=(5, 6), queries=(2, 3), D=64)
+    memory = torch.zeros(1 << 20, dtype=torch.uint8, device=cuda_device)
+    x = getattr(b, name)
+    shared = memory[:x.numel() * x.element_size()].view(x.dtype).view(x.shape)
+    shared.copy_(x)
+    setattr(b, name, shared)
+    before = shared.clone()
+    out = _inside(memory, b.query.shape, b.query.dtype)
+    argument = {"cache": "kv_cache", "tables": "block_tables", "own": "own_tokens",
+                "starts": "query_starts", "prefix_ids": "prefix_block_ids"}.get(name, name)
+    with pytest.raises(RuntimeError, match=f"out must not overlap {argument}"):
+        b.run(out=out)
+    lse = _inside(memory, b.query.shape[:2], torch.float32)
+    plain = torch.empty_like(b.query)
+
+    def direct(out, lse):
+        return _ext.ext().shared_prefix_attention(
+            b.query, b.cache, b.prefix_ids, b.prefix, b.tables, b.own, b.starts, None, None, None,
+            1.0, 1.0, out, lse)
+
+    with pytest.raises(RuntimeError, match=f"lse must not overlap {argument}"):
+        direct(plain, lse)
+    with pytest.raises(RuntimeError, match="out must not overlap lse"):
+        both = torch.zeros(b.query.numel(), dtype=b.dtype, device=cuda_device)
+        direct(both.view(b.query.shape), both.view(torch.float32)[:lse.numel()].view(lse.shape))
+    assert torch.equal(shared.view(torch.uint8), before.view(torch.uint8))
+    direct(plain, torch.zeros(lse.shape, device=cuda_device))
+
+
+def test_attention_refuses_strided_outputs_over_each_other(cuda_device):
+    b = Batch(cuda_device, prefix=20, own=(5, 6), D=64)
+    plain = b.run()[0]
+    rows = torch.zeros(2, 20, 64, dtype=b.dtype, device=cuda_device)
+    rows[:, :8] = b.query
+    b.query = rows[:, :8]
+    for out in (rows[:, :8], rows[:, 7:15], rows[:, :1].expand(2, 8, 64),
+                rows.as_strided((2, 8, 64), (1280, 48, 1), 512)):
+        with pytest.raises(RuntimeError, match="out must not overlap"):
+            b.run(out=out)
+    assert torch.equal(b.run(out=rows[:, 12:])[0], plain)
+    assert torch.equal(rows[:, 12:], plain)

@@ -1,8 +1,11 @@
 """Refusals of the C entry points of the operators on the paged cache; no GPU is needed, since
 they are checked before anything is launched."""
-import pytest
+import random
 
-from origami_amd import _native
+import pytest
+import torch
+
+from origami_amd import _ext, _native
 
 BF16, FP8, F32 = _native.DTYPE_BFLOAT16, _native.DTYPE_FLOAT8_E4M3FN, _native.DTYPE_FLOAT32
 
@@ -177,3 +180,57 @@ def test_attention_refuses_numbers_that_binary32_does_not_hold(change, message):
     with pytest.raises(_native.OrigamiNativeError, match=message) as e:
         _attend(**change)
     assert e.value.code == _native.ORIGAMI_ERR_INVALID
+
+
+def _bytes(t):
+    at = torch.zeros((), dtype=torch.int64)
+    for n, step in zip(t.shape, t.stride()):
+        at = at[..., None] + torch.arange(n) * step
+    at = (t.data_ptr() + at.reshape(-1) * t.element_size())[:, None]
+    return (at + torch.arange(t.element_size())).reshape(-1)
+
+
+def _view(rng, memory, dtype):
+    """A view of `memory` with any strides, inside it."""
+    typed = memory.view(dtype)
+    shape = [rng.choice([0, 1, 1, 2, 3, 5, 7]) if rng.random() < 0.1 else rng.randint(1, 6)
+             for _ in range(rng.randint(1, 3))]
+    while True:
+        strides = [rng.choice([0, 1, 1, 2, 3, 8, 9, 16, 24, 25, 48, 50]) for _ in shape]
+        room = typed.numel() - sum(max(n - 1, 0) * s for n, s in zip(shape, strides))
+        if room > 0:
+            return typed.as_strided(shape, strides, rng.randrange(room))
+
+
+def test_overlap_of_strided_tensors():
+    """Which tensors share bytes, against sets of their bytes."""
+    ext, rng, found = _ext.ext(), random.Random(0), [0, 0, 0]
+    memory = torch.zeros(2048, dtype=torch.uint8)
+    types = [torch.uint8, torch.bfloat16, torch.float32, torch.int64]
+    for _ in range(4000):
+        a, b = (_view(rng, memory, rng.choice(types)) for _ in range(2))
+        x, y = _bytes(a), _bytes(b)
+        both = len(set(x.tolist()) & set(y.tolist())) > 0
+        assert ext._tensors_overlap(a, b) == both == ext._tensors_overlap(b, a), (a.shape, b.shape)
+        assert ext._tensor_overlaps_itself(a) == (len(set(x.tolist())) < x.numel())
+        found[0] += both
+        found[1] += not both and bool(x.numel() and y.numel() and x.min() <= y.max()
+                                      and y.min() <= x.max())
+        found[2] += len(set(x.tolist())) < x.numel()
+    assert min(found) > 100  # overlaps, views in each other's gaps, and overlaps with oneself
+
+
+def test_overlap_of_a_projections_parts():
+    """The views of a large projection, whose parts lie between each other's rows."""
+    ext = _ext.ext()
+    rows = torch.empty(100_000, 48, 8, dtype=torch.bfloat16)
+    query, key, value = rows[:, :32], rows[:, 32:40], rows[:, 40:]
+    for a, b in ((query, key), (key, value), (query, value), (rows[::2], rows[1::2]),
+                 (rows[:, :, :4], rows[:, :, 4:]), (rows[:50_000], rows[50_000:])):
+        assert not ext._tensors_overlap(a, b) and not ext._tensors_overlap(b, a)
+    for a, b in ((query, rows[:, 31:35]), (rows[:-1, :32], rows[1:, :32]), (query, query[777:778]),
+                 (rows.transpose(0, 1)[:32], query), (key, rows.view(-1)[32 * 8:32 * 8 + 1])):
+        assert ext._tensors_overlap(a, b) and ext._tensors_overlap(b, a)
+    assert not ext._tensor_overlaps_itself(query)
+    assert ext._tensor_overlaps_itself(rows[:, :1].expand(-1, 2, -1))
+    assert ext._tensor_overlaps_itself(rows.view(-1).as_strided((5, 2, 8), (16, 7, 1)))
