@@ -430,3 +430,46 @@ def test_rows_of_scores_of_minus_infinity(cuda_device, own, group, value):
     got, lse = b.run()
     assert not got[:, ::2].any() and (lse[:, ::2] == -math.inf).all()
     assert got[:, 1::2].isnan().all()
+
+
+# requests, their queries and rows of a KV head a query: workgroups of 16, 64, 128 and 256 rows
+# for the batch and for a request, as far as a head size has them
+SHAPES = {"16_16": (2, 1, 4), "64_16": (8, 1, 4), "64_64": (2, 5, 5), "128_16": (20, 1, 5),
+          "128_64": (6, 5, 5), "128_128": (3, 20, 5), "one_128": (1, 21, 5), "256": (2, 31, 5)}
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("D", [40, 64, 72, 80, 96, 120, 128, 136, 192, 256])
+@pytest.mark.parametrize("dtype,cache_dtype", [(BF16, FP8), (F16, FP8), (BF16, BF16), (F16, F16)])
+def test_every_type_and_size_in_every_shape(cuda_device, shape, D, dtype, cache_dtype):
+    requests, queries, group = SHAPES[shape]
+    own = [queries + (53 * i) % 170 for i in range(requests)]
+    counts = [queries - i % 2 * (queries // 3) for i in range(requests)]
+    b = Batch(cuda_device, prefix=397, own=own, queries=counts if queries > 1 else None, heads=2,
+              group=group, D=D, dtype=dtype, cache_dtype=cache_dtype, bs=(5, 24, 16)[D // 8 % 3],
+              order=("kv_first", "blocks_first")[D // 8 % 2], seed=D)
+    b.check(*b.run(max_query_tokens=queries))
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("D,bs", [(64, 16), (80, 24), (128, 5), (136, 24)])
+def test_odd_values_of_an_e4m3_cache(cuda_device, shape, D, bs):
+    """NaN among the values, in tiles that all rows see and in those that some see."""
+    requests, queries, group = SHAPES[shape]
+    own = [queries + (53 * i) % 170 for i in range(requests)]
+    b = Batch(cuda_device, prefix=130, own=own, queries=[queries] * requests, heads=2, group=group,
+              D=D, cache_dtype=FP8, bs=bs, seed=D)
+    bound = dict(max_query_tokens=queries)
+    whole, whole_lse = b.run(**bound)
+    b.check(whole, whole_lse)
+    marks = [(b.prefix_ids, 3, 0, 5), (b.prefix_ids, 129, 1, 6), (b.tables[0], own[0] - 1, 0, 9),
+             (b.tables[-1], max(own[-1] - 3, 0), 1, D - 1), (b.tables[-1], 0, 1, 0)]
+    cells = b.cache.view(torch.uint8)
+    for table, t, h, d in marks:
+        cells[1, int(table[t // bs]), t % bs, h, d] = 0x7f + 0x80 * (d % 2)
+    got, lse = b.run(**bound)
+    ref = pagedref.attend(b.query, b.cache, b.prefix_ids, b.prefix, b.tables, b.own, b.starts,
+                          None, b.k_scale, b.v_scale)[0]
+    fine = ref.isfinite()
+    assert not fine.all() and torch.equal(got.isfinite(), fine)
+    assert torch.equal(got[fine], whole[fine]) and torch.equal(lse, whole_lse)
