@@ -7,6 +7,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from origami_amd import _ext
+from origami_amd.lossless import native_gpu
 from tests.test_gpu_append import Tokens
 from tests.test_gpu_prefix_attention import Batch
 
@@ -216,3 +217,26 @@ def test_attention_refuses_strided_outputs_over_each_other(cuda_device):
             b.run(out=out)
     assert torch.equal(b.run(out=rows[:, 12:])[0], plain)
     assert torch.equal(rows[:, 12:], plain)
+
+
+def test_refused_appends_leave_the_cache_and_the_output(cuda_device):
+    t = Tokens(cuda_device, rot=32, norm=True)
+    out = torch.full_like(t.query, 3.0)
+    t.cache.fill_(5.0)
+    w, table = t.kw["key_norm"], t.kw["cos_sin"]
+    for change in (dict(key=t.key[:, :1]), dict(value=t.value[:3]), dict(query=t.query[:3]),
+                   dict(slots=t.slots[:3]), dict(slots=t.slots.int()), dict(positions=None),
+                   dict(cos_sin=table.double()), dict(cos_sin=table[:, :5].contiguous()),
+                   dict(cos_sin=table[:0]), dict(key_norm=w[:7]), dict(key_norm=w.float()),
+                   dict(key_norm=w.half(), query_norm=None), dict(k_scale=2.0), dict(eps=-1.0),
+                   dict(eps=float("nan")), dict(key=t.key.clone().requires_grad_()),
+                   dict(query_out=out[:, :1]), dict(query_out=out.float()),
+                   dict(kv_cache=t.cache.half()), dict(query=None)):
+        args = dict(key=t.key, value=t.value, kv_cache=t.cache, slots=t.slots, query=t.query,
+                    query_out=out, **t.kw)
+        args.update(change)
+        with pytest.raises(RuntimeError):
+            native_gpu.append_kv_cache(**args)
+    assert (t.cache == 5.0).all() and (out == 3.0).all()
+    t.run(query_out=out)
+    assert (t.cache != 5.0).any() and (out != 3.0).any()
