@@ -480,7 +480,9 @@ int origami_append_kv_cache(
  * the first prefix_tokens tokens (in blocks prefix_block_ids): each query row
  * is softmax(scale * k_scale * q . k) over the prefix and, causally, over its
  * request's own tokens, times v_scale * v.  The prefix is read once for the whole
- * batch.
+ * batch where max_query_tokens * (query_heads / heads) is below 128 (64 for more than
+ * 128 channels); else each request reads it for itself, in tiles of many rows, also a
+ * request of few.
  *
  * query and out are [tokens, query_heads, head_dim] of dtype FLOAT16 or
  * BFLOAT16, channels contiguous; strides (host, [4]) are the token and head

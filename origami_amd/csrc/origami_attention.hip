@@ -8,14 +8,16 @@
 // the exponentials are rounded to the queries' type for the matrix instruction, which adds half a
 // step of the weighted mean of |v|, about what rounding the result does.
 //
-// The rows of all requests that share the prefix are one matrix against each tile of it, so its
-// keys and values are read once (64 requests over 32768 tokens and 33 thousand of their own: 282 MB
-// from memory of 281 that there are).  With few rows a call is bound by memory and, below some
+// Where requests have too few rows to fill workgroups by themselves, the rows of all of them are one
+// matrix against each tile of the prefix, so its keys and values are read once (64 requests over
+// 32768 tokens and 33 thousand of their own: 282 MB from memory of 281 that there are).  Else
+// each request reads the prefix with its own tokens; the bound of a request's queries decides for
+// the whole batch (plan_of).  With few rows a call is bound by memory and, below some
 // tens of microseconds, by the chain of loads at a workgroup's start (lengths, block ids, rows);
 // with rows by the hundred by the vector instructions of the softmax, which are as many cycles as
-// the products' matrix instructions and run beside them only in part: 815 TFLOP/s for prompts of
-// up to 1024 tokens after 8192, at about 40% of the matrix cycles, where a large library
-// product reaches 1150.
+// the products' matrix instructions and run beside them only in part: 710 to 815 TFLOP/s (600 to
+// 525 us, on different boxes) for prompts of up to 1024 tokens after 8192, with the matrix units busy
+// in 46% of the CUs' busy cycles, where a large library product reaches 1150.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -38,7 +40,9 @@ using origami_internal::fail;
 // beside another's products (against eight waves: 93 us for 103 for 64 requests over 32768
 // tokens, 34 for 40 for 16 over 16384 in e4m3).  The last shape, for requests of many rows and 65
 // to 128 channels, shares tiles among eight waves: 536 us for 616 for prompts of up to 1024 tokens
-// after 8192.  With more channels there are the first two shapes, and a workgroup to a CU.
+// after 8192.  With 64 channels it is the slower one: 427 us for 406 to 413 for the same prompts, 242
+// for 199 to 209 with 12 heads in half precision.  With more channels there are the first two
+// shapes, and a workgroup to a CU.
 constexpr int kShapeRows[4] = {16, 64, 128, 256};
 constexpr int kShapeWaves[4] = {4, 4, 4, 8};
 
@@ -287,8 +291,10 @@ constexpr int kTeamTokens = WR == 8 || (WR == 4 && DP == 64) ? 64 : 32;
 // One workgroup: WR MR rows of one KV head over a range of tokens.  Its NW waves are WR row waves
 // by WT token waves: a wave takes MR rows, and of every WT kTeamTokens tokens its share.  Rows
 // (queries, results, sums) stay in registers; keys and values go through LDS, where the WR waves
-// of a team share them, and the next ones are on their way to registers meanwhile.  They do not go
-// from memory to LDS directly: e4m3 is widened and odd values are dropped in between.  With
+// of a team share them, and the next ones are on their way to registers meanwhile.  They go
+// through registers for e4m3, which is widened on the way, and for the tiles that some rows see in
+// part, whose odd values are dropped; other tiles do not need it, but loads of theirs
+// straight to LDS have not been measured.  With
 // WR = 1 no wave needs another until the end; else buffers take turns, so that one barrier a
 // tile is enough.
 template <typename T, bool FP8, int DP, int MR, int WR, int NW>
@@ -788,7 +794,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams p, 
 
 // For many parts: a workgroup takes `4 lanes` channels of one row.  It first lists the parts that
 // have tokens with their weights, then its lane groups add them up in turn, several loads each on
-// their way: 7 us for 128 rows of 411 parts, where one wave a row after the other took 55.  Waves
+// their way: 8 us for 128 rows of 412 parts, where one wave a row after the other took 55.  Waves
 // meet three times; a tree of steps through LDS and maxima by its crossbar cost 0.5 us more.
 template <typename T>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendParams p, int lanes, int blocks) {
@@ -970,7 +976,8 @@ double call_time(const Kind& k0, int64_t s0, const Kind& k1, int64_t s1, int64_t
 Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_dim,
              int64_t prefix, int64_t requests, int64_t max_query, int64_t max_own, int64_t cell) {
   const int64_t G = query_heads / heads, last = head_dim <= 128 ? 2 : 1;
-  // A request whose rows fill workgroups by themselves reads the prefix with its own tokens.
+  // Where the bound of a request's rows fills workgroups by itself, every request reads the prefix
+  // with its own tokens; that is slow for requests of few rows beside one of many.
   const bool apart = requests > 1 && prefix > 0 && max_query * G < kShapeRows[last];
   const auto kind_of = [&](int shape, int64_t n, int64_t rows, int64_t all_rows, int64_t span) {
     Kind k;

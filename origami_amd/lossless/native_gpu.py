@@ -765,7 +765,11 @@ def shared_prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor,
                             k_scale: float = 1.0, v_scale: float = 1.0,
                             out: torch.Tensor | None = None, return_lse: bool = False):
     """Attention of a batch over the paged cache, where all requests share the first
-    prefix_tokens tokens (in blocks prefix_block_ids): the prefix is read once for the batch.
+    prefix_tokens tokens (in blocks prefix_block_ids).  The prefix is read once for the batch
+    where max_query_tokens * (query_heads // heads) is below 128 (64 for more than 128
+    channels); else each request reads it for itself, in tiles of many rows, also a request
+    of few.  So give max_query_tokens with query_starts, whose default, all rows, is seldom
+    below, and call once for prompts and once for single tokens.
 
     query is float16 or bfloat16 [tokens, query_heads, head_dim]; kv_cache has its dtype or
     is float8_e4m3fn with k_scale / v_scale; query head h uses cache head
