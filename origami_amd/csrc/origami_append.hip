@@ -18,10 +18,9 @@
 // adds, and the root is the instruction's.  8192 tokens of 32 + 8 + 8 heads of 128 with norms take
 // 38 us (5.4 TB/s; all times are of passes in a graph) and, with nothing in a cache, 53; with
 // kinds mixed in a wave, exchanges through the LDS crossbar and the exact root and quotient it was
-// 50 and 68.  128 threads take 42 and 52 and
-// leave half of a workgroup idle where a layer has few heads; 256 take 45; a token's workgroups in
-// a row 43; loads of weights and angles ahead of the row's sum 42.  One token takes 2.9 us, which
-// is a launch.
+// 50 and 68.  128 threads take 42 and 52 and leave half of a workgroup idle where a layer has few
+// heads; 256 take 45; a token's workgroups in a row 43; loads of weights and angles ahead of the
+// row's sum 42.  One token takes 2.9 us, which is a launch.
 #include <cmath>
 
 #include "origami_element.h"

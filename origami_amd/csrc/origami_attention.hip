@@ -8,15 +8,15 @@
 // the exponentials are rounded to the queries' type for the matrix instruction, which adds half a
 // step of the weighted mean of |v|, about what rounding the result does.
 //
-// Where requests have too few rows to fill workgroups by themselves, the rows of all of them are one
-// matrix against each tile of the prefix, so its keys and values are read once (64 requests over
-// 32768 tokens and 33 thousand of their own: 282 MB from memory of 281 that there are).  Else
+// Where requests have too few rows to fill workgroups by themselves, the rows of all of them are
+// one matrix against each tile of the prefix, so its keys and values are read once (64 requests
+// over 32768 tokens and 33 thousand of their own: 282 MB from memory of 281 that there are).  Else
 // each request reads the prefix with its own tokens; the bound of a request's queries decides for
-// the whole batch (plan_of).  With few rows a call is bound by memory and, below some
-// tens of microseconds, by the chain of loads at a workgroup's start (lengths, block ids, rows);
-// with rows by the hundred by the vector instructions of the softmax, which are as many cycles as
-// the products' matrix instructions and run beside them only in part: 710 to 815 TFLOP/s (600 to
-// 525 us, on different boxes) for prompts of up to 1024 tokens after 8192, with the matrix units busy
+// the whole batch (plan_of).  With few rows a call is bound by memory and, below some tens of
+// microseconds, by the chain of loads at a workgroup's start (lengths, block ids, rows); with rows
+// by the hundred by the vector instructions of the softmax, which are as many cycles as the
+// products' matrix instructions and run beside them only in part: 710 to 815 TFLOP/s (600 to 525
+// us, on different boxes) for prompts of up to 1024 tokens after 8192, with the matrix units busy
 // in 46% of the CUs' busy cycles, where a large library product reaches 1150.
 #include <algorithm>
 #include <cmath>
@@ -40,8 +40,8 @@ using origami_internal::fail;
 // beside another's products (against eight waves: 93 us for 103 for 64 requests over 32768
 // tokens, 34 for 40 for 16 over 16384 in e4m3).  The last shape, for requests of many rows and 65
 // to 128 channels, shares tiles among eight waves: 536 us for 616 for prompts of up to 1024 tokens
-// after 8192.  With 64 channels it is the slower one: 427 us for 406 to 413 for the same prompts, 242
-// for 199 to 209 with 12 heads in half precision.  With more channels there are the first two
+// after 8192.  With 64 channels it is the slower one: 427 us for 406 to 413 for the same prompts,
+// 242 for 199 to 209 with 12 heads in half precision.  With more channels there are the first two
 // shapes, and a workgroup to a CU.
 constexpr int kShapeRows[4] = {16, 64, 128, 256};
 constexpr int kShapeWaves[4] = {4, 4, 4, 8};
@@ -293,10 +293,9 @@ constexpr int kTeamTokens = WR == 8 || (WR == 4 && DP == 64) ? 64 : 32;
 // (queries, results, sums) stay in registers; keys and values go through LDS, where the WR waves
 // of a team share them, and the next ones are on their way to registers meanwhile.  They go
 // through registers for e4m3, which is widened on the way, and for the tiles that some rows see in
-// part, whose odd values are dropped; other tiles do not need it, but loads of theirs
-// straight to LDS have not been measured.  With
-// WR = 1 no wave needs another until the end; else buffers take turns, so that one barrier a
-// tile is enough.
+// part, whose odd values are dropped; other tiles do not need it, but loads of theirs straight to
+// LDS have not been measured.  With WR = 1 no wave needs another until the end; else buffers take
+// turns, so that one barrier a tile is enough.
 template <typename T, bool FP8, int DP, int MR, int WR, int NW>
 __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, int unit, bool batch,
                                        uint8_t* lds, float* ml) {

@@ -451,10 +451,12 @@ int64_t paged_dtype_code(at::ScalarType t, const char* name) {
 // this call gave.
 void require_eager() {
   using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
   bool recorded = torch::jit::tracer::isTracing();
-  for (const auto mode : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY,
-                          TorchDispatchModeKey::FUNCTIONAL})
-    recorded |= c10::impl::TorchDispatchModeTLS::get_mode(mode).has_value();
+  if (TorchDispatchModeTLS::any_modes_set())
+    for (const auto mode : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY,
+                            TorchDispatchModeKey::FUNCTIONAL})
+      recorded |= TorchDispatchModeTLS::get_mode(mode).has_value();
   TORCH_CHECK(!recorded, "this operator cannot be traced");
 }
 
@@ -488,9 +490,11 @@ Extent extent_of(const at::Tensor& t) {
   if (t.numel() == 0) return e;
   e.base = static_cast<const char*>(t.data_ptr());
   e.run = t.element_size();
-  TORCH_CHECK(t.dim() <= 8, "tensors of more than 8 dimensions are not compared");
-  for (int64_t d = t.dim() - 1; d >= 0; --d) {
-    const int64_t n = t.size(d), step = t.stride(d) * t.element_size();
+  const at::IntArrayRef sizes = t.sizes(), strides = t.strides();
+  TORCH_CHECK(sizes.size() <= 8, "tensors of more than 8 dimensions are not compared");
+  const int64_t cell = e.run;
+  for (size_t d = sizes.size(); d-- > 0;) {
+    const int64_t n = sizes[d], step = strides[d] * cell;
     if (n == 1) continue;
     if (step == 0) {
       e.repeated = true;
@@ -579,10 +583,9 @@ bool same_elements(const at::Tensor& a, const at::Tensor& b) {
 }
 
 // What a call writes may not be what it reads: launches have no order between their workgroups.
-void require_apart(const at::Tensor& result, const char* result_name, const at::Tensor& input,
+void require_apart(const Extent& result, const char* result_name, const Extent& input,
                    const char* name) {
-  TORCH_CHECK(!share_bytes(extent_of(result), extent_of(input)), result_name,
-              " must not overlap ", name);
+  TORCH_CHECK(!share_bytes(result, input), result_name, " must not overlap ", name);
 }
 
 // A [tokens, heads, head_dim] tensor whose channels are contiguous.
@@ -634,6 +637,7 @@ c10::optional<at::Tensor> append_kv_cache(
   const c10::OptionalDeviceGuard guard(kv_cache.device());
 
   c10::optional<at::Tensor> out;
+  Extent out_extent;  // of a new tensor: none
   int64_t query_heads = 0;
   if (query) {
     require_rows(*query, "query", kv_cache, key.scalar_type());
@@ -642,9 +646,10 @@ c10::optional<at::Tensor> append_kv_cache(
     if (query_out) {
       require_rows(*query_out, "query_out", kv_cache, key.scalar_type());
       TORCH_CHECK(query_out->sizes() == query->sizes(), "query_out must have the query's shape");
-      TORCH_CHECK(!shares_with_itself(extent_of(*query_out)), "query_out must not overlap itself");
+      out_extent = extent_of(*query_out);
+      TORCH_CHECK(!shares_with_itself(out_extent), "query_out must not overlap itself");
       if (!same_elements(*query_out, *query))
-        require_apart(*query_out, "query_out", *query, "another row's query");
+        require_apart(out_extent, "query_out", extent_of(*query), "another row's query");
     }
     out = query_out ? *query_out : at::empty({tokens, query_heads, D}, query->options());
     strides[4] = query->stride(0);
@@ -682,15 +687,17 @@ c10::optional<at::Tensor> append_kv_cache(
     }
   TORCH_CHECK(!query_norm || !key_norm || query_norm->scalar_type() == key_norm->scalar_type(),
               "norm weights must have the same dtype");
+  const Extent cache_extent = extent_of(kv_cache);
   const auto apart = [&](const at::Tensor& t, const char* name) {
-    require_apart(kv_cache, "kv_cache", t, name);
-    if (query_out) require_apart(*query_out, "query_out", t, name);
+    const Extent e = extent_of(t);
+    require_apart(cache_extent, "kv_cache", e, name);
+    require_apart(out_extent, "query_out", e, name);
   };
   apart(key, "key");
   apart(value, "value");
   apart(slots, "slots");
-  if (query) require_apart(kv_cache, "kv_cache", *query, "query");
-  if (query_out) require_apart(*query_out, "query_out", kv_cache, "kv_cache");
+  if (query) require_apart(cache_extent, "kv_cache", extent_of(*query), "query");
+  require_apart(out_extent, "query_out", cache_extent, "kv_cache");
   if (cos_sin) {
     apart(*positions, "positions");
     apart(*cos_sin, "cos_sin");
@@ -753,11 +760,13 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
   const c10::OptionalDeviceGuard guard(kv_cache.device());
 
   at::Tensor out;
+  Extent out_extent, lse_extent;  // of new tensors: none
   if (out_) {
     out = *out_;
     require_rows(out, "out", kv_cache, query.scalar_type());
     TORCH_CHECK(out.sizes() == query.sizes(), "out must have the query's shape");
-    TORCH_CHECK(!shares_with_itself(extent_of(out)), "out must not overlap itself");
+    out_extent = extent_of(out);
+    TORCH_CHECK(!shares_with_itself(out_extent), "out must not overlap itself");
   } else {
     // rows of no request are not written: zero in a new tensor
     out = starts ? at::zeros({tokens, Hq, D}, query.options())
@@ -770,17 +779,21 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
                     lse->dim() == 2 && lse->size(0) == tokens && lse->size(1) == Hq,
                 "lse must be float32 [tokens, query heads] on the kv_cache device");
   }
-  if (out_ && lse) require_apart(out, "out", *lse, "lse");
-  const auto apart = [&](const at::Tensor& t, const char* name) {
-    if (out_) require_apart(out, "out", t, name);
-    if (lse) require_apart(*lse, "lse", t, name);
-  };
-  apart(query, "query");
-  apart(kv_cache, "kv_cache");
-  apart(block_tables, "block_tables");
-  apart(own_tokens, "own_tokens");
-  if (prefix_block_ids) apart(*prefix_block_ids, "prefix_block_ids");
-  if (query_starts) apart(*query_starts, "query_starts");
+  if (out_ || lse) {
+    if (lse) lse_extent = extent_of(*lse);
+    require_apart(out_extent, "out", lse_extent, "lse");
+    const auto apart = [&](const at::Tensor& t, const char* name) {
+      const Extent e = extent_of(t);
+      require_apart(out_extent, "out", e, name);
+      require_apart(lse_extent, "lse", e, name);
+    };
+    apart(query, "query");
+    apart(kv_cache, "kv_cache");
+    apart(block_tables, "block_tables");
+    apart(own_tokens, "own_tokens");
+    if (prefix_block_ids) apart(*prefix_block_ids, "prefix_block_ids");
+    if (query_starts) apart(*query_starts, "query_starts");
+  }
   const int64_t cache_dtype = paged_dtype_code(kv_cache.scalar_type(), "kv_cache");
   const int64_t bytes = origami_shared_prefix_attention_workspace(
       tokens, Hq, g.heads, D, prefix_tokens, requests, most, most_own, cache_dtype);

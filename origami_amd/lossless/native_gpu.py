@@ -749,8 +749,9 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tens
     query becomes zero.  Arithmetic is float32, rounded once.  A float8_e4m3fn kv_cache holds
     key / k_scale and value / v_scale, limited to +-448.  Returns the queries: query_out
     (which may be `query` itself, but must share no element with anything else) or a new tensor;
-    None without `query`.  No input may lie in the cache.  Overlaps are refused.  For inference only: inputs that require a gradient or carry a tangent
-    are refused, and so are traced and transformed calls."""
+    None without `query`.  No input may lie in the cache.  Overlaps are refused.  For inference
+    only: inputs that require a gradient or carry a tangent are refused, and so are traced and
+    transformed calls."""
     return _ext.ext().append_kv_cache(key, value, kv_cache, slots, query, positions, cos_sin,
                                       interleaved, query_norm, key_norm, eps, k_scale, v_scale,
                                       query_out)
