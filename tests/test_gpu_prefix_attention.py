@@ -473,3 +473,50 @@ def test_odd_values_of_an_e4m3_cache(cuda_device, shape, D, bs):
     fine = ref.isfinite()
     assert not fine.all() and torch.equal(got.isfinite(), fine)
     assert torch.equal(got[fine], whole[fine]) and torch.equal(lse, whole_lse)
+
+
+@pytest.mark.parametrize("cache_dtype", [BF16, FP8])
+def test_captured_ragged_queries_follow_starts_and_lengths(cuda_device, cache_dtype):
+    """A captured call with query_starts, replayed with other rows for each request, rows of no
+    request, and lengths past the bound; eager calls in between."""
+    b = Batch(cuda_device, prefix=300, own=(200, 200, 200), queries=(4, 4, 4), D=64,
+              cache_dtype=cache_dtype, seed=4)
+    bound = dict(max_query_tokens=9, max_own_tokens=160)
+    b.run(**bound)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, lse = b.run(**bound)
+    for starts, own in (((0, 4, 8, 12), (200, 170, 31)), ((1, 1, 10, 11), (5, 163, 160)),
+                        ((0, 9, 9, 9), (161, 0, 3)), ((2, 3, 5, 12), (1, 2, 168))):
+        b.starts.copy_(torch.tensor(starts))
+        b.own.copy_(torch.tensor(own))
+        b.query.normal_()
+        graph.replay()
+        eager, eager_lse = b.run(**bound)
+        torch.cuda.synchronize()
+        assert torch.equal(got, eager) and torch.equal(lse, eager_lse)
+        rows = torch.zeros(12, dtype=torch.bool)
+        rows[starts[0]:starts[-1]] = True
+        assert not got[~rows].any() and (lse[~rows] == -math.inf).all()
+        # each row against a request of its own with the tokens it sees
+        seen, request = [], []
+        for r in range(3):
+            n = starts[r + 1] - starts[r]
+            seen += [min(max(own[r] - n + i + 1, 0), 160) for i in range(n)]
+            request += [r] * n
+        one = Batch.__new__(Batch)
+        one.__dict__.update(b.__dict__)
+        one.query, one.starts = b.query[starts[0]:starts[-1]], None
+        one.tables, one.own = b.tables[request], torch.tensor(seen, device=cuda_device)
+        one.check(got[starts[0]:starts[-1]], lse[starts[0]:starts[-1]])
+
+
+def test_inference_mode(cuda_device):
+    b = Batch(cuda_device, prefix=50, own=(9, 20), D=64)
+    plain, lse = b.run()
+    with torch.inference_mode():
+        b.query = b.query.clone()
+        got, again = b.run()
+    assert torch.equal(got, plain) and torch.equal(again, lse)
+    b.check(*b.run())  # an inference tensor outside of it
