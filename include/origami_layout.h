@@ -60,8 +60,10 @@ typedef struct ihipStream_t* origami_stream_t; /* == hipStream_t */
 #define ORIGAMI_DTYPE_FLOAT16 1
 #define ORIGAMI_DTYPE_BFLOAT16 2
 #define ORIGAMI_DTYPE_FLOAT32 3
-/* element type of paged caches read and written by the append and the attention */
+/* element types of paged caches read and written by the append, the attention and the eviction:
+ * e4m3, and rows in 4 bits (origami_kv4_row_bytes) */
 #define ORIGAMI_DTYPE_FLOAT8_E4M3FN 4
+#define ORIGAMI_DTYPE_FLOAT4_E2M1 5
 
 /* KIVI symbol packing: LSB-first at `bits` bits (what the reference kernel
  * reads), or KIVI's own container, where 3-bit symbols sit one per nibble
@@ -439,6 +441,18 @@ int origami_kivi_quantize(const void* kv, int64_t dtype, int64_t tokens, int64_t
  * ------------------------------------------------------------------------- */
 
 /*
+ * Bytes of one row (a token's head) of a cache in 4 bits, whose order is that of other caches with
+ * these bytes in the place of the channels; -1 for an invalid head_dim.  head_dim / 2 bytes hold
+ * e2m1 values (sign, two exponent bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6), channel 2 i
+ * in the low half of byte i; then a byte s for each 32 channels, whose values are multiplied with
+ * 2^(s - 127) (255: NaN); then zeros up to whole dwords.  Appending takes the least power of two at
+ * which no value is further than half a step from what is held, but keeps it within 2^-23 and 2^13,
+ * so that float16 has every value of the cache: larger values become +-49152, infinities too, and a
+ * NaN makes its 32 channels NaN.  Rounding is to nearest even.
+ */
+int64_t origami_kv4_row_bytes(int64_t head_dim);
+
+/*
  * Appends `tokens` tokens to the paged cache, with the position rotation and,
  * for models that have them, norms of queries and keys per head on the way;
  * the queries are rotated in the same launch.
@@ -455,8 +469,8 @@ int origami_kivi_quantize(const void* kv, int64_t dtype, int64_t tokens, int64_t
  *    first rotary_dim channels are rotated in pairs (i, i + rotary_dim / 2), or
  *    (2 i, 2 i + 1) where `interleaved`: (a cos - b sin, b cos + a sin);
  *  - rounded once, to dtype, or for a cache of FLOAT8_E4M3FN divided by k_scale
- *    (values by v_scale), limited to +-448 and rounded to e4m3 (scales are 1
- *    for other caches, which have dtype).
+ *    (values by v_scale), limited to +-448 and rounded to e4m3, or for one of FLOAT4_E2M1
+ *    rounded to 4 bits (scales are 1 for these and for caches of dtype).
  * Token t goes to slot slots[t] = block * block_size + offset.  A token whose
  * slot is outside the cache (such as -1, for padding) is not written; neither is
  * one whose position is outside the table, and its query row becomes zero.
@@ -487,7 +501,8 @@ int origami_append_kv_cache(
  * query and out are [tokens, query_heads, head_dim] of dtype FLOAT16 or
  * BFLOAT16, channels contiguous; strides (host, [4]) are the token and head
  * strides of query and out.  Query head h uses cache head
- * h / (query_heads / heads).  kv_cache has dtype, or FLOAT8_E4M3FN with scales.
+ * h / (query_heads / heads).  kv_cache has dtype, or FLOAT8_E4M3FN with scales, or
+ * FLOAT4_E2M1.
  * Request r has own_tokens[r] tokens in blocks block_tables[r * table_stride ..]
  * (table_blocks of them), those of its queries included: its query tokens are
  * rows query_starts[r] .. query_starts[r + 1] - 1 of query (query_starts null:
@@ -523,6 +538,73 @@ int origami_shared_prefix_attention(
     const int64_t* own_tokens, int64_t requests, const int64_t* query_starts,
     int64_t max_query_tokens, int64_t max_own_tokens, double scale, double k_scale,
     double v_scale, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+    origami_stream_t stream);
+
+/*
+ * Reads the rows of `tokens` slots of the paged cache into key and value ([tokens, heads,
+ * head_dim] of dtype FLOAT16 or BFLOAT16, channels contiguous; strides (host, [4]): token and head
+ * strides of key and value, in elements): as they are from a cache of dtype, times k_scale and
+ * v_scale and rounded once from one of FLOAT8_E4M3FN, and exactly from one of FLOAT4_E2M1 that was
+ * appended to.  The rows of slots outside the cache are zero.  A slot may be given twice.  key and
+ * value share no memory with each other or with an input, and have no element twice (the Python
+ * module refuses such calls).
+ */
+int origami_read_kv_cache(const void* kv_cache, int64_t cache_dtype, int64_t cache_layout,
+                          int64_t num_blocks, int64_t block_size, int64_t heads,
+                          int64_t head_dim, const int64_t* slots, int64_t tokens, double k_scale,
+                          double v_scale, void* key, void* value, int64_t dtype,
+                          const int64_t* strides, origami_stream_t stream);
+
+/*
+ * Adds the weights that query rows give the cached tokens to sums of such weights: for request r,
+ * cache head h and place t,
+ *   out[r, h, t] = weights[r, h, t] + sum over rows of exp(scale * k_scale * q . k_t - lse)
+ * over the query rows of r whose head uses h and that see token t.  Request r has lengths[r]
+ * tokens in blocks block_tables[r * table_stride ..] (table_blocks of them); its query tokens are
+ * rows query_starts[r] .. query_starts[r + 1] - 1 of query (query_starts null: row r alone) and its
+ * last tokens, so that query i of n sees tokens 0 .. lengths[r] - n + i.  lse is a contiguous
+ * float32 [tokens, query_heads], what the attention returned; a row of -infinity gives nothing.
+ * weights (null: zeros) and out are float32 [requests, heads, places], places contiguous, with
+ * request and head strides weight_strides (host, [4]: of weights, then of out); out may be weights
+ * itself.  Tokens past max_tokens and tokens in blocks outside the cache get nothing, and places
+ * that get nothing become weights' (0).
+ *
+ * Products are of dtype (e4m3 and 4 bits are widened exactly), scores, exponentials and sums
+ * binary32.  Each sum is made by one workgroup in a fixed order.  query, strides, kv_cache and scale
+ * are as for the attention.  out shares no memory with an input but weights, if it is all of it.
+ */
+int origami_accumulate_attention_weights(
+    const void* query, int64_t dtype, const int64_t* strides, int64_t tokens, int64_t query_heads,
+    const float* lse, const void* kv_cache, int64_t cache_dtype, int64_t cache_layout,
+    int64_t num_blocks, int64_t block_size, int64_t heads, int64_t head_dim,
+    const int64_t* block_tables, int64_t table_stride, int64_t table_blocks,
+    const int64_t* lengths, int64_t requests, const int64_t* query_starts, int64_t max_tokens,
+    double scale, double k_scale, const float* weights, float* out, int64_t places,
+    const int64_t* weight_strides, origami_stream_t stream);
+
+/*
+ * Moves the tokens that requests keep to blocks of their own, for each cache head by itself: with
+ * n = min(lengths[r], max_tokens) tokens, m = min(n, keep) are kept: the last min(recent, m) of
+ * them, and of the others those with the largest weights[r, h, t], of equal ones (0 and -0 are) the
+ * first; NaN is larger than infinity.  In their order, they become tokens 0 .. m - 1 of the request
+ * in blocks out_tables[r * out_table_stride ..] (out_table_blocks of them), keys and values as they
+ * are; kept (int64 [requests, heads, keep], contiguous) holds their places before, then -1, and
+ * out_weights (float32 [requests, heads, out_places]) their weights, then 0.
+ *
+ * weights are float32 [requests, heads, places]; weight_strides (host, [4]) are the request and
+ * head strides of weights and out_weights, places contiguous.  kv_cache may have any type of
+ * paged caches; head_dim counts channels.  A kept token in a block outside the cache becomes a row
+ * of zeros; one whose new block is outside is not written.  Blocks that are written must be in no
+ * other place of out_tables and in no block table of the call; blocks that are read may be shared.
+ * kept and out_weights share no memory with each other or with an input.
+ */
+int origami_evict_kv_cache(
+    void* kv_cache, int64_t cache_dtype, int64_t cache_layout, int64_t num_blocks,
+    int64_t block_size, int64_t heads, int64_t head_dim, const int64_t* block_tables,
+    int64_t table_stride, int64_t table_blocks, const int64_t* lengths, int64_t requests,
+    int64_t max_tokens, const float* weights, int64_t places, const int64_t* out_tables,
+    int64_t out_table_stride, int64_t out_table_blocks, int64_t keep, int64_t recent,
+    int64_t* kept, float* out_weights, int64_t out_places, const int64_t* weight_strides,
     origami_stream_t stream);
 
 #ifdef __cplusplus

@@ -26,6 +26,7 @@ DTYPE_FLOAT16 = 1
 DTYPE_BFLOAT16 = 2
 DTYPE_FLOAT32 = 3
 DTYPE_FLOAT8_E4M3FN = 4
+DTYPE_FLOAT4_E2M1 = 5
 
 KIVI_PACKED_LSB = 0
 KIVI_NIBBLE3 = 1
@@ -76,6 +77,15 @@ _SIGNATURES: dict[str, list] = {
     "origami_shared_prefix_attention": [
         _p, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p,
         _i64, _i64, _p, _i64, _p, _i64, _i64, _f64, _f64, _f64, _p, _p, _p, _i64, _p],
+    "origami_kv4_row_bytes": [_i64],
+    "origami_read_kv_cache": [
+        _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _f64, _f64, _p, _p, _i64, _p, _p],
+    "origami_accumulate_attention_weights": [
+        _p, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p,
+        _i64, _p, _i64, _f64, _f64, _p, _p, _i64, _p, _p],
+    "origami_evict_kv_cache": [
+        _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _i64,
+        _i64, _i64, _i64, _p, _p, _i64, _p, _p],
 }
 
 EXPORTED_SYMBOLS = ("origami_last_error", "origami_restore_plan_destroy",
@@ -113,6 +123,7 @@ def lib() -> ctypes.CDLL:
                 fn.argtypes = args
             L.origami_set_rows_grid_limit.restype = ctypes.c_int64
             L.origami_shared_prefix_attention_workspace.restype = ctypes.c_int64
+            L.origami_kv4_row_bytes.restype = ctypes.c_int64
             L.origami_restore_plan_destroy.restype = None
             L.origami_restore_plan_destroy.argtypes = [_p]
             L.origami_debug_counters.restype = None

@@ -1,11 +1,13 @@
 // origami_append.hip -- new tokens into the paged KV cache: queries and keys normalised per
-// head and rotated to their positions on the way, keys and values written to their slots.
+// head and rotated to their positions on the way, keys and values written to their slots; and the
+// rows of slots read back from it (read_kv_kernel).
 //
 // For a row x of D channels (one token, one head):
 //   y = x * (1 / sqrt(mean(x^2) + eps)) * w          (where a norm weight is given)
 //   for each pair (a, b) of the rotated channels, with the position's cos and sin:
 //   a' = a cos - b sin,  b' = b cos + a sin          (where a table is given)
-// in binary32, rounded once, to the type that is stored.
+// in binary32, rounded once, to the type that is stored; in 4 bits (origami_element.h) by blocks of
+// 32 channels, which are four neighbouring lanes.
 //
 // Every row is read and written once.  L lanes take a row, 8 channels each (16 bytes of a 16-bit
 // row), so that the mean and a pair's partner are exchanged between lanes of one wave and nothing
@@ -189,7 +191,7 @@ __device__ __forceinline__ void norm_rotate(const AppendParams& p, const T* row,
 
 // One workgroup: kThreads / L rows of one kind (blockIdx.y) of one token (blockIdx.x), whose
 // strides, slot, position and angles are the same for all of them.
-template <typename T, bool FP8, int L>
+template <typename T, Cell CELL, int L>
 __global__ __launch_bounds__(kThreads) void append_kv_kernel(AppendParams p) {
   constexpr int kRows = kThreads / L;
   const int64_t token = blockIdx.x;
@@ -229,12 +231,22 @@ __global__ __launch_bounds__(kThreads) void append_kv_kernel(AppendParams p) {
       for (int j = 0; j < 8; ++j) raw[j] = static_cast<T>(placed ? x[j] : 0.0f);
     }
   }
-  if (!live) return;
   if (kind == 0) {
+    if (!live) return;
     store8(static_cast<T*>(p.out.data) + token * p.out.token + h0 * p.out.head +
                row * p.out.head + 8 * c,
            raw, p.out.vec);
     return;
+  }
+  uint32_t scales = 0;  // of the 128 channels of 16 lanes
+  if constexpr (CELL == kFp4) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      most = max(most, __builtin_bit_cast(uint32_t, x[j]) & 0x7fffffffu);
+    most = max(most, lane_moved<0xb1>(most));
+    most = max(most, lane_moved<0x4e>(most));  // of the block's four lanes
+    scales = 32 * (c / 4) < p.D ? fp4_scale_byte(most) : 0;
   }
   const int64_t slot = p.slots[token];
   if (!placed || slot < 0 || slot >= p.num_slots) return;
@@ -242,8 +254,18 @@ __global__ __launch_bounds__(kThreads) void append_kv_kernel(AppendParams p) {
   const int block = divide(at_slot, p.block_size);
   const int64_t at = block * p.blk_stride + (at_slot - block * p.block_size.d) +
                      (kind == 1 ? 0 : p.half_stride);
+  if constexpr (CELL == kFp4) {
+    uint8_t* const dst = p.cache + (at * p.H + h0 + row) * fp4_row_bytes(p.D);
+    if (live) *reinterpret_cast<uint32_t*>(dst + 4 * c) = fp4_pack(x, fp4_scale(scales));
+    scales <<= 8 * (c / 4 % 4);
+    scales |= lane_moved<0x141>(scales);
+    if constexpr (L > 8) scales |= lane_moved<0x140>(scales);
+    if (c % 16 == 0) *reinterpret_cast<uint32_t*>(dst + p.D / 2 + 4 * (c / 16)) = scales;
+    return;
+  }
+  if (!live) return;
   const int64_t e = (at * p.H + h0) * p.D + (row * p.D + 8 * c);
-  if constexpr (FP8) {
+  if constexpr (CELL == kFp8) {
     const float scale = p.scale[kind - 1];
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = fp8_clamp(x[j] / scale);
@@ -260,21 +282,104 @@ __global__ __launch_bounds__(kThreads) void append_kv_kernel(AppendParams p) {
   }
 }
 
-template <typename T, bool FP8, int L>
+template <typename T, Cell CELL, int L>
 int launch_rows(AppendParams p, uint32_t tokens, hipStream_t stream) {
   constexpr int kRows = kThreads / L;
   p.query_groups = (p.Hq + kRows - 1) / kRows;
   p.groups = (p.H + kRows - 1) / kRows;
   const dim3 grid(tokens, p.query_groups + 2 * p.groups), block(kThreads);
-  hipLaunchKernelGGL((append_kv_kernel<T, FP8, L>), grid, block, 0, stream, p);
+  hipLaunchKernelGGL((append_kv_kernel<T, CELL, L>), grid, block, 0, stream, p);
   return check_launch("append_kv_kernel");
 }
 
-template <typename T, bool FP8>
+template <typename T, Cell CELL>
 int launch_append(const AppendParams& p, uint32_t tokens, hipStream_t stream) {
-  return p.D <= 64    ? launch_rows<T, FP8, 8>(p, tokens, stream)
-         : p.D <= 128 ? launch_rows<T, FP8, 16>(p, tokens, stream)
-                      : launch_rows<T, FP8, 32>(p, tokens, stream);
+  return p.D <= 64    ? launch_rows<T, CELL, 8>(p, tokens, stream)
+         : p.D <= 128 ? launch_rows<T, CELL, 16>(p, tokens, stream)
+                      : launch_rows<T, CELL, 32>(p, tokens, stream);
+}
+
+template <typename T>
+int launch_append(const AppendParams& p, int64_t cache_dtype, uint32_t tokens,
+                  hipStream_t stream) {
+  if (cell_of(cache_dtype) == kFp8) return launch_append<T, kFp8>(p, tokens, stream);
+  if (cell_of(cache_dtype) == kFp4) return launch_append<T, kFp4>(p, tokens, stream);
+  return launch_append<T, kWide>(p, tokens, stream);
+}
+
+struct ReadParams {
+  const uint8_t* cache;
+  int64_t blk_stride, half_stride, num_slots;  // rows of H * D, as cache_geometry
+  Divisor block_size, H;
+  const int64_t* slots;
+  Rows out[2];  // keys and values
+  float scale[2];
+  int32_t D, rows;  // tokens * H
+};
+
+constexpr int kReadThreads = 256;
+
+// The key and the value of one row (a token's head), 8 channels a lane, as T.  A row outside the
+// cache is zero.
+template <typename T, Cell CELL, int L>
+__global__ __launch_bounds__(kReadThreads) void read_kv_kernel(ReadParams p) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kReadThreads / L) + threadIdx.x / L;
+  const int c = threadIdx.x % L;
+  if (row >= p.rows || 8 * c >= p.D) return;
+  const int token = divide(static_cast<int>(row), p.H);
+  const int h = static_cast<int>(row) - token * p.H.d;
+  const int64_t slot = p.slots[token];
+  const bool in = slot >= 0 && slot < p.num_slots;
+  const int at_slot = in ? static_cast<int>(slot) : 0;
+  const int block = divide(at_slot, p.block_size);
+  const int64_t at = block * p.blk_stride + (at_slot - block * p.block_size.d);
+  const int bytes = row_bytes_of(CELL, p.D);
+  U32x4 v[2] = {};
+  if (in) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint8_t* const src = p.cache + ((at + half * p.half_stride) * p.H.d + h) * bytes;
+      if constexpr (CELL == kFp4) {
+        const uint32_t codes = *reinterpret_cast<const uint32_t*>(src + 4 * c);
+        v[half] = fp4_expand<T>(codes, fp4_scale(src[p.D / 2 + c / 4]));
+      } else if constexpr (CELL == kFp8) {
+        const Vec8<T> x = __builtin_bit_cast(
+            Vec8<T>, fp8_expand<T>(*reinterpret_cast<const U32x2*>(src + 8 * c)));
+        Vec8<T> y;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          y[j] = static_cast<T>(static_cast<float>(x[j]) * p.scale[half]);
+        v[half] = __builtin_bit_cast(U32x4, y);
+      } else {
+        v[half] = *reinterpret_cast<const U32x4*>(src + 16 * c);
+      }
+    }
+  }
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
+    store8(static_cast<T*>(p.out[half].data) + token * p.out[half].token + h * p.out[half].head +
+               8 * c,
+           __builtin_bit_cast(Vec8<T>, v[half]), p.out[half].vec);
+}
+
+template <typename T, Cell CELL>
+int launch_read(const ReadParams& p, hipStream_t stream) {
+  const int lanes = p.D <= 64 ? 8 : (p.D <= 128 ? 16 : 32), per = kReadThreads / lanes;
+  const dim3 grid((static_cast<unsigned>(p.rows) + per - 1) / per), block(kReadThreads);
+  if (lanes == 8)
+    hipLaunchKernelGGL((read_kv_kernel<T, CELL, 8>), grid, block, 0, stream, p);
+  else if (lanes == 16)
+    hipLaunchKernelGGL((read_kv_kernel<T, CELL, 16>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((read_kv_kernel<T, CELL, 32>), grid, block, 0, stream, p);
+  return check_launch("read_kv_kernel");
+}
+
+template <typename T>
+int launch_read(const ReadParams& p, int64_t cache_dtype, hipStream_t stream) {
+  if (cell_of(cache_dtype) == kFp8) return launch_read<T, kFp8>(p, stream);
+  if (cell_of(cache_dtype) == kFp4) return launch_read<T, kFp4>(p, stream);
+  return launch_read<T, kWide>(p, stream);
 }
 
 Rows rows_of(const void* data, const int64_t* strides) {
@@ -295,8 +400,9 @@ extern "C" int origami_append_kv_cache(
   AppendParams p{};
   ORIGAMI_REQUIRE(dtype == ORIGAMI_DTYPE_FLOAT16 || dtype == ORIGAMI_DTYPE_BFLOAT16,
                   "keys and values must be float16 or bfloat16");
-  ORIGAMI_REQUIRE(cache_dtype == dtype || cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN,
-                  "kv_cache must have the keys' dtype or be float8_e4m3fn");
+  ORIGAMI_REQUIRE(cache_dtype == dtype || cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN ||
+                      cache_dtype == ORIGAMI_DTYPE_FLOAT4_E2M1,
+                  "kv_cache must have the keys' dtype or be float8_e4m3fn or in 4 bits");
   ORIGAMI_REQUIRE(tokens >= 0 && query_heads >= 0 && heads > 0,
                   "tokens and heads must not be negative");
   ORIGAMI_REQUIRE(head_dim > 0 && head_dim % 8 == 0 && head_dim <= 256,
@@ -361,8 +467,64 @@ extern "C" int origami_append_kv_cache(
   p.inverse_D = 1.0f / static_cast<float>(head_dim);
   const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   const uint32_t n = static_cast<uint32_t>(tokens);
-  const bool fp8 = cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN;
-  if (dtype == ORIGAMI_DTYPE_BFLOAT16)
-    return fp8 ? launch_append<bf16, true>(p, n, stream) : launch_append<bf16, false>(p, n, stream);
-  return fp8 ? launch_append<f16, true>(p, n, stream) : launch_append<f16, false>(p, n, stream);
+  return dtype == ORIGAMI_DTYPE_BFLOAT16 ? launch_append<bf16>(p, cache_dtype, n, stream)
+                                         : launch_append<f16>(p, cache_dtype, n, stream);
+}
+
+extern "C" int64_t origami_kv4_row_bytes(int64_t head_dim) {
+  if (head_dim <= 0 || head_dim % 8 != 0 || head_dim > 256) {
+    fail(ORIGAMI_ERR_INVALID, "head_dim must be a multiple of 8, at most 256");
+    return -1;
+  }
+  return fp4_row_bytes(static_cast<int>(head_dim));
+}
+
+extern "C" int origami_read_kv_cache(const void* kv_cache, int64_t cache_dtype,
+                                     int64_t cache_layout, int64_t num_blocks, int64_t block_size,
+                                     int64_t heads, int64_t head_dim, const int64_t* slots,
+                                     int64_t tokens, double k_scale, double v_scale, void* key,
+                                     void* value, int64_t dtype, const int64_t* strides,
+                                     origami_stream_t stream) {
+  ReadParams p{};
+  ORIGAMI_REQUIRE(dtype == ORIGAMI_DTYPE_FLOAT16 || dtype == ORIGAMI_DTYPE_BFLOAT16,
+                  "keys and values must be float16 or bfloat16");
+  ORIGAMI_REQUIRE(cache_dtype == dtype || cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN ||
+                      cache_dtype == ORIGAMI_DTYPE_FLOAT4_E2M1,
+                  "kv_cache must have the keys' dtype or be float8_e4m3fn or in 4 bits");
+  ORIGAMI_REQUIRE(tokens >= 0 && heads > 0, "tokens and heads must not be negative");
+  ORIGAMI_REQUIRE(head_dim > 0 && head_dim % 8 == 0 && head_dim <= 256,
+                  "head_dim must be a multiple of 8, at most 256");
+  ORIGAMI_REQUIRE(num_blocks >= 0 && block_size > 0, "cache block size must be positive");
+  if (int rc = cache_geometry(cache_layout, num_blocks, block_size, &p.blk_stride,
+                              &p.half_stride))
+    return rc;
+  ORIGAMI_REQUIRE(block_size <= INT32_MAX / (num_blocks > 0 ? num_blocks : 1),
+                  "the cache has too many token slots");
+  ORIGAMI_REQUIRE(cache_scale(k_scale) && cache_scale(v_scale),
+                  "cache scales must be positive and finite in binary32");
+  ORIGAMI_REQUIRE(cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN || (k_scale == 1.0 && v_scale == 1.0),
+                  "cache scales are for float8_e4m3fn caches");
+  ORIGAMI_REQUIRE(aligned16(kv_cache), "kv_cache must be 16-byte aligned");
+  // rows are counted in 31 bits; a launch has at most 2^32 threads, 32 of which take a row at most
+  ORIGAMI_REQUIRE(tokens < (int64_t(1) << 27) / heads, "too many rows for one call");
+  for (int i = 0; i < 4; ++i)
+    ORIGAMI_REQUIRE(strides[i] >= 0, "row strides must not be negative");
+  if (tokens == 0) return ORIGAMI_OK;
+  ORIGAMI_REQUIRE(key != nullptr && value != nullptr && slots != nullptr &&
+                      (kv_cache != nullptr || num_blocks == 0),
+                  "keys, values, slots and the cache must not be null");
+  p.cache = static_cast<const uint8_t*>(kv_cache);
+  p.num_slots = num_blocks * block_size;
+  p.block_size = divisor(block_size);
+  p.H = divisor(heads);
+  p.slots = slots;
+  p.out[0] = rows_of(key, strides);
+  p.out[1] = rows_of(value, strides + 2);
+  p.scale[0] = static_cast<float>(k_scale);
+  p.scale[1] = static_cast<float>(v_scale);
+  p.D = static_cast<int32_t>(head_dim);
+  p.rows = static_cast<int32_t>(tokens * heads);
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return dtype == ORIGAMI_DTYPE_BFLOAT16 ? launch_read<bf16>(p, cache_dtype, s)
+                                         : launch_read<f16>(p, cache_dtype, s);
 }

@@ -134,11 +134,17 @@ __device__ __forceinline__ U32x2 read_column(const uint8_t* p) {
       (__attribute__((address_space(3))) Short4*)p));
 }
 
-// Four channels of a cache row.
-template <typename T, bool FP8>
-__device__ __forceinline__ Float4 four_values(const uint8_t* row, int ch) {
+// Four channels of a cache row (of D channels).
+template <typename T, Cell CELL>
+__device__ __forceinline__ Float4 four_values(const uint8_t* row, int ch, int D) {
   Float4 out;
-  if constexpr (FP8) {
+  if constexpr (CELL == kFp4) {
+    const uint32_t w = *reinterpret_cast<const uint16_t*>(row + ch / 2);
+    const float scale = fp4_scale(row[D / 2 + ch / 32]);
+    const Vec2<T> a = fp4_pair<0>(w, scale, T()), b = fp4_pair<1>(w, scale, T());
+    out = Float4{static_cast<float>(a[0]), static_cast<float>(a[1]), static_cast<float>(b[0]),
+                 static_cast<float>(b[1])};
+  } else if constexpr (CELL == kFp8) {
     const uint32_t w = *reinterpret_cast<const uint32_t*>(row + ch);
     const Vec2<T> a = fp8_pair<false>(w, T()), b = fp8_pair<true>(w, T());
     out = Float4{static_cast<float>(a[0]), static_cast<float>(a[1]), static_cast<float>(b[0]),
@@ -177,6 +183,57 @@ __device__ __forceinline__ bool drop_odd(U32x2& w) {
         w[i] &= ~(0xffu << j);
       }
   return odd;
+}
+
+// Eight 4-bit values and the byte of their scale.
+struct Fp4x8 {
+  uint32_t codes, scale;
+};
+// The same for those: T does not have all values of large scales, which no append writes, and 255
+// makes all NaN.
+template <typename T>
+__device__ __forceinline__ bool drop_odd(Fp4x8& w) {
+  constexpr uint32_t kLast = std::is_same<T, bf16>::value ? 252 : 127 + kMostScale;
+  if (w.scale <= kLast) return false;
+  const float scale = fp4_scale(w.scale);
+  bool odd = false;
+  for (int j = 0; j < 32; j += 4) {
+    const float v = static_cast<float>(fp4_pair<0>(w.codes >> j & 15u, scale, T())[0]);
+    if (!(fabsf(v) < INFINITY)) {
+      odd = true;
+      w.codes &= ~(15u << j);
+    }
+  }
+  w.scale = w.scale == 255 ? 0 : w.scale;
+  return odd;
+}
+
+// Eight values as they are loaded from a cache (the scale's byte is `to_scale` past them), and as
+// they go into a product.
+template <Cell CELL>
+using Raw = typename std::conditional<CELL == kFp4, Fp4x8,
+                                      typename std::conditional<CELL == kFp8, U32x2,
+                                                                U32x4>::type>::type;
+template <Cell CELL>
+__device__ __forceinline__ Raw<CELL> load_raw(const uint8_t* src, int to_scale, bool in,
+                                              const uint8_t* zeros) {
+  if constexpr (CELL == kFp4)
+    return Fp4x8{load_global<uint32_t>(in ? src : zeros),
+                 load_global<uint8_t>(in ? src + to_scale : zeros)};
+  else
+    return load_global<Raw<CELL>>(in ? src : zeros);
+}
+template <typename T>
+__device__ __forceinline__ U32x4 expand(Fp4x8 raw) {
+  return fp4_expand<T>(raw.codes, fp4_scale(raw.scale));
+}
+template <typename T>
+__device__ __forceinline__ U32x4 expand(U32x2 raw) {
+  return fp8_expand<T>(raw);
+}
+template <typename T>
+__device__ __forceinline__ U32x4 expand(U32x4 raw) {
+  return raw;
 }
 
 // Four values rounded to T; `vec`: rows start on 8 bytes.
@@ -296,7 +353,7 @@ constexpr int kTeamTokens = WR == 8 || (WR == 4 && DP == 64) ? 64 : 32;
 // part, whose odd values are dropped; other tiles do not need it, but loads of theirs straight to
 // LDS have not been measured.  With WR = 1 no wave needs another until the end; else buffers take
 // turns, so that one barrier a tile is enough.
-template <typename T, bool FP8, int DP, int MR, int WR, int NW>
+template <typename T, Cell CELL, int DP, int MR, int WR, int NW>
 __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, int unit, bool batch,
                                        uint8_t* lds, float* ml) {
   constexpr int WT = NW / WR, TT = kTeamTokens<DP, WR>;
@@ -400,10 +457,12 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
   uint8_t* const team = lds + wt * kBuffers * 2 * kTile;
   const int piece = lane % NCH, sub = lane / NCH;
   const bool has = 8 * piece < p.D;
-  constexpr int cell = FP8 ? 1 : 2;
-  const int64_t pitch = static_cast<int64_t>(p.H.d) * p.D * cell;
+  const int bytes = row_bytes_of(CELL, p.D);
+  const int64_t pitch = static_cast<int64_t>(p.H.d) * bytes;
+  constexpr int kPiece = CELL == kFp4 ? 4 : (CELL == kFp8 ? 8 : 16);  // bytes of 8 channels
   const uint8_t* const keys =
-      p.cache + (static_cast<int64_t>(h) * p.D + (has ? 8 * piece : 0)) * cell;
+      p.cache + (static_cast<int64_t>(h) * bytes + (has ? kPiece * piece : 0));
+  const int to_scale = p.D / 2 + piece / 4 - kPiece * piece;  // of 4-bit values
   const int64_t to_values = p.half_stride * pitch;
 
   // the cache row of token t, -1 where it has none
@@ -412,8 +471,7 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
     const int i = t < p.prefix ? t : t - p.prefix;
     return static_cast<int>(id * p.blk_stride + i - divide(i, p.block_size) * p.block_size.d);
   };
-  using Raw = typename std::conditional<FP8, U32x2, U32x4>::type;
-  Raw kr[IT], vr[IT];
+  Raw<CELL> kr[IT], vr[IT];
   const auto load_tile = [&](int mine) {
     const uint8_t* const zeros = reinterpret_cast<const uint8_t*>(&kZeros);
 #pragma unroll
@@ -421,8 +479,8 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
       const int r = __shfl(mine, (i * WR + wr) * RPI + sub);
       const bool in = r >= 0 && has;
       const uint8_t* const src = keys + r * pitch;
-      kr[i] = load_global<Raw>(in ? src : zeros);
-      vr[i] = load_global<Raw>(in ? src + to_values : zeros);
+      kr[i] = load_raw<CELL>(src, to_scale, in, zeros);
+      vr[i] = load_raw<CELL>(src + to_values, to_scale, in, zeros);
     }
   };
   // Where some rows may not see some of a tile's tokens: a hidden token's weight is 0, but 0 times
@@ -438,14 +496,7 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int tok = (i * WR + wr) * RPI + sub;
-      U32x4 kv, vv;
-      if constexpr (FP8) {
-        kv = fp8_expand<T>(kr[i]);
-        vv = fp8_expand<T>(vr[i]);
-      } else {
-        kv = kr[i];
-        vv = vr[i];
-      }
+      const U32x4 kv = expand<T>(kr[i]), vv = expand<T>(vr[i]);
       *reinterpret_cast<U32x4*>(buf + (tok * NCH + key_piece<DP>(tok, piece)) * 16) = kv;
       *reinterpret_cast<U32x4*>(buf + kTile + (tok * NCH + value_piece<DP, MR>(tok, piece)) * 16) =
           vv;
@@ -605,7 +656,7 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
     for (int i = max(t0, nearest - TT); i < min(t1, seen_by(row)); ++i) {
       const int at_row = row_of(i, block_of(i, t1));
       if (at_row >= 0)
-        add(p.cache + (at_row + p.half_stride) * pitch + static_cast<int64_t>(h) * p.D * cell);
+        add(p.cache + (at_row + p.half_stride) * pitch + static_cast<int64_t>(h) * bytes);
     }
   };
   const auto odd_part = [](Float4 v) {
@@ -679,7 +730,7 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
         }
         if (odd)
           each_odd_token(row0 + r, [&](const uint8_t* values) {
-            v += odd_part(four_values<T, FP8>(values, min(ch, p.D - 4)));
+            v += odd_part(four_values<T, CELL>(values, min(ch, p.D - 4), p.D));
           });
         put(row0 + r, ch, v, most, total);
       }
@@ -720,7 +771,7 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
 #pragma unroll
         for (int x = 0; x < ACC; x += 4) {
           const int ch = MR * d + 4 * q4 + 256 / MR * (x / 4);
-          const Float4 v = odd_part(four_values<T, FP8>(values, min(ch, p.D - 4)));
+          const Float4 v = odd_part(four_values<T, CELL>(values, min(ch, p.D - 4), p.D));
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[d][x + j] += v[j];
         }
@@ -733,16 +784,16 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
           Float4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]}, base, sum);
 }
 
-template <typename T, bool FP8, int DP, int SHAPE>
+template <typename T, Cell CELL, int DP, int SHAPE>
 __device__ __forceinline__ void attend_shape(const AttendParams& p, int kind, int unit,
                                              uint8_t* lds, float* ml) {
   constexpr int MR = SHAPE == 0 || DP == 256 ? 16 : 32;
-  attend<T, FP8, DP, MR, kShapeRows[SHAPE] / MR, kShapeWaves[SHAPE]>(p, p.group[kind], unit,
+  attend<T, CELL, DP, MR, kShapeRows[SHAPE] / MR, kShapeWaves[SHAPE]>(p, p.group[kind], unit,
                                                                     kind == 0, lds, ml);
 }
 
 // The prefix in workgroups of shape S0 and the requests in those of S1, in one launch.
-template <typename T, bool FP8, int DP, int S0, int S1>
+template <typename T, Cell CELL, int DP, int S0, int S1>
 __global__ __launch_bounds__(64 * kShapeWaves[S0], DP == 256 ? 1 : 2)
     void attend_kernel(AttendParams p) {
   __shared__ alignas(16) uint8_t lds[(S0 == 3 ? 768 : 512) * DP];
@@ -751,9 +802,9 @@ __global__ __launch_bounds__(64 * kShapeWaves[S0], DP == 256 ? 1 : 2)
   const int kind = unit >= p.group[0].units;
   unit -= kind ? p.group[0].units : 0;
   if (S0 == S1 || kind == 1)
-    attend_shape<T, FP8, DP, S1>(p, S0 == S1 ? kind : 1, unit, lds, ml);
+    attend_shape<T, CELL, DP, S1>(p, S0 == S1 ? kind : 1, unit, lds, ml);
   else
-    attend_shape<T, FP8, DP, S0>(p, 0, unit, lds, ml);
+    attend_shape<T, CELL, DP, S0>(p, 0, unit, lds, ml);
 }
 
 // Joins the parts of each row: out = v_scale sum_s w_s O_s / sum_s w_s l_s with
@@ -879,35 +930,35 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendParams p, int 
   if (p.lse && ch == 0) p.lse[row] = total == 0.0f ? -INFINITY : kLn2 * (best + log2f(total));
 }
 
-template <typename T, bool FP8, int DP, int S0, int S1>
+template <typename T, Cell CELL, int DP, int S0, int S1>
 int launch_shapes(const AttendParams& p, hipStream_t stream) {
   const dim3 grid(p.group[0].units + p.group[1].units), block(64 * kShapeWaves[S0]);
-  hipLaunchKernelGGL((attend_kernel<T, FP8, DP, S0, S1>), grid, block, 0, stream, p);
+  hipLaunchKernelGGL((attend_kernel<T, CELL, DP, S0, S1>), grid, block, 0, stream, p);
   return check_launch("attend_kernel");
 }
 
-template <typename T, bool FP8, int DP>
+template <typename T, Cell CELL, int DP>
 int launch_units(const AttendParams& p, hipStream_t stream) {
   // the batch has at least a request's rows: s0 >= s1
   const int s1 = p.group[1].shape, s0 = p.group[0].units ? p.group[0].shape : s1;
   if constexpr (DP == 128)
-    if (s0 == 3) return launch_shapes<T, FP8, DP, 3, 3>(p, stream);
+    if (s0 == 3) return launch_shapes<T, CELL, DP, 3, 3>(p, stream);
   if constexpr (DP <= 128)
     if (s0 == 2)
-      return s1 == 0   ? launch_shapes<T, FP8, DP, 2, 0>(p, stream)
-             : s1 == 1 ? launch_shapes<T, FP8, DP, 2, 1>(p, stream)
-                       : launch_shapes<T, FP8, DP, 2, 2>(p, stream);
+      return s1 == 0   ? launch_shapes<T, CELL, DP, 2, 0>(p, stream)
+             : s1 == 1 ? launch_shapes<T, CELL, DP, 2, 1>(p, stream)
+                       : launch_shapes<T, CELL, DP, 2, 2>(p, stream);
   if constexpr (DP <= 128)
-    if (s0 == 1 && s1 == 0) return launch_shapes<T, FP8, DP, 1, 0>(p, stream);
-  if (s0 == 1) return launch_shapes<T, FP8, DP, 1, 1>(p, stream);
-  return launch_shapes<T, FP8, DP, 0, 0>(p, stream);
+    if (s0 == 1 && s1 == 0) return launch_shapes<T, CELL, DP, 1, 0>(p, stream);
+  if (s0 == 1) return launch_shapes<T, CELL, DP, 1, 1>(p, stream);
+  return launch_shapes<T, CELL, DP, 0, 0>(p, stream);
 }
 
-template <typename T, bool FP8>
+template <typename T, Cell CELL>
 int launch_attend(const AttendParams& p, hipStream_t stream) {
-  const int rc = p.D <= 64    ? launch_units<T, FP8, 64>(p, stream)
-                 : p.D <= 128 ? launch_units<T, FP8, 128>(p, stream)
-                              : launch_units<T, FP8, 256>(p, stream);
+  const int rc = p.D <= 64    ? launch_units<T, CELL, 64>(p, stream)
+                 : p.D <= 128 ? launch_units<T, CELL, 128>(p, stream)
+                              : launch_units<T, CELL, 256>(p, stream);
   if (rc) return rc;
   const dim3 block(kJoinThreads);
   if (p.slots == 1) return ORIGAMI_OK;
@@ -924,6 +975,13 @@ int launch_attend(const AttendParams& p, hipStream_t stream) {
     hipLaunchKernelGGL(join_kernel<T>, joins, block, 0, stream, p, some, blocks);
   }
   return check_launch("join_kernel");
+}
+
+template <typename T>
+int launch_attend(const AttendParams& p, Cell cell, hipStream_t stream) {
+  if (cell == kFp8) return launch_attend<T, kFp8>(p, stream);
+  if (cell == kFp4) return launch_attend<T, kFp4>(p, stream);
+  return launch_attend<T, kWide>(p, stream);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -973,7 +1031,8 @@ double call_time(const Kind& k0, int64_t s0, const Kind& k1, int64_t s1, int64_t
 }
 
 Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_dim,
-             int64_t prefix, int64_t requests, int64_t max_query, int64_t max_own, int64_t cell) {
+             int64_t prefix, int64_t requests, int64_t max_query, int64_t max_own,
+             int64_t row_bytes) {
   const int64_t G = query_heads / heads, last = head_dim <= 128 ? 2 : 1;
   // Where the bound of a request's rows fills workgroups by itself, every request reads the prefix
   // with its own tokens; that is slow for requests of few rows beside one of many.
@@ -990,7 +1049,7 @@ Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_di
         std::min(k.count, heads * (ceil_div(all_rows, unit_rows) + n / 2)), 1);
     k.span = span;
     k.fill = head_dim <= 128 && k.shape < 3 ? 2 * kCus : kCus;  // workgroups that the CUs hold
-    k.token = k.fill / kCus * std::max(2.0 * head_dim * cell / kCuBytes,
+    k.token = k.fill / kCus * std::max(2.0 * row_bytes / kCuBytes,
                                      4.0 * head_dim * unit_rows / kCuFlops);
     return k;
   };
@@ -1073,13 +1132,13 @@ int64_t origami_shared_prefix_attention_workspace(int64_t tokens, int64_t query_
                                                   int64_t prefix_tokens, int64_t requests,
                                                   int64_t max_query_tokens,
                                                   int64_t max_own_tokens, int64_t cache_dtype) {
-  const int64_t cell_bytes = cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN ? 1 : 2;
   if (check_sizes(tokens, query_heads, heads, head_dim, prefix_tokens, requests, max_query_tokens,
                   max_own_tokens))
     return -1;
   max_query_tokens = bound_of_queries(max_query_tokens, tokens);
   return workspace_bytes_of(plan_of(tokens, query_heads, heads, head_dim, prefix_tokens,
-                                    requests, max_query_tokens, max_own_tokens, cell_bytes),
+                                    requests, max_query_tokens, max_own_tokens,
+                                    row_bytes_of(cell_of(cache_dtype), head_dim)),
                             tokens, query_heads, head_dim);
 }
 
@@ -1095,8 +1154,9 @@ int origami_shared_prefix_attention(
   AttendParams p{};
   ORIGAMI_REQUIRE(dtype == ORIGAMI_DTYPE_FLOAT16 || dtype == ORIGAMI_DTYPE_BFLOAT16,
                   "queries must be float16 or bfloat16");
-  ORIGAMI_REQUIRE(cache_dtype == dtype || cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN,
-                  "kv_cache must have the queries' dtype or be float8_e4m3fn");
+  ORIGAMI_REQUIRE(cache_dtype == dtype || cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN ||
+                      cache_dtype == ORIGAMI_DTYPE_FLOAT4_E2M1,
+                  "kv_cache must have the queries' dtype or be float8_e4m3fn or in 4 bits");
   if (int rc = check_sizes(tokens, query_heads, heads, head_dim, prefix_tokens, requests,
                            max_query_tokens, max_own_tokens))
     return rc;
@@ -1131,9 +1191,9 @@ int origami_shared_prefix_attention(
                       (block_tables != nullptr || max_own_tokens == 0),
                   "queries, output, lengths, tables and the cache must not be null");
 
-  const bool fp8 = cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN;
   const Plan plan = plan_of(tokens, query_heads, heads, head_dim, prefix_tokens, requests,
-                            max_query_tokens, max_own_tokens, fp8 ? 1 : 2);
+                            max_query_tokens, max_own_tokens,
+                            row_bytes_of(cell_of(cache_dtype), head_dim));
   ORIGAMI_REQUIRE(plan.units < kMostUnits, "too many row tiles for one call");
   ORIGAMI_REQUIRE(workspace_bytes >= workspace_bytes_of(plan, tokens, query_heads, head_dim) &&
                       (plan.slots == 1 || workspace != nullptr) && aligned16(workspace),
@@ -1172,9 +1232,8 @@ int origami_shared_prefix_attention(
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + parts * head_dim;
   const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-  if (dtype == ORIGAMI_DTYPE_BFLOAT16)
-    return fp8 ? launch_attend<bf16, true>(p, stream) : launch_attend<bf16, false>(p, stream);
-  return fp8 ? launch_attend<f16, true>(p, stream) : launch_attend<f16, false>(p, stream);
+  return dtype == ORIGAMI_DTYPE_BFLOAT16 ? launch_attend<bf16>(p, cell_of(cache_dtype), stream)
+                                         : launch_attend<f16>(p, cell_of(cache_dtype), stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,707 @@
+// origami_evict.hip -- eviction from the paged KV cache by accumulated attention weight.
+//
+// weigh_kernel adds up, for each cached token t and cache head, the weights that the queries give
+// it:  out_t = weights_t + sum_q exp(scale (q . k_t) - lse_q),  with lse_q the logarithm of the
+// sum of exponentials that the attention returned for the row, so that no maximum is needed.
+// select_kernel finds the tokens that a head keeps, the newest and those of the largest sums, and
+// move_kernel copies their rows, in order, to blocks of their own.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "origami_element.h"
+#include "origami_internal.h"
+
+namespace {
+
+using namespace origami_element;
+using origami_internal::aligned16;
+using origami_internal::cache_geometry;
+using origami_internal::cache_scale;
+using origami_internal::check_launch;
+using origami_internal::fail;
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ---------------------------------------------------------------------------
+// Adding up the weights
+// ---------------------------------------------------------------------------
+
+struct WeighParams {
+  const void* query;
+  int64_t q_token, q_head;  // strides, in elements
+  bool q_vec;               // its rows start on 16 bytes
+  const float* lse;         // [tokens, query heads]
+  const uint8_t* cache;     // the keys
+  int64_t blk_stride;       // rows of H * D, as cache_geometry
+  int64_t num_blocks;
+  const int64_t *tables, *lengths, *starts;
+  int64_t table_stride;
+  Divisor block_size, H, G, tiles;  // tiles: of a request's places, in eights
+  int32_t tokens, Hq, D, max_tokens, places;
+  float scale;  // includes the keys' scale
+  const float* weights;  // null: zeros
+  float* out;
+  int64_t w_request, w_head, o_request, o_head;  // strides, in elements
+};
+
+constexpr int kWeighThreads = 256, kWeighWaves = kWeighThreads / 64;
+
+template <int MR>
+using Tile = float __attribute__((ext_vector_type(MR * MR / 64)));
+
+// c + a b, where a lane has 8 values of row (a) and column (b) lane % MR, from 8 (lane / MR) on;
+// value x of the result is in column lane % MR and row 4 (lane / MR) + x % 4 + (256 / MR) (x / 4).
+template <typename T, int MR>
+__device__ __forceinline__ Tile<MR> mfma(Vec8<T> a, Vec8<T> b, Tile<MR> c) {
+  if constexpr (MR == 16) {
+    if constexpr (std::is_same<T, bf16>::value)
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  } else {
+    if constexpr (std::is_same<T, bf16>::value)
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+}
+
+// Where piece `piece` (16 bytes) of row `row` is in LDS: 16 lanes read the same piece of 16 rows.
+template <int DP>
+__device__ __forceinline__ int query_piece(int row, int piece) {
+  return row * (DP / 8) + (piece ^ (DP == 64 ? (row >> 1) & 7 : row & 15));
+}
+
+// Dwords of a cache row, which starts on four bytes where it holds 4-bit values.
+template <int DWORDS>
+struct __attribute__((aligned(4))) Dwords {
+  uint32_t w[DWORDS];
+};
+
+// One workgroup: 4 NT MR tokens of one KV head of one request, against all query rows that see
+// any of them, MR rows at a time.  The keys stay in registers, as the second operand, so that a
+// token's scores are in the lanes of one column and are added up where they are; the queries go
+// through LDS.
+//
+// The order of the channels in the products is free as long as keys and queries have the same: a
+// lane's 16 bytes of a key are 8, 16 or 32 channels in a row, whole loads of the cache's row.
+template <typename T, Cell CELL, int DP, int MR, int NT>
+__global__ __launch_bounds__(kWeighThreads) void weigh_kernel(WeighParams p) {
+  constexpr int NG = 64 / MR, KS = DP / (8 * NG), NCH = DP / 8, ACC = MR * MR / 64;
+  constexpr int kWhole = CELL == kFp4 ? 4 : (CELL == kFp8 ? 2 : 1);
+  constexpr int NPE = kWhole < KS ? kWhole : KS;  // pieces of 8 channels in a load
+  constexpr int kPiece = CELL == kFp4 ? 4 : (CELL == kFp8 ? 8 : 16);
+  constexpr int kTokens = kWeighWaves * NT * MR;
+  constexpr int QL = MR * NCH / kWeighThreads > 0 ? MR * NCH / kWeighThreads : 1;
+  __shared__ U32x4 queries[2][MR * NCH];
+  __shared__ alignas(16) float lses[2][MR];
+  __shared__ alignas(16) int limits[2][MR];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int c = lane % MR, q4 = lane / MR;
+
+  // The heads of the same tokens are 8 workgroups apart, on one chiplet: their rows share lines.
+  const int unit = static_cast<int>(blockIdx.x);
+  const int eighth = unit & 7;
+  int u = divide(unit >> 3, p.H);
+  const int h = (unit >> 3) - u * p.H.d;
+  const int r = divide(u, p.tiles);
+  const int tile = (u - r * p.tiles.d) * 8 + eighth;
+  const int t0 = tile * kTokens;
+  if (t0 >= p.places) return;
+
+  const int length =
+      static_cast<int>(min(max(p.lengths[r], int64_t(0)), int64_t(3) << 29));
+  const int end = min(length, p.max_tokens);
+  const float* const weights =
+      p.weights ? p.weights + r * p.w_request + h * p.w_head : nullptr;
+  float* const out = p.out + r * p.o_request + h * p.o_head;
+  const int first_t = t0 + wave * NT * MR;  // of this wave
+  if (t0 >= end) {
+    for (int i = threadIdx.x; i < kTokens; i += kWeighThreads)
+      if (t0 + i < p.places && out != weights)
+        out[t0 + i] = weights ? weights[t0 + i] : 0.0f;
+    return;
+  }
+
+  int q_first = r, q_count = 1;
+  if (p.starts) {
+    const int64_t n = p.tokens;
+    const int64_t a = min(max(p.starts[r], int64_t(0)), n);
+    q_first = static_cast<int>(a);
+    q_count = static_cast<int>(min(max(p.starts[r + 1], a), n) - a);
+  }
+  const int before = length - q_count;  // tokens before the queries' (may be negative)
+  const int rows = q_count * p.G.d;
+
+  // the keys
+  const int bytes = row_bytes_of(CELL, p.D);
+  Vec8<T> kf[NT][KS];
+  bool there[NT];
+  const int64_t* const table = p.tables + r * p.table_stride;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int t = first_t + n * MR + c;
+    const int block = divide(min(t, end - 1), p.block_size);
+    const int64_t id = table[block];
+    there[n] = t < end && id >= 0 && id < p.num_blocks;
+    const int64_t at = there[n] ? id * p.blk_stride + (t - block * p.block_size.d) : 0;
+    const uint8_t* const row = p.cache + (at * p.H.d + h) * bytes;
+#pragma unroll
+    for (int j = 0; j < KS / NPE; ++j) {
+      const int ch = (j * NG + q4) * NPE * 8;  // of the load's first piece
+      Dwords<NPE * kPiece / 4> raw = {};
+      const uint8_t* const src = row + ch / 8 * kPiece;
+      float scale = 0.0f;
+      if (there[n] && ch < p.D) {
+        if (ch + NPE * 8 <= p.D) {
+          raw = *reinterpret_cast<const Dwords<NPE * kPiece / 4>*>(src);
+        } else {
+#pragma unroll
+          for (int i = 0; i < NPE; ++i)
+            if (ch + 8 * i < p.D)
+#pragma unroll
+              for (int x = 0; x < kPiece / 4; ++x)
+                raw.w[i * kPiece / 4 + x] =
+                    *reinterpret_cast<const uint32_t*>(src + i * kPiece + 4 * x);
+        }
+        if constexpr (CELL == kFp4) scale = fp4_scale(row[p.D / 2 + ch / 32]);
+      }
+#pragma unroll
+      for (int i = 0; i < NPE; ++i) {
+        U32x4 wide;
+        if constexpr (CELL == kFp4)
+          wide = fp4_expand<T>(raw.w[i], scale);
+        else if constexpr (CELL == kFp8)
+          wide = fp8_expand<T>(U32x2{raw.w[2 * i], raw.w[2 * i + 1]});
+        else
+          wide = U32x4{raw.w[0], raw.w[1], raw.w[2], raw.w[3]};
+        kf[n][j * NPE + i] = __builtin_bit_cast(Vec8<T>, wide);
+      }
+    }
+  }
+
+  // Query i / G sees the tokens up to before + i / G: rows from the first that sees one of these.
+  const int row0 = min(max(t0 - before, 0), q_count) * p.G.d / MR * MR;
+  U32x4 qr[QL];
+  float lse = 0.0f;
+  int limit = 0;
+  const auto load_rows = [&](int from) {
+#pragma unroll
+    for (int l = 0; l < QL; ++l) {
+      const int i = l * kWeighThreads + threadIdx.x, row = from + i / NCH, d = i % NCH * 8;
+      qr[l] = U32x4{0, 0, 0, 0};
+      if (i < MR * NCH && row < rows && d < p.D) {
+        const int qi = divide(row, p.G), head = h * p.G.d + row - qi * p.G.d;
+        const T* const src =
+            static_cast<const T*>(p.query) + (q_first + qi) * p.q_token + head * p.q_head + d;
+        if (p.q_vec) {
+          qr[l] = *reinterpret_cast<const U32x4*>(src);
+        } else {
+          Vec8<T> v;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = src[j];
+          qr[l] = __builtin_bit_cast(U32x4, v);
+        }
+      }
+    }
+    if (threadIdx.x < MR) {
+      const int row = from + threadIdx.x;
+      limit = 0;
+      lse = 0.0f;
+      if (row < rows) {
+        const int qi = divide(row, p.G), head = h * p.G.d + row - qi * p.G.d;
+        lse = p.lse[static_cast<int64_t>(q_first + qi) * p.Hq + head];
+        // a row that saw nothing gives no weight
+        limit = lse == -INFINITY ? 0 : max(before + qi + 1, 0);
+      }
+    }
+  };
+  const auto store_rows = [&](int buf) {
+#pragma unroll
+    for (int l = 0; l < QL; ++l) {
+      const int i = l * kWeighThreads + threadIdx.x;
+      if (i < MR * NCH) queries[buf][query_piece<DP>(i / NCH, i % NCH)] = qr[l];
+    }
+    if (threadIdx.x < MR) {
+      lses[buf][threadIdx.x] = lse;
+      limits[buf][threadIdx.x] = limit;
+    }
+  };
+
+  // sums of binary32 with what they lose
+  float sum[NT], lost[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) sum[n] = lost[n] = 0.0f;
+  int buf = 0;
+  if (row0 < rows) {
+    load_rows(row0);
+    store_rows(0);
+  }
+  for (int from = row0; from < rows; from += MR) {
+    __syncthreads();
+    const bool more = from + MR < rows;
+    if (more) load_rows(from + MR);
+    // rows of the result that this lane has, four at a time
+    const auto mine = [&](int x) { return 4 * q4 + 256 / MR * (x / 4); };
+    Tile<MR> s[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < ACC; ++x) s[n][x] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const int piece = (k / NPE * NG + q4) * NPE + k % NPE;
+      const Vec8<T> qf = __builtin_bit_cast(Vec8<T>, queries[buf][query_piece<DP>(c, piece)]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n] = mfma<T, MR>(qf, kf[n][k], s[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int t = first_t + n * MR + c;
+      float e[ACC];
+#pragma unroll
+      for (int x = 0; x < ACC; x += 4) {
+        const Float4 below = *reinterpret_cast<const Float4*>(&lses[buf][mine(x)]);
+        const auto until = *reinterpret_cast<const int __attribute__((ext_vector_type(4)))*>(
+            &limits[buf][mine(x)]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float v = fmaf(s[n][x + j], p.scale, -below[j]);
+          const float w = __builtin_amdgcn_exp2f(v * kLog2e);
+          e[x + j] = t < until[j] ? w : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int step = 1; step < ACC; step *= 2)
+#pragma unroll
+        for (int x = 0; x < ACC; x += 2 * step) e[x] += e[x + step];
+      const float add = e[0] - lost[n], next = sum[n] + add;
+      lost[n] = next < INFINITY ? (next - sum[n]) - add : 0.0f;
+      sum[n] = next;
+    }
+    buf ^= 1;
+    if (more) store_rows(buf);
+  }
+
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float v = sum[n];
+#pragma unroll
+    for (int x = MR; x < 64; x <<= 1) v += __shfl_xor(v, x);
+    const int t = first_t + n * MR + c;
+    if (q4 == 0 && t < p.places) {
+      const float old = weights ? weights[t] : 0.0f;
+      if (there[n])
+        out[t] = old + v;
+      else if (out != weights)
+        out[t] = old;
+    }
+  }
+}
+
+template <typename T, Cell CELL, int DP, int MR, int NT>
+int launch_weigh(WeighParams p, int64_t requests, hipStream_t stream) {
+  const int64_t tiles = ceil_div(p.places, kWeighWaves * NT * MR);
+  p.tiles = divisor(ceil_div(tiles, 8));
+  const int64_t units = requests * p.H.d * p.tiles.d * 8;
+  ORIGAMI_REQUIRE(units < (int64_t(1) << 32) / kWeighThreads, "too many tokens for one call");
+  const dim3 grid(static_cast<unsigned>(units)), block(kWeighThreads);
+  hipLaunchKernelGGL((weigh_kernel<T, CELL, DP, MR, NT>), grid, block, 0, stream, p);
+  return check_launch("weigh_kernel");
+}
+
+template <typename T, Cell CELL, int DP>
+int launch_weigh(const WeighParams& p, int64_t requests, hipStream_t stream) {
+  // tiles of 16 rows where the requests have no more, as in a decode step
+  if (static_cast<int64_t>(p.tokens) * p.G.d <= 16 * requests)
+    return launch_weigh<T, CELL, DP, 16, DP == 256 ? 2 : 4>(p, requests, stream);
+  return launch_weigh<T, CELL, DP, 32, 1>(p, requests, stream);
+}
+
+template <typename T, Cell CELL>
+int launch_weigh(const WeighParams& p, int64_t requests, hipStream_t stream) {
+  return p.D <= 64    ? launch_weigh<T, CELL, 64>(p, requests, stream)
+         : p.D <= 128 ? launch_weigh<T, CELL, 128>(p, requests, stream)
+                      : launch_weigh<T, CELL, 256>(p, requests, stream);
+}
+
+template <typename T>
+int launch_weigh(const WeighParams& p, Cell cell, int64_t requests, hipStream_t stream) {
+  if (cell == kFp8) return launch_weigh<T, kFp8>(p, requests, stream);
+  if (cell == kFp4) return launch_weigh<T, kFp4>(p, requests, stream);
+  return launch_weigh<T, kWide>(p, requests, stream);
+}
+
+// ---------------------------------------------------------------------------
+// Eviction
+// ---------------------------------------------------------------------------
+
+struct EvictParams {
+  uint8_t* cache;
+  int64_t blk_stride, half_stride, num_blocks;  // rows of H * D, as cache_geometry
+  const int64_t *tables, *out_tables, *lengths;
+  int64_t table_stride, out_table_stride;
+  Divisor block_size, H;
+  int32_t max_tokens, keep, recent, out_places;
+  const float* weights;
+  float* out_weights;
+  int64_t w_request, w_head, o_request, o_head;  // strides, in elements
+  int64_t* kept;  // [requests, H, keep]
+  int32_t row_bytes;
+  Divisor pieces;     // of a row, in loads
+  Divisor row_tiles;  // of a request's kept tokens
+};
+
+constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64, kBins = 2048;
+
+// What is kept of one request's head: all of the newest `recent`, and of the others those with the
+// largest weights, of equal ones the first.
+struct Share {
+  int tokens, kept, older, need;  // `need` of the first `older` tokens
+};
+
+__device__ __forceinline__ Share share_of(const EvictParams& p, int r) {
+  Share s;
+  s.tokens = static_cast<int>(min(max(p.lengths[r], int64_t(0)), static_cast<int64_t>(p.max_tokens)));
+  s.kept = min(s.tokens, p.keep);
+  const int last = min(p.recent, s.kept);
+  s.older = s.tokens - last;
+  s.need = s.kept - last;
+  return s;
+}
+
+// Weights as whole numbers in the same order; both zeros are one, NaN is the largest.
+__device__ __forceinline__ uint32_t rank_of(float w) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, w);
+  if (w != w) return 0xffffffffu;
+  if (w == 0.0f) return 0x80000000u;
+  return b >> 31 ? ~b : b | 0x80000000u;
+}
+
+// One workgroup: the tokens that one head of one request keeps.  The rank of the last of them is
+// found by its digits, from the highest, from counts of the ranks that have the digits before it;
+// then waves list the tokens of a part of the places each.
+__global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
+  __shared__ uint32_t bins[kBins];
+  __shared__ uint32_t wave_sum[kSelectWaves], wave_same[kSelectWaves];
+  __shared__ uint32_t found[2];
+  const int r = divide(static_cast<int>(blockIdx.x), p.H);
+  const int h = static_cast<int>(blockIdx.x) - r * p.H.d;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Share s = share_of(p, r);
+  const float* const w = p.weights + r * p.w_request + h * p.w_head;
+  float* const out_w = p.out_weights + r * p.o_request + h * p.o_head;
+  int64_t* const kept = p.kept + static_cast<int64_t>(blockIdx.x) * p.keep;
+
+  // ranks above `cut` are kept, and the first `ties` of those equal to it
+  uint32_t cut = 0, ties = 0;
+  if (s.need == 0) {
+    cut = 0xffffffffu;
+  } else if (s.need < s.older) {
+    uint32_t left = s.need, known = 0;
+    for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : (shift == 10 ? 0 : -1)) {
+      const int width = shift == 0 ? 10 : 11;
+      for (int i = tid; i < kBins; i += kSelectThreads) bins[i] = 0;
+      __syncthreads();
+      for (int i = tid; i < s.older; i += kSelectThreads) {
+        const uint32_t k = rank_of(w[i]);
+        if (((k ^ cut) & known) == 0) atomicAdd(&bins[(k >> shift) & ((1u << width) - 1)], 1u);
+      }
+      __syncthreads();
+      // thread i has digits 2 i and 2 i + 1 from the highest down
+      const uint32_t high = bins[kBins - 1 - 2 * tid], low = bins[kBins - 2 - 2 * tid];
+      uint32_t upto = high + low;
+#pragma unroll
+      for (int x = 1; x < 64; x <<= 1) {
+        const uint32_t other = __shfl_up(upto, x);
+        upto += lane >= x ? other : 0;
+      }
+      if (lane == 63) wave_sum[wave] = upto;
+      __syncthreads();
+      for (int i = 0; i < wave; ++i) upto += wave_sum[i];
+      const uint32_t above = upto - high - low;
+      if (above < left && upto >= left) {
+        const bool second = above + high < left;
+        found[0] = kBins - 1 - 2 * tid - second;
+        found[1] = above + (second ? high : 0);
+      }
+      __syncthreads();
+      cut |= found[0] << shift;
+      left -= found[1];
+      known |= ((1u << width) - 1) << shift;
+    }
+    ties = left;
+  } else {
+    ties = s.older;  // all
+  }
+
+  // each wave lists its part of the places, 64 at a time
+  const int part = (s.tokens + kSelectThreads - 1) / kSelectThreads * 64;
+  const int first = min(wave * part, s.tokens), last = min(first + part, s.tokens);
+  uint32_t sure = 0, same = 0;
+  for (int i = first; i < last; i += 64) {
+    const int t = i + lane;
+    const uint32_t k = t < s.older ? rank_of(w[t]) : 0;
+    sure += __popcll(__ballot(t < last && (t >= s.older || k > cut)));
+    same += __popcll(__ballot(t < last && t < s.older && k == cut));
+  }
+  __syncthreads();
+  if (lane == 0) {
+    wave_sum[wave] = sure;
+    wave_same[wave] = same;
+  }
+  __syncthreads();
+  uint32_t sure_before = 0, same_before = 0;
+  for (int i = 0; i < wave; ++i) {
+    sure_before += wave_sum[i];
+    same_before += wave_same[i];
+  }
+  for (int i = first; i < last; i += 64) {
+    const int t = i + lane;
+    const bool in = t < last;
+    const float weight = in ? w[t] : 0.0f;
+    const uint32_t k = t < s.older ? rank_of(weight) : 0;
+    const uint64_t lower = (1ull << lane) - 1;
+    const uint64_t sures = __ballot(in && (t >= s.older || k > cut));
+    const uint64_t sames = __ballot(in && t < s.older && k == cut);
+    const uint32_t same_rank = same_before + __popcll(sames & lower);
+    const bool mine = ((sures >> lane) & 1) || (((sames >> lane) & 1) && same_rank < ties);
+    if (mine) {
+      const uint32_t at = sure_before + __popcll(sures & lower) + min(same_rank, ties);
+      kept[at] = t;
+      out_w[at] = weight;
+    }
+    sure_before += __popcll(sures);
+    same_before += __popcll(sames);
+  }
+  for (int i = s.kept + tid; i < p.keep; i += kSelectThreads) kept[i] = -1;
+  for (int i = s.kept + tid; i < p.out_places; i += kSelectThreads) out_w[i] = 0.0f;
+}
+
+constexpr int kMoveThreads = 256, kMoveTokens = 8;
+
+// One workgroup: kMoveTokens new tokens of a request, all heads, keys and values.  V: what a load
+// has.
+template <typename V>
+__global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictParams p) {
+  const int r = divide(static_cast<int>(blockIdx.x), p.row_tiles);
+  const int j0 = (static_cast<int>(blockIdx.x) - r * p.row_tiles.d) * kMoveTokens;
+  const int kept = share_of(p, r).kept;
+  if (j0 >= kept) return;
+  const int count = min(kMoveTokens, kept - j0);
+  const int64_t* const table = p.tables + r * p.table_stride;
+  const int64_t* const out_table = p.out_tables + r * p.out_table_stride;
+  const int rows = count * p.H.d, all = rows * p.pieces.d;
+  for (int i = threadIdx.x; i < all; i += kMoveThreads) {
+    const int row = divide(i, p.pieces), piece = i - row * p.pieces.d;
+    const int j = j0 + divide(row, p.H), h = row - (j - j0) * p.H.d;
+    const int t = static_cast<int>(p.kept[(static_cast<int64_t>(r) * p.H.d + h) * p.keep + j]);
+    const int from_block = divide(t, p.block_size), to_block = divide(j, p.block_size);
+    const int64_t from = table[from_block], to = out_table[to_block];
+    if (to < 0 || to >= p.num_blocks) continue;
+    const bool in = from >= 0 && from < p.num_blocks;
+    const int64_t src =
+        (in ? from : 0) * p.blk_stride + (t - from_block * p.block_size.d);
+    const int64_t dst = to * p.blk_stride + (j - to_block * p.block_size.d);
+    V v[2] = {};
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+      if (in)
+        v[half] = *reinterpret_cast<const V*>(
+            p.cache + ((src + half * p.half_stride) * p.H.d + h) * p.row_bytes +
+            piece * static_cast<int>(sizeof(V)));
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+      *reinterpret_cast<V*>(p.cache + ((dst + half * p.half_stride) * p.H.d + h) * p.row_bytes +
+                            piece * static_cast<int>(sizeof(V))) = v[half];
+  }
+}
+
+int check_cache(int64_t cache_layout, int64_t num_blocks, int64_t block_size, int64_t heads,
+                int64_t head_dim, const void* kv_cache, int64_t* blk_stride,
+                int64_t* half_stride) {
+  ORIGAMI_REQUIRE(heads > 0, "heads must be positive");
+  ORIGAMI_REQUIRE(head_dim > 0 && head_dim % 8 == 0 && head_dim <= 256,
+                  "head_dim must be a multiple of 8, at most 256");
+  ORIGAMI_REQUIRE(num_blocks >= 0 && block_size > 0, "cache block size must be positive");
+  if (int rc = cache_geometry(cache_layout, num_blocks, block_size, blk_stride, half_stride))
+    return rc;
+  ORIGAMI_REQUIRE(block_size <= INT32_MAX / 2 / std::max<int64_t>(num_blocks, 1),
+                  "the cache has too many token slots");
+  ORIGAMI_REQUIRE(aligned16(kv_cache), "kv_cache must be 16-byte aligned");
+  return ORIGAMI_OK;
+}
+
+bool paged_dtype(int64_t dtype) {
+  return dtype == ORIGAMI_DTYPE_FLOAT16 || dtype == ORIGAMI_DTYPE_BFLOAT16 ||
+         dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN || dtype == ORIGAMI_DTYPE_FLOAT4_E2M1;
+}
+
+constexpr int64_t kMostTokens = int64_t(1) << 30;
+
+}  // namespace
+
+extern "C" {
+
+int origami_accumulate_attention_weights(
+    const void* query, int64_t dtype, const int64_t* strides, int64_t tokens, int64_t query_heads,
+    const float* lse, const void* kv_cache, int64_t cache_dtype, int64_t cache_layout,
+    int64_t num_blocks, int64_t block_size, int64_t heads, int64_t head_dim,
+    const int64_t* block_tables, int64_t table_stride, int64_t table_blocks,
+    const int64_t* lengths, int64_t requests, const int64_t* query_starts, int64_t max_tokens,
+    double scale, double k_scale, const float* weights, float* out, int64_t places,
+    const int64_t* weight_strides, origami_stream_t stream_) {
+  WeighParams p{};
+  int64_t half_stride;
+  ORIGAMI_REQUIRE(dtype == ORIGAMI_DTYPE_FLOAT16 || dtype == ORIGAMI_DTYPE_BFLOAT16,
+                  "queries must be float16 or bfloat16");
+  ORIGAMI_REQUIRE(cache_dtype == dtype || cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN ||
+                      cache_dtype == ORIGAMI_DTYPE_FLOAT4_E2M1,
+                  "kv_cache must have the queries' dtype or be float8_e4m3fn or in 4 bits");
+  if (int rc = check_cache(cache_layout, num_blocks, block_size, heads, head_dim, kv_cache,
+                           &p.blk_stride, &half_stride))
+    return rc;
+  ORIGAMI_REQUIRE(query_heads > 0 && query_heads % heads == 0,
+                  "query heads must be a multiple of the cache's heads");
+  ORIGAMI_REQUIRE(tokens >= 0 && requests >= 0 && max_tokens >= 0 && places >= 0 &&
+                      table_blocks >= 0,
+                  "token counts must not be negative");
+  ORIGAMI_REQUIRE(places <= kMostTokens, "too many tokens for one call");
+  ORIGAMI_REQUIRE(tokens < (int64_t(1) << 24) / query_heads, "too many query rows for one call");
+  ORIGAMI_REQUIRE(requests < (int64_t(1) << 24) / heads, "too many requests for one call");
+  ORIGAMI_REQUIRE(max_tokens <= places, "max_tokens exceeds the weights' places");
+  ORIGAMI_REQUIRE(ceil_div(max_tokens, block_size) <= table_blocks,
+                  "max_tokens exceeds the block tables");
+  ORIGAMI_REQUIRE(query_starts != nullptr || tokens == requests,
+                  "without query_starts every request has one query token");
+  ORIGAMI_REQUIRE(cache_scale(k_scale), "cache scales must be positive and finite in binary32");
+  ORIGAMI_REQUIRE(cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN || k_scale == 1.0,
+                  "cache scales are for float8_e4m3fn caches");
+  p.scale = static_cast<float>(scale * k_scale);
+  ORIGAMI_REQUIRE(std::isfinite(p.scale), "scale must be finite in binary32");
+  ORIGAMI_REQUIRE(strides[0] >= 0 && strides[1] >= 0, "row strides must not be negative");
+  for (int i = 0; i < 4; ++i)
+    ORIGAMI_REQUIRE(weight_strides[i] >= 0, "weight strides must not be negative");
+  ORIGAMI_REQUIRE(table_stride >= 0, "the table stride must not be negative");
+  if (requests == 0 || places == 0) return ORIGAMI_OK;
+  ORIGAMI_REQUIRE((tokens == 0 || (query != nullptr && lse != nullptr)) && out != nullptr &&
+                      lengths != nullptr && (block_tables != nullptr || max_tokens == 0) &&
+                      (kv_cache != nullptr || num_blocks == 0),
+                  "queries, weights, lengths, tables and the cache must not be null");
+  p.query = query;
+  p.q_token = strides[0];
+  p.q_head = strides[1];
+  p.q_vec = aligned16(query) && strides[0] % 8 == 0 && strides[1] % 8 == 0;
+  p.lse = lse;
+  p.cache = static_cast<const uint8_t*>(kv_cache);
+  p.num_blocks = num_blocks;
+  p.tables = block_tables;
+  p.lengths = lengths;
+  p.starts = query_starts;
+  p.table_stride = table_stride;
+  p.block_size = divisor(block_size);
+  p.H = divisor(heads);
+  p.G = divisor(query_heads / heads);
+  p.tokens = static_cast<int32_t>(tokens);
+  p.Hq = static_cast<int32_t>(query_heads);
+  p.D = static_cast<int32_t>(head_dim);
+  p.max_tokens = static_cast<int32_t>(max_tokens);
+  p.places = static_cast<int32_t>(places);
+  p.weights = weights;
+  p.out = out;
+  p.w_request = weight_strides[0];
+  p.w_head = weight_strides[1];
+  p.o_request = weight_strides[2];
+  p.o_head = weight_strides[3];
+  const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  return dtype == ORIGAMI_DTYPE_BFLOAT16
+             ? launch_weigh<bf16>(p, cell_of(cache_dtype), requests, stream)
+             : launch_weigh<f16>(p, cell_of(cache_dtype), requests, stream);
+}
+
+int origami_evict_kv_cache(
+    void* kv_cache, int64_t cache_dtype, int64_t cache_layout, int64_t num_blocks,
+    int64_t block_size, int64_t heads, int64_t head_dim, const int64_t* block_tables,
+    int64_t table_stride, int64_t table_blocks, const int64_t* lengths, int64_t requests,
+    int64_t max_tokens, const float* weights, int64_t places, const int64_t* out_tables,
+    int64_t out_table_stride, int64_t out_table_blocks, int64_t keep, int64_t recent,
+    int64_t* kept, float* out_weights, int64_t out_places, const int64_t* weight_strides,
+    origami_stream_t stream_) {
+  EvictParams p{};
+  ORIGAMI_REQUIRE(paged_dtype(cache_dtype),
+                  "kv_cache must be float16, bfloat16 or float8_e4m3fn or in 4 bits");
+  if (int rc = check_cache(cache_layout, num_blocks, block_size, heads, head_dim, kv_cache,
+                           &p.blk_stride, &p.half_stride))
+    return rc;
+  ORIGAMI_REQUIRE(requests >= 0 && max_tokens >= 0 && places >= 0 && keep >= 0 && recent >= 0 &&
+                      out_places >= 0 && table_blocks >= 0 && out_table_blocks >= 0,
+                  "token counts must not be negative");
+  ORIGAMI_REQUIRE(max_tokens <= kMostTokens && keep <= kMostTokens && out_places <= kMostTokens,
+                  "too many tokens for one call");
+  ORIGAMI_REQUIRE(requests < (int64_t(1) << 22) / heads, "too many requests for one call");
+  ORIGAMI_REQUIRE(max_tokens <= places, "max_tokens exceeds the weights' places");
+  const int64_t most = std::min(keep, max_tokens);
+  ORIGAMI_REQUIRE(most <= out_places, "what is kept exceeds the places of out_weights");
+  ORIGAMI_REQUIRE(ceil_div(max_tokens, block_size) <= table_blocks,
+                  "max_tokens exceeds the block tables");
+  ORIGAMI_REQUIRE(ceil_div(most, block_size) <= out_table_blocks,
+                  "what is kept exceeds the new block tables");
+  for (int i = 0; i < 4; ++i)
+    ORIGAMI_REQUIRE(weight_strides[i] >= 0, "weight strides must not be negative");
+  ORIGAMI_REQUIRE(table_stride >= 0 && out_table_stride >= 0,
+                  "the table strides must not be negative");
+  const int row_bytes = row_bytes_of(cell_of(cache_dtype), static_cast<int>(head_dim));
+  // rows that are whole 16 bytes move so, others by 4
+  const int load = row_bytes % 16 == 0 ? 16 : 4;
+  ORIGAMI_REQUIRE(heads <= INT32_MAX / kMoveTokens / 128, "too many heads for one call");
+  const int64_t tiles = std::max<int64_t>(ceil_div(most, kMoveTokens), 1);
+  ORIGAMI_REQUIRE(tiles < (int64_t(1) << 24) / std::max<int64_t>(requests, 1),
+                  "too many tokens for one call");
+  if (requests == 0) return ORIGAMI_OK;
+  ORIGAMI_REQUIRE(lengths != nullptr && (weights != nullptr || max_tokens == 0) &&
+                      (kept != nullptr || keep == 0) && (out_weights != nullptr || out_places == 0) &&
+                      (block_tables != nullptr || max_tokens == 0) &&
+                      (out_tables != nullptr || most == 0) &&
+                      (kv_cache != nullptr || num_blocks == 0),
+                  "weights, lengths, tables, results and the cache must not be null");
+  p.cache = static_cast<uint8_t*>(kv_cache);
+  p.num_blocks = num_blocks;
+  p.tables = block_tables;
+  p.out_tables = out_tables;
+  p.lengths = lengths;
+  p.table_stride = table_stride;
+  p.out_table_stride = out_table_stride;
+  p.block_size = divisor(block_size);
+  p.H = divisor(heads);
+  p.max_tokens = static_cast<int32_t>(max_tokens);
+  p.keep = static_cast<int32_t>(keep);
+  p.recent = static_cast<int32_t>(std::min(recent, kMostTokens));
+  p.out_places = static_cast<int32_t>(out_places);
+  p.weights = weights;
+  p.out_weights = out_weights;
+  p.w_request = weight_strides[0];
+  p.w_head = weight_strides[1];
+  p.o_request = weight_strides[2];
+  p.o_head = weight_strides[3];
+  p.kept = kept;
+  p.row_bytes = row_bytes;
+  p.pieces = divisor(row_bytes / load);
+  p.row_tiles = divisor(tiles);
+  const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  hipLaunchKernelGGL(select_kernel, dim3(static_cast<unsigned>(requests * heads)),
+                     dim3(kSelectThreads), 0, stream, p);
+  if (int rc = check_launch("select_kernel")) return rc;
+  if (most == 0) return ORIGAMI_OK;
+  const dim3 grid(static_cast<unsigned>(requests * tiles)), block(kMoveThreads);
+  if (load == 16)
+    hipLaunchKernelGGL(move_kernel<U32x4>, grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL(move_kernel<uint32_t>, grid, block, 0, stream, p);
+  return check_launch("move_kernel");
+}
+
+}  // extern "C"

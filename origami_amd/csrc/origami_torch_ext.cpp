@@ -447,6 +447,34 @@ int64_t paged_dtype_code(at::ScalarType t, const char* name) {
   return dtype_code(t, name);
 }
 
+// The element type of a paged cache: uint8 holds rows in 4 bits.
+int64_t cache_dtype_code(const at::Tensor& cache) {
+  if (cache.scalar_type() == at::kByte) return ORIGAMI_DTYPE_FLOAT4_E2M1;
+  return paged_dtype_code(cache.scalar_type(), "kv_cache");
+}
+
+// The channels of a head of the cache, whose rows in 4 bits are as many bytes as `rows` (a tensor
+// of rows of it) says.
+int64_t head_dim_of(const at::Tensor& cache, const at::Tensor& rows, const char* name) {
+  if (cache.scalar_type() != at::kByte) return cache.size(4);
+  TORCH_CHECK(rows.dim() == 3, name, " must be [tokens, heads, head_dim]");
+  const int64_t D = rows.size(2), bytes = origami_kv4_row_bytes(D);
+  TORCH_CHECK(bytes >= 0, origami_last_error());
+  TORCH_CHECK(cache.size(4) == bytes, "a kv_cache in 4 bits must have rows of ", bytes,
+              " bytes for ", D, " channels, not of ", cache.size(4));
+  return D;
+}
+
+// The channels of a head of the cache; those of rows in 4 bits follow from their bytes.
+int64_t channels_of(const at::Tensor& cache) {
+  if (cache.scalar_type() != at::kByte) return cache.size(4);
+  int64_t D = 8;
+  while (D < 256 && origami_kv4_row_bytes(D) < cache.size(4)) D += 8;
+  TORCH_CHECK(origami_kv4_row_bytes(D) == cache.size(4), "no head_dim has rows of ",
+              cache.size(4), " bytes in 4 bits");
+  return D;
+}
+
 // No record is kept of operations: it would leave a launch on addresses out, and play back what
 // this call gave.
 void require_eager() {
@@ -590,13 +618,13 @@ void require_apart(const Extent& result, const char* result_name, const Extent& 
 
 // A [tokens, heads, head_dim] tensor whose channels are contiguous.
 void require_rows(const at::Tensor& t, const char* name, const at::Tensor& cache,
-                  at::ScalarType dtype) {
+                  at::ScalarType dtype, int64_t head_dim) {
   require_plain(t, name);
   TORCH_CHECK(t.is_cuda() && t.device() == cache.device(), name,
               " must be on the kv_cache device");
   TORCH_CHECK(t.dim() == 3, name, " must be [tokens, heads, head_dim]");
   TORCH_CHECK(t.scalar_type() == dtype, name, " must have the same dtype as the other rows");
-  TORCH_CHECK(t.size(2) == cache.size(4), name, " head_dim differs from the kv_cache's");
+  TORCH_CHECK(t.size(2) == head_dim, name, " head_dim differs from the kv_cache's");
   TORCH_CHECK(t.stride(2) == 1 || t.numel() == 0, name, " channels must be contiguous");
 }
 
@@ -610,6 +638,15 @@ const int64_t* require_index(const at::Tensor& t, const char* name, const at::Te
               " must be a contiguous int64 vector");
   TORCH_CHECK(t.numel() == count, name, " must have ", count, " values, not ", t.numel());
   return count > 0 ? t.data_ptr<int64_t>() : nullptr;
+}
+
+void require_tables(const at::Tensor& t, const char* name, const at::Tensor& cache) {
+  require_plain(t, name);
+  TORCH_CHECK(t.is_cuda() && t.device() == cache.device(), name,
+              " must be on the kv_cache device");
+  TORCH_CHECK(t.scalar_type() == at::kLong && t.dim() == 2 &&
+                  (t.stride(1) == 1 || t.size(1) <= 1),
+              name, " must be int64 [requests, blocks] with contiguous rows");
 }
 
 // New tokens into the cache; returns the rotated queries (an undefined tensor, None in
@@ -626,9 +663,10 @@ c10::optional<at::Tensor> append_kv_cache(
   const CacheGeom g = layout_cache_geometry(kv_cache);
   const int64_t dtype = paged_dtype_code(key.scalar_type(), "key");
   TORCH_CHECK(dtype != ORIGAMI_DTYPE_FLOAT8_E4M3FN, "key must be float16 or bfloat16");
-  require_rows(key, "key", kv_cache, key.scalar_type());
-  require_rows(value, "value", kv_cache, key.scalar_type());
-  const int64_t tokens = key.size(0), D = kv_cache.size(4);
+  const int64_t D = head_dim_of(kv_cache, key, "key");
+  require_rows(key, "key", kv_cache, key.scalar_type(), D);
+  require_rows(value, "value", kv_cache, key.scalar_type(), D);
+  const int64_t tokens = key.size(0);
   TORCH_CHECK(key.size(1) == g.heads && value.size(1) == g.heads,
               "key and value heads differ from the kv_cache's");
   TORCH_CHECK(value.size(0) == tokens, "key and value must have the same tokens");
@@ -640,11 +678,11 @@ c10::optional<at::Tensor> append_kv_cache(
   Extent out_extent;  // of a new tensor: none
   int64_t query_heads = 0;
   if (query) {
-    require_rows(*query, "query", kv_cache, key.scalar_type());
+    require_rows(*query, "query", kv_cache, key.scalar_type(), D);
     TORCH_CHECK(query->size(0) == tokens, "query and key must have the same tokens");
     query_heads = query->size(1);
     if (query_out) {
-      require_rows(*query_out, "query_out", kv_cache, key.scalar_type());
+      require_rows(*query_out, "query_out", kv_cache, key.scalar_type(), D);
       TORCH_CHECK(query_out->sizes() == query->sizes(), "query_out must have the query's shape");
       out_extent = extent_of(*query_out);
       TORCH_CHECK(!shares_with_itself(out_extent), "query_out must not overlap itself");
@@ -707,8 +745,7 @@ c10::optional<at::Tensor> append_kv_cache(
   check(origami_append_kv_cache(
       key.data_ptr(), value.data_ptr(), query ? query->data_ptr() : nullptr,
       out ? out->data_ptr() : nullptr, dtype, strides, tokens, query_heads, kv_cache.data_ptr(),
-      paged_dtype_code(kv_cache.scalar_type(), "kv_cache"), g.layout, g.num_blocks, g.block_size,
-      g.heads, D, slot, position, cos_sin ? cos_sin->data_ptr<float>() : nullptr, table_rows,
+      cache_dtype_code(kv_cache), g.layout, g.num_blocks, g.block_size, g.heads, D, slot, position, cos_sin ? cos_sin->data_ptr<float>() : nullptr, table_rows,
       rotary_dim, interleaved, query_norm ? query_norm->data_ptr() : nullptr,
       key_norm ? key_norm->data_ptr() : nullptr, norm_dtype, eps, k_scale, v_scale,
       current_stream(kv_cache)));
@@ -731,14 +768,10 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
   const CacheGeom g = layout_cache_geometry(kv_cache);
   const int64_t dtype = paged_dtype_code(query.scalar_type(), "query");
   TORCH_CHECK(dtype != ORIGAMI_DTYPE_FLOAT8_E4M3FN, "query must be float16 or bfloat16");
-  require_rows(query, "query", kv_cache, query.scalar_type());
-  const int64_t tokens = query.size(0), Hq = query.size(1), D = kv_cache.size(4);
-  require_plain(block_tables, "block_tables");
-  TORCH_CHECK(block_tables.is_cuda() && block_tables.device() == kv_cache.device(),
-              "block_tables must be on the kv_cache device");
-  TORCH_CHECK(block_tables.scalar_type() == at::kLong && block_tables.dim() == 2 &&
-                  (block_tables.stride(1) == 1 || block_tables.size(1) <= 1),
-              "block_tables must be int64 [requests, blocks] with contiguous rows");
+  const int64_t D = head_dim_of(kv_cache, query, "query");
+  require_rows(query, "query", kv_cache, query.scalar_type(), D);
+  const int64_t tokens = query.size(0), Hq = query.size(1);
+  require_tables(block_tables, "block_tables", kv_cache);
   const int64_t requests = block_tables.size(0), blocks = block_tables.size(1);
   const int64_t* const own = require_index(own_tokens, "own_tokens", kv_cache, requests);
   const int64_t *prefix = nullptr, *starts = nullptr;
@@ -763,7 +796,7 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
   Extent out_extent, lse_extent;  // of new tensors: none
   if (out_) {
     out = *out_;
-    require_rows(out, "out", kv_cache, query.scalar_type());
+    require_rows(out, "out", kv_cache, query.scalar_type(), D);
     TORCH_CHECK(out.sizes() == query.sizes(), "out must have the query's shape");
     out_extent = extent_of(out);
     TORCH_CHECK(!shares_with_itself(out_extent), "out must not overlap itself");
@@ -794,7 +827,7 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
     if (prefix_block_ids) apart(*prefix_block_ids, "prefix_block_ids");
     if (query_starts) apart(*query_starts, "query_starts");
   }
-  const int64_t cache_dtype = paged_dtype_code(kv_cache.scalar_type(), "kv_cache");
+  const int64_t cache_dtype = cache_dtype_code(kv_cache);
   const int64_t bytes = origami_shared_prefix_attention_workspace(
       tokens, Hq, g.heads, D, prefix_tokens, requests, most, most_own, cache_dtype);
   TORCH_CHECK(bytes >= 0, origami_last_error());
@@ -810,6 +843,197 @@ at::Tensor shared_prefix_attention(at::Tensor query, at::Tensor kv_cache,
       v_scale, out.data_ptr(), lse ? lse->data_ptr<float>() : nullptr,
       bytes > 0 ? work.data_ptr() : nullptr, bytes, current_stream(kv_cache)));
   return out;
+}
+
+// The rows of slots of the cache, as (key, value).
+std::tuple<at::Tensor, at::Tensor> read_kv_cache(at::Tensor kv_cache, at::Tensor slots,
+                                                 at::ScalarType dtype, double k_scale,
+                                                 double v_scale,
+                                                 c10::optional<at::Tensor> key_out,
+                                                 c10::optional<at::Tensor> value_out) {
+  require_eager();
+  require_plain(kv_cache, "kv_cache");
+  require_device(kv_cache, "kv_cache");
+  const CacheGeom g = layout_cache_geometry(kv_cache);
+  const int64_t out_dtype = paged_dtype_code(dtype, "dtype");
+  TORCH_CHECK(out_dtype != ORIGAMI_DTYPE_FLOAT8_E4M3FN, "dtype must be float16 or bfloat16");
+  const int64_t tokens = slots.numel(), cache_dtype = cache_dtype_code(kv_cache);
+  const int64_t* const slot = require_index(slots, "slots", kv_cache, tokens);
+  const int64_t head_dim = channels_of(kv_cache);
+  const c10::OptionalDeviceGuard guard(kv_cache.device());
+  at::Tensor out[2];
+  Extent extents[2];  // of new tensors: none
+  const char* const names[2] = {"key_out", "value_out"};
+  for (int i = 0; i < 2; ++i) {
+    const auto& given = i == 0 ? key_out : value_out;
+    if (!given) {
+      out[i] = at::empty({tokens, g.heads, head_dim}, kv_cache.options().dtype(dtype));
+      continue;
+    }
+    out[i] = *given;
+    require_rows(out[i], names[i], kv_cache, dtype, head_dim);
+    TORCH_CHECK(out[i].size(0) == tokens && out[i].size(1) == g.heads, names[i],
+                " must be [slots, heads, head_dim]");
+    extents[i] = extent_of(out[i]);
+    TORCH_CHECK(!shares_with_itself(extents[i]), names[i], " must not overlap itself");
+    require_apart(extents[i], names[i], extent_of(kv_cache), "kv_cache");
+    require_apart(extents[i], names[i], extent_of(slots), "slots");
+  }
+  require_apart(extents[0], names[0], extents[1], names[1]);
+  const int64_t strides[4] = {out[0].stride(0), out[0].stride(1), out[1].stride(0),
+                              out[1].stride(1)};
+  check(origami_read_kv_cache(kv_cache.data_ptr(), cache_dtype, g.layout, g.num_blocks,
+                              g.block_size, g.heads, head_dim, slot, tokens, k_scale, v_scale,
+                              out[0].data_ptr(), out[1].data_ptr(), out_dtype, strides,
+                              current_stream(kv_cache)));
+  return {out[0], out[1]};
+}
+
+// A float32 [requests, heads, places] tensor whose places are contiguous.
+void require_weights(const at::Tensor& t, const char* name, const at::Tensor& cache,
+                     int64_t requests, int64_t heads) {
+  require_plain(t, name);
+  TORCH_CHECK(t.is_cuda() && t.device() == cache.device(), name,
+              " must be on the kv_cache device");
+  TORCH_CHECK(t.scalar_type() == at::kFloat && t.dim() == 3 && t.size(0) == requests &&
+                  t.size(1) == heads,
+              name, " must be float32 [requests, heads, places]");
+  TORCH_CHECK(t.stride(2) == 1 || t.size(2) <= 1, name, " places must be contiguous");
+}
+
+// The most tokens of a request: what is given, or what the block tables hold.
+int64_t most_tokens(c10::optional<int64_t> given, int64_t blocks, int64_t block_size) {
+  int64_t most;
+  if (given) return *given;
+  return __builtin_mul_overflow(blocks, block_size, &most) ? INT64_MAX : most;
+}
+
+// Sums of attention weights with those of the query rows added; `out` or a new tensor.
+at::Tensor accumulate_attention_weights(
+    at::Tensor query, at::Tensor kv_cache, at::Tensor block_tables, at::Tensor tokens,
+    at::Tensor lse, c10::optional<at::Tensor> weights, c10::optional<at::Tensor> query_starts,
+    c10::optional<int64_t> max_tokens, c10::optional<double> scale, double k_scale,
+    c10::optional<at::Tensor> out_) {
+  require_eager();
+  require_plain(kv_cache, "kv_cache");
+  require_device(kv_cache, "kv_cache");
+  const CacheGeom g = layout_cache_geometry(kv_cache);
+  const int64_t dtype = paged_dtype_code(query.scalar_type(), "query");
+  TORCH_CHECK(dtype != ORIGAMI_DTYPE_FLOAT8_E4M3FN, "query must be float16 or bfloat16");
+  const int64_t D = head_dim_of(kv_cache, query, "query");
+  require_rows(query, "query", kv_cache, query.scalar_type(), D);
+  const int64_t rows = query.size(0), Hq = query.size(1);
+  require_tables(block_tables, "block_tables", kv_cache);
+  const int64_t requests = block_tables.size(0), blocks = block_tables.size(1);
+  const int64_t* const lengths = require_index(tokens, "tokens", kv_cache, requests);
+  const int64_t* starts = nullptr;
+  if (query_starts) starts = require_index(*query_starts, "query_starts", kv_cache, requests + 1);
+  TORCH_CHECK(starts || rows == requests, "without query_starts every request has one query token");
+  require_plain(lse, "lse");
+  require_device(lse, "lse");
+  TORCH_CHECK(lse.device() == kv_cache.device() && lse.scalar_type() == at::kFloat &&
+                  lse.dim() == 2 && lse.size(0) == rows && lse.size(1) == Hq,
+              "lse must be float32 [tokens, query heads] on the kv_cache device");
+  const int64_t most = most_tokens(max_tokens, blocks, g.block_size);
+  if (weights) require_weights(*weights, "weights", kv_cache, requests, g.heads);
+  const c10::OptionalDeviceGuard guard(kv_cache.device());
+
+  at::Tensor out;
+  if (out_) {
+    out = *out_;
+    require_weights(out, "out", kv_cache, requests, g.heads);
+    TORCH_CHECK(!weights || out.size(2) == weights->size(2), "out must have the weights' shape");
+    const Extent extent = extent_of(out);
+    TORCH_CHECK(!shares_with_itself(extent), "out must not overlap itself");
+    const auto apart = [&](const at::Tensor& t, const char* name) {
+      require_apart(extent, "out", extent_of(t), name);
+    };
+    apart(query, "query");
+    apart(kv_cache, "kv_cache");
+    apart(block_tables, "block_tables");
+    apart(tokens, "tokens");
+    apart(lse, "lse");
+    if (query_starts) apart(*query_starts, "query_starts");
+    if (weights && !same_elements(out, *weights)) apart(*weights, "other elements of weights");
+  } else {
+    TORCH_CHECK(most >= 0 && (weights || most <= (int64_t(1) << 30)),
+                "max_tokens must not be negative or too many");
+    out = at::empty({requests, g.heads, weights ? weights->size(2) : most},
+                    query.options().dtype(at::kFloat));
+  }
+  const at::Tensor& in = weights ? *weights : out;
+  const int64_t strides[2] = {query.stride(0), query.stride(1)};
+  const int64_t weight_strides[4] = {in.stride(0), in.stride(1), out.stride(0), out.stride(1)};
+  check(origami_accumulate_attention_weights(
+      query.data_ptr(), dtype, strides, rows, Hq, lse.numel() > 0 ? lse.data_ptr<float>() : nullptr,
+      kv_cache.data_ptr(), cache_dtype_code(kv_cache), g.layout, g.num_blocks, g.block_size,
+      g.heads, D, block_tables.numel() ? block_tables.data_ptr<int64_t>() : nullptr,
+      block_tables.stride(0), blocks, lengths, requests, starts, most,
+      scale ? *scale : 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(D, 1))), k_scale,
+      weights && weights->numel() ? weights->data_ptr<float>() : nullptr,
+      out.numel() ? out.data_ptr<float>() : nullptr, out.size(2), weight_strides,
+      current_stream(kv_cache)));
+  return out;
+}
+
+// The tokens that requests keep, moved to blocks of their own: (their places before, their
+// weights).
+std::tuple<at::Tensor, at::Tensor> evict_kv_cache(at::Tensor kv_cache, at::Tensor block_tables,
+                                                  at::Tensor tokens, at::Tensor weights,
+                                                  at::Tensor out_tables, int64_t keep,
+                                                  int64_t recent,
+                                                  c10::optional<int64_t> max_tokens,
+                                                  c10::optional<at::Tensor> out_weights_) {
+  require_eager();
+  require_plain(kv_cache, "kv_cache");
+  require_device(kv_cache, "kv_cache");
+  const CacheGeom g = layout_cache_geometry(kv_cache);
+  const int64_t cache_dtype = cache_dtype_code(kv_cache);
+  const int64_t D = channels_of(kv_cache);
+  require_tables(block_tables, "block_tables", kv_cache);
+  const int64_t requests = block_tables.size(0), blocks = block_tables.size(1);
+  const int64_t* const lengths = require_index(tokens, "tokens", kv_cache, requests);
+  require_weights(weights, "weights", kv_cache, requests, g.heads);
+  require_tables(out_tables, "out_tables", kv_cache);
+  TORCH_CHECK(out_tables.size(0) == requests, "out_tables must have a row for every request");
+  TORCH_CHECK(keep >= 0 && keep <= (int64_t(1) << 30), "keep must not be negative or too many");
+  const int64_t most = most_tokens(max_tokens, blocks, g.block_size);
+  const c10::OptionalDeviceGuard guard(kv_cache.device());
+  const Extent cache_extent = extent_of(kv_cache);
+  Extent extent;  // of a new tensor: none
+  at::Tensor out;
+  if (out_weights_) {
+    out = *out_weights_;
+    require_weights(out, "out_weights", kv_cache, requests, g.heads);
+    extent = extent_of(out);
+    TORCH_CHECK(!shares_with_itself(extent), "out_weights must not overlap itself");
+    require_apart(extent, "out_weights", cache_extent, "kv_cache");
+  } else {
+    out = at::empty({requests, g.heads, std::max(weights.size(2), std::min(keep, most))},
+                    weights.options());
+  }
+  const auto apart = [&](const at::Tensor& t, const char* name) {
+    const Extent e = extent_of(t);
+    require_apart(cache_extent, "kv_cache", e, name);
+    require_apart(extent, "out_weights", e, name);
+  };
+  apart(block_tables, "block_tables");
+  apart(tokens, "tokens");
+  apart(weights, "weights");
+  apart(out_tables, "out_tables");
+  const at::Tensor kept = at::empty({requests, g.heads, keep}, tokens.options());
+  const int64_t weight_strides[4] = {weights.stride(0), weights.stride(1), out.stride(0),
+                                     out.stride(1)};
+  check(origami_evict_kv_cache(
+      kv_cache.data_ptr(), cache_dtype, g.layout, g.num_blocks, g.block_size, g.heads, D,
+      block_tables.numel() ? block_tables.data_ptr<int64_t>() : nullptr, block_tables.stride(0),
+      blocks, lengths, requests, most, weights.numel() ? weights.data_ptr<float>() : nullptr,
+      weights.size(2), out_tables.numel() ? out_tables.data_ptr<int64_t>() : nullptr,
+      out_tables.stride(0), out_tables.size(1), keep, recent,
+      kept.numel() ? kept.data_ptr<int64_t>() : nullptr,
+      out.numel() ? out.data_ptr<float>() : nullptr, out.size(2), weight_strides,
+      current_stream(kv_cache)));
+  return {kept, out};
 }
 
 }  // namespace
@@ -832,7 +1056,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("restore_plan_destroy", &restore_plan_destroy);
   m.def("append_kv_cache", &append_kv_cache);
   m.def("shared_prefix_attention", &shared_prefix_attention);
-  // how both find results that overlap inputs, for tests on any device
+  m.def("read_kv_cache", &read_kv_cache);
+  m.def("accumulate_attention_weights", &accumulate_attention_weights);
+  m.def("evict_kv_cache", &evict_kv_cache);
+  // how they find results that overlap inputs, for tests on any device
   m.def("_tensors_overlap", [](const at::Tensor& a, const at::Tensor& b) {
     return share_bytes(extent_of(a), extent_of(b));
   });

@@ -728,6 +728,21 @@ def kivi_quantize(kv: torch.Tensor, *, dims: Sequence[int], strides: Sequence[in
 # Operators on the paged cache that follow a restore (no reference counterpart)
 # ---------------------------------------------------------------------------
 
+def kv4_row_bytes(head_dim: int) -> int:
+    """Bytes of a row (one token's head of head_dim channels) of a paged cache in 4 bits: a uint8
+    tensor [2, blocks, block_size, heads, kv4_row_bytes(head_dim)] or [blocks, 2, ...], which
+    append_kv_cache, read_kv_cache, shared_prefix_attention, accumulate_attention_weights and
+    evict_kv_cache take in the place of a 16-bit or fp8 cache.
+
+    A row holds head_dim / 2 bytes of e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign; channel
+    2 i in the low half of byte i), then a byte s for each 32 channels, whose values are multiplied
+    with 2 ** (s - 127), filled up to whole dwords: 4.25 bits a channel of 128."""
+    size = _native.lib().origami_kv4_row_bytes(int(head_dim))
+    if size < 0:
+        raise ValueError("head_dim must be a multiple of 8, at most 256")
+    return size
+
+
 def append_kv_cache(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor,
                     slots: torch.Tensor, *, query: torch.Tensor | None = None,
                     positions: torch.Tensor | None = None, cos_sin: torch.Tensor | None = None,
@@ -747,7 +762,10 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tens
     (int64 [tokens]) are given: channels (i, i + rotary_dim / 2) are a pair, or (2 i, 2 i + 1)
     with `interleaved`.  A token whose position is outside the table is not written, and its
     query becomes zero.  Arithmetic is float32, rounded once.  A float8_e4m3fn kv_cache holds
-    key / k_scale and value / v_scale, limited to +-448.  Returns the queries: query_out
+    key / k_scale and value / v_scale, limited to +-448.  A uint8 kv_cache holds 4 bits a channel
+    (kv4_row_bytes): each 32 channels are rounded to e2m1 values times the least power of two, of
+    2 ** -23 to 2 ** 13, at which none is further than half a step from what is held; larger
+    values become +-49152, infinities too, and a NaN makes its 32 channels NaN.  Returns the queries: query_out
     (which may be `query` itself, but must share no element with anything else) or a new tensor;
     None without `query`.  No input may lie in the cache.  Overlaps are refused.  For inference
     only: inputs that require a gradient or carry a tangent are refused, and so are traced and
@@ -755,6 +773,23 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tens
     return _ext.ext().append_kv_cache(key, value, kv_cache, slots, query, positions, cos_sin,
                                       interleaved, query_norm, key_norm, eps, k_scale, v_scale,
                                       query_out)
+
+
+def read_kv_cache(kv_cache: torch.Tensor, slots: torch.Tensor, *,
+                  dtype: torch.dtype | None = None, k_scale: float = 1.0, v_scale: float = 1.0,
+                  key_out: torch.Tensor | None = None, value_out: torch.Tensor | None = None
+                  ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(key, value) [slots, heads, head_dim] as the paged cache holds them, of dtype float16 or
+    bfloat16 (default: the cache's, else bfloat16): what append_kv_cache wrote to these slots
+    (int64, block id * block size + offset).  Rows of a 16-bit cache come as they are, of a
+    float8_e4m3fn one times k_scale and v_scale, rounded once, and of one in 4 bits exactly.  Slots
+    outside the cache, such as -1, give zeros; a slot may be given twice.  key_out and value_out
+    (channels contiguous) may be given for the results; overlaps are refused.  For inference only,
+    as append_kv_cache."""
+    if dtype is None:
+        wide = kv_cache.dtype in (torch.float16, torch.bfloat16)
+        dtype = kv_cache.dtype if wide else torch.bfloat16
+    return _ext.ext().read_kv_cache(kv_cache, slots, dtype, k_scale, v_scale, key_out, value_out)
 
 
 def shared_prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor,
@@ -773,8 +808,8 @@ def shared_prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor,
     below, and call once for prompts and once for single tokens.
 
     query is float16 or bfloat16 [tokens, query_heads, head_dim]; kv_cache has its dtype or
-    is float8_e4m3fn with k_scale / v_scale; query head h uses cache head
-    h // (query_heads // heads).  Request r has own_tokens[r] tokens of its own in blocks
+    is float8_e4m3fn with k_scale / v_scale or uint8 with rows in 4 bits (kv4_row_bytes); query
+    head h uses cache head h // (query_heads // heads).  Request r has own_tokens[r] tokens of its own in blocks
     block_tables[r] (int64, rows contiguous), those of its queries included.  Without
     query_starts, row r of query is request r's newest token; with it (int64
     [requests + 1]) rows query_starts[r] .. query_starts[r + 1] - 1 are request r's newest
@@ -804,6 +839,61 @@ def shared_prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor,
     return (result, lse) if return_lse else result
 
 
+def accumulate_attention_weights(query: torch.Tensor, kv_cache: torch.Tensor,
+                                 block_tables: torch.Tensor, tokens: torch.Tensor,
+                                 lse: torch.Tensor, weights: torch.Tensor | None = None, *,
+                                 query_starts: torch.Tensor | None = None,
+                                 max_tokens: int | None = None, scale: float | None = None,
+                                 k_scale: float = 1.0, out: torch.Tensor | None = None
+                                 ) -> torch.Tensor:
+    """Sums of the attention weights that cached tokens get, from which evict_kv_cache chooses:
+    out[r, h, t] = weights[r, h, t] + the sum of exp(scale * q . k_t - lse) over the query rows of
+    request r that see token t and whose query head uses cache head h.
+
+    Request r has tokens[r] tokens in blocks block_tables[r] (a prefix shared with others is part of
+    them here), and its query rows are its newest ones: row r of query, or with query_starts rows
+    query_starts[r] .. query_starts[r + 1] - 1; all of a prompt's rows or some last ones may be
+    given.  query, kv_cache, k_scale and scale are those of shared_prefix_attention, and lse
+    (float32 [rows, query_heads]) is what it returned with return_lse for these rows over all of
+    the request's tokens.  weights (default: zeros) and the result are float32 [requests, heads,
+    places]; place t is the request's token t.  `out` may be `weights` itself; without weights and
+    out the result has max_tokens places (default: the block table's slots).  Tokens past max_tokens
+    and in blocks outside the cache get nothing.  Lengths and tables are read on the device, so a
+    call can be captured in a graph.  Each sum is float32, in a fixed order.  Overlaps are refused
+    but of out with weights.  For inference only, as shared_prefix_attention."""
+    return _ext.ext().accumulate_attention_weights(
+        query, kv_cache, block_tables, tokens, lse, weights, query_starts, max_tokens, scale,
+        k_scale, out)
+
+
+def evict_kv_cache(kv_cache: torch.Tensor, block_tables: torch.Tensor, tokens: torch.Tensor,
+                   weights: torch.Tensor, out_tables: torch.Tensor, keep: int, *,
+                   recent: int = 0, max_tokens: int | None = None,
+                   out_weights: torch.Tensor | None = None
+                   ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Evicts all but `keep` tokens of each request, for each cache head by itself: the newest
+    `recent` stay, and of the others those with the largest weights[r, h, t] (float32 [requests,
+    heads, places], as accumulate_attention_weights makes them), of equal ones the first (NaN is
+    larger than infinity).
+
+    Request r has tokens[r] tokens in blocks block_tables[r], of which the first max_tokens count
+    (default: the block table's slots).  What it keeps, min(tokens[r], keep) rows a head, is copied
+    in its order to blocks out_tables[r] of the same cache, keys and values bit by bit whatever the
+    cache's type, and is the request from then on: with out_tables as its block table and
+    tokens.clamp(max=keep) tokens.  Blocks that are read stay as they are, so a prefix may be shared
+    with other requests; blocks that are written must be in no table that is read, and in
+    out_tables once.  A row of a block outside the cache is copied as zeros, and to one outside it
+    not at all.  Since rows are copied, it pays to let a cache grow by some tens of tokens between
+    two calls.
+
+    Returns (kept, out_weights): int64 [requests, heads, keep] places that the rows had, then -1,
+    and their weights, then zeros, in `out_weights` or a new tensor of the weights' shape (at least
+    what is kept), so that new tokens start at zero.  Nothing is read back, so a call can be
+    captured in a graph.  Overlaps are refused."""
+    return _ext.ext().evict_kv_cache(kv_cache, block_tables, tokens, weights, out_tables, keep,
+                                     recent, max_tokens, out_weights)
+
+
 # ---------------------------------------------------------------------------
 # Reference extension surface (origami_bitpack_cuda_v6, cpp:894-903)
 # ---------------------------------------------------------------------------
@@ -831,5 +921,6 @@ __all__ = [
     "gather_kv_blocks", "kv_symbol_layout", "CACHE_KV_FIRST", "CACHE_BLOCKS_FIRST",
     "cachegen_unpack_dequantize_to_kv_cache", "cachegen_unpack_dequantize",
     "kivi_dequantize_to_kv_cache", "dequant_cache_geometry", "append_kv_cache",
-    "shared_prefix_attention",
+    "shared_prefix_attention", "kv4_row_bytes", "read_kv_cache", "accumulate_attention_weights",
+    "evict_kv_cache",
 ]
