@@ -68,7 +68,7 @@ struct Group {
   int32_t units;   // workgroups
   int32_t shape;   // kShapeRows[shape] rows each, at most
   Divisor tiles;   // row tiles of a request, or of the batch
-  int32_t splits;  // ranges of `chunk` tokens
+  Divisor splits;  // ranges of `chunk` tokens
   int32_t chunk;
   int32_t slot;    // the partial results' first slot
   int32_t first;   // the first token of range 0
@@ -101,8 +101,14 @@ __device__ __forceinline__ V load_global(const uint8_t* p) {
   return *(const __attribute__((address_space(1))) V*)(reinterpret_cast<uintptr_t>(p));
 }
 
+// Dwords that start on four bytes.
+template <int N>
+using Dwords = uint32_t __attribute__((ext_vector_type(N), aligned(4)));
+
 // What a lane reads of a row that is not in the cache, and of channels past the last.
 __device__ const U32x4 kZeros = {0, 0, 0, 0};
+// A row in 4 bits that is not in the cache.
+__device__ const U32x4 kZeroRow[fp4_row_bytes(256) / 16 + 1] = {};
 
 // MR x MR scores or results: value x of a lane is in column lane % MR and in row
 // 4 (lane / MR) + x % 4 + (256 / MR) (x / 4).
@@ -236,6 +242,50 @@ __device__ __forceinline__ U32x4 expand(U32x4 raw) {
   return raw;
 }
 
+// 8 W channels next to each other of a row in 4 bits, and the bytes of their scales.
+template <int W>
+struct Fp4Lane {
+  static constexpr int kScales = (W + 3) / 4;
+  uint32_t codes[W], scale[kScales];
+};
+// From where they are in a row, whose scales are `to_scale` further.  Where not all WHOLE lanes
+// have their channels, there are `end` dwords of them.
+template <int W, bool WHOLE>
+__device__ __forceinline__ Fp4Lane<W> load_lane(const uint8_t* src, int to_scale, int end) {
+  Fp4Lane<W> out;
+  constexpr int N = W < 4 ? W : 4;
+#pragma unroll
+  for (int b = 0; b < Fp4Lane<W>::kScales; ++b) {
+    out.scale[b] = load_global<uint8_t>(src + to_scale + b);
+    if constexpr (WHOLE) {
+      const auto w = load_global<Dwords<N>>(src + 16 * b);
+#pragma unroll
+      for (int j = 0; j < N; ++j) out.codes[4 * b + j] = w[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        out.codes[4 * b + j] = load_global<uint32_t>(src + 4 * min(4 * b + j, end - 1));
+    }
+  }
+  return out;
+}
+template <typename T, int W>
+__device__ __forceinline__ bool drop_odd(Fp4Lane<W>& x) {
+  bool odd = false;
+#pragma unroll
+  for (int b = 0; b < Fp4Lane<W>::kScales; ++b) {
+    const uint32_t scale = x.scale[b];
+#pragma unroll
+    for (int j = 4 * b; j < W && j < 4 * b + 4; ++j) {
+      Fp4x8 part{x.codes[j], scale};
+      odd |= drop_odd<T>(part);
+      x.codes[j] = part.codes;
+      x.scale[b] = part.scale;
+    }
+  }
+  return odd;
+}
+
 // Four values rounded to T; `vec`: rows start on 8 bytes.
 template <typename T>
 __device__ __forceinline__ void store4(T* dst, Float4 v, bool vec) {
@@ -275,6 +325,20 @@ __device__ __forceinline__ Request request_of(const AttendParams& p, int r) {
   return q;
 }
 
+// The request and the range of tokens number `at` of a cache in 4 bits, whose heads are on one
+// chiplet: ranges of a request follow each other, so that they are spread over the chiplets
+// whatever its length, and start elsewhere for each request, since the last ones may have no
+// tokens (requests by turns took 120 us for 95 with lengths of 1000 to 16384).
+__device__ __forceinline__ bool range_of(const AttendParams& p, const Group& g, bool batch, int at,
+                                         int* r, int* split) {
+  *r = batch ? 0 : divide(at, g.splits);
+  *split = at - *r * g.splits.d;
+  if (batch || *r >= p.requests.d) return batch && *split < g.splits.d;
+  const int turned = *split + *r;
+  *split = turned - divide(turned, g.splits) * g.splits.d;
+  return true;
+}
+
 __device__ __forceinline__ uint32_t as_u32(float x) { return __builtin_bit_cast(uint32_t, x); }
 __device__ __forceinline__ float as_float(uint32_t x) { return __builtin_bit_cast(float, x); }
 
@@ -302,6 +366,32 @@ __device__ __forceinline__ float fold_wave(float x, Fold fold) {
   one = halves[0];
   other = halves[1];
   return fold(as_float(one), as_float(other));
+}
+
+// Four channels of a row's result, and with the first ones its maximum and sum.
+template <typename T>
+__device__ __forceinline__ void put_four(const AttendParams& p, const Group& g, const Request& rq,
+                                         int h, int split, int rows, int row, int ch, Float4 v,
+                                         float base, float sum) {
+  if (row >= rows || ch >= p.D) return;
+  const int qi = divide(row, p.G), head = h * p.G.d + row - qi * p.G.d;
+  const int64_t n = rq.first + qi, at = n * p.Hq + head;
+  if (p.slots > 1) {
+    const int64_t slot = (g.slot + split) * (static_cast<int64_t>(p.tokens) * p.Hq) + at;
+    if (ch == 0) {
+      p.part_ml[2 * slot] = base - kLift<T>;
+      p.part_ml[2 * slot + 1] = sum;
+    }
+    // without a token the join does not read the rest
+    if (sum != 0.0f) *reinterpret_cast<Float4*>(p.part_o + slot * p.D + ch) = v;
+  } else {
+    // a row without a weight is zero also where a value is infinite or NaN
+    if (sum == 0.0f) v = Float4{0.0f, 0.0f, 0.0f, 0.0f};
+    const float inv = sum == 0.0f ? 0.0f : p.v_scale / sum;
+    store4(static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + ch, v * inv, p.out_vec);
+    if (p.lse && ch == 0)
+      p.lse[at] = sum == 0.0f ? -INFINITY : kLn2 * (base - kLift<T> + log2f(sum));
+  }
 }
 
 // Where the 16-byte piece `piece` of token `tok`'s row is in LDS, in pieces of its row.  Keys are
@@ -341,6 +431,13 @@ __device__ __forceinline__ Vec8<T> read_values(const uint8_t* values, int lane, 
 template <int N>
 using Int = std::integral_constant<int, N>;
 
+// Bytes of LDS of a wave of attend_four: the values of 32 tokens, or 16 rows of its part.
+template <int DP, bool JOIN>
+constexpr int kFourLds = JOIN ? 16 * (DP + 4) * 4 : 32 * DP * 2;
+// Waves of its workgroups.  Without a join they are independent.
+template <int DP, bool JOIN>
+constexpr int kFourWaves = JOIN && DP <= 128 ? 8 : 4;
+
 // Tokens that a team of waves (the WR waves with the same tokens) has in LDS at a time.
 template <int DP, int WR>
 constexpr int kTeamTokens = WR == 8 || (WR == 4 && DP == 64) ? 64 : 32;
@@ -375,18 +472,23 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
   const int c = lane % MR, q4 = lane / MR;
 
   // The unit: row tiles of the same keys are 8 units apart, so that they run on the same chiplet
-  // at about the same time and its L2 gives the keys to all but the first.
+  // at about the same time and its L2 gives the keys to all but the first.  So are the heads of the
+  // same tokens in 4 bits, whose rows share lines.
   const int eight = unit >> 3, eighth = unit & 7;
   int u = divide(eight, g.tiles);
   const int tile = eight - u * g.tiles.d;
-  u = u * 8 + eighth;
-  const int uh = divide(u, p.H), h = u - uh * p.H.d;
+  if constexpr (CELL != kFp4) u = u * 8 + eighth;
+  int uh = divide(u, p.H);
+  const int h = u - uh * p.H.d;
+  if constexpr (CELL == kFp4) uh = uh * 8 + eighth;
   int r = 0, split = uh;
-  if (!batch) {
+  if constexpr (CELL == kFp4) {
+    if (!range_of(p, g, batch, uh, &r, &split)) return;
+  } else if (!batch) {
     split = divide(uh, p.requests);
     r = uh - split * p.requests.d;
   }
-  if (split >= g.splits) return;
+  if (split >= g.splits.d) return;
   const int t0 = g.first + split * g.chunk;
   const int64_t* const table = p.tables + static_cast<int64_t>(r) * p.table_stride;
   // The block of token t.  Blocks of the first tokens are asked for before the request's length is
@@ -664,28 +766,8 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
     for (int j = 0; j < 4; ++j) v[j] = fabsf(v[j]) < INFINITY ? 0.0f : v[j];
     return v;
   };
-  // Four channels of a row's result, and with the first ones its maximum and sum.
   const auto put = [&](int row, int ch, Float4 v, float base, float sum) {
-    if (row >= rows || ch >= p.D) return;
-    const int qi = divide(row, p.G), head = h * p.G.d + row - qi * p.G.d;
-    const int64_t n = rq.first + qi, at = n * p.Hq + head;
-    if (p.slots > 1) {
-      const int64_t slot =
-          (g.slot + split) * (static_cast<int64_t>(p.tokens) * p.Hq) + at;
-      if (ch == 0) {
-        p.part_ml[2 * slot] = base - kLift<T>;
-        p.part_ml[2 * slot + 1] = sum;
-      }
-      // without a token the join does not read the rest
-      if (sum != 0.0f) *reinterpret_cast<Float4*>(p.part_o + slot * p.D + ch) = v;
-    } else {
-      // a row without a weight is zero also where a value is infinite or NaN
-      if (sum == 0.0f) v = Float4{0.0f, 0.0f, 0.0f, 0.0f};
-      const float inv = sum == 0.0f ? 0.0f : p.v_scale / sum;
-      store4(static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + ch, v * inv, p.out_vec);
-      if (p.lse && ch == 0)
-        p.lse[at] = sum == 0.0f ? -INFINITY : kLn2 * (base - kLift<T> + log2f(sum));
-    }
+    put_four<T>(p, g, rq, h, split, rows, row, ch, v, base, sum);
   };
 
   if constexpr (WT > 1) {
@@ -782,6 +864,290 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
     for (int x = 0; x < ACC; x += 4)
       put(again, MR * d + 4 * q4 + 256 / MR * (x / 4),
           Float4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]}, base, sum);
+}
+
+// The rows of one KV head (16 at most) over a range of tokens in 4 bits, 32 at a step: of one wave,
+// or with JOIN of the waves of a workgroup, which take steps in turn and join their parts in LDS.
+//
+// A decode step's few rows leave time for little else than the bytes, so nothing waits here for
+// another wave until the end.  Where there are units enough, waves by themselves have the longest
+// ranges and no join; waves next to each other are then heads of the same tokens, whose rows of 68
+// bytes (of 128 channels) share lines.  With few units the parts of eight waves are one.
+// Four lanes next to each other load a row, a quarter each: that is one access to the cache for a
+// row, where rows over lanes (as the products take them) are one for each lane.  Two steps are on
+// their way while one is computed.  The keys' quarters change lanes through LDS as they are, and
+// are widened where the product K Q takes them, 32 channels with one scale in a lane (the queries
+// have the same order of channels); the values are widened on their way to LDS, which transposes
+// them for V P.
+template <typename T, int DP, bool WHOLE, bool JOIN>
+__device__ __forceinline__ void attend_four(const AttendParams& p, const Group& g, int unit,
+                                            bool batch, int wave, uint8_t* wave_lds, float* ml) {
+  constexpr int kStride = JOIN ? 32 * kFourWaves<DP, JOIN> : 32;  // tokens between a wave's steps
+  uint8_t* const lds = wave_lds + wave * kFourLds<DP, JOIN>;
+  constexpr int MR = 16, NG = 4, TT = 32, KS = DP / 32, DT = DP / MR, NCH = DP / 8, W = KS;
+  constexpr int kRawPitch = 18 * 4 * W;  // bytes: quarters of two rows are in different banks
+  static_assert(8 * kRawPitch <= kFourLds<DP, JOIN> && TT * DP * 2 <= kFourLds<DP, JOIN>, "LDS");
+  using Codes = uint32_t __attribute__((ext_vector_type(W)));
+  const int lane = threadIdx.x & 63, c = lane % MR, q4 = lane / MR;
+  const int uh = divide(unit, p.H), h = unit - uh * p.H.d;
+  int r, split;
+  if (!range_of(p, g, batch, uh, &r, &split)) return;
+  const int t0 = g.first + split * g.chunk;
+  const int64_t* const table = p.tables + static_cast<int64_t>(r) * p.table_stride;
+  const int bound = batch ? p.prefix : p.prefix + p.max_own;
+  const auto block_of = [&](int t, int before) -> int64_t {
+    if (t >= before) return -1;
+    const bool pre = t < p.prefix;
+    return (pre ? p.prefix_ids : table)[divide(pre ? t : t - p.prefix, p.block_size)];
+  };
+  const int tl = lane % TT;
+  const int first = t0 + (JOIN ? wave * TT : 0);
+  const int64_t id = block_of(first + tl, bound), id1 = block_of(first + kStride + tl, bound);
+  int64_t ahead = block_of(first + 2 * kStride + tl, bound);
+
+  const Request rq = batch ? Request{0, p.tokens, 0, 0} : request_of(p, r);
+  const int rows = rq.count * p.G.d;
+  if (rows == 0) return;
+  const int end = batch ? p.prefix : p.prefix + rq.own;
+  const int row = c;
+  const auto seen_by = [&](int i) -> int {  // tokens that row i sees
+    return p.prefix + (batch ? 0 : min(max(rq.before + divide(i, p.G) + 1, 0), rq.own));
+  };
+  const int limit = seen_by(row);
+  const float scale = p.scale == 0.0f ? 1.0f : fabsf(p.scale);  // as in attend
+  Vec8<T> qf[KS];
+  {
+    const int qi = divide(row, p.G), head = h * p.G.d + row - qi * p.G.d;
+    const T* const src =
+        static_cast<const T*>(p.query) + (rq.first + qi) * p.q_token + head * p.q_head;
+    const bool vec =
+        ((reinterpret_cast<uintptr_t>(p.query) | 2 * p.q_token | 2 * p.q_head) & 15) == 0;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const int d = q4 * (DP / NG) + 8 * k;
+      qf[k] = Vec8<T>{};
+      if (row < rows && d < p.D) {
+        if (vec) {
+          qf[k] = *reinterpret_cast<const Vec8<T>*>(src + d);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) qf[k][j] = src[d + j];
+        }
+        if (p.scale <= 0.0f) qf[k] = p.scale == 0.0f ? Vec8<T>{} : -qf[k];
+      }
+    }
+  }
+  const int most = seen_by(rows - 1), nearest = seen_by(0);  // tokens that some, all rows see
+  const int t1 = min(min(end, most), t0 + g.chunk);
+
+  // what this lane loads; past the last channel it is some others, whose queries are zero
+  const int tok = lane >> 2, slot_ch = (lane & 3) * (DP / NG), ch = slot_ch < p.D ? slot_ch : 0;
+  const int lane_end = min(p.D - ch, DP / NG) / 8, lane_scale = p.D / 2 + ch / 32 - ch / 2;
+  const int bytes = fp4_row_bytes(p.D);
+  const uint32_t pitch = static_cast<uint32_t>(p.H.d) * bytes;
+  const int64_t to_values = p.half_stride * pitch;
+  const uint8_t* const lane_rows = p.cache + (static_cast<int64_t>(h) * bytes + ch / 2);
+  const uint8_t* const no_row = reinterpret_cast<const uint8_t*>(kZeroRow) + ch / 2;
+  const auto row_of = [&](int t, int64_t id) -> int {  // of the cache, -1 where t has none
+    if (t >= t1 || id < 0 || id >= p.num_blocks) return -1;
+    const int i = t < p.prefix ? t : t - p.prefix;
+    return static_cast<int>(id * p.blk_stride + i - divide(i, p.block_size) * p.block_size.d);
+  };
+  struct Step {
+    Fp4Lane<W> keys[2], values[2];
+    uint32_t there;  // its tokens that are in the cache
+  };
+  const auto load_step = [&](Step& s, int mine) {
+    s.there = static_cast<uint32_t>(__ballot(mine >= 0));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = __shfl(mine, 16 * i + tok);
+      const uint8_t* const src = lane_rows + static_cast<uint64_t>(static_cast<uint32_t>(at)) * pitch;
+      s.keys[i] = load_lane<W, WHOLE>(at >= 0 ? src : no_row, lane_scale, lane_end);
+      s.values[i] =
+          load_lane<W, WHOLE>(at >= 0 ? src + to_values : no_row, lane_scale, lane_end);
+    }
+  };
+
+  Tile<MR> o[DT];
+  float base = -INFINITY, sum = 0.0f;
+  bool odd = false;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) o[d] = Tile<MR>{};
+
+  const auto compute = [&](Step& s, int t, auto reload) {
+    // hidden values that are no numbers: see attend
+    if (min(t + TT, t1) > nearest)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) odd |= drop_odd<T>(s.values[i]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      Codes w;
+#pragma unroll
+      for (int k = 0; k < W; ++k) w[k] = s.keys[i].codes[k];
+      *reinterpret_cast<Codes*>(lds + ((lane & 3) + 4 * i) * kRawPitch + tok * 4 * W) = w;
+    }
+    __builtin_amdgcn_wave_barrier();
+    Codes kw[2];
+    float scales[2][Fp4Lane<W>::kScales];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      kw[i] = *reinterpret_cast<const Codes*>(lds + (q4 + 4 * i) * kRawPitch + c * 4 * W);
+#pragma unroll
+      for (int b = 0; b < Fp4Lane<W>::kScales; ++b)
+        scales[i][b] = fp4_scale(__shfl(s.keys[i].scale[b], 4 * c + q4));
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const int at = 16 * i + tok;
+        *reinterpret_cast<U32x4*>(
+            lds + (at * NCH + value_piece<DP, MR>(at, slot_ch / 8 + k)) * 16) =
+            fp4_expand<T>(s.values[i].codes[k], fp4_scale(s.values[i].scale[k / 4]));
+      }
+    __builtin_amdgcn_wave_barrier();
+    const uint32_t there = s.there;
+    reload();
+    Tile<MR> sc[2] = {};
+#pragma unroll
+    for (int k = 0; k < W; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        sc[i] = mfma<T, MR>(
+            __builtin_bit_cast(Vec8<T>, fp4_expand<T>(kw[i][k], scales[i][k / 4])), qf[k], sc[i]);
+    if (there != ~0u || t + TT > nearest) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = 16 * (i / 4) + 4 * q4 + i % 4;
+        if (t + at >= limit || !((there >> at) & 1)) sc[i / 4][i % 4] = -INFINITY;
+      }
+    }
+    float best = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) best = fmaxf(best, sc[i / 4][i % 4]);
+    best = max_over_groups<MR>(best) * scale;
+    const bool rises = best > base + kSlack<T>;
+    if (__any(rises)) {
+      const float next = rises ? best : base;
+      const float keep = __builtin_amdgcn_exp2f(base - (next == -INFINITY ? 0.0f : next));
+      base = next;
+      sum *= keep;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= keep;
+    }
+    const float below = kLift<T> - (base == -INFINITY ? 0.0f : base);
+    Vec8<T> pf;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float e = __builtin_amdgcn_exp2f(fmaf(sc[i / 4][i % 4], scale, below));
+      sum += e;
+      pf[i] = static_cast<T>(e);
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      o[d] = mfma<T, MR>(read_values<T, DP, MR>(lds, lane, 0, d), pf, o[d]);
+    __builtin_amdgcn_wave_barrier();
+  };
+
+  if (first < t1) {
+    // Block ids are asked for before the rows that come after them, whose arrival they would else
+    // wait for; steps' loads stay in their order, since waits count what came after.
+    Step even, other;
+    int next = row_of(first + 2 * kStride + tl, ahead);
+    ahead = block_of(min(first + 3 * kStride + tl, t1 - 1), t1);
+    load_step(even, row_of(first + tl, id));
+    __builtin_amdgcn_sched_barrier(0);
+    load_step(other, row_of(first + kStride + tl, id1));
+    const auto advance = [&](Step& s, int t) {  // to the rows of the step after the next
+      const int mine = next;
+      next = row_of(t + 3 * kStride + tl, ahead);
+      ahead = block_of(min(t + 4 * kStride + tl, t1 - 1), t1);
+      load_step(s, mine);
+    };
+    for (int t = first; t < t1; t += 2 * kStride) {
+      compute(even, t, [&] { advance(even, t); });
+      if (t + kStride >= t1) break;
+      compute(other, t + kStride, [&] { advance(other, t + kStride); });
+    }
+  }
+
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+  odd = JOIN ? __syncthreads_or(odd) : __any(odd);
+  // calls add(row of the cache's values) for the tokens whose odd values were left out, and some
+  // before them, as far as row i sees them: see attend
+  const auto each_odd_token = [&](int i, auto add) {
+    for (int t = max(t0, nearest - TT); t < min(t1, seen_by(i)); ++t) {
+      const int at = row_of(t, block_of(t, t1));
+      if (at >= 0)
+        add(p.cache + (at + p.half_stride) * pitch + static_cast<int64_t>(h) * bytes);
+    }
+  };
+  const auto odd_part = [&](const uint8_t* values, int ch) {
+    Float4 v = four_values<T, kFp4>(values, min(ch, p.D - 4), p.D);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = fabsf(v[j]) < INFINITY ? 0.0f : v[j];
+    return v;
+  };
+  if constexpr (JOIN) {
+    constexpr int NW = kFourWaves<DP, JOIN>, kPitch = DP + 4;
+    const auto part_row = [&](int w, int i) {
+      return reinterpret_cast<float*>(wave_lds + w * kFourLds<DP, JOIN>) + i * kPitch;
+    };
+    if (q4 == 0) {
+      ml[(wave * MR + c) * 2] = base;
+      ml[(wave * MR + c) * 2 + 1] = sum;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      *reinterpret_cast<Float4*>(part_row(wave, c) + MR * d + 4 * q4) = o[d];
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(rows, MR) * (DP / 4); i += 64 * NW) {
+      const int at = i / (DP / 4), d = 4 * (i % (DP / 4));
+      float top = -INFINITY, total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[(w * MR + at) * 2]);
+      const float zero = top == -INFINITY ? 0.0f : top;
+      Float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float weight = __builtin_amdgcn_exp2f(ml[(w * MR + at) * 2] - zero);
+        total += ml[(w * MR + at) * 2 + 1] * weight;
+        v += *reinterpret_cast<const Float4*>(part_row(w, at) + d) * weight;
+      }
+      if (odd) each_odd_token(at, [&](const uint8_t* values) { v += odd_part(values, d); });
+      put_four<T>(p, g, rq, h, split, rows, at, d, v, top, total);
+    }
+  } else {
+    if (odd)
+      each_odd_token(row, [&](const uint8_t* values) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] += odd_part(values, MR * d + 4 * q4);
+      });
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      put_four<T>(p, g, rq, h, split, rows, row, MR * d + 4 * q4, o[d], base, sum);
+  }
+}
+
+// `beside` workgroups that follow each other in the units' order are 8 apart: on one chiplet.
+template <typename T, int DP, bool WHOLE, bool JOIN>
+__global__ __launch_bounds__((64 * kFourWaves<DP, JOIN>), JOIN || DP == 256 ? 1 : (WHOLE ? 3 : 2))
+    void attend_four_kernel(AttendParams p, Divisor beside) {
+  constexpr int NW = kFourWaves<DP, JOIN>;
+  __shared__ alignas(16) uint8_t lds[NW * kFourLds<DP, JOIN>];
+  __shared__ float ml[JOIN ? NW * 32 : 1];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int eight = static_cast<int>(blockIdx.x >> 3);
+  const int some = divide(eight, beside);
+  int unit = (some * 8 + static_cast<int>(blockIdx.x & 7)) * beside.d + eight - some * beside.d;
+  if constexpr (!JOIN) unit = unit * NW + wave;
+  const int kind = unit >= p.group[0].units;
+  unit -= kind ? p.group[0].units : 0;
+  if (unit >= p.group[kind].units) return;
+  attend_four<T, DP, WHOLE, JOIN>(p, p.group[kind], unit, kind == 0, wave, lds, ml);
 }
 
 template <typename T, Cell CELL, int DP, int SHAPE>
@@ -930,6 +1296,8 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendParams p, int 
   if (p.lse && ch == 0) p.lse[row] = total == 0.0f ? -INFINITY : kLn2 * (best + log2f(total));
 }
 
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
 template <typename T, Cell CELL, int DP, int S0, int S1>
 int launch_shapes(const AttendParams& p, hipStream_t stream) {
   const dim3 grid(p.group[0].units + p.group[1].units), block(64 * kShapeWaves[S0]);
@@ -954,11 +1322,42 @@ int launch_units(const AttendParams& p, hipStream_t stream) {
   return launch_shapes<T, CELL, DP, 0, 0>(p, stream);
 }
 
+// How plan_of has attention computed: by attend, or by attend_four with or without a join.
+enum Way { kTiles, kFourJoined, kFourWavesAlone };
+
+template <typename T, int DP, bool WHOLE, bool JOIN>
+int launch_four(const AttendParams& p, hipStream_t stream) {
+  constexpr int NW = kFourWaves<DP, JOIN>;
+  const int units = p.group[0].units + p.group[1].units;
+  const Divisor beside = divisor(JOIN ? 1 : std::max(p.H.d / NW, 1));
+  const int64_t workgroups = ceil_div(units, JOIN ? 1 : NW);
+  const dim3 grid(static_cast<unsigned>(ceil_div(workgroups, 8 * beside.d) * 8 * beside.d));
+  hipLaunchKernelGGL((attend_four_kernel<T, DP, WHOLE, JOIN>), grid, dim3(64 * NW), 0, stream, p,
+                     beside);
+  return check_launch("attend_four_kernel");
+}
+
+template <typename T, int DP>
+int launch_four(const AttendParams& p, Way way, hipStream_t stream) {
+  if (p.D % (DP / 4) == 0)
+    return way == kFourJoined ? launch_four<T, DP, true, true>(p, stream)
+                              : launch_four<T, DP, true, false>(p, stream);
+  return way == kFourJoined ? launch_four<T, DP, false, true>(p, stream)
+                            : launch_four<T, DP, false, false>(p, stream);
+}
+
+template <typename T, Cell CELL, int DP>
+int launch_units(const AttendParams& p, Way way, hipStream_t stream) {
+  if constexpr (CELL == kFp4)
+    if (way != kTiles) return launch_four<T, DP>(p, way, stream);
+  return launch_units<T, CELL, DP>(p, stream);
+}
+
 template <typename T, Cell CELL>
-int launch_attend(const AttendParams& p, hipStream_t stream) {
-  const int rc = p.D <= 64    ? launch_units<T, CELL, 64>(p, stream)
-                 : p.D <= 128 ? launch_units<T, CELL, 128>(p, stream)
-                              : launch_units<T, CELL, 256>(p, stream);
+int launch_attend(const AttendParams& p, Way way, hipStream_t stream) {
+  const int rc = p.D <= 64    ? launch_units<T, CELL, 64>(p, way, stream)
+                 : p.D <= 128 ? launch_units<T, CELL, 128>(p, way, stream)
+                              : launch_units<T, CELL, 256>(p, way, stream);
   if (rc) return rc;
   const dim3 block(kJoinThreads);
   if (p.slots == 1) return ORIGAMI_OK;
@@ -978,18 +1377,17 @@ int launch_attend(const AttendParams& p, hipStream_t stream) {
 }
 
 template <typename T>
-int launch_attend(const AttendParams& p, Cell cell, hipStream_t stream) {
-  if (cell == kFp8) return launch_attend<T, kFp8>(p, stream);
-  if (cell == kFp4) return launch_attend<T, kFp4>(p, stream);
-  return launch_attend<T, kWide>(p, stream);
+int launch_attend(const AttendParams& p, Cell cell, Way way, hipStream_t stream) {
+  if (cell == kFp8) return launch_attend<T, kFp8>(p, way, stream);
+  if (cell == kFp4) return launch_attend<T, kFp4>(p, way, stream);
+  return launch_attend<T, kWide>(p, way, stream);
 }
-
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The split of a call into units, from sizes that the host has.
 struct Plan {
   Group group[2];
   int64_t slots, units;
+  Way way;
 };
 
 // Units of one kind, before they are split: `count` of them, `live` with rows if the requests are
@@ -1012,6 +1410,14 @@ struct Kind {
 // any of the three is half or twice as large: the split needs to be near only.
 constexpr double kUnitTime = 6.0, kCuBytes = 20e3, kCuFlops = 3.2e6;
 
+// Caches in 4 bits with few rows.  Waves by themselves pay where there are enough of them with 256
+// tokens, and ranges of 256 to 1024 tokens that make about 2048 waves: 1 request of 32000 tokens
+// and 8 heads takes 24 us and, with joins in workgroups, 24; 8 of 4000 take 18 and 24, 64 of 2000 42
+// and 63 (49 with 3072 waves), 32 of 1000 to 16384 105 and 145.  Below, workgroups that join eight
+// waves, and a single part where it is short: 1 request of 1029 tokens takes 10.2 us, with two
+// parts 11.8, in waves by themselves 14.4; of 8000 tokens 15.0 and 14.6 to 16.3.
+constexpr int64_t kFourMany = 512, kFourWavesWanted = 2048;
+
 // Microseconds of a call whose kinds are split in s0 and s1 ranges: workgroups of the first kind go
 // to the CUs in order, then those of the second; and joining the parts of `rows` rows.
 double call_time(const Kind& k0, int64_t s0, const Kind& k1, int64_t s1, int64_t rows,
@@ -1032,7 +1438,8 @@ double call_time(const Kind& k0, int64_t s0, const Kind& k1, int64_t s1, int64_t
 
 Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_dim,
              int64_t prefix, int64_t requests, int64_t max_query, int64_t max_own,
-             int64_t row_bytes) {
+             Cell cell) {
+  const int64_t row_bytes = row_bytes_of(cell, head_dim);
   const int64_t G = query_heads / heads, last = head_dim <= 128 ? 2 : 1;
   // Where the bound of a request's rows fills workgroups by itself, every request reads the prefix
   // with its own tokens; that is slow for requests of few rows beside one of many.
@@ -1077,13 +1484,29 @@ Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_di
     if (s1 < want) break;
   }
   Plan plan{};
+  plan.way = kTiles;
+  if (cell == kFp4 && k1.shape == 0 && (!apart || k0.shape == 0)) {
+    plan.way = (k0.count + k1.count) * ceil_div(std::max(k0.span, k1.span), 256) >= kFourMany
+                   ? kFourWavesAlone
+                   : kFourJoined;
+    const auto ranges = [&](const Kind& k) {
+      if (plan.way == kFourJoined) return k.splits(k.span <= 1536 ? 1 : ceil_div(k.span, 512));
+      return k.splits(std::min(std::max(kFourWavesWanted / k.count, ceil_div(k.span, 1024)),
+                               ceil_div(k.span, 256)));
+    };
+    best0 = apart ? ranges(k0) : 1;
+    best1 = ranges(k1);
+  }
   const auto put = [&](Group& g, const Kind& k, int64_t splits, int64_t first) {
-    const int64_t units = ceil_div(k.count / k.tiles * splits, 8) * 8 * k.tiles;
+    const int64_t spread = cell == kFp4 ? heads : 1;  // see attend: units of the same tokens
+    const int64_t units = plan.way != kTiles
+                              ? k.count * splits
+                              : ceil_div(k.count / k.tiles / spread * splits, 8) * 8 * spread * k.tiles;
     plan.units += units;
     g.units = static_cast<int32_t>(std::min<int64_t>(units, INT32_MAX));
     g.shape = k.shape;
     g.tiles = divisor(k.tiles);
-    g.splits = static_cast<int32_t>(splits);
+    g.splits = divisor(splits);
     g.chunk = static_cast<int32_t>(k.chunk(splits));
     g.slot = static_cast<int32_t>(plan.slots);  // of the partial results
     g.first = static_cast<int32_t>(first);
@@ -1138,7 +1561,7 @@ int64_t origami_shared_prefix_attention_workspace(int64_t tokens, int64_t query_
   max_query_tokens = bound_of_queries(max_query_tokens, tokens);
   return workspace_bytes_of(plan_of(tokens, query_heads, heads, head_dim, prefix_tokens,
                                     requests, max_query_tokens, max_own_tokens,
-                                    row_bytes_of(cell_of(cache_dtype), head_dim)),
+                                    cell_of(cache_dtype)),
                             tokens, query_heads, head_dim);
 }
 
@@ -1193,7 +1616,7 @@ int origami_shared_prefix_attention(
 
   const Plan plan = plan_of(tokens, query_heads, heads, head_dim, prefix_tokens, requests,
                             max_query_tokens, max_own_tokens,
-                            row_bytes_of(cell_of(cache_dtype), head_dim));
+                            cell_of(cache_dtype));
   ORIGAMI_REQUIRE(plan.units < kMostUnits, "too many row tiles for one call");
   ORIGAMI_REQUIRE(workspace_bytes >= workspace_bytes_of(plan, tokens, query_heads, head_dim) &&
                       (plan.slots == 1 || workspace != nullptr) && aligned16(workspace),
@@ -1232,8 +1655,8 @@ int origami_shared_prefix_attention(
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + parts * head_dim;
   const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-  return dtype == ORIGAMI_DTYPE_BFLOAT16 ? launch_attend<bf16>(p, cell_of(cache_dtype), stream)
-                                         : launch_attend<f16>(p, cell_of(cache_dtype), stream);
+  return dtype == ORIGAMI_DTYPE_BFLOAT16 ? launch_attend<bf16>(p, cell_of(cache_dtype), plan.way, stream)
+                                         : launch_attend<f16>(p, cell_of(cache_dtype), plan.way, stream);
 }
 
 }  // extern "C"
