@@ -570,9 +570,16 @@ int origami_read_kv_cache(const void* kv_cache, int64_t cache_dtype, int64_t cac
  * that get nothing become weights' (0).
  *
  * Products are of dtype (e4m3 and 4 bits are widened exactly), scores, exponentials and sums
- * binary32.  Each sum is made by one workgroup in a fixed order.  query, strides, kv_cache and scale
- * are as for the attention.  out shares no memory with an input but weights, if it is all of it.
+ * binary32.  Sums are made in a fixed order.  query, strides, kv_cache and scale
+ * are as for the attention.  workspace is a 16-byte aligned device buffer of at least
+ * origami_accumulate_attention_weights_workspace bytes (0: may be null; -1: invalid sizes), in use
+ * until the call's work is done; calls that can run at the same time need their own.  out and
+ * workspace share no memory with each other or with an input, but out with weights, if it is all of
+ * it.
  */
+int64_t origami_accumulate_attention_weights_workspace(int64_t tokens, int64_t query_heads,
+                                                       int64_t heads, int64_t requests,
+                                                       int64_t places);
 int origami_accumulate_attention_weights(
     const void* query, int64_t dtype, const int64_t* strides, int64_t tokens, int64_t query_heads,
     const float* lse, const void* kv_cache, int64_t cache_dtype, int64_t cache_layout,
@@ -580,7 +587,8 @@ int origami_accumulate_attention_weights(
     const int64_t* block_tables, int64_t table_stride, int64_t table_blocks,
     const int64_t* lengths, int64_t requests, const int64_t* query_starts, int64_t max_tokens,
     double scale, double k_scale, const float* weights, float* out, int64_t places,
-    const int64_t* weight_strides, origami_stream_t stream);
+    const int64_t* weight_strides, void* workspace, int64_t workspace_bytes,
+    origami_stream_t stream);
 
 /*
  * Moves the tokens that requests keep to blocks of their own, for each cache head by itself: with

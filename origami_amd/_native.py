@@ -82,7 +82,8 @@ _SIGNATURES: dict[str, list] = {
         _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _f64, _f64, _p, _p, _i64, _p, _p],
     "origami_accumulate_attention_weights": [
         _p, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p,
-        _i64, _p, _i64, _f64, _f64, _p, _p, _i64, _p, _p],
+        _i64, _p, _i64, _f64, _f64, _p, _p, _i64, _p, _p, _i64, _p],
+    "origami_accumulate_attention_weights_workspace": [_i64] * 5,
     "origami_evict_kv_cache": [
         _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _i64,
         _i64, _i64, _i64, _p, _p, _i64, _p, _p],
@@ -124,6 +125,7 @@ def lib() -> ctypes.CDLL:
             L.origami_set_rows_grid_limit.restype = ctypes.c_int64
             L.origami_shared_prefix_attention_workspace.restype = ctypes.c_int64
             L.origami_kv4_row_bytes.restype = ctypes.c_int64
+            L.origami_accumulate_attention_weights_workspace.restype = ctypes.c_int64
             L.origami_restore_plan_destroy.restype = None
             L.origami_restore_plan_destroy.argtypes = [_p]
             L.origami_debug_counters.restype = None

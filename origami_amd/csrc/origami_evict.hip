@@ -25,6 +25,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+constexpr int64_t kWeighUnits = 2048, kMostWeighParts = 32;
+
 // ---------------------------------------------------------------------------
 // Adding up the weights
 // ---------------------------------------------------------------------------
@@ -39,15 +41,23 @@ struct WeighParams {
   int64_t num_blocks;
   const int64_t *tables, *lengths, *starts;
   int64_t table_stride;
-  Divisor block_size, H, G, tiles;  // tiles: of a request's places, in eights
+  Divisor block_size, requests, H, G;
+  Divisor tiles;  // of a request's places, in eights where the rows are few
+  Divisor parts;  // of the rows that see a tile, each of which a workgroup adds up
   int32_t tokens, Hq, D, max_tokens, places;
-  float scale;  // includes the keys' scale
+  float scale;  // includes log2 e and the keys' scale
   const float* weights;  // null: zeros
   float* out;
   int64_t w_request, w_head, o_request, o_head;  // strides, in elements
+  float* part_sums;  // [parts][requests][H][places], where there are several
 };
 
-constexpr int kWeighThreads = 256, kWeighWaves = kWeighThreads / 64;
+// Workgroups of eight waves with 32 tokens each, and stages of 64 rows, where there are many rows;
+// else of four waves with 64 tokens each (32 past 128 channels).
+template <int MR>
+constexpr int kWeighWaves = MR == 32 ? 8 : 4;
+template <int MR>
+constexpr int kStageTiles = MR == 32 ? 2 : 1;
 
 template <int MR>
 using Tile = float __attribute__((ext_vector_type(MR * MR / 64)));
@@ -81,34 +91,46 @@ struct __attribute__((aligned(4))) Dwords {
   uint32_t w[DWORDS];
 };
 
-// One workgroup: 4 NT MR tokens of one KV head of one request, against all query rows that see
-// any of them, MR rows at a time.  The keys stay in registers, as the second operand, so that a
-// token's scores are in the lanes of one column and are added up where they are; the queries go
-// through LDS.
+// One workgroup: NT MR tokens of one KV head of one request a wave, against the query rows that see
+// any of them or a part of those rows, MR rows at a time.  The keys stay in registers, as the
+// second operand, so that a token's scores are in the lanes of one column and are added up where
+// they are; the queries go through LDS, a stage ahead.
 //
 // The order of the channels in the products is free as long as keys and queries have the same: a
 // lane's 16 bytes of a key are 8, 16 or 32 channels in a row, whole loads of the cache's row.
 template <typename T, Cell CELL, int DP, int MR, int NT>
-__global__ __launch_bounds__(kWeighThreads) void weigh_kernel(WeighParams p) {
+__global__ __launch_bounds__(64 * kWeighWaves<MR>, MR == 32 && DP <= 128 ? 2 : 1)
+    void weigh_kernel(WeighParams p) {
+  constexpr int NW = kWeighWaves<MR>, kThreads = 64 * NW, SUB = kStageTiles<MR>, ROWS = SUB * MR;
   constexpr int NG = 64 / MR, KS = DP / (8 * NG), NCH = DP / 8, ACC = MR * MR / 64;
   constexpr int kWhole = CELL == kFp4 ? 4 : (CELL == kFp8 ? 2 : 1);
   constexpr int NPE = kWhole < KS ? kWhole : KS;  // pieces of 8 channels in a load
   constexpr int kPiece = CELL == kFp4 ? 4 : (CELL == kFp8 ? 8 : 16);
-  constexpr int kTokens = kWeighWaves * NT * MR;
-  constexpr int QL = MR * NCH / kWeighThreads > 0 ? MR * NCH / kWeighThreads : 1;
-  __shared__ U32x4 queries[2][MR * NCH];
-  __shared__ alignas(16) float lses[2][MR];
-  __shared__ alignas(16) int limits[2][MR];
+  constexpr int kTokens = NW * NT * MR;
+  constexpr int QL = (ROWS * NCH + kThreads - 1) / kThreads;
+  __shared__ U32x4 queries[2][ROWS * NCH];
+  __shared__ alignas(16) float lses[2][ROWS];
+  __shared__ alignas(16) int limits[2][ROWS];
+  __shared__ int least[2][SUB];  // the smallest limit of a tile's rows
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c = lane % MR, q4 = lane / MR;
 
-  // The heads of the same tokens are 8 workgroups apart, on one chiplet: their rows share lines.
-  const int unit = static_cast<int>(blockIdx.x);
-  const int eighth = unit & 7;
-  int u = divide(unit >> 3, p.H);
-  const int h = (unit >> 3) - u * p.H.d;
-  const int r = divide(u, p.tiles);
-  const int tile = (u - r * p.tiles.d) * 8 + eighth;
+  int r, h, tile, part = 0;
+  if constexpr (MR == 16) {
+    // the heads of the same tokens are 8 workgroups apart, on one chiplet: their rows share lines
+    int u = divide(static_cast<int>(blockIdx.x >> 3), p.H);
+    h = static_cast<int>(blockIdx.x >> 3) - u * p.H.d;
+    r = divide(u, p.tiles);
+    tile = (u - r * p.tiles.d) * 8 + static_cast<int>(blockIdx.x & 7);
+  } else {
+    // the first tokens, which most rows see, first; the same part of the rows on the same chiplet
+    int u = divide(static_cast<int>(blockIdx.x), p.parts);
+    part = static_cast<int>(blockIdx.x) - u * p.parts.d;
+    int v = divide(u, p.H);
+    h = u - v * p.H.d;
+    tile = divide(v, p.requests);
+    r = v - tile * p.requests.d;
+  }
   const int t0 = tile * kTokens;
   if (t0 >= p.places) return;
 
@@ -118,9 +140,13 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_kernel(WeighParams p) {
   const float* const weights =
       p.weights ? p.weights + r * p.w_request + h * p.w_head : nullptr;
   float* const out = p.out + r * p.o_request + h * p.o_head;
+  float* const sums =
+      p.part_sums + ((static_cast<int64_t>(part) * p.requests.d + r) * p.H.d + h) * p.places;
   const int first_t = t0 + wave * NT * MR;  // of this wave
   if (t0 >= end) {
-    for (int i = threadIdx.x; i < kTokens; i += kWeighThreads)
+    // of several parts the join takes care of these
+    if (p.parts.d > 1) return;
+    for (int i = threadIdx.x; i < kTokens; i += kThreads)
       if (t0 + i < p.places && out != weights)
         out[t0 + i] = weights ? weights[t0 + i] : 0.0f;
     return;
@@ -134,7 +160,6 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_kernel(WeighParams p) {
     q_count = static_cast<int>(min(max(p.starts[r + 1], a), n) - a);
   }
   const int before = length - q_count;  // tokens before the queries' (may be negative)
-  const int rows = q_count * p.G.d;
 
   // the keys
   const int bytes = row_bytes_of(CELL, p.D);
@@ -184,16 +209,23 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_kernel(WeighParams p) {
   }
 
   // Query i / G sees the tokens up to before + i / G: rows from the first that sees one of these.
-  const int row0 = min(max(t0 - before, 0), q_count) * p.G.d / MR * MR;
+  const int all_rows = q_count * p.G.d;
+  int row0 = min(max(t0 - before, 0), q_count) * p.G.d / MR * MR, rows = all_rows;
+  if (p.parts.d > 1) {
+    const int stages = (rows - row0 + ROWS - 1) / ROWS;
+    const int each = divide(stages + p.parts.d - 1, p.parts) * ROWS;
+    row0 = min(row0 + part * each, rows);
+    rows = min(row0 + each, rows);
+  }
   U32x4 qr[QL];
   float lse = 0.0f;
   int limit = 0;
   const auto load_rows = [&](int from) {
 #pragma unroll
     for (int l = 0; l < QL; ++l) {
-      const int i = l * kWeighThreads + threadIdx.x, row = from + i / NCH, d = i % NCH * 8;
+      const int i = l * kThreads + threadIdx.x, row = from + i / NCH, d = i % NCH * 8;
       qr[l] = U32x4{0, 0, 0, 0};
-      if (i < MR * NCH && row < rows && d < p.D) {
+      if (i < ROWS * NCH && row < rows && d < p.D) {
         const int qi = divide(row, p.G), head = h * p.G.d + row - qi * p.G.d;
         const T* const src =
             static_cast<const T*>(p.query) + (q_first + qi) * p.q_token + head * p.q_head + d;
@@ -207,7 +239,7 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_kernel(WeighParams p) {
         }
       }
     }
-    if (threadIdx.x < MR) {
+    if (threadIdx.x < ROWS) {
       const int row = from + threadIdx.x;
       limit = 0;
       lse = 0.0f;
@@ -222,12 +254,18 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_kernel(WeighParams p) {
   const auto store_rows = [&](int buf) {
 #pragma unroll
     for (int l = 0; l < QL; ++l) {
-      const int i = l * kWeighThreads + threadIdx.x;
-      if (i < MR * NCH) queries[buf][query_piece<DP>(i / NCH, i % NCH)] = qr[l];
+      const int i = l * kThreads + threadIdx.x;
+      if (i < ROWS * NCH) queries[buf][query_piece<DP>(i / NCH, i % NCH)] = qr[l];
     }
-    if (threadIdx.x < MR) {
-      lses[buf][threadIdx.x] = lse;
-      limits[buf][threadIdx.x] = limit;
+    if (wave == 0) {  // ROWS <= 64
+      int low = lane < ROWS ? limit : INT32_MAX;
+#pragma unroll
+      for (int x = 1; x < MR; x <<= 1) low = min(low, __shfl_xor(low, x));
+      if (lane < ROWS) {
+        lses[buf][lane] = lse * kLog2e;
+        limits[buf][lane] = limit;
+        if (c == 0) least[buf][lane / MR] = low;
+      }
     }
   };
 
@@ -240,47 +278,53 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_kernel(WeighParams p) {
     load_rows(row0);
     store_rows(0);
   }
-  for (int from = row0; from < rows; from += MR) {
+  for (int from = row0; from < rows; from += ROWS) {
     __syncthreads();
-    const bool more = from + MR < rows;
-    if (more) load_rows(from + MR);
-    // rows of the result that this lane has, four at a time
-    const auto mine = [&](int x) { return 4 * q4 + 256 / MR * (x / 4); };
-    Tile<MR> s[NT];
+    const bool more = from + ROWS < rows;
+    if (more) load_rows(from + ROWS);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int m = 0; m < SUB; ++m) {
+      // rows of the result that this lane has, four at a time
+      const auto mine = [&](int x) { return MR * m + 4 * q4 + 256 / MR * (x / 4); };
+      Tile<MR> s[NT];
 #pragma unroll
-      for (int x = 0; x < ACC; ++x) s[n][x] = 0.0f;
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const int piece = (k / NPE * NG + q4) * NPE + k % NPE;
-      const Vec8<T> qf = __builtin_bit_cast(Vec8<T>, queries[buf][query_piece<DP>(c, piece)]);
+        for (int x = 0; x < ACC; ++x) s[n][x] = 0.0f;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s[n] = mfma<T, MR>(qf, kf[n][k], s[n]);
-    }
+      for (int k = 0; k < KS; ++k) {
+        const int piece = (k / NPE * NG + q4) * NPE + k % NPE;
+        const Vec8<T> qf =
+            __builtin_bit_cast(Vec8<T>, queries[buf][query_piece<DP>(MR * m + c, piece)]);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int t = first_t + n * MR + c;
-      float e[ACC];
-#pragma unroll
-      for (int x = 0; x < ACC; x += 4) {
-        const Float4 below = *reinterpret_cast<const Float4*>(&lses[buf][mine(x)]);
-        const auto until = *reinterpret_cast<const int __attribute__((ext_vector_type(4)))*>(
-            &limits[buf][mine(x)]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float v = fmaf(s[n][x + j], p.scale, -below[j]);
-          const float w = __builtin_amdgcn_exp2f(v * kLog2e);
-          e[x + j] = t < until[j] ? w : 0.0f;
-        }
+        for (int n = 0; n < NT; ++n) s[n] = mfma<T, MR>(qf, kf[n][k], s[n]);
       }
+      const bool whole =
+          __builtin_amdgcn_readfirstlane(least[buf][m]) >= first_t + NT * MR;
 #pragma unroll
-      for (int step = 1; step < ACC; step *= 2)
+      for (int n = 0; n < NT; ++n) {
+        const int t = first_t + n * MR + c;
+        float e[ACC];
 #pragma unroll
-        for (int x = 0; x < ACC; x += 2 * step) e[x] += e[x + step];
-      const float add = e[0] - lost[n], next = sum[n] + add;
-      lost[n] = next < INFINITY ? (next - sum[n]) - add : 0.0f;
-      sum[n] = next;
+        for (int x = 0; x < ACC; x += 4) {
+          const Float4 below = *reinterpret_cast<const Float4*>(&lses[buf][mine(x)]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            e[x + j] = __builtin_amdgcn_exp2f(fmaf(s[n][x + j], p.scale, -below[j]));
+        }
+        if (!whole) {
+#pragma unroll
+          for (int x = 0; x < ACC; ++x)
+            e[x] = t < limits[buf][mine(x) + x % 4] ? e[x] : 0.0f;
+        }
+#pragma unroll
+        for (int step = 1; step < ACC; step *= 2)
+#pragma unroll
+          for (int x = 0; x < ACC; x += 2 * step) e[x] += e[x + step];
+        const float add = e[0] - lost[n], next = sum[n] + add;
+        lost[n] = next < INFINITY ? (next - sum[n]) - add : 0.0f;
+        sum[n] = next;
+      }
     }
     buf ^= 1;
     if (more) store_rows(buf);
@@ -292,25 +336,64 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_kernel(WeighParams p) {
 #pragma unroll
     for (int x = MR; x < 64; x <<= 1) v += __shfl_xor(v, x);
     const int t = first_t + n * MR + c;
-    if (q4 == 0 && t < p.places) {
-      const float old = weights ? weights[t] : 0.0f;
-      if (there[n])
-        out[t] = old + v;
-      else if (out != weights)
-        out[t] = old;
+    if (q4 != 0 || t >= p.places) continue;
+    if (p.parts.d > 1) {
+      sums[t] = there[n] ? v : 0.0f;
+      continue;
     }
+    const float old = weights ? weights[t] : 0.0f;
+    if (there[n])
+      out[t] = old + v;
+    else if (out != weights)
+      out[t] = old;
   }
+}
+
+// Adds the parts of each place, in their order.
+__global__ __launch_bounds__(256) void weigh_join_kernel(WeighParams p) {
+  const int row = static_cast<int>(blockIdx.y), r = divide(row, p.H), h = row - r * p.H.d;
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= p.places) return;
+  const float* const weights = p.weights ? p.weights + r * p.w_request + h * p.w_head : nullptr;
+  float* const out = p.out + r * p.o_request + h * p.o_head;
+  const int end = static_cast<int>(
+      min(max(p.lengths[r], int64_t(0)), static_cast<int64_t>(p.max_tokens)));
+  float sum = 0.0f;
+  if (t < end) {  // past it there may be no parts
+    const int64_t all = static_cast<int64_t>(p.requests.d) * p.H.d * p.places;
+    const float* const src = p.part_sums + static_cast<int64_t>(row) * p.places + t;
+#pragma unroll 4
+    for (int i = 0; i < p.parts.d; ++i) sum += src[i * all];
+  }
+  out[t] = (weights ? weights[t] : 0.0f) + sum;
+}
+
+// Parts of the rows: as many as give every CU a few workgroups, of four stages at least.
+int64_t weigh_parts(int64_t tokens, int64_t query_heads, int64_t heads, int64_t requests,
+                    int64_t places) {
+  const int64_t rows = tokens * (query_heads / heads);
+  if (requests == 0 || rows <= 16 * requests) return 1;
+  const int64_t units = requests * heads * std::max<int64_t>(ceil_div(places, 256), 1);
+  const int64_t most = std::min<int64_t>(rows / requests / 256, kMostWeighParts);
+  return std::max<int64_t>(std::min(ceil_div(kWeighUnits, units), most), 1);
 }
 
 template <typename T, Cell CELL, int DP, int MR, int NT>
 int launch_weigh(WeighParams p, int64_t requests, hipStream_t stream) {
-  const int64_t tiles = ceil_div(p.places, kWeighWaves * NT * MR);
-  p.tiles = divisor(ceil_div(tiles, 8));
-  const int64_t units = requests * p.H.d * p.tiles.d * 8;
-  ORIGAMI_REQUIRE(units < (int64_t(1) << 32) / kWeighThreads, "too many tokens for one call");
-  const dim3 grid(static_cast<unsigned>(units)), block(kWeighThreads);
+  constexpr int kTokens = kWeighWaves<MR> * NT * MR, kThreads = 64 * kWeighWaves<MR>;
+  int64_t tiles = ceil_div(p.places, kTokens);
+  if (MR == 16) tiles = ceil_div(tiles, 8);
+  p.tiles = divisor(tiles);
+  const int64_t units = requests * p.H.d * tiles * (MR == 16 ? 8 : p.parts.d);
+  ORIGAMI_REQUIRE(units < (int64_t(1) << 32) / kThreads, "too many tokens for one call");
+  const dim3 grid(static_cast<unsigned>(units)), block(kThreads);
   hipLaunchKernelGGL((weigh_kernel<T, CELL, DP, MR, NT>), grid, block, 0, stream, p);
-  return check_launch("weigh_kernel");
+  if (int rc = check_launch("weigh_kernel")) return rc;
+  if (p.parts.d == 1) return ORIGAMI_OK;
+  const dim3 joins(static_cast<unsigned>(ceil_div(p.places, 256)),
+                   static_cast<unsigned>(requests * p.H.d));
+  hipLaunchKernelGGL(weigh_join_kernel, joins, dim3(256), 0, stream, p);
+  return check_launch("weigh_join_kernel");
 }
 
 template <typename T, Cell CELL, int DP>
@@ -543,9 +626,33 @@ bool paged_dtype(int64_t dtype) {
 
 constexpr int64_t kMostTokens = int64_t(1) << 30;
 
+int check_weigh_sizes(int64_t tokens, int64_t query_heads, int64_t heads, int64_t requests,
+                      int64_t places) {
+  ORIGAMI_REQUIRE(heads > 0 && query_heads > 0 && query_heads % heads == 0,
+                  "query heads must be a multiple of the cache's heads");
+  ORIGAMI_REQUIRE(tokens >= 0 && requests >= 0 && places >= 0,
+                  "token counts must not be negative");
+  ORIGAMI_REQUIRE(places <= kMostTokens, "too many tokens for one call");
+  ORIGAMI_REQUIRE(tokens < (int64_t(1) << 24) / query_heads, "too many query rows for one call");
+  ORIGAMI_REQUIRE(requests < (int64_t(1) << 24) / heads, "too many requests for one call");
+  return ORIGAMI_OK;
+}
+
+int64_t weigh_workspace(int64_t parts, int64_t requests, int64_t heads, int64_t places) {
+  return parts > 1 ? parts * requests * heads * places * 4 : 0;
+}
+
 }  // namespace
 
 extern "C" {
+
+int64_t origami_accumulate_attention_weights_workspace(int64_t tokens, int64_t query_heads,
+                                                       int64_t heads, int64_t requests,
+                                                       int64_t places) {
+  if (check_weigh_sizes(tokens, query_heads, heads, requests, places)) return -1;
+  return weigh_workspace(weigh_parts(tokens, query_heads, heads, requests, places), requests,
+                         heads, places);
+}
 
 int origami_accumulate_attention_weights(
     const void* query, int64_t dtype, const int64_t* strides, int64_t tokens, int64_t query_heads,
@@ -554,7 +661,8 @@ int origami_accumulate_attention_weights(
     const int64_t* block_tables, int64_t table_stride, int64_t table_blocks,
     const int64_t* lengths, int64_t requests, const int64_t* query_starts, int64_t max_tokens,
     double scale, double k_scale, const float* weights, float* out, int64_t places,
-    const int64_t* weight_strides, origami_stream_t stream_) {
+    const int64_t* weight_strides, void* workspace, int64_t workspace_bytes,
+    origami_stream_t stream_) {
   WeighParams p{};
   int64_t half_stride;
   ORIGAMI_REQUIRE(dtype == ORIGAMI_DTYPE_FLOAT16 || dtype == ORIGAMI_DTYPE_BFLOAT16,
@@ -565,14 +673,8 @@ int origami_accumulate_attention_weights(
   if (int rc = check_cache(cache_layout, num_blocks, block_size, heads, head_dim, kv_cache,
                            &p.blk_stride, &half_stride))
     return rc;
-  ORIGAMI_REQUIRE(query_heads > 0 && query_heads % heads == 0,
-                  "query heads must be a multiple of the cache's heads");
-  ORIGAMI_REQUIRE(tokens >= 0 && requests >= 0 && max_tokens >= 0 && places >= 0 &&
-                      table_blocks >= 0,
-                  "token counts must not be negative");
-  ORIGAMI_REQUIRE(places <= kMostTokens, "too many tokens for one call");
-  ORIGAMI_REQUIRE(tokens < (int64_t(1) << 24) / query_heads, "too many query rows for one call");
-  ORIGAMI_REQUIRE(requests < (int64_t(1) << 24) / heads, "too many requests for one call");
+  ORIGAMI_REQUIRE(max_tokens >= 0 && table_blocks >= 0, "token counts must not be negative");
+  if (int rc = check_weigh_sizes(tokens, query_heads, heads, requests, places)) return rc;
   ORIGAMI_REQUIRE(max_tokens <= places, "max_tokens exceeds the weights' places");
   ORIGAMI_REQUIRE(ceil_div(max_tokens, block_size) <= table_blocks,
                   "max_tokens exceeds the block tables");
@@ -581,7 +683,7 @@ int origami_accumulate_attention_weights(
   ORIGAMI_REQUIRE(cache_scale(k_scale), "cache scales must be positive and finite in binary32");
   ORIGAMI_REQUIRE(cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN || k_scale == 1.0,
                   "cache scales are for float8_e4m3fn caches");
-  p.scale = static_cast<float>(scale * k_scale);
+  p.scale = static_cast<float>(scale * k_scale * 1.4426950408889634);
   ORIGAMI_REQUIRE(std::isfinite(p.scale), "scale must be finite in binary32");
   ORIGAMI_REQUIRE(strides[0] >= 0 && strides[1] >= 0, "row strides must not be negative");
   for (int i = 0; i < 4; ++i)
@@ -592,6 +694,15 @@ int origami_accumulate_attention_weights(
                       lengths != nullptr && (block_tables != nullptr || max_tokens == 0) &&
                       (kv_cache != nullptr || num_blocks == 0),
                   "queries, weights, lengths, tables and the cache must not be null");
+  const int64_t parts = weigh_parts(tokens, query_heads, heads, requests, places);
+  // the join has a workgroup row for every request and head
+  ORIGAMI_REQUIRE(parts == 1 || requests * heads <= 65535, "too many requests for one call");
+  ORIGAMI_REQUIRE(workspace_bytes >= weigh_workspace(parts, requests, heads, places) &&
+                      (parts == 1 || workspace != nullptr) && aligned16(workspace),
+                  "the workspace of the weights is too small");
+  p.parts = divisor(parts);
+  p.requests = divisor(requests);
+  p.part_sums = static_cast<float*>(workspace);
   p.query = query;
   p.q_token = strides[0];
   p.q_head = strides[1];

@@ -964,6 +964,11 @@ at::Tensor accumulate_attention_weights(
   const at::Tensor& in = weights ? *weights : out;
   const int64_t strides[2] = {query.stride(0), query.stride(1)};
   const int64_t weight_strides[4] = {in.stride(0), in.stride(1), out.stride(0), out.stride(1)};
+  const int64_t bytes = origami_accumulate_attention_weights_workspace(rows, Hq, g.heads, requests,
+                                                                       out.size(2));
+  TORCH_CHECK(bytes >= 0, origami_last_error());
+  at::Tensor work;
+  if (bytes > 0) work = at::empty({bytes}, query.options().dtype(at::kByte));
   check(origami_accumulate_attention_weights(
       query.data_ptr(), dtype, strides, rows, Hq, lse.numel() > 0 ? lse.data_ptr<float>() : nullptr,
       kv_cache.data_ptr(), cache_dtype_code(kv_cache), g.layout, g.num_blocks, g.block_size,
@@ -972,7 +977,7 @@ at::Tensor accumulate_attention_weights(
       scale ? *scale : 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(D, 1))), k_scale,
       weights && weights->numel() ? weights->data_ptr<float>() : nullptr,
       out.numel() ? out.data_ptr<float>() : nullptr, out.size(2), weight_strides,
-      current_stream(kv_cache)));
+      bytes > 0 ? work.data_ptr() : nullptr, bytes, current_stream(kv_cache)));
   return out;
 }
 

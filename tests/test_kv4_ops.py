@@ -106,7 +106,7 @@ def _weigh(**kw):
              cache_dtype=FP4, layout=0, num_blocks=4, block_size=16, heads=2, head_dim=64,
              tables=16, table_stride=2, table_blocks=2, lengths=16, requests=3, starts=None,
              max_tokens=32, scale=1.0, k_scale=1.0, weights=16, out=16, places=40,
-             weight_strides=[8] * 4, stream=None)
+             weight_strides=[8] * 4, workspace=16, workspace_bytes=1 << 40, stream=None)
     a.update(kw)
     strides, more = (_native.i64_array(a[n]) for n in ("strides", "weight_strides"))
     a["strides"], a["weight_strides"] = strides.ctypes.data, more.ctypes.data
@@ -136,6 +136,23 @@ def _weigh(**kw):
      "too many tokens for one call")])
 def test_weights_refuse(change, message):
     refused(_weigh, change, message)
+
+
+@pytest.mark.parametrize("change", [dict(workspace_bytes=8), dict(workspace=None),
+                                    dict(workspace=8)])
+def test_weights_refuse_workspaces(change):
+    prompt = dict(tokens=4096, requests=1, starts=16, places=4096)
+    refused(_weigh, dict(prompt, **change), "workspace of the weights is too small")
+
+
+def test_weights_workspace_sizes():
+    size = _native.lib().origami_accumulate_attention_weights_workspace
+    assert size(4096, 8, 2, 1, 4096) > 0 and size(4096, 8, 2, 1, 4096) % (2 * 4096 * 4) == 0
+    assert size(64, 32, 8, 64, 32768) == 0  # single tokens: one part
+    assert size(64, 8, 2, 0, 100) == 0
+    for sizes in ((-1, 4, 2, 1, 8), (1, 3, 2, 1, 8), (1, 4, 0, 1, 8), (1, 4, 2, BIG, 8),
+                  (BIG, 4, 2, 1, 8), (1, 4, 2, 1, BIG)):
+        assert size(*sizes) == -1
 
 
 def test_nothing_to_weigh():
