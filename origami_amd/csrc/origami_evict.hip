@@ -464,13 +464,45 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
   return b >> 31 ? ~b : b | 0x80000000u;
 }
 
+// The sum of x over a wave's first 16 lanes, of which the others have the same.
+__device__ __forceinline__ uint32_t sum16(uint32_t x) {
+  x += lane_moved<0xb1>(x);
+  x += lane_moved<0x4e>(x);
+  x += lane_moved<0x141>(x);
+  x += lane_moved<0x140>(x);
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+// x summed over this lane and those before it.
+__device__ __forceinline__ uint32_t sum_upto(uint32_t x, int lane) {
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) {
+    const uint32_t other = __shfl_up(x, i);
+    x += lane >= i ? other : 0;
+  }
+  return x;
+}
+
+__device__ __forceinline__ float weight_of(uint32_t rank) {
+  return __builtin_bit_cast(float, rank >> 31 ? rank ^ 0x80000000u : ~rank);
+}
+
 // One workgroup: the tokens that one head of one request keeps.  The rank of the last of them is
-// found by its digits, from the highest, from counts of the ranks that have the digits before it;
-// then waves list the tokens of a part of the places each.
+// found by its digits, from the highest, from counts of the ranks that have the digits before it
+// (four counts of each digit, for lanes in turn, since weights have few exponents); then the tokens
+// are listed in their order, KEYS times 1024 of them at a time.
+//
+// The workgroup has a CU to itself, and instructions bound it: a lane keeps the ranks of KEYS
+// places, which are read and made once, and the lists are counted with scalar instructions.  4
+// requests of 8 heads and 20000 to 32768 tokens take 32 us; with weights kept in place of ranks 39,
+// with weights read anew in each pass 50.  More than KEYS times 1024 tokens are read five times.
+template <int KEYS>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
-  __shared__ uint32_t bins[kBins];
-  __shared__ uint32_t wave_sum[kSelectWaves], wave_same[kSelectWaves];
+  constexpr int kCopies = 4, kStep = kSelectThreads, kRound = KEYS * kStep;
+  __shared__ alignas(16) uint32_t bins[kCopies * kBins];
+  __shared__ uint32_t wave_sum[kSelectWaves];
   __shared__ uint32_t found[2];
+  __shared__ uint32_t sure_count[KEYS * kSelectWaves], same_count[KEYS * kSelectWaves];
   const int r = divide(static_cast<int>(blockIdx.x), p.H);
   const int h = static_cast<int>(blockIdx.x) - r * p.H.d;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -480,6 +512,20 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
   float* const out_w = p.out_weights + r * p.o_request + h * p.o_head;
   int64_t* const kept = p.kept + static_cast<int64_t>(blockIdx.x) * p.keep;
 
+  // This lane's ranks from place `from` on: of places from + j kStep + tid, and 0, which no weight
+  // has, where there is no older token.
+  uint32_t rank[KEYS] = {};
+  const auto load_ranks = [&](int from) {
+    float x[KEYS];
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j)
+      x[j] = w[max(min(from + j * kStep + tid, s.older - 1), 0)];
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j)
+      rank[j] = from + j * kStep + tid < s.older ? rank_of(x[j]) : 0;
+  };
+  if (s.older > 0) load_ranks(0);
+
   // ranks above `cut` are kept, and the first `ties` of those equal to it
   uint32_t cut = 0, ties = 0;
   if (s.need == 0) {
@@ -487,25 +533,30 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
   } else if (s.need < s.older) {
     uint32_t left = s.need, known = 0;
     for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : (shift == 10 ? 0 : -1)) {
-      const int width = shift == 0 ? 10 : 11;
-      for (int i = tid; i < kBins; i += kSelectThreads) bins[i] = 0;
+      const uint32_t digit = shift == 0 ? 0x3ffu : 0x7ffu;
+      for (int i = tid; i < kCopies * kBins / 4; i += kSelectThreads)
+        reinterpret_cast<U32x4*>(bins)[i] = U32x4{0, 0, 0, 0};
       __syncthreads();
-      for (int i = tid; i < s.older; i += kSelectThreads) {
-        const uint32_t k = rank_of(w[i]);
-        if (((k ^ cut) & known) == 0) atomicAdd(&bins[(k >> shift) & ((1u << width) - 1)], 1u);
+      for (int from = 0; from < s.older; from += kRound) {
+        if (s.older > kRound) load_ranks(from);
+#pragma unroll
+        for (int j = 0; j < KEYS; ++j) {
+          if (rank[j] != 0 && ((rank[j] ^ cut) & known) == 0)
+            atomicAdd(&bins[kCopies * ((rank[j] >> shift) & digit) + lane % kCopies], 1u);
+        }
       }
       __syncthreads();
       // thread i has digits 2 i and 2 i + 1 from the highest down
-      const uint32_t high = bins[kBins - 1 - 2 * tid], low = bins[kBins - 2 - 2 * tid];
-      uint32_t upto = high + low;
-#pragma unroll
-      for (int x = 1; x < 64; x <<= 1) {
-        const uint32_t other = __shfl_up(upto, x);
-        upto += lane >= x ? other : 0;
-      }
+      const auto count = [&](int d) {
+        const U32x4 c = *reinterpret_cast<const U32x4*>(&bins[kCopies * d]);
+        return c[0] + c[1] + c[2] + c[3];
+      };
+      const uint32_t high = count(kBins - 1 - 2 * tid), low = count(kBins - 2 - 2 * tid);
+      uint32_t upto = sum_upto(high + low, lane);
       if (lane == 63) wave_sum[wave] = upto;
       __syncthreads();
-      for (int i = 0; i < wave; ++i) upto += wave_sum[i];
+      const int one = lane % kSelectWaves;
+      upto += sum16(one < wave ? wave_sum[one] : 0);
       const uint32_t above = upto - high - low;
       if (above < left && upto >= left) {
         const bool second = above + high < left;
@@ -515,51 +566,75 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
       __syncthreads();
       cut |= found[0] << shift;
       left -= found[1];
-      known |= ((1u << width) - 1) << shift;
+      known |= digit << shift;
     }
     ties = left;
-  } else {
-    ties = s.older;  // all
-  }
+  }  // else all
 
-  // each wave lists its part of the places, 64 at a time
-  const int part = (s.tokens + kSelectThreads - 1) / kSelectThreads * 64;
-  const int first = min(wave * part, s.tokens), last = min(first + part, s.tokens);
-  uint32_t sure = 0, same = 0;
-  for (int i = first; i < last; i += 64) {
-    const int t = i + lane;
-    const uint32_t k = t < s.older ? rank_of(w[t]) : 0;
-    sure += __popcll(__ballot(t < last && (t >= s.older || k > cut)));
-    same += __popcll(__ballot(t < last && t < s.older && k == cut));
-  }
-  __syncthreads();
-  if (lane == 0) {
-    wave_sum[wave] = sure;
-    wave_same[wave] = same;
-  }
-  __syncthreads();
-  uint32_t sure_before = 0, same_before = 0;
-  for (int i = 0; i < wave; ++i) {
-    sure_before += wave_sum[i];
-    same_before += wave_same[i];
-  }
-  for (int i = first; i < last; i += 64) {
-    const int t = i + lane;
-    const bool in = t < last;
-    const float weight = in ? w[t] : 0.0f;
-    const uint32_t k = t < s.older ? rank_of(weight) : 0;
-    const uint64_t lower = (1ull << lane) - 1;
-    const uint64_t sures = __ballot(in && (t >= s.older || k > cut));
-    const uint64_t sames = __ballot(in && t < s.older && k == cut);
-    const uint32_t same_rank = same_before + __popcll(sames & lower);
-    const bool mine = ((sures >> lane) & 1) || (((sames >> lane) & 1) && same_rank < ties);
-    if (mine) {
-      const uint32_t at = sure_before + __popcll(sures & lower) + min(same_rank, ties);
-      kept[at] = t;
-      out_w[at] = weight;
+  // The sure ones and those equal to the cut among 64 places each, as bits of the lanes.
+  const auto sures_of = [&](int j, int from) -> uint64_t {
+    const int at = from + j * kStep + wave * 64;  // the first of the places
+    const uint64_t above = __ballot(rank[j] > cut);
+    if (at + 64 <= s.older) return above;
+    return above | __ballot(at + lane >= s.older && at + lane < s.tokens);
+  };
+  const auto sames_of = [&](int j) { return ties ? __ballot(rank[j] == cut) : 0ull; };
+  uint32_t sure_base = 0, same_base = 0;
+  for (int from = 0; from < s.tokens; from += kRound) {
+    if (s.tokens > kRound && s.older > 0) load_ranks(from);
+    uint32_t sures_here = 0, sames_here = 0;  // lane j: of step j
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j) {
+      const uint32_t a = __popcll(sures_of(j, from)), b = __popcll(sames_of(j));
+      sures_here = lane == j ? a : sures_here;
+      sames_here = lane == j ? b : sames_here;
     }
-    sure_before += __popcll(sures);
-    same_before += __popcll(sames);
+    __syncthreads();
+    if (lane < KEYS) {
+      sure_count[lane * kSelectWaves + wave] = sures_here;
+      same_count[lane * kSelectWaves + wave] = sames_here;
+    }
+    __syncthreads();
+    if (wave < 2) {  // a wave for each kind: the sums before each count
+      uint32_t* const counts = wave == 0 ? sure_count : same_count;
+      constexpr int kEach = KEYS * kSelectWaves / 64;
+      uint32_t c[kEach], total = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        c[i] = counts[lane * kEach + i];
+        total += c[i];
+      }
+      const uint32_t upto = sum_upto(total, lane);
+      uint32_t before = upto - total;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        counts[lane * kEach + i] = before;
+        before += c[i];
+      }
+      if (lane == 63) found[wave] = upto;
+    }
+    __syncthreads();
+    if (lane < KEYS) {
+      sures_here = sure_count[lane * kSelectWaves + wave];
+      sames_here = same_count[lane * kSelectWaves + wave];
+    }
+#pragma unroll
+    for (int j = 0; j < KEYS; ++j) {
+      asm volatile("" : "+v"(rank[j]));  // bits are made anew: there are no registers for all
+      const uint64_t sures = sures_of(j, from), sames = sames_of(j);
+      if ((sures | sames) == 0) continue;
+      const uint32_t same_rank = same_base + __builtin_amdgcn_readlane(sames_here, j) +
+                                 __popcll(sames & ((1ull << lane) - 1));
+      if (((sures >> lane) & 1) || (((sames >> lane) & 1) && same_rank < ties)) {
+        const int t = from + j * kStep + tid;
+        const uint32_t at = sure_base + __builtin_amdgcn_readlane(sures_here, j) +
+                            __popcll(sures & ((1ull << lane) - 1)) + min(same_rank, ties);
+        kept[at] = t;
+        out_w[at] = t < s.older ? weight_of(rank[j]) : w[t];
+      }
+    }
+    sure_base += found[0];
+    same_base += found[1];
   }
   for (int i = s.kept + tid; i < p.keep; i += kSelectThreads) kept[i] = -1;
   for (int i = s.kept + tid; i < p.out_places; i += kSelectThreads) out_w[i] = 0.0f;
@@ -803,8 +878,11 @@ int origami_evict_kv_cache(
   p.pieces = divisor(row_bytes / load);
   p.row_tiles = divisor(tiles);
   const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-  hipLaunchKernelGGL(select_kernel, dim3(static_cast<unsigned>(requests * heads)),
-                     dim3(kSelectThreads), 0, stream, p);
+  const dim3 lists(static_cast<unsigned>(requests * heads)), threads(kSelectThreads);
+  if (max_tokens <= 4 * kSelectThreads)
+    hipLaunchKernelGGL(select_kernel<4>, lists, threads, 0, stream, p);
+  else
+    hipLaunchKernelGGL(select_kernel<32>, lists, threads, 0, stream, p);
   if (int rc = check_launch("select_kernel")) return rc;
   if (most == 0) return ORIGAMI_OK;
   const dim3 grid(static_cast<unsigned>(requests * tiles)), block(kMoveThreads);
