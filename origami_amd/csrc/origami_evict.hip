@@ -25,7 +25,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-constexpr int64_t kWeighUnits = 2048, kMostWeighParts = 32;
+constexpr int64_t kWeighUnits = 2048, kMostWeighParts = 32, kWeighWaves = 2048;
 
 // ---------------------------------------------------------------------------
 // Adding up the weights
@@ -42,7 +42,7 @@ struct WeighParams {
   const int64_t *tables, *lengths, *starts;
   int64_t table_stride;
   Divisor block_size, requests, H, G;
-  Divisor tiles;  // of a request's places, in eights where the rows are few
+  Divisor tiles;  // ranges of a request's places, where the rows are few
   Divisor parts;  // of the rows that see a tile, each of which a workgroup adds up
   int32_t tokens, Hq, D, max_tokens, places;
   float scale;  // includes log2 e and the keys' scale
@@ -52,12 +52,6 @@ struct WeighParams {
   float* part_sums;  // [parts][requests][H][places], where there are several
 };
 
-// Workgroups of eight waves with 32 tokens each, and stages of 64 rows, where there are many rows;
-// else of four waves with 64 tokens each (32 past 128 channels).
-template <int MR>
-constexpr int kWeighWaves = MR == 32 ? 8 : 4;
-template <int MR>
-constexpr int kStageTiles = MR == 32 ? 2 : 1;
 
 template <int MR>
 using Tile = float __attribute__((ext_vector_type(MR * MR / 64)));
@@ -91,17 +85,16 @@ struct __attribute__((aligned(4))) Dwords {
   uint32_t w[DWORDS];
 };
 
-// One workgroup: NT MR tokens of one KV head of one request a wave, against the query rows that see
-// any of them or a part of those rows, MR rows at a time.  The keys stay in registers, as the
+// One workgroup: 32 tokens of one KV head of one request for each of eight waves, against the query
+// rows that see any of them or a part of those rows, in stages of 64.  The keys stay in registers, as the
 // second operand, so that a token's scores are in the lanes of one column and are added up where
 // they are; the queries go through LDS, a stage ahead.
 //
 // The order of the channels in the products is free as long as keys and queries have the same: a
 // lane's 16 bytes of a key are 8, 16 or 32 channels in a row, whole loads of the cache's row.
-template <typename T, Cell CELL, int DP, int MR, int NT>
-__global__ __launch_bounds__(64 * kWeighWaves<MR>, MR == 32 && DP <= 128 ? 2 : 1)
-    void weigh_kernel(WeighParams p) {
-  constexpr int NW = kWeighWaves<MR>, kThreads = 64 * NW, SUB = kStageTiles<MR>, ROWS = SUB * MR;
+template <typename T, Cell CELL, int DP>
+__global__ __launch_bounds__(512, DP <= 128 ? 2 : 1) void weigh_kernel(WeighParams p) {
+  constexpr int MR = 32, NT = 1, NW = 8, kThreads = 64 * NW, SUB = 2, ROWS = SUB * MR;
   constexpr int NG = 64 / MR, KS = DP / (8 * NG), NCH = DP / 8, ACC = MR * MR / 64;
   constexpr int kWhole = CELL == kFp4 ? 4 : (CELL == kFp8 ? 2 : 1);
   constexpr int NPE = kWhole < KS ? kWhole : KS;  // pieces of 8 channels in a load
@@ -115,25 +108,23 @@ __global__ __launch_bounds__(64 * kWeighWaves<MR>, MR == 32 && DP <= 128 ? 2 : 1
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c = lane % MR, q4 = lane / MR;
 
-  int r, h, tile, part = 0;
-  if constexpr (MR == 16) {
-    // the heads of the same tokens are 8 workgroups apart, on one chiplet: their rows share lines
-    int u = divide(static_cast<int>(blockIdx.x >> 3), p.H);
-    h = static_cast<int>(blockIdx.x >> 3) - u * p.H.d;
-    r = divide(u, p.tiles);
-    tile = (u - r * p.tiles.d) * 8 + static_cast<int>(blockIdx.x & 7);
-  } else {
-    // the first tokens, which most rows see, first; the same part of the rows on the same chiplet
-    int u = divide(static_cast<int>(blockIdx.x), p.parts);
-    part = static_cast<int>(blockIdx.x) - u * p.parts.d;
-    int v = divide(u, p.H);
-    h = u - v * p.H.d;
-    tile = divide(v, p.requests);
-    r = v - tile * p.requests.d;
-  }
+  // the first tokens, which most rows see, first; the same part of the rows on the same chiplet
+  int u = divide(static_cast<int>(blockIdx.x), p.parts);
+  const int part = static_cast<int>(blockIdx.x) - u * p.parts.d;
+  const int v = divide(u, p.H), h = u - v * p.H.d;
+  const int tile = divide(v, p.requests), r = v - tile * p.requests.d;
   const int t0 = tile * kTokens;
   if (t0 >= p.places) return;
 
+  // The blocks and the sums so far are asked for before the length is known: up to the bounds that
+  // the host has they can be read.
+  const int first_t = t0 + wave * NT * MR;  // of this wave
+  const int64_t* const table = p.tables + r * p.table_stride;
+  int64_t ids[NT] = {};
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+    if (p.max_tokens > 0)
+      ids[n] = table[divide(min(first_t + n * MR + c, p.max_tokens - 1), p.block_size)];
   const int length =
       static_cast<int>(min(max(p.lengths[r], int64_t(0)), int64_t(3) << 29));
   const int end = min(length, p.max_tokens);
@@ -142,7 +133,6 @@ __global__ __launch_bounds__(64 * kWeighWaves<MR>, MR == 32 && DP <= 128 ? 2 : 1
   float* const out = p.out + r * p.o_request + h * p.o_head;
   float* const sums =
       p.part_sums + ((static_cast<int64_t>(part) * p.requests.d + r) * p.H.d + h) * p.places;
-  const int first_t = t0 + wave * NT * MR;  // of this wave
   if (t0 >= end) {
     // of several parts the join takes care of these
     if (p.parts.d > 1) return;
@@ -165,13 +155,14 @@ __global__ __launch_bounds__(64 * kWeighWaves<MR>, MR == 32 && DP <= 128 ? 2 : 1
   const int bytes = row_bytes_of(CELL, p.D);
   Vec8<T> kf[NT][KS];
   bool there[NT];
-  const int64_t* const table = p.tables + r * p.table_stride;
+  float old[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int t = first_t + n * MR + c;
-    const int block = divide(min(t, end - 1), p.block_size);
-    const int64_t id = table[block];
+    const int block = divide(t, p.block_size);
+    const int64_t id = ids[n];
     there[n] = t < end && id >= 0 && id < p.num_blocks;
+    old[n] = weights && p.parts.d == 1 && t < p.places ? weights[t] : 0.0f;
     const int64_t at = there[n] ? id * p.blk_stride + (t - block * p.block_size.d) : 0;
     const uint8_t* const row = p.cache + (at * p.H.d + h) * bytes;
 #pragma unroll
@@ -341,11 +332,10 @@ __global__ __launch_bounds__(64 * kWeighWaves<MR>, MR == 32 && DP <= 128 ? 2 : 1
       sums[t] = there[n] ? v : 0.0f;
       continue;
     }
-    const float old = weights ? weights[t] : 0.0f;
     if (there[n])
-      out[t] = old + v;
+      out[t] = old[n] + v;
     else if (out != weights)
-      out[t] = old;
+      out[t] = old[n];
   }
 }
 
@@ -378,30 +368,239 @@ int64_t weigh_parts(int64_t tokens, int64_t query_heads, int64_t heads, int64_t 
   return std::max<int64_t>(std::min(ceil_div(kWeighUnits, units), most), 1);
 }
 
-template <typename T, Cell CELL, int DP, int MR, int NT>
-int launch_weigh(WeighParams p, int64_t requests, hipStream_t stream) {
-  constexpr int kTokens = kWeighWaves<MR> * NT * MR, kThreads = 64 * kWeighWaves<MR>;
-  int64_t tiles = ceil_div(p.places, kTokens);
-  if (MR == 16) tiles = ceil_div(tiles, 8);
-  p.tiles = divisor(tiles);
-  const int64_t units = requests * p.H.d * tiles * (MR == 16 ? 8 : p.parts.d);
-  ORIGAMI_REQUIRE(units < (int64_t(1) << 32) / kThreads, "too many tokens for one call");
-  const dim3 grid(static_cast<unsigned>(units)), block(kThreads);
-  hipLaunchKernelGGL((weigh_kernel<T, CELL, DP, MR, NT>), grid, block, 0, stream, p);
+// Zeros, for what a lane reads of rows that are not in the cache and of channels past the last.
+__device__ const U32x4 kZeroRow[33] = {};
+
+// One wave: a range of the tokens of one KV head of one request against its query rows, 16 at a
+// time, for requests of few rows, as in a decode step.  The queries stay in registers; the keys come
+// 64 tokens at a step (32 past 128 channels) and a step ahead, and their blocks two steps, so that a
+// wave waits for memory as seldom as can be (workgroups that ended after 256 tokens took 46 us
+// for 16 requests of 2048 to 8192 tokens, and as long in e4m3 and in 4 bits).  Waves next to each
+// other are heads of the same tokens, and ranges of a request follow each other over the
+// chiplets, as in the attention.
+template <typename T, Cell CELL, int DP, bool WHOLE>
+__global__ __launch_bounds__(256, 2) void weigh_few_kernel(WeighParams p, Divisor beside,
+                                                           int chunk) {
+  constexpr int MR = 16, NG = 4, NT = DP == 256 ? 2 : 4, KS = DP / (8 * NG), STEP = NT * MR;
+  constexpr int kWhole = CELL == kFp4 ? 4 : (CELL == kFp8 ? 2 : 1);
+  constexpr int NPE = kWhole < KS ? kWhole : KS;  // pieces of 8 channels in a load
+  constexpr int kPiece = CELL == kFp4 ? 4 : (CELL == kFp8 ? 8 : 16);
+  constexpr int LJ = KS / NPE, DW = NPE * kPiece / 4;  // loads of a key, and their dwords
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int c = lane % MR, q4 = lane / MR;
+  const int eight = static_cast<int>(blockIdx.x >> 3), some = divide(eight, beside);
+  const int unit = ((some * 8 + static_cast<int>(blockIdx.x & 7)) * beside.d + eight -
+                    some * beside.d) * 4 + wave;
+  const int u = divide(unit, p.H), h = unit - u * p.H.d;
+  const int r = divide(u, p.tiles);
+  if (r >= p.requests.d) return;
+  const int turned = u - r * p.tiles.d + r;
+  const int t0 = (turned - divide(turned, p.tiles) * p.tiles.d) * chunk;
+
+  const int64_t* const table = p.tables + r * p.table_stride;
+  const int tl = lane % STEP;
+  const auto block_of = [&](int t) -> int64_t {  // up to max_tokens the tables can be read
+    return t < p.max_tokens ? table[divide(t, p.block_size)] : -1;
+  };
+  const int64_t id = block_of(t0 + tl);
+  int64_t ahead = block_of(t0 + STEP + tl);
+  const int length =
+      static_cast<int>(min(max(p.lengths[r], int64_t(0)), int64_t(3) << 29));
+  const int end = min(length, p.max_tokens);
+  const float* const weights =
+      p.weights ? p.weights + r * p.w_request + h * p.w_head : nullptr;
+  float* const out = p.out + r * p.o_request + h * p.o_head;
+  // places past the tokens are copied, if they are elsewhere
+  const int t1 = min(t0 + chunk, out == weights ? end : p.places);
+  if (t0 >= t1) return;
+  int q_first = r, q_count = 1;
+  if (p.starts) {
+    const int64_t n = p.tokens;
+    const int64_t a = min(max(p.starts[r], int64_t(0)), n);
+    q_first = static_cast<int>(a);
+    q_count = static_cast<int>(min(max(p.starts[r + 1], a), n) - a);
+  }
+  const int before = length - q_count, rows = q_count * p.G.d;
+
+  const int bytes = row_bytes_of(CELL, p.D);
+  const uint32_t pitch = static_cast<uint32_t>(p.H.d) * bytes;
+  const uint8_t* const head_rows = p.cache + static_cast<int64_t>(h) * bytes;
+  const uint8_t* const zeros = reinterpret_cast<const uint8_t*>(kZeroRow);
+  const auto row_of = [&](int t, int64_t id) -> int {  // of the cache, -1 where t has none
+    if (t >= end || id < 0 || id >= p.num_blocks) return -1;
+    return static_cast<int>(id * p.blk_stride + t - divide(t, p.block_size) * p.block_size.d);
+  };
+  struct Step {
+    Dwords<DW> raw[NT][LJ];
+    uint32_t scale[NT][LJ];
+    float old;   // the sum so far of token number `lane` of the step
+    bool there;  // whether it is in the cache
+  };
+  const auto load_step = [&](Step& s, int mine, int t, const float* sums) {
+    s.there = mine >= 0;
+    s.old = sums && t + tl < t1 ? sums[t + tl] : 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int at = __shfl(mine, MR * n + c);
+      const uint8_t* const row =
+          head_rows + static_cast<uint64_t>(static_cast<uint32_t>(at)) * pitch;
+#pragma unroll
+      for (int j = 0; j < LJ; ++j) {
+        const int ch = (j * NG + q4) * NPE * 8;
+        const bool in = at >= 0 && ch < p.D;
+        if constexpr (WHOLE) {
+          s.raw[n][j] =
+              *reinterpret_cast<const Dwords<DW>*>(in ? row + ch / 8 * kPiece : zeros);
+        } else {
+#pragma unroll
+          for (int i = 0; i < NPE; ++i) {
+            const auto piece = *reinterpret_cast<const Dwords<kPiece / 4>*>(
+                in && ch + 8 * i < p.D ? row + (ch / 8 + i) * kPiece : zeros);
+#pragma unroll
+            for (int x = 0; x < kPiece / 4; ++x) s.raw[n][j].w[i * kPiece / 4 + x] = piece.w[x];
+          }
+        }
+        if constexpr (CELL == kFp4) s.scale[n][j] = *(in ? row + p.D / 2 + ch / 32 : zeros);
+      }
+    }
+  };
+
+  // With no query row the sums stay what they are; with more than 16 the later rows are added to
+  // what the first ones left in `out`.
+  int from = 0;
+  do {
+    Vec8<T> qf[KS];
+    {
+      const int row = from + c, qi = divide(row, p.G), head = h * p.G.d + row - qi * p.G.d;
+      const T* const src =
+          static_cast<const T*>(p.query) + (q_first + qi) * p.q_token + head * p.q_head;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int d = ((k / NPE * NG + q4) * NPE + k % NPE) * 8;
+        qf[k] = Vec8<T>{};
+        if (row < rows && d < p.D) {
+          if (p.q_vec) {
+            qf[k] = *reinterpret_cast<const Vec8<T>*>(src + d);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) qf[k][j] = src[d + j];
+          }
+        }
+      }
+    }
+    float below[4];  // of rows 4 q4 .. 4 q4 + 3, which are this lane's in the result
+    int limit[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int row = from + 4 * q4 + x, qi = divide(row, p.G);
+      below[x] = 0.0f;
+      limit[x] = 0;
+      if (row < rows) {
+        const float lse =
+            p.lse[static_cast<int64_t>(q_first + qi) * p.Hq + h * p.G.d + row - qi * p.G.d];
+        below[x] = lse * kLog2e;
+        // a row that saw nothing gives no weight
+        limit[x] = lse == -INFINITY ? 0 : before + qi + 1;
+      }
+    }
+    const float* const sums = from == 0 ? weights : out;
+    const auto compute = [&](const Step& s, int t) {
+      float v[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        Tile<MR> score = {};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const int j = k / NPE, i = k % NPE;
+          U32x4 wide;
+          if constexpr (CELL == kFp4)
+            wide = fp4_expand<T>(s.raw[n][j].w[i], fp4_scale(s.scale[n][j]));
+          else if constexpr (CELL == kFp8)
+            wide = fp8_expand<T>(U32x2{s.raw[n][j].w[2 * i], s.raw[n][j].w[2 * i + 1]});
+          else
+            wide = U32x4{s.raw[n][j].w[0], s.raw[n][j].w[1], s.raw[n][j].w[2], s.raw[n][j].w[3]};
+          score = mfma<T, MR>(qf[k], __builtin_bit_cast(Vec8<T>, wide), score);
+        }
+        const int at = t + MR * n + c;
+        float e[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          e[x] = __builtin_amdgcn_exp2f(fmaf(score[x], p.scale, -below[x]));
+          e[x] = at < limit[x] ? e[x] : 0.0f;
+        }
+        v[n] = (e[0] + e[1]) + (e[2] + e[3]);
+        v[n] += __shfl_xor(v[n], 16);
+        v[n] += __shfl_xor(v[n], 32);
+      }
+      float mine = v[0];  // of token number `lane`, which is in tile lane / 16
+#pragma unroll
+      for (int n = 1; n < NT; ++n) mine = q4 % NT == n ? v[n] : mine;
+      if (lane < STEP && t + tl < t1) {
+        if (s.there)
+          out[t + tl] = s.old + mine;
+        else if (out != sums)
+          out[t + tl] = s.old;
+      }
+    };
+
+    Step even, other;
+    int64_t next_id = from == 0 ? id : block_of(t0 + tl);
+    if (from > 0) ahead = block_of(t0 + STEP + tl);
+    load_step(even, row_of(t0 + tl, next_id), t0, sums);
+    __builtin_amdgcn_sched_barrier(0);
+    for (int t = t0; t < t1; t += 2 * STEP) {
+      int mine = row_of(t + STEP + tl, ahead);
+      ahead = block_of(t + 2 * STEP + tl);
+      load_step(other, mine, t + STEP, sums);
+      compute(even, t);
+      if (t + STEP >= t1) break;
+      mine = row_of(t + 2 * STEP + tl, ahead);
+      ahead = block_of(t + 3 * STEP + tl);
+      load_step(even, mine, t + 2 * STEP, sums);
+      compute(other, t + STEP);
+    }
+    from += MR;
+  } while (from < rows);
+}
+
+template <typename T, Cell CELL, int DP>
+int launch_weigh_few(WeighParams p, int64_t requests, hipStream_t stream) {
+  // ranges of 64 tokens and more, for about 2048 waves
+  const int64_t most = std::max<int64_t>(ceil_div(p.places, 64), 1);
+  const int64_t wanted = std::min(std::max<int64_t>(kWeighWaves / (requests * p.H.d), 1), most);
+  const int64_t chunk = ceil_div(ceil_div(p.places, wanted), 64) * 64;
+  p.tiles = divisor(ceil_div(p.places, chunk));
+  const int64_t units = requests * p.H.d * p.tiles.d;
+  const Divisor beside = divisor(std::max(p.H.d / 4, 1));
+  const int64_t workgroups = ceil_div(ceil_div(units, 4), 8 * beside.d) * 8 * beside.d;
+  ORIGAMI_REQUIRE(workgroups < (int64_t(1) << 32) / 256, "too many tokens for one call");
+  const dim3 grid(static_cast<unsigned>(workgroups)), block(256);
+  constexpr int kLoad = CELL == kFp4 ? 32 : (CELL == kFp8 ? 16 : 8);
+  constexpr int kChannels = kLoad < DP / 4 ? kLoad : DP / 4;  // of a load
+  if (p.D % kChannels == 0)
+    hipLaunchKernelGGL((weigh_few_kernel<T, CELL, DP, true>), grid, block, 0, stream, p, beside,
+                       static_cast<int>(chunk));
+  else if constexpr (kChannels > 8)
+    hipLaunchKernelGGL((weigh_few_kernel<T, CELL, DP, false>), grid, block, 0, stream, p, beside,
+                       static_cast<int>(chunk));
+  return check_launch("weigh_few_kernel");
+}
+
+template <typename T, Cell CELL, int DP>
+int launch_weigh(const WeighParams& p, int64_t requests, hipStream_t stream) {
+  // rows of 16 where the requests have no more on average
+  if (static_cast<int64_t>(p.tokens) * p.G.d <= 16 * requests)
+    return launch_weigh_few<T, CELL, DP>(p, requests, stream);
+  const int64_t units = requests * p.H.d * ceil_div(p.places, 256) * p.parts.d;
+  ORIGAMI_REQUIRE(units < (int64_t(1) << 32) / 512, "too many tokens for one call");
+  const dim3 grid(static_cast<unsigned>(units)), block(512);
+  hipLaunchKernelGGL((weigh_kernel<T, CELL, DP>), grid, block, 0, stream, p);
   if (int rc = check_launch("weigh_kernel")) return rc;
   if (p.parts.d == 1) return ORIGAMI_OK;
   const dim3 joins(static_cast<unsigned>(ceil_div(p.places, 256)),
                    static_cast<unsigned>(requests * p.H.d));
   hipLaunchKernelGGL(weigh_join_kernel, joins, dim3(256), 0, stream, p);
   return check_launch("weigh_join_kernel");
-}
-
-template <typename T, Cell CELL, int DP>
-int launch_weigh(const WeighParams& p, int64_t requests, hipStream_t stream) {
-  // tiles of 16 rows where the requests have no more, as in a decode step
-  if (static_cast<int64_t>(p.tokens) * p.G.d <= 16 * requests)
-    return launch_weigh<T, CELL, DP, 16, DP == 256 ? 2 : 4>(p, requests, stream);
-  return launch_weigh<T, CELL, DP, 32, 1>(p, requests, stream);
 }
 
 template <typename T, Cell CELL>
@@ -683,6 +882,8 @@ int check_cache(int64_t cache_layout, int64_t num_blocks, int64_t block_size, in
                 int64_t head_dim, const void* kv_cache, int64_t* blk_stride,
                 int64_t* half_stride) {
   ORIGAMI_REQUIRE(heads > 0, "heads must be positive");
+  // a token's bytes, 512 a head at most, are counted in 31 bits
+  ORIGAMI_REQUIRE(heads <= INT32_MAX / 512, "too many heads for one call");
   ORIGAMI_REQUIRE(head_dim > 0 && head_dim % 8 == 0 && head_dim <= 256,
                   "head_dim must be a multiple of 8, at most 256");
   ORIGAMI_REQUIRE(num_blocks >= 0 && block_size > 0, "cache block size must be positive");

@@ -901,11 +901,13 @@ void require_weights(const at::Tensor& t, const char* name, const at::Tensor& ca
   TORCH_CHECK(t.stride(2) == 1 || t.size(2) <= 1, name, " places must be contiguous");
 }
 
-// The most tokens of a request: what is given, or what the block tables hold.
-int64_t most_tokens(c10::optional<int64_t> given, int64_t blocks, int64_t block_size) {
+// The most tokens of a request: what is given, or what the block tables and the weights hold.
+int64_t most_tokens(c10::optional<int64_t> given, int64_t blocks, int64_t block_size,
+                    const c10::optional<at::Tensor>& weights) {
   int64_t most;
   if (given) return *given;
-  return __builtin_mul_overflow(blocks, block_size, &most) ? INT64_MAX : most;
+  if (__builtin_mul_overflow(blocks, block_size, &most)) most = INT64_MAX;
+  return weights ? std::min(most, weights->size(2)) : most;
 }
 
 // Sums of attention weights with those of the query rows added; `out` or a new tensor.
@@ -934,8 +936,8 @@ at::Tensor accumulate_attention_weights(
   TORCH_CHECK(lse.device() == kv_cache.device() && lse.scalar_type() == at::kFloat &&
                   lse.dim() == 2 && lse.size(0) == rows && lse.size(1) == Hq,
               "lse must be float32 [tokens, query heads] on the kv_cache device");
-  const int64_t most = most_tokens(max_tokens, blocks, g.block_size);
   if (weights) require_weights(*weights, "weights", kv_cache, requests, g.heads);
+  const int64_t most = most_tokens(max_tokens, blocks, g.block_size, weights);
   const c10::OptionalDeviceGuard guard(kv_cache.device());
 
   at::Tensor out;
@@ -1002,7 +1004,7 @@ std::tuple<at::Tensor, at::Tensor> evict_kv_cache(at::Tensor kv_cache, at::Tenso
   require_tables(out_tables, "out_tables", kv_cache);
   TORCH_CHECK(out_tables.size(0) == requests, "out_tables must have a row for every request");
   TORCH_CHECK(keep >= 0 && keep <= (int64_t(1) << 30), "keep must not be negative or too many");
-  const int64_t most = most_tokens(max_tokens, blocks, g.block_size);
+  const int64_t most = most_tokens(max_tokens, blocks, g.block_size, weights);
   const c10::OptionalDeviceGuard guard(kv_cache.device());
   const Extent cache_extent = extent_of(kv_cache);
   Extent extent;  // of a new tensor: none

@@ -857,8 +857,8 @@ def accumulate_attention_weights(query: torch.Tensor, kv_cache: torch.Tensor,
     (float32 [rows, query_heads]) is what it returned with return_lse for these rows over all of
     the request's tokens.  weights (default: zeros) and the result are float32 [requests, heads,
     places]; place t is the request's token t.  `out` may be `weights` itself; without weights and
-    out the result has max_tokens places (default: the block table's slots).  Tokens past max_tokens
-    and in blocks outside the cache get nothing.  Lengths and tables are read on the device, so a
+    out the result has max_tokens places (default: the block table's slots, or as many as weights has
+    places).  Tokens past max_tokens and in blocks outside the cache get nothing.  Lengths and tables are read on the device, so a
     call can be captured in a graph.  Each sum is float32, in a fixed order.  Overlaps are refused
     but of out with weights.  For inference only, as shared_prefix_attention."""
     return _ext.ext().accumulate_attention_weights(
@@ -877,7 +877,7 @@ def evict_kv_cache(kv_cache: torch.Tensor, block_tables: torch.Tensor, tokens: t
     larger than infinity).
 
     Request r has tokens[r] tokens in blocks block_tables[r], of which the first max_tokens count
-    (default: the block table's slots).  What it keeps, min(tokens[r], keep) rows a head, is copied
+    (default: the block table's slots, or as many as weights has places).  What it keeps, min(tokens[r], keep) rows a head, is copied
     in its order to blocks out_tables[r] of the same cache, keys and values bit by bit whatever the
     cache's type, and is the request from then on: with out_tables as its block table and
     tokens.clamp(max=keep) tokens.  Blocks that are read stay as they are, so a prefix may be shared

@@ -122,6 +122,7 @@ def _weigh(**kw):
     (dict(tokens=-1), "must not be negative"), (dict(places=-1), "must not be negative"),
     (dict(places=BIG), "too many tokens"), (dict(tokens=1 << 22, starts=16), "too many query rows"),
     (dict(requests=BIG, starts=16), "too many requests"),
+    (dict(heads=1 << 22, query_heads=1 << 22), "too many heads"),
     (dict(max_tokens=41), "exceeds the weights' places"),
     (dict(max_tokens=33), "exceeds the block tables"), (dict(tokens=4), "one query token"),
     (dict(k_scale=0.5), "for float8_e4m3fn"), (dict(cache_dtype=FP8, k_scale=0.0), "be positive"),
@@ -181,7 +182,8 @@ def _evict(**kw):
     (dict(recent=-1), "must not be negative"), (dict(out_places=-5), "must not be negative"),
     (dict(max_tokens=BIG, places=BIG), "too many tokens"),
     (dict(keep=BIG, out_places=BIG), "too many tokens"),
-    (dict(requests=BIG), "too many requests"), (dict(heads=BIG), "too many requests"),
+    (dict(requests=BIG), "too many requests"), (dict(heads=BIG), "too many heads"),
+    (dict(heads=1 << 22), "too many heads"), (dict(heads=1 << 21, requests=2), "too many requests"),
     (dict(max_tokens=41), "exceeds the weights' places"),
     (dict(max_tokens=33), "exceeds the block tables"),
     (dict(out_places=9), "places of out_weights"), (dict(keep=17), "new block tables"),
