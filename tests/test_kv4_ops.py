@@ -133,7 +133,7 @@ def _weigh(**kw):
     (dict(lse=None), "must not be null"), (dict(out=None), "must not be null"),
     (dict(lengths=None), "must not be null"), (dict(tables=None), "must not be null"),
     (dict(kv_cache=None), "must not be null"),
-    (dict(places=1 << 30, requests=1 << 20, starts=16, heads=1, query_heads=1),
+    (dict(places=1 << 30, requests=1 << 10, starts=16, tokens=1 << 20),
      "too many tokens for one call")])
 def test_weights_refuse(change, message):
     refused(_weigh, change, message)
