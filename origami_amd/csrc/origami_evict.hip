@@ -45,7 +45,7 @@ struct WeighParams {
   Divisor tiles;  // ranges of a request's places, where the rows are few
   Divisor parts;  // of the rows that see a tile, each of which a workgroup adds up
   int32_t tokens, Hq, D, max_tokens, places;
-  float scale;  // includes log2 e and the keys' scale
+  float scale;  // includes the keys' scale
   const float* weights;  // null: zeros
   float* out;
   int64_t w_request, w_head, o_request, o_head;  // strides, in elements
@@ -253,7 +253,7 @@ __global__ __launch_bounds__(512, DP <= 128 ? 2 : 1) void weigh_kernel(WeighPara
 #pragma unroll
       for (int x = 1; x < MR; x <<= 1) low = min(low, __shfl_xor(low, x));
       if (lane < ROWS) {
-        lses[buf][lane] = lse * kLog2e;
+        lses[buf][lane] = lse;
         limits[buf][lane] = limit;
         if (c == 0) least[buf][lane / MR] = low;
       }
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(512, DP <= 128 ? 2 : 1) void weigh_kernel(WeighPara
           const Float4 below = *reinterpret_cast<const Float4*>(&lses[buf][mine(x)]);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            e[x + j] = __builtin_amdgcn_exp2f(fmaf(s[n][x + j], p.scale, -below[j]));
+            e[x + j] = __builtin_amdgcn_exp2f(kLog2e * fmaf(s[n][x + j], p.scale, -below[j]));
         }
         if (!whole) {
 #pragma unroll
@@ -498,7 +498,7 @@ __global__ __launch_bounds__(256, 2) void weigh_few_kernel(WeighParams p, Diviso
       if (row < rows) {
         const float lse =
             p.lse[static_cast<int64_t>(q_first + qi) * p.Hq + h * p.G.d + row - qi * p.G.d];
-        below[x] = lse * kLog2e;
+        below[x] = lse;
         // a row that saw nothing gives no weight
         limit[x] = lse == -INFINITY ? 0 : before + qi + 1;
       }
@@ -525,7 +525,7 @@ __global__ __launch_bounds__(256, 2) void weigh_few_kernel(WeighParams p, Diviso
         float e[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          e[x] = __builtin_amdgcn_exp2f(fmaf(score[x], p.scale, -below[x]));
+          e[x] = __builtin_amdgcn_exp2f(kLog2e * fmaf(score[x], p.scale, -below[x]));
           e[x] = at < limit[x] ? e[x] : 0.0f;
         }
         v[n] = (e[0] + e[1]) + (e[2] + e[3]);
@@ -959,7 +959,7 @@ int origami_accumulate_attention_weights(
   ORIGAMI_REQUIRE(cache_scale(k_scale), "cache scales must be positive and finite in binary32");
   ORIGAMI_REQUIRE(cache_dtype == ORIGAMI_DTYPE_FLOAT8_E4M3FN || k_scale == 1.0,
                   "cache scales are for float8_e4m3fn caches");
-  p.scale = static_cast<float>(scale * k_scale * 1.4426950408889634);
+  p.scale = static_cast<float>(scale * k_scale);
   ORIGAMI_REQUIRE(std::isfinite(p.scale), "scale must be finite in binary32");
   ORIGAMI_REQUIRE(strides[0] >= 0 && strides[1] >= 0, "row strides must not be negative");
   for (int i = 0; i < 4; ++i)
