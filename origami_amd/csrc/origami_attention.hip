@@ -91,6 +91,8 @@ struct AttendParams {
   int32_t tokens, Hq, D;
   float scale, v_scale;  // scale includes log2 e and the keys' scale
   Group group[2];        // the prefix with the whole batch's rows; each request's rows
+  Divisor shares, full_shares;  // see share_of: of a head (0 without); one a request less
+  int32_t least_share;   // steps of a share, at least
   int32_t slots;
   float *part_o, *part_ml;  // [slots][rows][D], [slots][rows][2]
 };
@@ -866,13 +868,13 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
           Float4{o[d][x], o[d][x + 1], o[d][x + 2], o[d][x + 3]}, base, sum);
 }
 
-// The rows of one KV head (16 at most) over a range of tokens in 4 bits, 32 at a step: of one wave,
-// or with JOIN of the waves of a workgroup, which take steps in turn and join their parts in LDS.
+// The rows of one KV head (16 at most) of a request (or of the batch, over the prefix) over the
+// tokens from t0 to `stop` in 4 bits, 32 at a step: of one wave, or with JOIN of the waves of a
+// workgroup, which take steps in turn and join their parts in LDS.
 //
 // A decode step's few rows leave time for little else than the bytes, so nothing waits here for
-// another wave until the end.  Where there are units enough, waves by themselves have the longest
-// ranges and no join; waves next to each other are then heads of the same tokens, whose rows of 68
-// bytes (of 128 channels) share lines.  With few units the parts of eight waves are one.
+// another wave until the end.  Where there is work enough, waves by themselves have the longest
+// ranges and no join (attend_alone); with little of it the parts of eight waves are one.
 // Four lanes next to each other load a row, a quarter each: that is one access to the cache for a
 // row, where rows over lanes (as the products take them) are one for each lane.  Two steps are on
 // their way while one is computed.  The keys' quarters change lanes through LDS as they are, and
@@ -880,8 +882,9 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
 // have the same order of channels); the values are widened on their way to LDS, which transposes
 // them for V P.
 template <typename T, int DP, bool WHOLE, bool JOIN>
-__device__ __forceinline__ void attend_four(const AttendParams& p, const Group& g, int unit,
-                                            bool batch, int wave, uint8_t* wave_lds, float* ml) {
+__device__ __forceinline__ void attend_four(const AttendParams& p, const Group& g, bool batch, int r,
+                                            const Request& rq, int h, int split, int t0, int stop,
+                                            int wave, uint8_t* wave_lds, float* ml) {
   constexpr int kStride = JOIN ? 32 * kFourWaves<DP, JOIN> : 32;  // tokens between a wave's steps
   uint8_t* const lds = wave_lds + wave * kFourLds<DP, JOIN>;
   constexpr int MR = 16, NG = 4, TT = 32, KS = DP / 32, DT = DP / MR, NCH = DP / 8, W = KS;
@@ -889,10 +892,6 @@ __device__ __forceinline__ void attend_four(const AttendParams& p, const Group& 
   static_assert(8 * kRawPitch <= kFourLds<DP, JOIN> && TT * DP * 2 <= kFourLds<DP, JOIN>, "LDS");
   using Codes = uint32_t __attribute__((ext_vector_type(W)));
   const int lane = threadIdx.x & 63, c = lane % MR, q4 = lane / MR;
-  const int uh = divide(unit, p.H), h = unit - uh * p.H.d;
-  int r, split;
-  if (!range_of(p, g, batch, uh, &r, &split)) return;
-  const int t0 = g.first + split * g.chunk;
   const int64_t* const table = p.tables + static_cast<int64_t>(r) * p.table_stride;
   const int bound = batch ? p.prefix : p.prefix + p.max_own;
   const auto block_of = [&](int t, int before) -> int64_t {
@@ -905,7 +904,6 @@ __device__ __forceinline__ void attend_four(const AttendParams& p, const Group& 
   const int64_t id = block_of(first + tl, bound), id1 = block_of(first + kStride + tl, bound);
   int64_t ahead = block_of(first + 2 * kStride + tl, bound);
 
-  const Request rq = batch ? Request{0, p.tokens, 0, 0} : request_of(p, r);
   const int rows = rq.count * p.G.d;
   if (rows == 0) return;
   const int end = batch ? p.prefix : p.prefix + rq.own;
@@ -938,7 +936,7 @@ __device__ __forceinline__ void attend_four(const AttendParams& p, const Group& 
     }
   }
   const int most = seen_by(rows - 1), nearest = seen_by(0);  // tokens that some, all rows see
-  const int t1 = min(min(end, most), t0 + g.chunk);
+  const int t1 = min(min(end, most), stop);
 
   // what this lane loads; past the last channel it is some others, whose queries are zero
   const int tok = lane >> 2, slot_ch = (lane & 3) * (DP / NG), ch = slot_ch < p.D ? slot_ch : 0;
@@ -1132,22 +1130,130 @@ __device__ __forceinline__ void attend_four(const AttendParams& p, const Group& 
   }
 }
 
-// `beside` workgroups that follow each other in the units' order are 8 apart: on one chiplet.
+// The sum of x over this lane and those before it, without a trip through LDS.
+__device__ __forceinline__ int sum_upto(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // from the lane before in 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);  // 2, 4 and 8 before
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the last of the 16 before
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // and of the 32 before
+  return x;
+}
+
+constexpr int kShared = 256;  // requests whose shares a wave finds: their steps stay in registers
+
+// Share `share` of those that one KV head's steps of 32 tokens are cut into: part `part` of `parts`
+// of request `r`, of `each` steps; false if there are fewer shares.  A request has as many parts as
+// leave none more than some number of steps, the least at which there are no more shares than
+// waves.  Every wave finds that from the lengths (about 1 us), so that all have about the same work
+// and every CU as many waves: with as many ranges for every request, lengths of 1000 to 16384 took
+// 105 us for 89.  A share that went on with the next request would start anew there, for 5 us.
+__device__ __forceinline__ bool share_of(const AttendParams& p, int share, int* r, int* part,
+                                         int* parts, int* each) {
+  constexpr int kKept = kShared / 64;
+  const int lane = threadIdx.x & 63;
+  const auto sum = [](int x) { return __builtin_amdgcn_readlane(sum_upto(x), 63); };
+  int steps[kKept], all = 0;
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) {
+    steps[i] = 0;
+    if (64 * i + lane < p.requests.d) {
+      const Request q = request_of(p, 64 * i + lane);
+      steps[i] = q.count == 0 ? 0 : max((p.prefix + q.own + 31) / 32, 1);
+    }
+    all += steps[i];
+  }
+  all = sum(all);
+  // a size that is large enough, since no request has more than one share that is not full
+  int size = max(divide(all + p.shares.d - p.requests.d - 1, p.full_shares), p.least_share);
+  int low = max(divide(all + p.shares.d - 1, p.shares), p.least_share);
+  while (low < size) {
+    const int mid = (low + size) / 2;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) count += (steps[i] + mid - 1) / mid;
+    if (sum(count) <= p.shares.d)
+      size = mid;
+    else
+      low = mid + 1;
+  }
+  int before = 0;
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) {
+    const int mine = (steps[i] + size - 1) / size;
+    const int upto = before + sum_upto(mine);
+    if (const uint64_t past = __ballot(upto > share)) {
+      const int at = __builtin_ctzll(past);
+      *r = 64 * i + at;
+      *parts = __builtin_amdgcn_readlane(mine, at);
+      *part = share - (__builtin_amdgcn_readlane(upto, at) - *parts);
+      *each = (__builtin_amdgcn_readlane(steps[i], at) + *parts - 1) / *parts;
+      return true;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// One wave by itself: a share of one KV head's steps, or where there are too many requests for that
+// a range of those that all of them have.
+template <typename T, int DP, bool WHOLE>
+__device__ __forceinline__ void attend_alone(const AttendParams& p, int unit, int wave,
+                                             uint8_t* wave_lds) {
+  const Group& g = p.group[1];
+  const int at = divide(unit, p.H), h = unit - at * p.H.d;
+  int r, part, parts = g.splits.d, each = g.chunk / 32;
+  if (p.shares.d ? !share_of(p, at, &r, &part, &parts, &each)
+                 : !range_of(p, g, false, at, &r, &part))
+    return;
+  const Request q = request_of(p, r);
+  const int t0 = 32 * part * each;
+  attend_four<T, DP, WHOLE, false>(p, g, false, r, q, h, part, t0, t0 + 32 * each, wave, wave_lds,
+                                   nullptr);
+  if (part != parts - 1) return;
+  // the last part says that there are no more
+  const int rows = q.count * p.G.d, none = (p.slots - parts) * rows;
+  for (int i = threadIdx.x & 63; i < none; i += 64) {
+    const int slot = i / rows, row = i - slot * rows, qi = divide(row, p.G);
+    const int64_t at_row =
+        static_cast<int64_t>(q.first + qi) * p.Hq + h * p.G.d + row - qi * p.G.d;
+    float* const ml =
+        p.part_ml + 2 * ((parts + slot) * (static_cast<int64_t>(p.tokens) * p.Hq) + at_row);
+    ml[0] = -INFINITY;
+    ml[1] = 0.0f;
+  }
+}
+
+// `beside` workgroups that follow each other in the units' order are 8 apart: on one chiplet, for
+// heads of the same tokens, whose rows of 68 bytes (of 128 channels) share lines.
 template <typename T, int DP, bool WHOLE, bool JOIN>
-__global__ __launch_bounds__((64 * kFourWaves<DP, JOIN>), JOIN || DP == 256 ? 1 : (WHOLE ? 3 : 2))
+__global__ __launch_bounds__((64 * kFourWaves<DP, JOIN>), JOIN || DP == 256 ? 1 : 2)
     void attend_four_kernel(AttendParams p, Divisor beside) {
   constexpr int NW = kFourWaves<DP, JOIN>;
   __shared__ alignas(16) uint8_t lds[NW * kFourLds<DP, JOIN>];
-  __shared__ float ml[JOIN ? NW * 32 : 1];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int eight = static_cast<int>(blockIdx.x >> 3);
   const int some = divide(eight, beside);
   int unit = (some * 8 + static_cast<int>(blockIdx.x & 7)) * beside.d + eight - some * beside.d;
-  if constexpr (!JOIN) unit = unit * NW + wave;
-  const int kind = unit >= p.group[0].units;
-  unit -= kind ? p.group[0].units : 0;
-  if (unit >= p.group[kind].units) return;
-  attend_four<T, DP, WHOLE, JOIN>(p, p.group[kind], unit, kind == 0, wave, lds, ml);
+  if constexpr (JOIN) {
+    __shared__ float ml[NW * 32];
+    const int kind = unit >= p.group[0].units;
+    unit -= kind ? p.group[0].units : 0;
+    const Group& g = p.group[kind];
+    if (unit >= g.units) return;
+    const int uh = divide(unit, p.H), h = unit - uh * p.H.d;
+    int r, split;
+    if (!range_of(p, g, kind == 0, uh, &r, &split)) return;
+    const int t0 = g.first + split * g.chunk;
+    const Request rq = kind == 0 ? Request{0, p.tokens, 0, 0} : request_of(p, r);
+    attend_four<T, DP, WHOLE, true>(p, g, kind == 0, r, rq, h, split, t0, t0 + g.chunk, wave, lds,
+                                    ml);
+  } else {
+    unit = unit * NW + wave;
+    if (unit >= p.group[1].units) return;
+    attend_alone<T, DP, WHOLE>(p, unit, wave, lds);
+  }
 }
 
 template <typename T, Cell CELL, int DP, int SHAPE>
@@ -1322,8 +1428,9 @@ int launch_units(const AttendParams& p, hipStream_t stream) {
   return launch_shapes<T, CELL, DP, 0, 0>(p, stream);
 }
 
-// How plan_of has attention computed: by attend, or by attend_four with or without a join.
-enum Way { kTiles, kFourJoined, kFourWavesAlone };
+// How plan_of has attention computed: by attend, or by attend_four in workgroups that join, or by
+// attend_alone in ranges that all requests have or in shares.
+enum Way { kTiles, kFourJoined, kFourRanges, kFourShares };
 
 template <typename T, int DP, bool WHOLE, bool JOIN>
 int launch_four(const AttendParams& p, hipStream_t stream) {
@@ -1388,6 +1495,7 @@ struct Plan {
   Group group[2];
   int64_t slots, units;
   Way way;
+  int64_t shares, least_share;  // see share_of
 };
 
 // Units of one kind, before they are split: `count` of them, `live` with rows if the requests are
@@ -1410,12 +1518,14 @@ struct Kind {
 // any of the three is half or twice as large: the split needs to be near only.
 constexpr double kUnitTime = 6.0, kCuBytes = 20e3, kCuFlops = 3.2e6;
 
-// Caches in 4 bits with few rows.  Waves by themselves pay where there are enough of them with 256
-// tokens, and ranges of 256 to 1024 tokens that make about 2048 waves: 1 request of 32000 tokens
-// and 8 heads takes 24 us and, with joins in workgroups, 24; 8 of 4000 take 18 and 24, 64 of 2000 42
-// and 63 (49 with 3072 waves), 32 of 1000 to 16384 105 and 145.  Below, workgroups that join eight
-// waves, and a single part where it is short: 1 request of 1029 tokens takes 10.2 us, with two
-// parts 11.8, in waves by themselves 14.4; of 8000 tokens 15.0 and 14.6 to 16.3.
+// Caches in 4 bits with few rows.  Waves by themselves, about 2048 of them, pay where the requests
+// have 512 times 256 tokens and heads: 8 requests of 4000 tokens and 8 heads take 18 us and, with
+// joins in workgroups, 24; 64 of 2000 take 43 and 63, and 49 in 1536 waves; 32 of 1000 to 16384 take
+// 89 and 145.  Below, workgroups join eight waves, and a single part is best where it is short: 1
+// request of 1029 tokens takes 10.2 us, with two parts 11.8, in waves by themselves 14.4; of 8000
+// tokens 15.0 and 14.6 to 16.3.  Past 256 requests their ranges are the same for all, since to find
+// shares takes longer with each request and many requests fill the CUs evenly by their number (200 of
+// 10 to 3000 tokens: 120 us in shares, 117 in ranges).
 constexpr int64_t kFourMany = 512, kFourWavesWanted = 2048;
 
 // Microseconds of a call whose kinds are split in s0 and s1 ranges: workgroups of the first kind go
@@ -1486,22 +1596,36 @@ Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_di
   Plan plan{};
   plan.way = kTiles;
   if (cell == kFp4 && k1.shape == 0 && (!apart || k0.shape == 0)) {
-    plan.way = (k0.count + k1.count) * ceil_div(std::max(k0.span, k1.span), 256) >= kFourMany
-                   ? kFourWavesAlone
-                   : kFourJoined;
+    const int64_t steps = std::max<int64_t>(ceil_div(k1.span, 32), 1);
     const auto ranges = [&](const Kind& k) {
-      if (plan.way == kFourJoined) return k.splits(k.span <= 1536 ? 1 : ceil_div(k.span, 512));
-      return k.splits(std::min(std::max(kFourWavesWanted / k.count, ceil_div(k.span, 1024)),
-                               ceil_div(k.span, 256)));
+      return k.splits(k.span <= 1536 ? 1 : ceil_div(k.span, 512));
     };
     best0 = apart ? ranges(k0) : 1;
     best1 = ranges(k1);
+    plan.way = kFourJoined;
+    if (!apart && k1.count * ceil_div(k1.span, 256) >= kFourMany) {
+      if (requests > kShared || requests * steps > INT32_MAX / 2) {
+        plan.way = kFourRanges;
+        best1 = k1.splits(std::min(
+            std::max(kFourWavesWanted / k1.count, ceil_div(k1.span, 1024)), ceil_div(k1.span, 256)));
+      } else {
+        plan.way = kFourShares;
+        // waves for the CUs once, or as often as the requests are half of them
+        const int64_t once = std::max<int64_t>(kFourWavesWanted / heads, 1);
+        plan.shares = std::max<int64_t>(ceil_div(2 * requests, once), 1) * once;
+        // a request's parts take memory: 32 of them, and more if there are few requests
+        const int64_t parts = std::min<int64_t>(
+            std::max<int64_t>(32, 2 * kFourWavesWanted / k1.count), kMaxParts / 2);
+        plan.least_share = std::max<int64_t>(8, ceil_div(steps, parts));
+        best1 = ceil_div(steps, plan.least_share);
+      }
+    }
   }
   const auto put = [&](Group& g, const Kind& k, int64_t splits, int64_t first) {
     const int64_t spread = cell == kFp4 ? heads : 1;  // see attend: units of the same tokens
-    const int64_t units = plan.way != kTiles
-                              ? k.count * splits
-                              : ceil_div(k.count / k.tiles / spread * splits, 8) * 8 * spread * k.tiles;
+    int64_t units = ceil_div(k.count / k.tiles / spread * splits, 8) * 8 * spread * k.tiles;
+    if (plan.way == kFourJoined || plan.way == kFourRanges) units = k.count * splits;
+    if (plan.way == kFourShares) units = plan.shares * heads;
     plan.units += units;
     g.units = static_cast<int32_t>(std::min<int64_t>(units, INT32_MAX));
     g.shape = k.shape;
@@ -1651,6 +1775,11 @@ int origami_shared_prefix_attention(
   p.group[0] = plan.group[0];
   p.group[1] = plan.group[1];
   p.slots = static_cast<int32_t>(plan.slots);
+  if (plan.shares > 0) {
+    p.shares = divisor(plan.shares);
+    p.full_shares = divisor(plan.shares - requests);
+  }
+  p.least_share = static_cast<int32_t>(plan.least_share);
   const int64_t parts = plan.slots * tokens * query_heads;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + parts * head_dim;

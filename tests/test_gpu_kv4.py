@@ -384,6 +384,115 @@ def test_attend_on_another_stream(cuda_device):
     assert torch.equal(got, want)
 
 
+# ---- attention over many tokens, whose requests are cut into shares by their lengths ----
+
+
+def lengths_of(requests, most, seed):
+    """Lengths with zeros, ones, and one far longer than the others."""
+    gen = torch.Generator().manual_seed(seed)
+    own = torch.randint(0, most // 8, (requests,), generator=gen)
+    own[torch.rand(requests, generator=gen) < 0.2] = 0
+    own[torch.rand(requests, generator=gen) < 0.1] = 1
+    own[requests // 2] = most
+    return tuple(own.tolist())
+
+
+# on both sides of 64 and 256 requests, of one and of several heads a workgroup
+@pytest.mark.parametrize("requests,heads,most", [
+    (1, 8, 17000), (2, 8, 9000), (5, 3, 9000), (63, 1, 3000), (64, 8, 1500), (65, 2, 2050),
+    (150, 5, 1031), (256, 1, 700), (257, 1, 700), (300, 4, 333)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_shares_of_any_lengths(cuda_device, requests, heads, most, D):
+    b = Batch4(cuda_device, heads=heads, group=2, D=D, prefix=0,
+               own=lengths_of(requests, most, requests), seed=requests)
+    got, lse = b.run()
+    b.check(got, lse)
+    if requests * heads > 4:  # every run is the same, sum for sum
+        again, again_lse = b.run()
+        assert torch.equal(got, again) and torch.equal(lse, again_lse)
+
+
+@pytest.mark.parametrize("own", [(0,) * 70, (1,) * 70, (0,) * 69 + (2500,), (2500,) + (0,) * 130])
+def test_attend_shares_of_empty_requests(cuda_device, own):
+    """The bound is of 2500 tokens for each, whatever they hold."""
+    b = Batch4(cuda_device, heads=8, group=3, prefix=0, own=own, seed=len(own))
+    if max(own) < 2500:
+        b.tables = torch.cat([b.tables, b.tables[:, :1].expand(-1, 160)], 1).contiguous()
+    got, lse = b.run()
+    b.check(got, lse)
+    empty = b.own == 0
+    assert (got[empty] == 0).all() and (lse[empty] == -math.inf).all()
+
+
+@pytest.mark.parametrize("D", [24, 80, 120, 200])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_attend_shares_of_odd_head_sizes(cuda_device, D, dtype):
+    b = Batch4(cuda_device, heads=4, group=5, D=D, dtype=dtype, prefix=0, bs=24,
+               own=(3000, 0, 77, 1999) * 5, seed=D)
+    b.check(*b.run())
+
+
+@pytest.mark.parametrize("queries", [(1, 0, 3, 2) * 20, (0,) * 79 + (1,), (2,) * 80])
+def test_attend_shares_of_several_queries(cuda_device, queries):
+    own = [n + q if n + q > 1 else q for n, q in zip(lengths_of(80, 1700, 7), queries)]
+    b = Batch4(cuda_device, heads=2, group=4, prefix=0, own=own, queries=queries, seed=80)
+    b.check(*b.run())
+
+
+def test_attend_shares_of_a_prefix(cuda_device):
+    """One request reads the prefix with its own tokens, in the same shares."""
+    for own, queries in (((900,), (3,)), ((0,), None), ((5,), (5,))):
+        b = Batch4(cuda_device, heads=8, group=4, prefix=17001, own=own, queries=queries, seed=9)
+        b.check(*b.run())
+
+
+@pytest.mark.parametrize("requests", [12, 90, 270])
+def test_attend_shares_captured_as_lengths_grow(cuda_device, requests):
+    """A bound far above the lengths, of which the graph knows nothing."""
+    b = Batch4(cuda_device, heads=4, group=2, prefix=0, own=lengths_of(requests, 2600, 3), seed=3)
+    grown = b.own.clone()
+    b.own.fill_(1)
+    b.run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = b.run()
+    for part in (0.0, 0.05, 0.5, 1.0, 0.0):
+        b.own.copy_((grown * part).long())
+        graph.replay()
+        b.check(out, lse)
+        eager, eager_lse = b.run()
+        assert torch.equal(out, eager) and torch.equal(lse, eager_lse)
+
+
+def test_attend_shares_of_lengths_past_the_bound(cuda_device):
+    """Lengths that the bound cuts off, up to the largest of their type, are no more than it."""
+    b = Batch4(cuda_device, heads=8, group=2, prefix=0, own=(2000,) * 40, seed=5)
+    whole, whole_lse = b.run(max_own_tokens=1600)
+    b.own[:] = 1600
+    want, want_lse = b.run(max_own_tokens=1600)
+    assert torch.equal(whole, want) and torch.equal(whole_lse, want_lse)
+    b.check(want, want_lse)
+    b.own[3], b.own[4], b.own[5] = 1 << 62, -7, torch.iinfo(torch.int64).min
+    got, lse = b.run(max_own_tokens=1600)
+    assert (got[4:6] == 0).all() and (lse[4:6] == -math.inf).all()
+    b.own[3], b.own[4], b.own[5] = 1600, 0, 0
+    b.check(got, lse)
+
+
+def test_attend_shares_nan_in_one_request(cuda_device):
+    b = Batch4(cuda_device, heads=4, group=2, prefix=0, own=(1500, 2500, 0, 900) * 10, seed=6)
+    whole, whole_lse = b.run()
+    for r, t in ((1, 0), (1, 2499), (36, 1499), (39, 33)):
+        b.cache[0, int(b.tables[r, t // b.bs]), t % b.bs, 2, b.D // 2] = 255
+    got, lse = b.run()
+    hit = torch.zeros(got.shape[:2], dtype=torch.bool, device=cuda_device)
+    for r in (1, 36, 39):
+        hit[r, 4:6] = True
+    assert got[hit].isnan().all() and lse[hit].isnan().all()
+    assert torch.equal(got[~hit], whole[~hit]) and torch.equal(lse[~hit], whole_lse[~hit])
+
+
 def test_refusals(cuda_device):
     b = Batch4(cuda_device, prefix=0, own=(40, 3), D=128)
     whole = b.cache
