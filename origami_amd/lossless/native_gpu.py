@@ -765,11 +765,11 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tens
     key / k_scale and value / v_scale, limited to +-448.  A uint8 kv_cache holds 4 bits a channel
     (kv4_row_bytes): each 32 channels are rounded to e2m1 values times the least power of two, of
     2 ** -23 to 2 ** 13, at which none is further than half a step from what is held; larger
-    values become +-49152, infinities too, and a NaN makes its 32 channels NaN.  Returns the queries: query_out
-    (which may be `query` itself, but must share no element with anything else) or a new tensor;
-    None without `query`.  No input may lie in the cache.  Overlaps are refused.  For inference
-    only: inputs that require a gradient or carry a tangent are refused, and so are traced and
-    transformed calls."""
+    values become +-49152, infinities too, and a NaN makes its 32 channels NaN.  Returns the
+    queries: query_out (which may be `query` itself, but must share no element with anything else)
+    or a new tensor; None without `query`.  No input may lie in the cache.  Overlaps are refused.
+    For inference only: inputs that require a gradient or carry a tangent are refused, and so are
+    traced and transformed calls."""
     return _ext.ext().append_kv_cache(key, value, kv_cache, slots, query, positions, cos_sin,
                                       interleaved, query_norm, key_norm, eps, k_scale, v_scale,
                                       query_out)
@@ -809,8 +809,8 @@ def shared_prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor,
 
     query is float16 or bfloat16 [tokens, query_heads, head_dim]; kv_cache has its dtype or
     is float8_e4m3fn with k_scale / v_scale or uint8 with rows in 4 bits (kv4_row_bytes); query
-    head h uses cache head h // (query_heads // heads).  Request r has own_tokens[r] tokens of its own in blocks
-    block_tables[r] (int64, rows contiguous), those of its queries included.  Without
+    head h uses cache head h // (query_heads // heads).  Request r has own_tokens[r] tokens of its
+    own in blocks block_tables[r] (int64, rows contiguous), those of its queries included.  Without
     query_starts, row r of query is request r's newest token; with it (int64
     [requests + 1]) rows query_starts[r] .. query_starts[r + 1] - 1 are request r's newest
     tokens.  A row sees the whole prefix and its request's own tokens up to itself; it
@@ -857,10 +857,11 @@ def accumulate_attention_weights(query: torch.Tensor, kv_cache: torch.Tensor,
     (float32 [rows, query_heads]) is what it returned with return_lse for these rows over all of
     the request's tokens.  weights (default: zeros) and the result are float32 [requests, heads,
     places]; place t is the request's token t.  `out` may be `weights` itself; without weights and
-    out the result has max_tokens places (default: the block table's slots, or as many as weights has
-    places).  Tokens past max_tokens and in blocks outside the cache get nothing.  Lengths and tables are read on the device, so a
-    call can be captured in a graph.  Each sum is float32, in a fixed order.  Overlaps are refused
-    but of out with weights.  For inference only, as shared_prefix_attention."""
+    out the result has max_tokens places (default: the block table's slots, or as many as weights
+    has places).  Tokens past max_tokens and in blocks outside the cache get nothing.  Lengths and
+    tables are read on the device, so a call can be captured in a graph.  Each sum is float32, in a
+    fixed order.  Overlaps are refused but of out with weights.  For inference only, as
+    shared_prefix_attention."""
     return _ext.ext().accumulate_attention_weights(
         query, kv_cache, block_tables, tokens, lse, weights, query_starts, max_tokens, scale,
         k_scale, out)
@@ -877,10 +878,10 @@ def evict_kv_cache(kv_cache: torch.Tensor, block_tables: torch.Tensor, tokens: t
     larger than infinity).
 
     Request r has tokens[r] tokens in blocks block_tables[r], of which the first max_tokens count
-    (default: the block table's slots, or as many as weights has places).  What it keeps, min(tokens[r], keep) rows a head, is copied
-    in its order to blocks out_tables[r] of the same cache, keys and values bit by bit whatever the
-    cache's type, and is the request from then on: with out_tables as its block table and
-    tokens.clamp(max=keep) tokens.  Blocks that are read stay as they are, so a prefix may be shared
+    (default: the block table's slots, or as many as weights has places).  What it keeps,
+    min(tokens[r], keep) rows a head, is copied in its order to blocks out_tables[r] of the same
+    cache, keys and values bit by bit whatever the cache's type, and is the request from then on:
+    with out_tables as its block table and tokens.clamp(max=keep) tokens.  Blocks that are read stay as they are, so a prefix may be shared
     with other requests; blocks that are written must be in no table that is read, and in
     out_tables once.  A row of a block outside the cache is copied as zeros, and to one outside it
     not at all.  Since rows are copied, it pays to let a cache grow by some tens of tokens between
