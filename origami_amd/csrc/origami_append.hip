@@ -23,7 +23,7 @@
 // 50 and 68.  128 threads take 42 and 52 and leave half of a workgroup idle where a layer has few
 // heads; 256 take 45; a token's workgroups in a row 43; loads of weights and angles ahead of the
 // row's sum 42.  One token takes 2.9 us, which is a launch.  Into a cache in 4 bits the 8192 tokens
-// take 37 us: 27 MB less is written, and the rounding takes what that saves.
+// take 37 us: 25 MB less is written, and the rounding takes what that saves.
 #include <cmath>
 
 #include "origami_element.h"

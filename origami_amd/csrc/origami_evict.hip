@@ -686,6 +686,12 @@ __device__ __forceinline__ uint32_t sum_upto(uint32_t x, int lane) {
   return x;
 }
 
+// How many of the bits are of lanes before this one.
+__device__ __forceinline__ uint32_t before_lane(uint64_t bits) {
+  return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(bits >> 32),
+                                   __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(bits), 0));
+}
+
 __device__ __forceinline__ float weight_of(uint32_t rank) {
   return __builtin_bit_cast(float, rank >> 31 ? rank ^ 0x80000000u : ~rank);
 }
@@ -696,9 +702,11 @@ __device__ __forceinline__ float weight_of(uint32_t rank) {
 // are listed in their order, KEYS times 1024 of them at a time.
 //
 // The workgroup has a CU to itself, and instructions bound it: a lane keeps the ranks of KEYS
-// places, which are read and made once, and the lists are counted with scalar instructions.  4
-// requests of 8 heads and 20000 to 32768 tokens take 32 us; with weights kept in place of ranks 39,
-// with weights read anew in each pass 50.  More than KEYS times 1024 tokens are read five times.
+// places, which are read and made once, steps without tokens are left out, and the lists are counted
+// with scalar instructions.  4 requests of 8 heads and 20000 to 32768 tokens take 27 us, 8000 to 8192
+// tokens 13, with the 32 places that long lists need 17; with every step taken 31 and 22.  With
+// weights kept in place of ranks 20000 to 32768 took 39, with weights read anew in each pass 50.
+// More than KEYS times 1024 tokens are read five times.
 template <int KEYS>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
   constexpr int kCopies = 4, kStep = kSelectThreads, kRound = KEYS * kStep;
@@ -715,14 +723,24 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
   float* const out_w = p.out_weights + r * p.o_request + h * p.o_head;
   int64_t* const kept = p.kept + static_cast<int64_t>(blockIdx.x) * p.keep;
 
+  // This wave's steps of the places from..end, counted anew for each loop: else the compiler keeps
+  // all their conditions.
+  const auto steps_of = [&](int from, int end) __attribute__((always_inline)) -> int {
+    int n = __builtin_amdgcn_readfirstlane((end - from - wave * 64 + kStep - 1) / kStep);
+    asm volatile("" : "+s"(n));
+    return n;
+  };
+
   // This lane's ranks from place `from` on: of places from + j kStep + tid, and 0, which no weight
   // has, where there is no older token.
   uint32_t rank[KEYS] = {};
-  const auto load_ranks = [&](int from) {
-    float x[KEYS];
+  const auto load_ranks = [&](int from) __attribute__((always_inline)) {
+    float x[KEYS] = {};
+    const int steps = steps_of(from, s.older);
 #pragma unroll
-    for (int j = 0; j < KEYS; ++j)
-      x[j] = w[max(min(from + j * kStep + tid, s.older - 1), 0)];
+    for (int j = 0; j < KEYS; ++j) {
+      if (j < steps) x[j] = w[min(from + j * kStep + tid, s.older - 1)];
+    }
 #pragma unroll
     for (int j = 0; j < KEYS; ++j)
       rank[j] = from + j * kStep + tid < s.older ? rank_of(x[j]) : 0;
@@ -734,18 +752,22 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
   if (s.need == 0) {
     cut = 0xffffffffu;
   } else if (s.need < s.older) {
-    uint32_t left = s.need, known = 0;
-    for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : (shift == 10 ? 0 : -1)) {
-      const uint32_t digit = shift == 0 ? 0x3ffu : 0x7ffu;
+    uint32_t left = s.need;
+    // the digit of BITS bits from SHIFT on; 0 in place of a rank is below all and changes nothing
+    const auto find = [&](auto shift_, auto bits_) __attribute__((always_inline)) {
+      constexpr int SHIFT = decltype(shift_)::value, BITS = decltype(bits_)::value;
+      constexpr int DONE = SHIFT + BITS;  // the digits from this bit on are known
       for (int i = tid; i < kCopies * kBins / 4; i += kSelectThreads)
         reinterpret_cast<U32x4*>(bins)[i] = U32x4{0, 0, 0, 0};
       __syncthreads();
       for (int from = 0; from < s.older; from += kRound) {
         if (s.older > kRound) load_ranks(from);
+        const int steps = steps_of(from, s.older);
 #pragma unroll
         for (int j = 0; j < KEYS; ++j) {
-          if (rank[j] != 0 && ((rank[j] ^ cut) & known) == 0)
-            atomicAdd(&bins[kCopies * ((rank[j] >> shift) & digit) + lane % kCopies], 1u);
+          if (j < steps && (DONE == 32 || (rank[j] >> (DONE % 32)) == (cut >> (DONE % 32))))
+            atomicAdd(&bins[kCopies * ((rank[j] >> SHIFT) & ((1u << BITS) - 1)) + lane % kCopies],
+                      1u);
         }
       }
       __syncthreads();
@@ -767,10 +789,12 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
         found[1] = above + (second ? high : 0);
       }
       __syncthreads();
-      cut |= found[0] << shift;
+      cut |= found[0] << SHIFT;
       left -= found[1];
-      known |= digit << shift;
-    }
+    };
+    find(std::integral_constant<int, 21>{}, std::integral_constant<int, 11>{});
+    find(std::integral_constant<int, 10>{}, std::integral_constant<int, 11>{});
+    find(std::integral_constant<int, 0>{}, std::integral_constant<int, 10>{});
     ties = left;
   }  // else all
 
@@ -786,8 +810,10 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
   for (int from = 0; from < s.tokens; from += kRound) {
     if (s.tokens > kRound && s.older > 0) load_ranks(from);
     uint32_t sures_here = 0, sames_here = 0;  // lane j: of step j
+    const int steps = steps_of(from, s.tokens);
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) {
+      if (j >= steps) continue;
       const uint32_t a = __popcll(sures_of(j, from)), b = __popcll(sames_of(j));
       sures_here = lane == j ? a : sures_here;
       sames_here = lane == j ? b : sames_here;
@@ -821,17 +847,25 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
       sures_here = sure_count[lane * kSelectWaves + wave];
       sames_here = same_count[lane * kSelectWaves + wave];
     }
+    const int again = steps_of(from, s.tokens);
 #pragma unroll
     for (int j = 0; j < KEYS; ++j) {
+      if (j >= again) continue;
       asm volatile("" : "+v"(rank[j]));  // bits are made anew: there are no registers for all
       const uint64_t sures = sures_of(j, from), sames = sames_of(j);
       if ((sures | sames) == 0) continue;
-      const uint32_t same_rank = same_base + __builtin_amdgcn_readlane(sames_here, j) +
-                                 __popcll(sames & ((1ull << lane) - 1));
-      if (((sures >> lane) & 1) || (((sames >> lane) & 1) && same_rank < ties)) {
+      const uint32_t same = same_base + __builtin_amdgcn_readlane(sames_here, j);
+      uint32_t at = sure_base + __builtin_amdgcn_readlane(sures_here, j) + before_lane(sures);
+      bool keep = __builtin_amdgcn_inverse_ballot_w64(sures);
+      if (sames == 0) {
+        at += min(same, ties);
+      } else {
+        const uint32_t same_rank = same + before_lane(sames);
+        keep |= __builtin_amdgcn_inverse_ballot_w64(sames) && same_rank < ties;
+        at += min(same_rank, ties);
+      }
+      if (keep) {
         const int t = from + j * kStep + tid;
-        const uint32_t at = sure_base + __builtin_amdgcn_readlane(sures_here, j) +
-                            __popcll(sures & ((1ull << lane) - 1)) + min(same_rank, ties);
         kept[at] = t;
         out_w[at] = t < s.older ? weight_of(rank[j]) : w[t];
       }
@@ -1087,6 +1121,8 @@ int origami_evict_kv_cache(
   const dim3 lists(static_cast<unsigned>(requests * heads)), threads(kSelectThreads);
   if (max_tokens <= 4 * kSelectThreads)
     hipLaunchKernelGGL(select_kernel<4>, lists, threads, 0, stream, p);
+  else if (max_tokens <= 16 * kSelectThreads)
+    hipLaunchKernelGGL(select_kernel<16>, lists, threads, 0, stream, p);
   else
     hipLaunchKernelGGL(select_kernel<32>, lists, threads, 0, stream, p);
   if (int rc = check_launch("select_kernel")) return rc;

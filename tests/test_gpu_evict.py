@@ -261,6 +261,17 @@ def test_evict_long(cuda_device):
     Eviction(cuda_device, tokens=(70001,), keep=30000, recent=1, heads=1, D=8).check()
 
 
+@pytest.mark.parametrize("most", [4096, 4097, 8191, 16384, 16385, 32768, 32769, 49155])
+@pytest.mark.parametrize("keep,recent", [(0, 0), (700, 0), (700, 65), (5000, 4999)])
+def test_evict_on_both_sides_of_a_lane_s_places(cuda_device, most, keep, recent):
+    """Requests of all lengths in one call, with weights that are all different, few, or one."""
+    e = Eviction(cuda_device, tokens=(most, most - 1, 0, 1, keep + 1, most // 2 + 1), keep=keep,
+                 recent=recent, heads=3, D=8, seed=most + keep)
+    e.weights[:, 1] = (e.weights[:, 1] * 8).round() - 3.0
+    e.weights[:, 2] = -0.0
+    e.check()
+
+
 def test_evict_ties_and_odd_weights(cuda_device):
     """Equal weights go to the first places; both zeros are equal; NaN is larger than infinity;
     ranks that differ in their last bit."""
