@@ -1614,9 +1614,11 @@ Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_di
         // waves for the CUs once, or as often as the requests are half of them
         const int64_t once = std::max<int64_t>(kFourWavesWanted / heads, 1);
         plan.shares = std::max<int64_t>(ceil_div(2 * requests, once), 1) * once;
-        // a request's parts take memory: 32 of them, and more if there are few requests
+        // a request's parts take memory: 32 of them, and more if there are few requests or the
+        // bound, which may be far above the lengths, is past 32768 tokens
         const int64_t parts = std::min<int64_t>(
-            std::max<int64_t>(32, 2 * kFourWavesWanted / k1.count), kMaxParts / 2);
+            std::max<int64_t>({32, 2 * kFourWavesWanted / k1.count, ceil_div(steps, 32)}),
+            kMaxParts / 2);
         plan.least_share = std::max<int64_t>(8, ceil_div(steps, parts));
         best1 = ceil_div(steps, plan.least_share);
       }

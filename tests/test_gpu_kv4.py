@@ -465,6 +465,15 @@ def test_attend_shares_captured_as_lengths_grow(cuda_device, requests):
         assert torch.equal(out, eager) and torch.equal(lse, eager_lse)
 
 
+@pytest.mark.parametrize("blocks", [1100, 4400, 9000])
+def test_attend_shares_of_bounds_far_above_the_lengths(cuda_device, blocks):
+    """Block tables of up to 144000 tokens for requests of up to 1700."""
+    b = Batch4(cuda_device, heads=8, group=2, prefix=0, own=lengths_of(24, 1700, 11), seed=11)
+    b.tables = torch.cat([b.tables, torch.full((24, blocks - b.tables.shape[1]), -1,
+                                               device=cuda_device)], 1)
+    b.check(*b.run())
+
+
 def test_attend_shares_of_lengths_past_the_bound(cuda_device):
     """Lengths that the bound cuts off, up to the largest of their type, are no more than it."""
     b = Batch4(cuda_device, heads=8, group=2, prefix=0, own=(2000,) * 40, seed=5)
