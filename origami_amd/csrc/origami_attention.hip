@@ -74,6 +74,11 @@ struct Group {
   int32_t first;   // the first token of range 0
 };
 
+// The parts of a row that is cut into shares: the first one's place, and how many there are.
+struct alignas(8) RowParts {
+  int32_t first, count;
+};
+
 struct AttendParams {
   const void* query;
   int64_t q_token, q_head;  // strides, in elements
@@ -93,8 +98,11 @@ struct AttendParams {
   Group group[2];        // the prefix with the whole batch's rows; each request's rows
   Divisor shares, full_shares;  // see share_of: of a head (0 without); one a request less
   int32_t least_share;   // steps of a share, at least
-  int32_t slots;
-  float *part_o, *part_ml;  // [slots][rows][D], [slots][rows][2]
+  int32_t share_rows;    // rows of a share and head that there is room for
+  int32_t slots;         // parts of a row, at most
+  // [slots][rows][D], [slots][rows][2], or of shares [shares][H][share_rows][..]
+  float *part_o, *part_ml;
+  RowParts* row_parts;  // [rows], of shares
 };
 
 // A load that is known to be from memory and not from LDS (whose waits it would share).
@@ -370,16 +378,22 @@ __device__ __forceinline__ float fold_wave(float x, Fold fold) {
   return fold(as_float(one), as_float(other));
 }
 
-// Four channels of a row's result, and with the first ones its maximum and sum.
-template <typename T>
-__device__ __forceinline__ void put_four(const AttendParams& p, const Group& g, const Request& rq,
-                                         int h, int split, int rows, int row, int ch, Float4 v,
+// The place of the first row's partial result, of one range.
+__device__ __forceinline__ int64_t first_place(const AttendParams& p, const Group& g, int split) {
+  return (g.slot + split) * (static_cast<int64_t>(p.tokens) * p.Hq);
+}
+
+// Four channels of a row's result, and with the first ones its maximum and sum; as a part, its
+// place is that of its row of the batch after `first`, or, of a share, of its request.
+template <typename T, bool SHARES = false>
+__device__ __forceinline__ void put_four(const AttendParams& p, const Request& rq, int h,
+                                         int64_t first, int rows, int row, int ch, Float4 v,
                                          float base, float sum) {
   if (row >= rows || ch >= p.D) return;
   const int qi = divide(row, p.G), head = h * p.G.d + row - qi * p.G.d;
   const int64_t n = rq.first + qi, at = n * p.Hq + head;
   if (p.slots > 1) {
-    const int64_t slot = (g.slot + split) * (static_cast<int64_t>(p.tokens) * p.Hq) + at;
+    const int64_t slot = first + (SHARES && p.share_rows ? row : at);
     if (ch == 0) {
       p.part_ml[2 * slot] = base - kLift<T>;
       p.part_ml[2 * slot + 1] = sum;
@@ -769,7 +783,7 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
     return v;
   };
   const auto put = [&](int row, int ch, Float4 v, float base, float sum) {
-    put_four<T>(p, g, rq, h, split, rows, row, ch, v, base, sum);
+    put_four<T>(p, rq, h, first_place(p, g, split), rows, row, ch, v, base, sum);
   };
 
   if constexpr (WT > 1) {
@@ -883,8 +897,8 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
 // them for V P.  Memory bounds it: 32 requests of 1000 to 16384 tokens with 8 heads of 128 (327 MB)
 // take 83 us, 4.0 TB/s, and without the products as long; with rows over lanes and no step ahead 165.
 template <typename T, int DP, bool WHOLE, bool JOIN>
-__device__ __forceinline__ void attend_four(const AttendParams& p, const Group& g, bool batch,
-                                            int r, const Request& rq, int h, int split, int t0,
+__device__ __forceinline__ void attend_four(const AttendParams& p, bool batch, int r,
+                                            const Request& rq, int h, int64_t place, int t0,
                                             int stop, int wave, uint8_t* wave_lds, float* ml) {
   constexpr int kStride = JOIN ? 32 * kFourWaves<DP, JOIN> : 32;  // tokens between a wave's steps
   uint8_t* const lds = wave_lds + wave * kFourLds<DP, JOIN>;
@@ -1117,7 +1131,7 @@ __device__ __forceinline__ void attend_four(const AttendParams& p, const Group& 
         v += *reinterpret_cast<const Float4*>(part_row(w, at) + d) * weight;
       }
       if (odd) each_odd_token(at, [&](const uint8_t* values) { v += odd_part(values, d); });
-      put_four<T>(p, g, rq, h, split, rows, at, d, v, top, total);
+      put_four<T>(p, rq, h, place, rows, at, d, v, top, total);
     }
   } else {
     if (odd)
@@ -1127,7 +1141,7 @@ __device__ __forceinline__ void attend_four(const AttendParams& p, const Group& 
       });
 #pragma unroll
     for (int d = 0; d < DT; ++d)
-      put_four<T>(p, g, rq, h, split, rows, row, MR * d + 4 * q4, o[d], base, sum);
+      put_four<T, true>(p, rq, h, place, rows, row, MR * d + 4 * q4, o[d], base, sum);
   }
 }
 
@@ -1204,25 +1218,22 @@ __device__ __forceinline__ void attend_alone(const AttendParams& p, int unit, in
                                              uint8_t* wave_lds) {
   const Group& g = p.group[1];
   const int at = divide(unit, p.H), h = unit - at * p.H.d;
-  int r, part, parts = g.splits.d, each = g.chunk / 32;
+  int r, part, parts, each = g.chunk / 32;
   if (p.shares.d ? !share_of(p, at, &r, &part, &parts, &each)
                  : !range_of(p, g, false, at, &r, &part))
     return;
   const Request q = request_of(p, r);
   const int t0 = 32 * part * each;
-  attend_four<T, DP, WHOLE, false>(p, g, false, r, q, h, part, t0, t0 + 32 * each, wave, wave_lds,
+  const int64_t place = p.shares.d ? static_cast<int64_t>(at * p.H.d + h) * p.share_rows
+                                   : first_place(p, g, part);
+  attend_four<T, DP, WHOLE, false>(p, false, r, q, h, place, t0, t0 + 32 * each, wave, wave_lds,
                                    nullptr);
-  if (part != parts - 1) return;
-  // the last part says that there are no more
-  const int rows = q.count * p.G.d, none = (p.slots - parts) * rows;
-  for (int i = threadIdx.x & 63; i < none; i += 64) {
-    const int slot = i / rows, row = i - slot * rows, qi = divide(row, p.G);
-    const int64_t at_row =
-        static_cast<int64_t>(q.first + qi) * p.Hq + h * p.G.d + row - qi * p.G.d;
-    float* const ml =
-        p.part_ml + 2 * ((parts + slot) * (static_cast<int64_t>(p.tokens) * p.Hq) + at_row);
-    ml[0] = -INFINITY;
-    ml[1] = 0.0f;
+  if (!p.shares.d || part != 0 || p.slots == 1) return;
+  // where the join finds the parts, share after share
+  for (int i = threadIdx.x & 63; i < q.count * p.G.d; i += 64) {
+    const int qi = divide(i, p.G);
+    p.row_parts[static_cast<int64_t>(q.first + qi) * p.Hq + h * p.G.d + i - qi * p.G.d] =
+        RowParts{static_cast<int32_t>(place) + i, parts};
   }
 }
 
@@ -1248,8 +1259,8 @@ __global__ __launch_bounds__((64 * kFourWaves<DP, JOIN>), JOIN || DP == 256 ? 1 
     if (!range_of(p, g, kind == 0, uh, &r, &split)) return;
     const int t0 = g.first + split * g.chunk;
     const Request rq = kind == 0 ? Request{0, p.tokens, 0, 0} : request_of(p, r);
-    attend_four<T, DP, WHOLE, true>(p, g, kind == 0, r, rq, h, split, t0, t0 + g.chunk, wave, lds,
-                                    ml);
+    attend_four<T, DP, WHOLE, true>(p, kind == 0, r, rq, h, first_place(p, g, split), t0,
+                                    t0 + g.chunk, wave, lds, ml);
   } else {
     unit = unit * NW + wave;
     if (unit >= p.group[1].units) return;
@@ -1280,6 +1291,21 @@ __global__ __launch_bounds__(64 * kShapeWaves[S0], DP == 256 ? 1 : 2)
     attend_shape<T, CELL, DP, S0>(p, 0, unit, lds, ml);
 }
 
+// Where the parts of row `row` are: the first one's place, and from each to the next.  What a
+// request has of rows past its bound was written by nobody: any number is taken to a part that
+// there is.
+struct Parts {
+  int64_t first, step;
+  int32_t count;
+};
+__device__ __forceinline__ Parts parts_of(const AttendParams& p, int64_t row, int most) {
+  if (!p.shares.d) return {row, static_cast<int64_t>(p.tokens) * p.Hq, p.slots};
+  const RowParts mine = p.row_parts[row];
+  const int step = p.H.d * p.share_rows, last = p.shares.d * step - 1;
+  const int first = min(max(mine.first, 0), last);
+  return {first, step, min(min(max(mine.count, 1), (last - first) / step + 1), most)};
+}
+
 // Joins the parts of each row: out = v_scale sum_s w_s O_s / sum_s w_s l_s with
 // w_s = 2^(m_s - max m).  For few parts: 4 channels a lane, `lanes` lanes a row.  Sums are loaded
 // once it is known which there are: loading them beside the maxima cost 0.3 us of 12.2 for one
@@ -1293,12 +1319,13 @@ __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams p, 
   if (row >= all || ch >= p.D) return;
   const int64_t n = row / p.Hq, head = row - n * p.Hq;
   if (p.starts && (n < p.starts[0] || n >= p.starts[p.requests.d])) return;
+  const Parts parts = parts_of(p, row, kFewParts);
   float m[kFewParts], l[kFewParts], best = -INFINITY, total = 0.0f;
 #pragma unroll
   for (int s = 0; s < kFewParts; ++s) {
-    const int64_t slot = min(s, p.slots - 1) * all + row;
+    const int64_t slot = parts.first + min(s, parts.count - 1) * parts.step;
     m[s] = p.part_ml[2 * slot];
-    l[s] = s < p.slots ? p.part_ml[2 * slot + 1] : 0.0f;
+    l[s] = s < parts.count ? p.part_ml[2 * slot + 1] : 0.0f;
     best = fmaxf(best, m[s]);
   }
   const float zero = best == -INFINITY ? 0.0f : best;
@@ -1308,7 +1335,8 @@ __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams p, 
     if (l[s] != 0.0f) {  // else no token: nothing was written
       const float w = __builtin_amdgcn_exp2f(m[s] - zero);
       total += l[s] * w;
-      o += *reinterpret_cast<const Float4*>(p.part_o + (s * all + row) * p.D + ch) * w;
+      o += *reinterpret_cast<const Float4*>(p.part_o + (parts.first + s * parts.step) * p.D + ch) *
+           w;
     }
   const float inv = total == 0.0f ? 0.0f : p.v_scale / total;
   store4(static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + ch, o * inv, p.out_vec);
@@ -1326,7 +1354,6 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendParams p, int 
   __shared__ float wave_best[kJoinWaves], wave_sum[kJoinWaves];
   __shared__ int counts[kMaxParts / kJoinThreads][kJoinWaves];
   __shared__ Float4 part[kJoinThreads];
-  const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
   const int64_t row = blockIdx.x / blocks;
   const int ch = 4 * (static_cast<int>(blockIdx.x % blocks) * lanes + threadIdx.x % lanes);
   const int team = threadIdx.x / lanes, teams = kJoinThreads / lanes;
@@ -1334,6 +1361,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendParams p, int 
   const int64_t n = row / p.Hq, head = row - n * p.Hq;
   if (p.starts && (n < p.starts[0] || n >= p.starts[p.requests.d])) return;
 
+  const Parts of = parts_of(p, row, kMaxParts);
   constexpr int kEach = kMaxParts / kJoinThreads;
   float m[kEach], l[kEach], best = -INFINITY;
 #pragma unroll
@@ -1341,9 +1369,9 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendParams p, int 
     const int s = i * kJoinThreads + threadIdx.x;
     m[i] = -INFINITY;
     l[i] = 0.0f;
-    if (s < p.slots) {
-      m[i] = p.part_ml[2 * (s * all + row)];
-      l[i] = p.part_ml[2 * (s * all + row) + 1];
+    if (s < of.count) {
+      m[i] = p.part_ml[2 * (of.first + s * of.step)];
+      l[i] = p.part_ml[2 * (of.first + s * of.step) + 1];
     }
     best = fmaxf(best, m[i]);
   }
@@ -1381,11 +1409,11 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendParams p, int 
   if (lane == 0) wave_sum[wave] = sum;
   __syncthreads();
 
-  const float* const src = p.part_o + row * p.D + min(ch, p.D - 4);
+  const float* const src = p.part_o + of.first * p.D + min(ch, p.D - 4);
   Float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
   for (int s = team; s < parts; s += teams)
-    o += *reinterpret_cast<const Float4*>(src + which[s] * all * p.D) * weight[s];
+    o += *reinterpret_cast<const Float4*>(src + which[s] * of.step * p.D) * weight[s];
   for (int x = lanes; x < 64; x <<= 1)
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] += __shfl_xor(o[j], x);
@@ -1497,6 +1525,7 @@ struct Plan {
   int64_t slots, units;
   Way way;
   int64_t shares, least_share;  // see share_of
+  int64_t places;               // of partial results: rows of all slots, or of all shares
 };
 
 // Units of one kind, before they are split: `count` of them, `live` with rows if the requests are
@@ -1528,6 +1557,9 @@ constexpr double kUnitTime = 6.0, kCuBytes = 20e3, kCuFlops = 3.2e6;
 // shares takes longer with each request and many requests fill the CUs evenly by their number (200 of
 // 10 to 3000 tokens: 120 us in shares, 117 in ranges).
 constexpr int64_t kFourMany = 512, kFourWavesWanted = 2048;
+// Bytes that such ranges' parts may take, past what is needed for as many waves: 15 parts a row of
+// 512 requests with 64 heads of 128 channels.
+constexpr int64_t kFourBytes = int64_t(256) << 20;
 
 // Microseconds of a call whose kinds are split in s0 and s1 ranges: workgroups of the first kind go
 // to the CUs in order, then those of the second; and joining the parts of `rows` rows.
@@ -1607,20 +1639,19 @@ Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_di
     if (!apart && k1.count * ceil_div(k1.span, 256) >= kFourMany) {
       if (requests > kShared || requests * steps > INT32_MAX / 2) {
         plan.way = kFourRanges;
-        best1 = k1.splits(std::min(std::max(kFourWavesWanted / k1.count, ceil_div(k1.span, 1024)),
-                                   ceil_div(k1.span, 256)));
+        // every row has a part for each range of the bound, whatever its request's length
+        const int64_t room =
+            kFourBytes / (std::max<int64_t>(tokens * query_heads, 1) * (head_dim + 2) * 4);
+        best1 = k1.splits(std::min(
+            std::max(kFourWavesWanted / k1.count, std::min(ceil_div(k1.span, 1024), room)),
+            ceil_div(k1.span, 256)));
       } else {
         plan.way = kFourShares;
         // waves for the CUs once, or as often as the requests are half of them
         const int64_t once = std::max<int64_t>(kFourWavesWanted / heads, 1);
         plan.shares = std::max<int64_t>(ceil_div(2 * requests, once), 1) * once;
-        // a request's parts take memory: 32 of them, and more if there are few requests or the
-        // bound, which may be far above the lengths, is past 32768 tokens
-        const int64_t parts = std::min<int64_t>(
-            std::max<int64_t>({32, 2 * kFourWavesWanted / k1.count, ceil_div(steps, 32)}),
-            kMaxParts / 2);
-        plan.least_share = std::max<int64_t>(8, ceil_div(steps, parts));
-        best1 = ceil_div(steps, plan.least_share);
+        plan.least_share = std::max<int64_t>(8, ceil_div(steps, kMaxParts / 2));
+        best1 = std::min(ceil_div(steps, plan.least_share), plan.shares);
       }
     }
   }
@@ -1641,12 +1672,16 @@ Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_di
   };
   if (apart) put(plan.group[0], k0, best0, 0);
   put(plan.group[1], k1, best1, apart ? prefix : 0);
+  plan.places = plan.way == kFourShares ? plan.shares * heads * max_query * G
+                                        : plan.slots * tokens * query_heads;
   return plan;
 }
 
 int64_t workspace_bytes_of(const Plan& plan, int64_t tokens, int64_t query_heads,
                            int64_t head_dim) {
-  return plan.slots > 1 ? plan.slots * tokens * query_heads * (head_dim + 2) * 4 : 0;
+  if (plan.slots <= 1) return 0;
+  const int64_t lists = plan.way == kFourShares ? tokens * query_heads * sizeof(RowParts) : 0;
+  return plan.places * (head_dim + 2) * 4 + lists;
 }
 
 // A request's query tokens at most: no more than there are, and one, which each has where no
@@ -1781,11 +1816,12 @@ int origami_shared_prefix_attention(
   if (plan.shares > 0) {
     p.shares = divisor(plan.shares);
     p.full_shares = divisor(plan.shares - requests);
+    p.share_rows = static_cast<int32_t>(max_query_tokens * (query_heads / heads));
   }
   p.least_share = static_cast<int32_t>(plan.least_share);
-  const int64_t parts = plan.slots * tokens * query_heads;
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + parts * head_dim;
+  p.part_ml = p.part_o + plan.places * head_dim;
+  p.row_parts = reinterpret_cast<RowParts*>(p.part_ml + plan.places * 2);
   const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
   return dtype == ORIGAMI_DTYPE_BFLOAT16 ? launch_attend<bf16>(p, cell_of(cache_dtype), plan.way, stream)
                                          : launch_attend<f16>(p, cell_of(cache_dtype), plan.way, stream);

@@ -544,3 +544,60 @@ def test_refusals(cuda_device):
     cache = memory[:2 * 4 * 16 * 2 * 36].view(2, 4, 16, 2, 36)
     with pytest.raises(RuntimeError, match="must not overlap kv_cache"):
         read(cache, slots, key_out=memory[512:512 + 768].view(BF16).view(3, 2, 64))
+
+
+def test_attend_shares_memory_is_not_of_the_bound(cuda_device):
+    """What a call takes beside its results follows from the batch, not from its block tables."""
+    requests, heads, group = 128, 8, 8
+    b = Batch4(cuda_device, heads=heads, group=group, prefix=0, own=lengths_of(requests, 900, 4))
+    used = []
+    for blocks in (b.tables.shape[1], 2048, 65536):
+        b.tables = torch.cat([b.tables, torch.full((requests, blocks - b.tables.shape[1]), -1,
+                                                   device=cuda_device)], 1)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got, lse = b.run()
+        used.append(torch.cuda.max_memory_allocated() - before)
+        b.check(got, lse)
+    results = got.nbytes + lse.nbytes
+    # 2048 shares or two a request and head, with `group` rows each; lists of 8 bytes a row
+    most = (2048 + 2 * requests * heads) * group * 130 * 4 + 8 * lse.numel() + 4096
+    assert max(used) <= results + most
+
+
+@pytest.mark.parametrize("filled", [0xff, 0x7f, 0x00, 0x80])
+def test_attend_shares_leave_other_rows(cuda_device, filled):
+    """Rows before the first request and behind the last are left as they were; a request with more
+    queries than its bound harms no other, whatever the workspace held before."""
+    queries = (2, 1, 5, 0, 2, 1) * 9
+    own = [n + q for n, q in zip(lengths_of(54, 2300, 8), queries)]
+    b = Batch4(cuda_device, heads=4, group=4, prefix=0, own=own, queries=queries, seed=2)
+    b.query = torch.cat([b.query[:3], b.query, b.query[:4]])
+    b.starts = b.starts + 3
+    n = b.query.shape[0]
+    out = torch.full_like(b.query, 3.0)
+    # the memory that the call's workspace gets: its own size first, then filled
+    b.run(out=out, max_query_tokens=2)
+    workspaces = [torch.full((1 << k,), filled, dtype=torch.uint8, device=cuda_device)
+                  for k in range(21, 28)]
+    del workspaces
+    out.fill_(3.0)
+    got, lse = b.run(out=out, max_query_tokens=2)
+    assert (got[:3] == 3.0).all() and (got[n - 4:] == 3.0).all()
+    request = torch.repeat_interleave(torch.arange(54), torch.tensor(queries))
+    fine = torch.cat([torch.zeros(3, dtype=torch.bool), torch.tensor(queries)[request] <= 2,
+                      torch.zeros(4, dtype=torch.bool)]).to(cuda_device)
+    b.check(got, lse, rows=fine)
+
+
+@pytest.mark.parametrize("requests,bound", [(60, 4096), (256, 40960), (257, 40960), (400, 131072)])
+def test_attend_many_requests_with_a_bound_far_above(cuda_device, requests, bound):
+    """On both sides of where shares end; the longest request far beyond the others."""
+    b = Batch4(cuda_device, heads=2, group=3, D=64, prefix=0, seed=requests,
+               own=lengths_of(requests, 1500, requests))
+    want, want_lse = b.run()
+    b.check(want, want_lse)
+    b.tables = torch.cat([b.tables, torch.full((requests, bound // b.bs - b.tables.shape[1]), -1,
+                                               device=cuda_device)], 1)
+    b.check(*b.run())

@@ -201,3 +201,19 @@ def test_evict_refuses(change, message):
 
 def test_nothing_to_evict():
     assert _evict(requests=0, lengths=None, kept=None, out_weights=None) == 0
+
+
+@pytest.mark.parametrize("heads,query_heads", [(8, 64), (8, 32), (1, 16), (4, 28)])
+@pytest.mark.parametrize("requests", [1, 16, 128, 256, 257, 512, 2000])
+def test_attention_workspace_is_not_of_the_bound(heads, query_heads, requests):
+    """Decode steps over a cache in 4 bits, however far the bound is above what the requests hold.
+    There are shares for 2048 waves or two for each request and head, each with a request's rows of
+    D + 2 numbers, and 8 bytes a row; of equal ranges, past 256 requests, 256 MiB or what 2048 waves
+    take."""
+    size, D = _native.lib().origami_shared_prefix_attention_workspace, 128
+    row = (D + 2) * 4
+    for bound in (1, 4096, 32768, 131072, 1 << 20, 1 << 22):
+        got = size(requests, query_heads, heads, D, 0, requests, 1, bound, FP4)
+        waves = (2048 + 2 * requests * heads) * (query_heads // heads) * row
+        most = waves + requests * query_heads * 8 if requests <= 256 else max(256 << 20, waves)
+        assert 0 <= got <= most, (bound, got, most)
