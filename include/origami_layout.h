@@ -566,13 +566,14 @@ int origami_read_kv_cache(const void* kv_cache, int64_t cache_dtype, int64_t cac
  * float32 [tokens, query_heads], what the attention returned; a row of -infinity gives nothing.
  * weights (null: zeros) and out are float32 [requests, heads, places], places contiguous, with
  * request and head strides weight_strides (host, [4]: of weights, then of out); out may be weights
- * itself.  Tokens past max_tokens and tokens in blocks outside the cache get nothing, and places
- * that get nothing become weights' (0).
+ * itself.  Tokens past max_tokens, which shapes the launch, and tokens in blocks outside the cache
+ * get nothing, and places that get nothing become weights' (0).
  *
  * Products are of dtype (e4m3 and 4 bits are widened exactly), scores, exponentials and sums
  * binary32.  Sums are made in a fixed order.  query, strides, kv_cache and scale
  * are as for the attention.  workspace is a 16-byte aligned device buffer of at least
- * origami_accumulate_attention_weights_workspace bytes (0: may be null; -1: invalid sizes), in use
+ * origami_accumulate_attention_weights_workspace bytes, enough for any max_tokens up to places and
+ * 4 MiB at most (0: may be null; -1: invalid sizes), in use
  * until the call's work is done; calls that can run at the same time need their own.  out and
  * workspace share no memory with each other or with an input, but out with weights, if it is all of
  * it.

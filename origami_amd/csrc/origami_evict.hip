@@ -42,14 +42,15 @@ struct WeighParams {
   const int64_t *tables, *lengths, *starts;
   int64_t table_stride;
   Divisor block_size, requests, H, G;
-  Divisor tiles;  // ranges of a request's places, where the rows are few
+  Divisor tiles;  // ranges of a request's tokens, where the rows are few
+  int32_t rest;   // places past max_tokens that a range copies
   Divisor parts;  // of the rows that see a tile, each of which a workgroup adds up
   int32_t tokens, Hq, D, max_tokens, places;
   float scale;  // includes the keys' scale
   const float* weights;  // null: zeros
   float* out;
   int64_t w_request, w_head, o_request, o_head;  // strides, in elements
-  float* part_sums;  // [parts][requests][H][places], where there are several
+  float* part_sums;  // [parts][requests][H][max_tokens], where there are several
 };
 
 
@@ -136,7 +137,7 @@ __global__ __launch_bounds__(512, DP <= 128 ? 2 : 1) void weigh_kernel(WeighPara
       p.weights ? p.weights + r * p.w_request + h * p.w_head : nullptr;
   float* const out = p.out + r * p.o_request + h * p.o_head;
   float* const sums =
-      p.part_sums + ((static_cast<int64_t>(part) * p.requests.d + r) * p.H.d + h) * p.places;
+      p.part_sums + ((static_cast<int64_t>(part) * p.requests.d + r) * p.H.d + h) * p.max_tokens;
   if (t0 >= end) {
     // of several parts the join takes care of these
     if (p.parts.d > 1) return;
@@ -333,7 +334,7 @@ __global__ __launch_bounds__(512, DP <= 128 ? 2 : 1) void weigh_kernel(WeighPara
     const int t = first_t + n * MR + c;
     if (q4 != 0 || t >= p.places) continue;
     if (p.parts.d > 1) {
-      sums[t] = there[n] ? v : 0.0f;
+      if (t < p.max_tokens) sums[t] = there[n] ? v : 0.0f;
       continue;
     }
     if (there[n])
@@ -352,24 +353,29 @@ __global__ __launch_bounds__(256) void weigh_join_kernel(WeighParams p) {
   float* const out = p.out + r * p.o_request + h * p.o_head;
   const int end = static_cast<int>(
       min(max(p.lengths[r], int64_t(0)), static_cast<int64_t>(p.max_tokens)));
-  float sum = 0.0f;
-  if (t < end) {  // past it there may be no parts
-    const int64_t all = static_cast<int64_t>(p.requests.d) * p.H.d * p.places;
-    const float* const src = p.part_sums + static_cast<int64_t>(row) * p.places + t;
-#pragma unroll 4
-    for (int i = 0; i < p.parts.d; ++i) sum += src[i * all];
+  if (t >= end) {  // where there may be no parts
+    if (out != weights) out[t] = weights ? weights[t] : 0.0f;
+    return;
   }
+  const int64_t all = static_cast<int64_t>(p.requests.d) * p.H.d * p.max_tokens;
+  const float* const src = p.part_sums + static_cast<int64_t>(row) * p.max_tokens + t;
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < p.parts.d; ++i) sum += src[i * all];
   out[t] = (weights ? weights[t] : 0.0f) + sum;
 }
 
 // Parts of the rows: as many as give every CU a few workgroups, of four stages at least.
-int64_t weigh_parts(int64_t tokens, int64_t query_heads, int64_t heads, int64_t requests,
-                    int64_t places) {
+int64_t most_weigh_parts(int64_t tokens, int64_t query_heads, int64_t heads, int64_t requests) {
   const int64_t rows = tokens * (query_heads / heads);
   if (requests == 0 || rows <= 16 * requests) return 1;
-  const int64_t units = requests * heads * std::max<int64_t>(ceil_div(places, 256), 1);
-  const int64_t most = std::min<int64_t>(rows / requests / 256, kMostWeighParts);
-  return std::max<int64_t>(std::min(ceil_div(kWeighUnits, units), most), 1);
+  return std::max<int64_t>(std::min(rows / requests / 256, kMostWeighParts), 1);
+}
+int64_t weigh_parts(int64_t tokens, int64_t query_heads, int64_t heads, int64_t requests,
+                    int64_t max_tokens) {
+  const int64_t most = most_weigh_parts(tokens, query_heads, heads, requests);
+  if (most == 1 || max_tokens == 0) return 1;
+  return std::min(ceil_div(kWeighUnits, requests * heads * ceil_div(max_tokens, 256)), most);
 }
 
 // Zeros, for what a lane reads of rows that are not in the cache and of channels past the last.
@@ -414,8 +420,23 @@ __global__ __launch_bounds__(256, 2) void weigh_few_kernel(WeighParams p, Diviso
   const float* const weights =
       p.weights ? p.weights + r * p.w_request + h * p.w_head : nullptr;
   float* const out = p.out + r * p.o_request + h * p.o_head;
-  // places past the tokens are copied, if they are elsewhere
-  const int t1 = min(t0 + chunk, out == weights ? end : p.places);
+  // places past the tokens are copied, if they are elsewhere: those up to the bound with the range's,
+  // those past it with all ranges alike
+  if (out != weights && p.rest > 0) {
+    constexpr int kEach = 8;
+    const int64_t rest0 = p.max_tokens + static_cast<int64_t>(t0 / chunk) * p.rest;
+    const int rest1 = static_cast<int>(min(rest0 + p.rest, static_cast<int64_t>(p.places)));
+    for (int64_t t = rest0 + lane; t < rest1; t += 64 * kEach) {
+      float w[kEach];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        w[i] = weights && t + 64 * i < rest1 ? weights[t + 64 * i] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (t + 64 * i < rest1) out[t + 64 * i] = w[i];
+    }
+  }
+  const int t1 = min(t0 + chunk, out == weights ? end : p.max_tokens);
   if (t0 >= t1) return;
   int q_first = r, q_count = 1;
   if (p.starts) {
@@ -567,13 +588,25 @@ __global__ __launch_bounds__(256, 2) void weigh_few_kernel(WeighParams p, Diviso
   } while (from < rows);
 }
 
+// Whether there are places past max_tokens that are copied: not if they are where they go.
+bool copies_rest(const WeighParams& p) {
+  return p.places > p.max_tokens && (p.out != p.weights || p.w_request != p.o_request ||
+                                     p.w_head != p.o_head);
+}
+
 template <typename T, Cell CELL, int DP>
 int launch_weigh_few(WeighParams p, int64_t requests, hipStream_t stream) {
-  // ranges of 64 tokens and more, for about 2048 waves
-  const int64_t most = std::max<int64_t>(ceil_div(p.places, 64), 1);
-  const int64_t wanted = std::min(std::max<int64_t>(kWeighWaves / (requests * p.H.d), 1), most);
-  const int64_t chunk = ceil_div(ceil_div(p.places, wanted), 64) * 64;
-  p.tiles = divisor(ceil_div(p.places, chunk));
+  // ranges of 64 tokens and more, for about 2048 waves; ranges without tokens where places past the
+  // bound are copied, 512 and more of them each
+  const int64_t most = std::max<int64_t>(ceil_div(p.max_tokens, 64), 1);
+  const int64_t waves = std::max<int64_t>(kWeighWaves / (requests * p.H.d), 1);
+  const int64_t wanted = std::min(waves, most);
+  const int64_t chunk = std::max<int64_t>(ceil_div(ceil_div(p.max_tokens, wanted), 64), 1) * 64;
+  const int64_t rest = copies_rest(p) ? p.places - p.max_tokens : 0;
+  const int64_t tiles = std::max({ceil_div(p.max_tokens, chunk),
+                                  std::min(waves, ceil_div(rest, 512)), int64_t(1)});
+  p.tiles = divisor(tiles);
+  p.rest = static_cast<int32_t>(ceil_div(rest, tiles));
   const int64_t units = requests * p.H.d * p.tiles.d;
   const Divisor beside = divisor(std::max(p.H.d / 4, 1));
   const int64_t workgroups = ceil_div(ceil_div(units, 4), 8 * beside.d) * 8 * beside.d;
@@ -595,14 +628,20 @@ int launch_weigh(const WeighParams& p, int64_t requests, hipStream_t stream) {
   // rows of 16 where the requests have no more on average
   if (static_cast<int64_t>(p.tokens) * p.G.d <= 16 * requests)
     return launch_weigh_few<T, CELL, DP>(p, requests, stream);
-  const int64_t units = requests * p.H.d * ceil_div(p.places, 256) * p.parts.d;
-  ORIGAMI_REQUIRE(units < (int64_t(1) << 32) / 512, "too many tokens for one call");
+  constexpr int64_t kMost = (int64_t(1) << 32) / 512;  // workgroups of a launch
+  ORIGAMI_REQUIRE(requests * p.H.d * ceil_div(p.places, 256) < kMost,
+                  "too many tokens for one call");
+  const int64_t tiles = ceil_div(copies_rest(p) ? p.places : p.max_tokens, 256);
+  if (tiles == 0) return ORIGAMI_OK;  // no tokens, and no places elsewhere
+  // of several parts the join copies what is past the bound
+  const int64_t units =
+      requests * p.H.d * (p.parts.d > 1 ? ceil_div(p.max_tokens, 256) * p.parts.d : tiles);
+  ORIGAMI_REQUIRE(units < kMost, "too many tokens for one call");
   const dim3 grid(static_cast<unsigned>(units)), block(512);
   hipLaunchKernelGGL((weigh_kernel<T, CELL, DP>), grid, block, 0, stream, p);
   if (int rc = check_launch("weigh_kernel")) return rc;
   if (p.parts.d == 1) return ORIGAMI_OK;
-  const dim3 joins(static_cast<unsigned>(ceil_div(p.places, 256)),
-                   static_cast<unsigned>(requests * p.H.d));
+  const dim3 joins(static_cast<unsigned>(tiles), static_cast<unsigned>(requests * p.H.d));
   hipLaunchKernelGGL(weigh_join_kernel, joins, dim3(256), 0, stream, p);
   return check_launch("weigh_join_kernel");
 }
@@ -953,8 +992,8 @@ int check_weigh_sizes(int64_t tokens, int64_t query_heads, int64_t heads, int64_
   return ORIGAMI_OK;
 }
 
-int64_t weigh_workspace(int64_t parts, int64_t requests, int64_t heads, int64_t places) {
-  return parts > 1 ? parts * requests * heads * places * 4 : 0;
+int64_t weigh_workspace(int64_t parts, int64_t requests, int64_t heads, int64_t max_tokens) {
+  return parts > 1 ? parts * requests * heads * max_tokens * 4 : 0;
 }
 
 }  // namespace
@@ -965,8 +1004,13 @@ int64_t origami_accumulate_attention_weights_workspace(int64_t tokens, int64_t q
                                                        int64_t heads, int64_t requests,
                                                        int64_t places) {
   if (check_weigh_sizes(tokens, query_heads, heads, requests, places)) return -1;
-  return weigh_workspace(weigh_parts(tokens, query_heads, heads, requests, places), requests,
-                         heads, places);
+  // the largest for any bound up to `places`: of those with some number of parts the last one
+  int64_t bytes = 0;
+  for (int64_t n = most_weigh_parts(tokens, query_heads, heads, requests); n > 1; --n) {
+    const int64_t tiles = (kWeighUnits - 1) / (requests * heads * (n - 1));
+    bytes = std::max(bytes, weigh_workspace(n, requests, heads, std::min(tiles * 256, places)));
+  }
+  return bytes;
 }
 
 int origami_accumulate_attention_weights(
@@ -1009,10 +1053,10 @@ int origami_accumulate_attention_weights(
                       lengths != nullptr && (block_tables != nullptr || max_tokens == 0) &&
                       (kv_cache != nullptr || num_blocks == 0),
                   "queries, weights, lengths, tables and the cache must not be null");
-  const int64_t parts = weigh_parts(tokens, query_heads, heads, requests, places);
+  const int64_t parts = weigh_parts(tokens, query_heads, heads, requests, max_tokens);
   // the join has a workgroup row for every request and head
   ORIGAMI_REQUIRE(parts == 1 || requests * heads <= 65535, "too many requests for one call");
-  ORIGAMI_REQUIRE(workspace_bytes >= weigh_workspace(parts, requests, heads, places) &&
+  ORIGAMI_REQUIRE(workspace_bytes >= weigh_workspace(parts, requests, heads, max_tokens) &&
                       (parts == 1 || workspace != nullptr) && aligned16(workspace),
                   "the workspace of the weights is too small");
   p.parts = divisor(parts);

@@ -858,8 +858,9 @@ def accumulate_attention_weights(query: torch.Tensor, kv_cache: torch.Tensor,
     the request's tokens.  weights (default: zeros) and the result are float32 [requests, heads,
     places]; place t is the request's token t.  `out` may be `weights` itself; without weights and
     out the result has max_tokens places (default: the block table's slots, or as many as weights
-    has places).  Tokens past max_tokens and in blocks outside the cache get nothing.  Lengths and
-    tables are read on the device, so a call can be captured in a graph.  Each sum is float32, in a
+    has places).  Tokens past max_tokens and in blocks outside the cache get nothing.  max_tokens
+    shapes the launch, not the places: in place, a buffer of sums for the longest context takes no
+    time beyond it.  Lengths and tables are read on the device, so a call can be captured in a graph.  Each sum is float32, in a
     fixed order.  Overlaps are refused but of out with weights.  For inference only, as
     shared_prefix_attention."""
     return _ext.ext().accumulate_attention_weights(

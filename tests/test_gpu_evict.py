@@ -479,3 +479,36 @@ def test_refusals(cuda_device):
         native_gpu.evict_kv_cache(e.cache.float(), e.tables, e.tokens, e.weights, e.out_tables, 20,
                                   max_tokens=50)
     assert torch.equal(e.cache, before)
+
+
+@pytest.mark.parametrize("tokens,queries", [((70, 300, 0, 33), None), ((70, 300, 0, 33), (9, 40, 0, 2)),
+                                            ((2000, 1500), (2000, 700)), ((5,) * 40, None)])
+@pytest.mark.parametrize("spare", [1, 63, 20000])
+@pytest.mark.parametrize("bound", ["most", "half", 0, None])
+def test_weights_places_far_past_the_tokens(cuda_device, tokens, queries, spare, bound):
+    """Sums for more tokens than there are, as a buffer that is kept for the longest context: the
+    places past the bound are the sums before in a new buffer, and stay in the same one."""
+    w = Weights(cuda_device, tokens=tokens, queries=queries, D=64, spare=spare, seed=spare)
+    bound = {"most": w.most, "half": w.most // 2}.get(bound, bound)
+    want = w.run(max_tokens=bound)
+    cut = min(w.most if bound is None else bound, w.most)
+    for start in (w.weights, torch.zeros_like(w.weights)):
+        got = w.run(max_tokens=bound, weights=start)
+        kv = kv4ref.cells(w.cache, w.D, w.k_scale)
+        sums, added, largest = kv4ref.weigh(w.query, kv, w.tables, w.tokens, w.lse, start, w.starts)
+        sums[..., cut:], added[..., cut:] = start[..., cut:].double(), 0.0
+        tol = kv4ref.weigh_tolerance(w.D, largest, w.lse, added, sums)
+        assert (got.double() - sums).abs().le(tol).all()
+        assert torch.equal(got[..., cut:], start[..., cut:])
+    B, H, S = w.weights.shape
+    room = torch.full((H, B, S + 9), 5.0, device=cuda_device)  # a buffer of other strides
+    out = room[..., 4:4 + S].transpose(0, 1)
+    w.run(max_tokens=bound, out=out)
+    assert torch.equal(out, want)
+    assert (room[..., :4] == 5.0).all() and (room[..., 4 + S:] == 5.0).all()
+    out.fill_(7.0)
+    zero = w.run(max_tokens=min(bound, S) if bound is not None else w.most, weights=None, out=out)
+    assert (zero[..., cut:] == 0).all()
+    same = w.weights.clone()
+    w.run(max_tokens=bound, weights=same, out=same)
+    assert torch.equal(same, want)

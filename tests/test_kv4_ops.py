@@ -146,6 +146,24 @@ def test_weights_refuse_workspaces(change):
     refused(_weigh, dict(prompt, **change), "workspace of the weights is too small")
 
 
+@pytest.mark.parametrize("places", [4096, 131072, 1 << 30])
+def test_weights_are_split_by_the_bound(places):
+    """Two prompts of 4096 tokens take parts of their rows (and room for their sums), however wide
+    the buffer of the sums is."""
+    prompts = dict(tokens=8000, requests=2, starts=16, heads=4, query_heads=28, table_blocks=256,
+                   max_tokens=4096, places=places)
+    refused(_weigh, dict(prompts, workspace_bytes=8), "workspace of the weights is too small")
+
+
+def test_weights_workspace_is_enough_for_every_bound():
+    size = _native.lib().origami_accumulate_attention_weights_workspace
+    for requests, heads in ((1, 1), (1, 8), (2, 4), (60, 8), (300, 8)):
+        sizes = [size(1 << 18, 4 * heads, heads, requests, n)
+                 for n in (1, 255, 256, 257, 1000, 4096, 20000, 131072, 1 << 30)]
+        assert sizes == sorted(sizes) and sizes[-1] <= 2 * 2048 * 256 * 4
+        assert sizes[0] >= 0 and (sizes[0] > 0) == (requests * heads < 2048)
+
+
 def test_weights_workspace_sizes():
     size = _native.lib().origami_accumulate_attention_weights_workspace
     assert size(4096, 8, 2, 1, 4096) > 0 and size(4096, 8, 2, 1, 4096) % (2 * 4096 * 4) == 0
