@@ -381,8 +381,8 @@ int64_t weigh_parts(int64_t tokens, int64_t query_heads, int64_t heads, int64_t 
 // Zeros, for what a lane reads of rows that are not in the cache and of channels past the last.
 __device__ const U32x4 kZeroRow[33] = {};
 
-// One wave: a range of the tokens of one KV head of one request against its query rows, 16 at a
-// time, for requests of few rows, as in a decode step.  Memory bounds it.  The queries stay in
+// One wave: a range of the tokens of one KV head of one request against its query rows, 16 and fewer
+// as in a decode step, or 16 at a time.  Memory bounds it.  The queries stay in
 // registers; the keys come 64 tokens at a step (32 past 128 channels) and a step ahead, and their
 // blocks two steps, so that a wave waits for memory as seldom as can be: 16 requests of 2048 to 8192
 // tokens and 8 heads of 128 take 47 us among other work (39 alone, 4.3 TB/s) and in 4 bits 20; with
@@ -490,11 +490,13 @@ __global__ __launch_bounds__(256, 2) void weigh_few_kernel(WeighParams p, Diviso
     }
   };
 
-  // With no query row the sums stay what they are; with more than 16 the later rows are added to
-  // what the first ones left in `out`.
-  int from = 0;
-  do {
-    Vec8<T> qf[KS];
+  // 16 query rows: of the product, and of what this lane has of its result (rows 4 q4 .. 4 q4 + 3).
+  struct Rows16 {
+    Vec8<T> q[KS];
+    float below[4];
+    int limit[4];
+  };
+  const auto load_rows = [&](Rows16& o, int from) {
     {
       const int row = from + c, qi = divide(row, p.G), head = h * p.G.d + row - qi * p.G.d;
       const T* const src =
@@ -502,90 +504,122 @@ __global__ __launch_bounds__(256, 2) void weigh_few_kernel(WeighParams p, Diviso
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const int d = ((k / NPE * NG + q4) * NPE + k % NPE) * 8;
-        qf[k] = Vec8<T>{};
+        o.q[k] = Vec8<T>{};
         if (row < rows && d < p.D) {
           if (p.q_vec) {
-            qf[k] = *reinterpret_cast<const Vec8<T>*>(src + d);
+            o.q[k] = *reinterpret_cast<const Vec8<T>*>(src + d);
           } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) qf[k][j] = src[d + j];
+            for (int j = 0; j < 8; ++j) o.q[k][j] = src[d + j];
           }
         }
       }
     }
-    float below[4];  // of rows 4 q4 .. 4 q4 + 3, which are this lane's in the result
-    int limit[4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int row = from + 4 * q4 + x, qi = divide(row, p.G);
-      below[x] = 0.0f;
-      limit[x] = 0;
+      o.below[x] = 0.0f;
+      o.limit[x] = 0;
       if (row < rows) {
         const float lse =
             p.lse[static_cast<int64_t>(q_first + qi) * p.Hq + h * p.G.d + row - qi * p.G.d];
-        below[x] = lse;
+        o.below[x] = lse;
         // a row that saw nothing gives no weight
-        limit[x] = lse == -INFINITY ? 0 : before + qi + 1;
+        o.limit[x] = lse == -INFINITY ? 0 : before + qi + 1;
       }
     }
-    const float* const sums = from == 0 ? weights : out;
-    const auto compute = [&](const Step& s, int t) {
-      float v[NT];
+  };
+  // What this lane's rows give the token of its column in tile n.
+  const auto weights_of = [&](const Rows16& q, const Step& s, int n, int t) -> float {
+    Tile<MR> score = {};
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        Tile<MR> score = {};
+    for (int k = 0; k < KS; ++k) {
+      const int j = k / NPE, i = k % NPE;
+      U32x4 wide;
+      if constexpr (CELL == kFp4)
+        wide = fp4_expand<T>(s.raw[n][j].w[i], fp4_scale(s.scale[n][j]));
+      else if constexpr (CELL == kFp8)
+        wide = fp8_expand<T>(U32x2{s.raw[n][j].w[2 * i], s.raw[n][j].w[2 * i + 1]});
+      else
+        wide = U32x4{s.raw[n][j].w[0], s.raw[n][j].w[1], s.raw[n][j].w[2], s.raw[n][j].w[3]};
+      score = mfma<T, MR>(q.q[k], __builtin_bit_cast(Vec8<T>, wide), score);
+    }
+    const int at = t + MR * n + c;
+    float e[4];
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const int j = k / NPE, i = k % NPE;
-          U32x4 wide;
-          if constexpr (CELL == kFp4)
-            wide = fp4_expand<T>(s.raw[n][j].w[i], fp4_scale(s.scale[n][j]));
-          else if constexpr (CELL == kFp8)
-            wide = fp8_expand<T>(U32x2{s.raw[n][j].w[2 * i], s.raw[n][j].w[2 * i + 1]});
-          else
-            wide = U32x4{s.raw[n][j].w[0], s.raw[n][j].w[1], s.raw[n][j].w[2], s.raw[n][j].w[3]};
-          score = mfma<T, MR>(qf[k], __builtin_bit_cast(Vec8<T>, wide), score);
-        }
-        const int at = t + MR * n + c;
-        float e[4];
+    for (int x = 0; x < 4; ++x) {
+      e[x] = __builtin_amdgcn_exp2f(kLog2e * fmaf(score[x], p.scale, -q.below[x]));
+      e[x] = at < q.limit[x] ? e[x] : 0.0f;
+    }
+    return (e[0] + e[1]) + (e[2] + e[3]);
+  };
+  const auto finish = [&](const Step& s, float (&v)[NT], int t) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          e[x] = __builtin_amdgcn_exp2f(kLog2e * fmaf(score[x], p.scale, -below[x]));
-          e[x] = at < limit[x] ? e[x] : 0.0f;
-        }
-        v[n] = (e[0] + e[1]) + (e[2] + e[3]);
-        v[n] += __shfl_xor(v[n], 16);
-        v[n] += __shfl_xor(v[n], 32);
-      }
-      float mine = v[0];  // of token number `lane`, which is in tile lane / 16
+    for (int n = 0; n < NT; ++n) {
+      v[n] += __shfl_xor(v[n], 16);
+      v[n] += __shfl_xor(v[n], 32);
+    }
+    float mine = v[0];  // of token number `lane`, which is in tile lane / 16
 #pragma unroll
-      for (int n = 1; n < NT; ++n) mine = q4 % NT == n ? v[n] : mine;
-      if (lane < STEP && t + tl < t1) {
-        if (s.there)
-          out[t + tl] = s.old + mine;
-        else if (out != sums)
-          out[t + tl] = s.old;
-      }
-    };
+    for (int n = 1; n < NT; ++n) mine = q4 % NT == n ? v[n] : mine;
+    if (lane < STEP && t + tl < t1) {
+      if (s.there)
+        out[t + tl] = s.old + mine;
+      else if (out != weights)
+        out[t + tl] = s.old;
+    }
+  };
 
-    Step even, other;
-    int64_t next_id = from == 0 ? id : block_of(t0 + tl);
-    if (from > 0) ahead = block_of(t0 + STEP + tl);
-    load_step(even, row_of(t0 + tl, next_id), t0, sums);
-    __builtin_amdgcn_sched_barrier(0);
-    for (int t = t0; t < t1; t += 2 * STEP) {
-      int mine = row_of(t + STEP + tl, ahead);
-      ahead = block_of(t + 2 * STEP + tl);
-      load_step(other, mine, t + STEP, sums);
-      compute(even, t);
-      if (t + STEP >= t1) break;
-      mine = row_of(t + 2 * STEP + tl, ahead);
-      ahead = block_of(t + 3 * STEP + tl);
-      load_step(even, mine, t + 2 * STEP, sums);
-      compute(other, t + STEP);
+  if (rows > MR) {
+    // One of the batch's longer requests: each step's keys against all rows that see any of them, 16
+    // at a time, in sums of binary32 with what they lose.
+    int64_t block = id;
+    for (int t = t0; t < t1; t += STEP) {
+      Step s;
+      load_step(s, row_of(t + tl, block), t, weights);
+      block = block_of(t + STEP + tl);
+      float sum[NT] = {}, lost[NT] = {};
+      int from = min(max(t - before, 0), q_count) * p.G.d / MR * MR;
+      Rows16 next;
+      if (from < rows) load_rows(next, from);
+      for (; from < rows; from += MR) {
+        const Rows16 q = next;
+        if (from + MR < rows) load_rows(next, from + MR);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float add = weights_of(q, s, n, t) - lost[n], total = sum[n] + add;
+          lost[n] = total < INFINITY ? (total - sum[n]) - add : 0.0f;
+          sum[n] = total;
+        }
+      }
+      finish(s, sum, t);
     }
-    from += MR;
-  } while (from < rows);
+    return;
+  }
+
+  // with no query row the sums stay what they are
+  Rows16 q;
+  load_rows(q, 0);
+  const auto compute = [&](const Step& s, int t) {
+    float v[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) v[n] = weights_of(q, s, n, t);
+    finish(s, v, t);
+  };
+  Step even, other;
+  load_step(even, row_of(t0 + tl, id), t0, weights);
+  __builtin_amdgcn_sched_barrier(0);
+  for (int t = t0; t < t1; t += 2 * STEP) {
+    int mine = row_of(t + STEP + tl, ahead);
+    ahead = block_of(t + 2 * STEP + tl);
+    load_step(other, mine, t + STEP, weights);
+    compute(even, t);
+    if (t + STEP >= t1) break;
+    mine = row_of(t + 2 * STEP + tl, ahead);
+    ahead = block_of(t + 3 * STEP + tl);
+    load_step(even, mine, t + 2 * STEP, weights);
+    compute(other, t + STEP);
+  }
 }
 
 // Whether there are places past max_tokens that are copied: not if they are where they go.

@@ -853,7 +853,8 @@ def accumulate_attention_weights(query: torch.Tensor, kv_cache: torch.Tensor,
     Request r has tokens[r] tokens in blocks block_tables[r] (a prefix shared with others is part of
     them here), and its query rows are its newest ones: row r of query, or with query_starts rows
     query_starts[r] .. query_starts[r + 1] - 1; all of a prompt's rows or some last ones may be
-    given.  query, kv_cache, k_scale and scale are those of shared_prefix_attention, and lse
+    given.  The average of the requests' rows shapes the launch, and a prompt among many single tokens
+    is slow: call once for prompts and once for single tokens.  query, kv_cache, k_scale and scale are those of shared_prefix_attention, and lse
     (float32 [rows, query_heads]) is what it returned with return_lse for these rows over all of
     the request's tokens.  weights (default: zeros) and the result are float32 [requests, heads,
     places]; place t is the request's token t.  `out` may be `weights` itself; without weights and

@@ -512,3 +512,24 @@ def test_weights_places_far_past_the_tokens(cuda_device, tokens, queries, spare,
     same = w.weights.clone()
     w.run(max_tokens=bound, weights=same, out=same)
     assert torch.equal(same, want)
+
+
+@pytest.mark.parametrize("cache_dtype", [BF16, U8])
+@pytest.mark.parametrize("requests,queries", [(64, 190), (20, 65), (300, 900)])
+def test_weights_of_one_long_request_among_many(cuda_device, cache_dtype, requests, queries):
+    """Requests of a row or two and one of many, whose sums lose no more than those of a prompt: its
+    rows are added to each other first, and to what there was once."""
+    at, group = requests // 2, 4
+    counts, tokens = [1] * requests, [1 + 37 * i % 200 for i in range(requests)]
+    counts[at], tokens[at], counts[-1], tokens[-2] = queries, queries + 70, 0, 0
+    w = Weights(cuda_device, heads=2, group=group, D=64, tokens=tokens, queries=counts,
+                cache_dtype=cache_dtype, seed=requests)
+    w.check(w.run())
+    same = w.weights.clone()
+    assert torch.equal(w.run(weights=same, out=same), w.run())
+    # 16 rows give 0.9, which is less than half a step of the sums before
+    w.query.zero_()
+    w.lse.fill_(math.log(16 / 0.9))
+    w.weights.fill_(2.0 ** 24)
+    added = w.check(w.run())
+    assert added[at, 0, 0] > 14  # of which the sums have all but a step
