@@ -344,7 +344,7 @@ __global__ __launch_bounds__(512, DP <= 128 ? 2 : 1) void weigh_kernel(WeighPara
   }
 }
 
-// Adds the parts of each place, in their order.
+// Adds the parts of each place, in their order, with what the sums lose.
 __global__ __launch_bounds__(256) void weigh_join_kernel(WeighParams p) {
   const int row = static_cast<int>(blockIdx.y), r = divide(row, p.H), h = row - r * p.H.d;
   const int t = blockIdx.x * 256 + threadIdx.x;
@@ -359,9 +359,13 @@ __global__ __launch_bounds__(256) void weigh_join_kernel(WeighParams p) {
   }
   const int64_t all = static_cast<int64_t>(p.requests.d) * p.H.d * p.max_tokens;
   const float* const src = p.part_sums + static_cast<int64_t>(row) * p.max_tokens + t;
-  float sum = 0.0f;
+  float sum = 0.0f, lost = 0.0f;
 #pragma unroll 4
-  for (int i = 0; i < p.parts.d; ++i) sum += src[i * all];
+  for (int i = 0; i < p.parts.d; ++i) {
+    const float add = src[i * all] - lost, next = sum + add;
+    lost = next < INFINITY ? (next - sum) - add : 0.0f;
+    sum = next;
+  }
   out[t] = (weights ? weights[t] : 0.0f) + sum;
 }
 

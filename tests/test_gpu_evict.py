@@ -533,3 +533,17 @@ def test_weights_of_one_long_request_among_many(cuda_device, cache_dtype, reques
     w.weights.fill_(2.0 ** 24)
     added = w.check(w.run())
     assert added[at, 0, 0] > 14  # of which the sums have all but a step
+
+
+def test_weights_of_parts_lose_nothing_between_them(cuda_device):
+    """8192 rows are 32 parts; all but the first give 0.9 each, less than half a step (1) of what
+    the first gives, and are not lost one by one."""
+    w = Weights(cuda_device, heads=1, group=8, D=64, tokens=(2048,), queries=(1024,))
+    w.query.zero_()
+    w.lse.fill_(math.inf)
+    w.lse[0, 0] = -math.log(1.5 * 2.0 ** 24)
+    first = w.run(weights=None)[0, 0, :1024].double()  # tokens that all rows see
+    assert ((first / 2.0 ** 24 - 1.5).abs() < 1e-4).all()
+    w.lse[32:] = math.log(256 / 0.9)
+    gain = w.run(weights=None)[0, 0, :1024].double() - first
+    assert ((gain - 31 * 0.9).abs() <= 2.0).all()
