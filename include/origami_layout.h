@@ -524,7 +524,10 @@ int origami_append_kv_cache(
  * sizes), in use until the call's work is done; calls that can run at the same
  * time need their own.  out, lse and workspace share no memory with each other or
  * with an input, and out has no element twice (the Python module refuses such
- * calls).  Results do not depend on timing.
+ * calls).  Results do not depend on timing.  What a request gets does not depend on the others'
+ * lengths either, but for caches of FLOAT4_E2M1: there up to 256 requests of few rows are split by
+ * all of their lengths, so that the sums of a request's parts may be rounded otherwise beside other
+ * ones.
  */
 int64_t origami_shared_prefix_attention_workspace(
     int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_dim, int64_t prefix_tokens,

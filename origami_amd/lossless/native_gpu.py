@@ -821,7 +821,9 @@ def shared_prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor,
     whole block table); own tokens past the bound are not seen, and a request with more query
     tokens than the bound gets no defined rows.  Tokens in blocks outside the cache are
     not seen.  scale defaults to head_dim ** -0.5.  An `out` that shares memory with an input
-    or has an element twice is refused.
+    or has an element twice is refused.  The same call gives the same bits.  A request's do not
+    depend on the others' lengths, but over rows in 4 bits: there a decode step of up to 256
+    requests is split by all of their lengths, and sums may be rounded otherwise beside other ones.
 
     Returns the output, and with return_lse also float32 [tokens, query_heads] natural
     logarithms of the rows' sums of exponentials (-inf for zero rows), with which results over

@@ -594,10 +594,33 @@ def test_attend_shares_leave_other_rows(cuda_device, filled):
 @pytest.mark.parametrize("requests,bound", [(60, 4096), (256, 40960), (257, 40960), (400, 131072)])
 def test_attend_many_requests_with_a_bound_far_above(cuda_device, requests, bound):
     """On both sides of where shares end; the longest request far beyond the others."""
-    b = Batch4(cuda_device, heads=2, group=3, D=64, prefix=0, seed=requests,
-               own=lengths_of(requests, 1500, requests))
+    b = Batch4(cuda_device, heads=1, group=3, D=64, prefix=0, seed=requests,
+               own=lengths_of(requests, 1100, requests))
     want, want_lse = b.run()
     b.check(want, want_lse)
     b.tables = torch.cat([b.tables, torch.full((requests, bound // b.bs - b.tables.shape[1]), -1,
                                                device=cuda_device)], 1)
     b.check(*b.run())
+
+
+@pytest.mark.parametrize("requests", [24, 200, 270])
+def test_attend_beside_other_lengths(cuda_device, requests):
+    """One request's length changes: the others' results are as near as before, but in shares (up to
+    256 requests) their sums may be made of other parts.  In equal ranges, and over other types of
+    caches, they are the same bits."""
+    own = [1 + n for n in lengths_of(requests, 2500 if requests < 100 else 700, 12)]
+    for make in (Batch4, Batch):
+        b = make(cuda_device, heads=4 if requests < 100 else 1, group=2, D=64, prefix=0, own=own,
+                 seed=4)
+        most, first = max(own), requests // 2
+        whole, whole_lse = b.run(max_own_tokens=most)
+        b.check(whole, whole_lse)
+        b.own[first] = 3  # the longest
+        got, lse = b.run(max_own_tokens=most)
+        b.check(got, lse)
+        again, again_lse = b.run(max_own_tokens=most)
+        assert torch.equal(got, again) and torch.equal(lse, again_lse)
+        others = torch.arange(requests, device=cuda_device) != first
+        if make is Batch or requests > 256:
+            assert torch.equal(got[others], whole[others])
+            assert torch.equal(lse[others], whole_lse[others])
