@@ -453,16 +453,20 @@ int64_t cache_dtype_code(const at::Tensor& cache) {
   return paged_dtype_code(cache.scalar_type(), "kv_cache");
 }
 
-// The channels of a head of the cache, whose rows in 4 bits are as many bytes as `rows` (a tensor
-// of rows of it) says.
-int64_t head_dim_of(const at::Tensor& cache, const at::Tensor& rows, const char* name) {
+// The channels of a head of the cache, whose rows in 4 bits are as many bytes as D of them take.
+int64_t head_dim_of(const at::Tensor& cache, int64_t D) {
   if (cache.scalar_type() != at::kByte) return cache.size(4);
-  TORCH_CHECK(rows.dim() == 3, name, " must be [tokens, heads, head_dim]");
-  const int64_t D = rows.size(2), bytes = origami_kv4_row_bytes(D);
+  const int64_t bytes = origami_kv4_row_bytes(D);
   TORCH_CHECK(bytes >= 0, origami_last_error());
   TORCH_CHECK(cache.size(4) == bytes, "a kv_cache in 4 bits must have rows of ", bytes,
               " bytes for ", D, " channels, not of ", cache.size(4));
   return D;
+}
+
+// As many as `rows` (a tensor of rows of it) says.
+int64_t head_dim_of(const at::Tensor& cache, const at::Tensor& rows, const char* name) {
+  TORCH_CHECK(rows.dim() == 3, name, " must be [tokens, heads, head_dim]");
+  return head_dim_of(cache, rows.size(2));
 }
 
 // The channels of a head of the cache; those of rows in 4 bits follow from their bytes.
@@ -850,7 +854,8 @@ std::tuple<at::Tensor, at::Tensor> read_kv_cache(at::Tensor kv_cache, at::Tensor
                                                  at::ScalarType dtype, double k_scale,
                                                  double v_scale,
                                                  c10::optional<at::Tensor> key_out,
-                                                 c10::optional<at::Tensor> value_out) {
+                                                 c10::optional<at::Tensor> value_out,
+                                                 c10::optional<int64_t> channels) {
   require_eager();
   require_plain(kv_cache, "kv_cache");
   require_device(kv_cache, "kv_cache");
@@ -859,7 +864,21 @@ std::tuple<at::Tensor, at::Tensor> read_kv_cache(at::Tensor kv_cache, at::Tensor
   TORCH_CHECK(out_dtype != ORIGAMI_DTYPE_FLOAT8_E4M3FN, "dtype must be float16 or bfloat16");
   const int64_t tokens = slots.numel(), cache_dtype = cache_dtype_code(kv_cache);
   const int64_t* const slot = require_index(slots, "slots", kv_cache, tokens);
-  const int64_t head_dim = channels_of(kv_cache);
+  if (!channels && (key_out || value_out)) {
+    const at::Tensor& given = key_out ? *key_out : *value_out;
+    if (given.dim() == 3) channels = given.size(2);
+  }
+  int64_t head_dim;
+  if (channels) {
+    head_dim = head_dim_of(kv_cache, *channels);
+    TORCH_CHECK(head_dim == *channels, "head_dim differs from the kv_cache's");
+  } else {
+    // rows of most 8-bit caches are such, too
+    TORCH_CHECK(kv_cache.scalar_type() != at::kByte || kv_cache.size(4) % 16 != 0,
+                "a uint8 kv_cache with rows of ", kv_cache.size(4),
+                " bytes may be one of 8 bits a channel: head_dim must be given, if it is in 4 bits");
+    head_dim = channels_of(kv_cache);
+  }
   const c10::OptionalDeviceGuard guard(kv_cache.device());
   at::Tensor out[2];
   Extent extents[2];  // of new tensors: none

@@ -777,19 +777,23 @@ def append_kv_cache(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tens
 
 def read_kv_cache(kv_cache: torch.Tensor, slots: torch.Tensor, *,
                   dtype: torch.dtype | None = None, k_scale: float = 1.0, v_scale: float = 1.0,
-                  key_out: torch.Tensor | None = None, value_out: torch.Tensor | None = None
-                  ) -> tuple[torch.Tensor, torch.Tensor]:
+                  key_out: torch.Tensor | None = None, value_out: torch.Tensor | None = None,
+                  head_dim: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(key, value) [slots, heads, head_dim] as the paged cache holds them, of dtype float16 or
     bfloat16 (default: the cache's, else bfloat16): what append_kv_cache wrote to these slots
     (int64, block id * block size + offset).  Rows of a 16-bit cache come as they are, of a
     float8_e4m3fn one times k_scale and v_scale, rounded once, and of one in 4 bits exactly.  Slots
     outside the cache, such as -1, give zeros; a slot may be given twice.  key_out and value_out
-    (channels contiguous) may be given for the results; overlaps are refused.  For inference only,
-    as append_kv_cache."""
+    (channels contiguous) may be given for the results; overlaps are refused.  head_dim is what the
+    cache is said to have, and another is refused.  A uint8 cache is one in 4 bits, whose head_dim
+    follows from its rows' bytes; where a row has a multiple of 16 bytes, as one of an 8-bit cache
+    seen as uint8 mostly has, head_dim (or a result) has to say that it is.  For inference only, as
+    append_kv_cache."""
     if dtype is None:
         wide = kv_cache.dtype in (torch.float16, torch.bfloat16)
         dtype = kv_cache.dtype if wide else torch.bfloat16
-    return _ext.ext().read_kv_cache(kv_cache, slots, dtype, k_scale, v_scale, key_out, value_out)
+    return _ext.ext().read_kv_cache(kv_cache, slots, dtype, k_scale, v_scale, key_out, value_out,
+                                    head_dim)
 
 
 def shared_prefix_attention(query: torch.Tensor, kv_cache: torch.Tensor,

@@ -624,3 +624,45 @@ def test_attend_beside_other_lengths(cuda_device, requests):
         if make is Batch or requests > 256:
             assert torch.equal(got[others], whole[others])
             assert torch.equal(lse[others], whole_lse[others])
+
+
+@pytest.mark.parametrize("D", [16, 32, 48, 64, 80, 96, 112, 128])
+def test_read_refuses_8_bit_caches_seen_as_bytes(cuda_device, D):
+    """A view of an e4m3 cache, as the layout calls take it, is not taken for 4 bits, though some
+    head size has rows of as many bytes."""
+    gen = torch.Generator().manual_seed(D)
+    cache = torch.randn(2, 4, 16, 3, D, generator=gen).to(FP8).to(cuda_device)
+    slots = torch.arange(33, device=cuda_device)
+    read = native_gpu.read_kv_cache
+    with pytest.raises(RuntimeError, match="head_dim must be given"):
+        read(cache.view(torch.uint8), slots)
+    with pytest.raises(RuntimeError, match=f"bytes for {D} channels, not of {D}"):
+        read(cache.view(torch.uint8), slots, head_dim=D)
+    room = torch.empty(33, 3, D, dtype=BF16, device=cuda_device)
+    with pytest.raises(RuntimeError, match=f"bytes for {D} channels, not of {D}"):
+        read(cache.view(torch.uint8), slots, value_out=room)
+    with pytest.raises(RuntimeError, match="head_dim differs from the kv_cache's"):
+        read(cache, slots, head_dim=D + 8)
+    key, value = read(cache, slots, head_dim=D)
+    for half, got in ((0, key), (1, value)):
+        assert torch.equal(got.float(), cache[half].flatten(0, 1)[:33].float())
+
+
+@pytest.mark.parametrize("D", [24, 56, 88, 120, 144, 176, 208, 240])
+def test_read_of_rows_of_whole_16_bytes(cuda_device, D):
+    """4-bit rows of as many bytes as common head sizes have in 8 bits, where it is said."""
+    gen = torch.Generator().manual_seed(D)
+    kv = torch.randn(2, 4, 16, 3, D, generator=gen)
+    cache = kv4ref.pack(kv).to(cuda_device)
+    assert cache.shape[-1] % 16 == 0
+    slots = torch.arange(33, device=cuda_device)
+    want = kv4ref.values(cache, D).flatten(1, 2)[:, :33]
+    room = torch.empty(33, 3, D, dtype=F16, device=cuda_device)
+    for kw in (dict(head_dim=D), dict(key_out=room), dict(value_out=room)):
+        key, value = native_gpu.read_kv_cache(cache, slots, dtype=F16, **kw)
+        assert torch.equal(key.double(), want[0]) and torch.equal(value.double(), want[1])
+    for other in (D + 8, D - 8):
+        with pytest.raises(RuntimeError, match=f"bytes for {other} channels"):
+            native_gpu.read_kv_cache(cache, slots, head_dim=other)
+    with pytest.raises(RuntimeError, match="multiple of 8"):
+        native_gpu.read_kv_cache(cache, slots, head_dim=D + 1)
