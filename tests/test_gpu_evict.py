@@ -547,3 +547,28 @@ def test_weights_of_parts_lose_nothing_between_them(cuda_device):
     w.lse[32:] = math.log(256 / 0.9)
     gain = w.run(weights=None)[0, 0, :1024].double() - first
     assert ((gain - 31 * 0.9).abs() <= 2.0).all()
+
+
+@pytest.mark.parametrize("queries", [None, (9, 40), (1, 65)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_weights_of_infinite_and_nan_keys(cuda_device, queries, dtype):
+    """What an odd key's token gets: infinity where a row's score is, nothing from scores of
+    -infinity, NaN where a score is; and what other tokens get is the same."""
+    w = Weights(cuda_device, tokens=(70, 300), queries=queries, dtype=dtype)
+    want, t = w.run(), 250  # which all rows see
+    clean, place = w.cache.clone(), (int(w.tables[1, t // w.bs]), t % w.bs)
+    w.query[:, :4, 7] = w.query[:, :4, 7].abs() + 0.5  # of head 0 all alike, of head 1 of both signs
+    base = w.run()
+    for value in (math.inf, -math.inf, math.nan):
+        w.cache.copy_(clean)
+        w.cache[0, place[0], place[1], :, 7] = value
+        got = w.run()
+        w.check(got)
+        others = torch.ones_like(got, dtype=torch.bool)
+        others[1, :, t] = False
+        assert torch.equal(got[others], base[others])
+        if math.isnan(value):
+            assert got[1, :, t].isnan().all()
+        else:
+            assert got[1, 0, t] == (math.inf if value > 0 else w.weights[1, 0, t])
+    assert torch.equal(want[:, 1], base[:, 1])
