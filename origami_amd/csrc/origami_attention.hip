@@ -895,7 +895,8 @@ __device__ __forceinline__ void attend(const AttendParams& p, const Group& g, in
 // are widened where the product K Q takes them, 32 channels with one scale in a lane (the queries
 // have the same order of channels); the values are widened on their way to LDS, which transposes
 // them for V P.  Memory bounds it: 32 requests of 1000 to 16384 tokens with 8 heads of 128 (327 MB)
-// take 83 us, 4.0 TB/s, and without the products as long; with rows over lanes and no step ahead 165.
+// take 83 us, 4.0 TB/s, and without the products as long; with rows over lanes and no step ahead
+// 165.
 template <typename T, int DP, bool WHOLE, bool JOIN>
 __device__ __forceinline__ void attend_four(const AttendParams& p, bool batch, int r,
                                             const Request& rq, int h, int64_t place, int t0,
@@ -975,7 +976,8 @@ __device__ __forceinline__ void attend_four(const AttendParams& p, bool batch, i
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int at = __shfl(mine, 16 * i + tok);
-      const uint8_t* const src = lane_rows + static_cast<uint64_t>(static_cast<uint32_t>(at)) * pitch;
+      const uint8_t* const src =
+          lane_rows + static_cast<uint64_t>(static_cast<uint32_t>(at)) * pitch;
       s.keys[i] = load_lane<W, WHOLE>(at >= 0 ? src : no_row, lane_scale, lane_end);
       s.values[i] =
           load_lane<W, WHOLE>(at >= 0 ? src + to_values : no_row, lane_scale, lane_end);
@@ -1650,7 +1652,10 @@ Plan plan_of(int64_t tokens, int64_t query_heads, int64_t heads, int64_t head_di
         // waves for the CUs once, or as often as the requests are half of them
         const int64_t once = std::max<int64_t>(kFourWavesWanted / heads, 1);
         plan.shares = std::max<int64_t>(ceil_div(2 * requests, once), 1) * once;
-        plan.least_share = std::max<int64_t>(8, ceil_div(steps, kMaxParts / 2));
+        // steps of a share at least, whatever the bound, if a request can have all of a head's
+        plan.least_share = 8;
+        if (plan.shares > kMaxParts)
+          plan.least_share = std::max<int64_t>(plan.least_share, ceil_div(steps, kMaxParts));
         best1 = std::min(ceil_div(steps, plan.least_share), plan.shares);
       }
     }
@@ -1823,8 +1828,9 @@ int origami_shared_prefix_attention(
   p.part_ml = p.part_o + plan.places * head_dim;
   p.row_parts = reinterpret_cast<RowParts*>(p.part_ml + plan.places * 2);
   const hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-  return dtype == ORIGAMI_DTYPE_BFLOAT16 ? launch_attend<bf16>(p, cell_of(cache_dtype), plan.way, stream)
-                                         : launch_attend<f16>(p, cell_of(cache_dtype), plan.way, stream);
+  const Cell cell = cell_of(cache_dtype);
+  return dtype == ORIGAMI_DTYPE_BFLOAT16 ? launch_attend<bf16>(p, cell, plan.way, stream)
+                                         : launch_attend<f16>(p, cell, plan.way, stream);
 }
 
 }  // extern "C"

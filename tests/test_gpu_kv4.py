@@ -666,3 +666,16 @@ def test_read_of_rows_of_whole_16_bytes(cuda_device, D):
             native_gpu.read_kv_cache(cache, slots, head_dim=other)
     with pytest.raises(RuntimeError, match="multiple of 8"):
         native_gpu.read_kv_cache(cache, slots, head_dim=D + 1)
+
+
+@pytest.mark.parametrize("heads,bound", [(1, 40000), (1, 1 << 20), (3, 1 << 20), (8, 1 << 22)])
+def test_attend_one_request_in_all_shares(cuda_device, heads, bound):
+    """A request beside empty ones is cut into as many parts as a row can have, whatever the bound
+    allows."""
+    own = (0,) * 5 + (40000,) + (1,) * 3
+    b = Batch4(cuda_device, heads=heads, group=2, D=8, prefix=0, own=own, seed=heads)
+    want, want_lse = b.run()
+    b.check(want, want_lse)
+    width = -(-bound // b.bs) - b.tables.shape[1]
+    b.tables = torch.cat([b.tables, torch.full((len(own), width), -1, device=cuda_device)], 1)
+    b.check(*b.run())
