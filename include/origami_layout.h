@@ -511,9 +511,9 @@ int origami_append_kv_cache(
  * and max_own_tokens bound a request's query and own tokens and shape the
  * launch: own tokens past the bound are not seen, and the rows of a request
  * with more query tokens than the bound have no defined values.  Rows that no
- * request has are left as they were.  Tokens in blocks outside [0, num_blocks) are not seen; what a row
- * does not see has no influence on it, NaN included.  A row that sees no token,
- * or only scores of -infinity, becomes zero.
+ * request has are left as they were.  Tokens in blocks outside [0, num_blocks)
+ * are not seen; what a row does not see has no influence on it, NaN included.  A
+ * row that sees no token, or only scores of -infinity, becomes zero.
  * lse (null: none) is a contiguous float32 [tokens, query_heads]: the natural
  * logarithm of each row's sum of exponentials, -infinity for zero rows.
  *

@@ -321,9 +321,9 @@ struct ReadParams {
 constexpr int kReadThreads = 256;
 
 // The key and the value of one row (a token's head), 8 channels a lane, as T.  A row outside the
-// cache is zero.  Memory bounds it, so a lane's store is 16 bytes and a row's lanes follow each other:
-// 32753 tokens of 8 heads of 128 in 4 bits take 37 us among other work (4.6 TB/s) and 27 alone,
-// where the rows stay in the last-level cache.
+// cache is zero.  Memory bounds it, so a lane's store is 16 bytes and a row's lanes follow each
+// other: 32753 tokens of 8 heads of 128 in 4 bits take 37 us among other work (4.6 TB/s) and 27
+// alone, where the rows stay in the last-level cache.
 template <typename T, Cell CELL, int L>
 __global__ __launch_bounds__(kReadThreads) void read_kv_kernel(ReadParams p) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kReadThreads / L) + threadIdx.x / L;

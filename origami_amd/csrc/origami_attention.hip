@@ -1551,13 +1551,13 @@ struct Kind {
 constexpr double kUnitTime = 6.0, kCuBytes = 20e3, kCuFlops = 3.2e6;
 
 // Caches in 4 bits with few rows.  Waves by themselves, about 2048 of them, pay where the requests
-// have 512 times 256 tokens and heads: 8 requests of 4000 tokens and 8 heads take 18 us and, with
-// joins in workgroups, 24; 64 of 2000 take 43 and 63, and 49 in 1536 waves; 32 of 1000 to 16384 take
-// 89 and 145.  Below, workgroups join eight waves, and a single part is best where it is short: 1
-// request of 1029 tokens takes 10.2 us, with two parts 11.8, in waves by themselves 14.4; of 8000
-// tokens 15.0 and 14.6 to 16.3.  Past 256 requests their ranges are the same for all, since to find
-// shares takes longer with each request and many requests fill the CUs evenly by their number (200 of
-// 10 to 3000 tokens: 120 us in shares, 117 in ranges).
+// have 512 times 256 tokens and heads: 8 requests of 4000 tokens and 8 heads take 19 us and, with
+// joins in workgroups, 24; 64 of 2000 take 44 and 63, and 49 in 1536 waves; 32 of 1000 to 16384
+// take 89 and 145.  Below, workgroups join eight waves, and a single part is best where it is
+// short: 1 request of 1029 tokens takes 10.2 us, with two parts 11.8, in waves by themselves 14.4;
+// of 8000 tokens 15.0 and 14.6 to 16.3.  Past 256 requests their ranges are the same for all, since
+// to find shares takes longer with each request and many requests fill the CUs evenly by their
+// number (200 of 10 to 3000 tokens: 121 us in shares, 117 in ranges).
 constexpr int64_t kFourMany = 512, kFourWavesWanted = 2048;
 // Bytes that such ranges' parts may take, past what is needed for as many waves: 15 parts a row of
 // 512 requests with 64 heads of 128 channels.

@@ -111,7 +111,8 @@ __device__ __forceinline__ U32x4 fp4_expand(uint32_t codes, float scale) {
 // 6 2^kMostScale; NaN makes the 32 values NaN.
 __device__ __forceinline__ uint32_t fp4_scale_byte(uint32_t most) {
   if (most > 0x7f800000u) return 255;
-  const int s = static_cast<int>((most + 0x1fffffu) >> 23) - 2;  // up by one past a mantissa of 1.75
+  // up by one past a mantissa of 1.75
+  const int s = static_cast<int>((most + 0x1fffffu) >> 23) - 2;
   return static_cast<uint32_t>(min(max(s, 127 + kLeastScale), 127 + kMostScale));
 }
 

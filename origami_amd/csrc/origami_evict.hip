@@ -1,10 +1,11 @@
 // origami_evict.hip -- eviction from the paged KV cache by accumulated attention weight.
 //
 // weigh_kernel (weigh_few_kernel where the rows are few) adds up, for each cached token t and cache
-// head, the weights that the queries give it:  out_t = weights_t + sum_q exp(scale (q . k_t) - lse_q),  with lse_q the logarithm of the
-// sum of exponentials that the attention returned for the row, so that no maximum is needed.
-// select_kernel finds the tokens that a head keeps, the newest and those of the largest sums, and
-// move_kernel copies their rows, in order, to blocks of their own.
+// head, the weights that the queries give it:
+//   out_t = weights_t + sum_q exp(scale (q . k_t) - lse_q)
+// with lse_q the logarithm of the sum of exponentials that the attention returned for the row, so
+// that no maximum is needed.  select_kernel finds the tokens that a head keeps, the newest and
+// those of the largest sums, and move_kernel copies their rows, in order, to blocks of their own.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -92,8 +93,9 @@ struct __attribute__((aligned(4))) Dwords {
 // where they are; the queries go through LDS, a stage ahead.
 //
 // The exponentials and masks beside the products bound it: two prompts of up to 4096 tokens, 28
-// query heads of 128 channels over 4 heads in 4 bits, take 139 us (723 TFLOP/s, matrix units busy in
-// 37% of the CUs' busy cycles); without parts of the rows and stages of 64 they took 926.
+// query heads of 128 channels over 4 heads in 4 bits, take 139 to 145 us (723 to 693 TFLOP/s,
+// matrix units busy in 37% of the CUs' busy cycles); without parts of the rows and stages of 64
+// they took 926.
 //
 // The order of the channels in the products is free as long as keys and queries have the same: a
 // lane's 16 bytes of a key are 8, 16 or 32 channels in a row, whole loads of the cache's row.
@@ -385,13 +387,19 @@ int64_t weigh_parts(int64_t tokens, int64_t query_heads, int64_t heads, int64_t 
 // Zeros, for what a lane reads of rows that are not in the cache and of channels past the last.
 __device__ const U32x4 kZeroRow[33] = {};
 
-// One wave: a range of the tokens of one KV head of one request against its query rows, 16 and fewer
-// as in a decode step, or 16 at a time.  Memory bounds it.  The queries stay in
-// registers; the keys come 64 tokens at a step (32 past 128 channels) and a step ahead, and their
-// blocks two steps, so that a wave waits for memory as seldom as can be: 16 requests of 2048 to 8192
-// tokens and 8 heads of 128 take 47 us among other work (39 alone, 4.3 TB/s) and in 4 bits 20; with
-// workgroups that ended after 256 tokens 52 and 33.  Waves next to each other are heads of the same
-// tokens, and ranges of a request follow each other over the chiplets, as in the attention.
+// One wave: a range of the tokens of one KV head of one request against its query rows, 16 and
+// fewer as in a decode step, or 16 at a time.  Memory bounds it.  The queries stay in registers;
+// the keys come 64 tokens at a step (32 past 128 channels) and a step ahead, and their blocks two
+// steps, so that a wave waits for memory as seldom as can be: 16 requests of 2048 to 8192 tokens
+// and 8 heads of 128 take 47 us among other work (39 alone, 4.3 TB/s), in e4m3 24 and in 4 bits 20;
+// with workgroups that ended after 256 tokens 52 and in 4 bits 33.  Waves next to each other are
+// heads of the same tokens, and ranges of a request follow each other over the chiplets, as in the
+// attention.
+//
+// Rows past 16 have their queries loaded anew for each step of keys, which is slow (1 us for 16
+// rows and a step), but their request alone is: one of 900 queries and 4 query heads a cache head
+// among 300 of one takes 3.5 ms.  To go over the keys anew for each 16 rows took 10.1, and a
+// rounding each.
 template <typename T, Cell CELL, int DP, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void weigh_few_kernel(WeighParams p, Divisor beside,
                                                            int chunk) {
@@ -424,8 +432,8 @@ __global__ __launch_bounds__(256, 2) void weigh_few_kernel(WeighParams p, Diviso
   const float* const weights =
       p.weights ? p.weights + r * p.w_request + h * p.w_head : nullptr;
   float* const out = p.out + r * p.o_request + h * p.o_head;
-  // places past the tokens are copied, if they are elsewhere: those up to the bound with the range's,
-  // those past it with all ranges alike
+  // places past the tokens are copied, if they are elsewhere: those up to the bound with the
+  // range's, those past it with all ranges alike
   if (out != weights && p.rest > 0) {
     constexpr int kEach = 8;
     const int64_t rest0 = p.max_tokens + static_cast<int64_t>(t0 / chunk) * p.rest;
@@ -575,8 +583,8 @@ __global__ __launch_bounds__(256, 2) void weigh_few_kernel(WeighParams p, Diviso
   };
 
   if (rows > MR) {
-    // One of the batch's longer requests: each step's keys against all rows that see any of them, 16
-    // at a time, in sums of binary32 with what they lose.
+    // One of the batch's longer requests: each step's keys against all rows that see any of them,
+    // 16 at a time, in sums of binary32 with what they lose.
     int64_t block = id;
     for (int t = t0; t < t1; t += STEP) {
       Step s;
@@ -728,7 +736,8 @@ struct Share {
 
 __device__ __forceinline__ Share share_of(const EvictParams& p, int r) {
   Share s;
-  s.tokens = static_cast<int>(min(max(p.lengths[r], int64_t(0)), static_cast<int64_t>(p.max_tokens)));
+  s.tokens =
+      static_cast<int>(min(max(p.lengths[r], int64_t(0)), static_cast<int64_t>(p.max_tokens)));
   s.kept = min(s.tokens, p.keep);
   const int last = min(p.recent, s.kept);
   s.older = s.tokens - last;
@@ -779,11 +788,11 @@ __device__ __forceinline__ float weight_of(uint32_t rank) {
 // are listed in their order, KEYS times 1024 of them at a time.
 //
 // The workgroup has a CU to itself, and instructions bound it: a lane keeps the ranks of KEYS
-// places, which are read and made once, steps without tokens are left out, and the lists are counted
-// with scalar instructions.  4 requests of 8 heads and 20000 to 32768 tokens take 27 us, 8000 to 8192
-// tokens 13, with the 32 places that long lists need 17; with every step taken 31 and 22.  With
-// weights kept in place of ranks 20000 to 32768 took 39, with weights read anew in each pass 50.
-// More than KEYS times 1024 tokens are read five times.
+// places, which are read and made once, steps without tokens are left out, and the lists are
+// counted with scalar instructions.  4 requests of 8 heads and 20000 to 32768 tokens take 27 us,
+// 8000 to 8192 tokens 13, with the 32 places that long lists need 17; with every step taken 31 and
+// 22.  With weights kept in place of ranks 20000 to 32768 took 39, with weights read anew in each
+// pass 50.  More than KEYS times 1024 tokens are read five times.
 template <int KEYS>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
   constexpr int kCopies = 4, kStep = kSelectThreads, kRound = KEYS * kStep;
@@ -957,8 +966,10 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
 constexpr int kMoveThreads = 256, kMoveTokens = 8;
 
 // One workgroup: kMoveTokens new tokens of a request, all heads, keys and values.  V: what a load
-// has.  Memory bounds it: 33 MB of keys and as much of values go in 22 to 24 us (5.7 TB/s, both ways
-// counted), as 1024 rows of 1024 channels in e4m3 or 4096 of 1024 in bfloat16 of each request.
+// has.  Memory bounds it where rows are whole 16 bytes: 33 MB of keys and as much of values go in
+// 22 to 24 us (5.7 TB/s, both ways counted), as 1024 rows of 1024 channels in e4m3 or 4096 of 1024
+// in bfloat16 of each request.  Rows in 4 bits go by dwords, with a quotient, a place and two block
+// ids for each: the same rows, 36 and 18 MB each way, take 21 and 13.5 us (3.4 and 2.6 TB/s).
 template <typename V>
 __global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictParams p) {
   const int r = divide(static_cast<int>(blockIdx.x), p.row_tiles);
@@ -1171,7 +1182,8 @@ int origami_evict_kv_cache(
                   "too many tokens for one call");
   if (requests == 0) return ORIGAMI_OK;
   ORIGAMI_REQUIRE(lengths != nullptr && (weights != nullptr || max_tokens == 0) &&
-                      (kept != nullptr || keep == 0) && (out_weights != nullptr || out_places == 0) &&
+                      (kept != nullptr || keep == 0) &&
+                      (out_weights != nullptr || out_places == 0) &&
                       (block_tables != nullptr || max_tokens == 0) &&
                       (out_tables != nullptr || most == 0) &&
                       (kv_cache != nullptr || num_blocks == 0),

@@ -749,8 +749,9 @@ c10::optional<at::Tensor> append_kv_cache(
   check(origami_append_kv_cache(
       key.data_ptr(), value.data_ptr(), query ? query->data_ptr() : nullptr,
       out ? out->data_ptr() : nullptr, dtype, strides, tokens, query_heads, kv_cache.data_ptr(),
-      cache_dtype_code(kv_cache), g.layout, g.num_blocks, g.block_size, g.heads, D, slot, position, cos_sin ? cos_sin->data_ptr<float>() : nullptr, table_rows,
-      rotary_dim, interleaved, query_norm ? query_norm->data_ptr() : nullptr,
+      cache_dtype_code(kv_cache), g.layout, g.num_blocks, g.block_size, g.heads, D, slot, position,
+      cos_sin ? cos_sin->data_ptr<float>() : nullptr, table_rows, rotary_dim, interleaved,
+      query_norm ? query_norm->data_ptr() : nullptr,
       key_norm ? key_norm->data_ptr() : nullptr, norm_dtype, eps, k_scale, v_scale,
       current_stream(kv_cache)));
   return out;
@@ -876,7 +877,8 @@ std::tuple<at::Tensor, at::Tensor> read_kv_cache(at::Tensor kv_cache, at::Tensor
     // rows of most 8-bit caches are such, too
     TORCH_CHECK(kv_cache.scalar_type() != at::kByte || kv_cache.size(4) % 16 != 0,
                 "a uint8 kv_cache with rows of ", kv_cache.size(4),
-                " bytes may be one of 8 bits a channel: head_dim must be given, if it is in 4 bits");
+                " bytes may be one of 8 bits a channel: head_dim must be given, if it is in 4 "
+                "bits");
     head_dim = channels_of(kv_cache);
   }
   const c10::OptionalDeviceGuard guard(kv_cache.device());

@@ -859,17 +859,17 @@ def accumulate_attention_weights(query: torch.Tensor, kv_cache: torch.Tensor,
     Request r has tokens[r] tokens in blocks block_tables[r] (a prefix shared with others is part of
     them here), and its query rows are its newest ones: row r of query, or with query_starts rows
     query_starts[r] .. query_starts[r + 1] - 1; all of a prompt's rows or some last ones may be
-    given.  The average of the requests' rows shapes the launch, and a prompt among many single tokens
-    is slow: call once for prompts and once for single tokens.  query, kv_cache, k_scale and scale are those of shared_prefix_attention, and lse
-    (float32 [rows, query_heads]) is what it returned with return_lse for these rows over all of
-    the request's tokens.  weights (default: zeros) and the result are float32 [requests, heads,
-    places]; place t is the request's token t.  `out` may be `weights` itself; without weights and
-    out the result has max_tokens places (default: the block table's slots, or as many as weights
-    has places).  Tokens past max_tokens and in blocks outside the cache get nothing.  max_tokens
+    given.  The average of the requests' rows shapes the launch, and a prompt among many single
+    tokens is slow: call once for prompts and once for single tokens.  query, kv_cache, k_scale and
+    scale are those of shared_prefix_attention, and lse (float32 [rows, query_heads]) is what it
+    returned with return_lse for these rows over all of the request's tokens.  weights (default:
+    zeros) and the result are float32 [requests, heads, places]; place t is the request's token t.
+    `out` may be `weights` itself; without weights and out the result has max_tokens places
+    (default: the block table's slots, or as many as weights has places).  Tokens past max_tokens and in blocks outside the cache get nothing.  max_tokens
     shapes the launch, not the places: in place, a buffer of sums for the longest context takes no
-    time beyond it.  Lengths and tables are read on the device, so a call can be captured in a graph.  Each sum is float32, in a
-    fixed order.  Overlaps are refused but of out with weights.  For inference only, as
-    shared_prefix_attention."""
+    time beyond it.  Lengths and tables are read on the device, so a call can be captured in a
+    graph.  Each sum is float32, in a fixed order.  Overlaps are refused but of out with weights.
+    For inference only, as shared_prefix_attention."""
     return _ext.ext().accumulate_attention_weights(
         query, kv_cache, block_tables, tokens, lse, weights, query_starts, max_tokens, scale,
         k_scale, out)
@@ -889,11 +889,11 @@ def evict_kv_cache(kv_cache: torch.Tensor, block_tables: torch.Tensor, tokens: t
     (default: the block table's slots, or as many as weights has places).  What it keeps,
     min(tokens[r], keep) rows a head, is copied in its order to blocks out_tables[r] of the same
     cache, keys and values bit by bit whatever the cache's type, and is the request from then on:
-    with out_tables as its block table and tokens.clamp(max=keep) tokens.  Blocks that are read stay as they are, so a prefix may be shared
-    with other requests; blocks that are written must be in no table that is read, and in
-    out_tables once.  A row of a block outside the cache is copied as zeros, and to one outside it
-    not at all.  Since rows are copied, it pays to let a cache grow by some tens of tokens between
-    two calls.
+    with out_tables as its block table and tokens.clamp(max=keep) tokens.  Blocks that are read
+    stay as they are, so a prefix may be shared with other requests; blocks that are written must
+    be in no table that is read, and in out_tables once.  A row of a block outside the cache is
+    copied as zeros, and to one outside it not at all.  Since rows are copied, it pays to let a
+    cache grow by some tens of tokens between two calls.
 
     Returns (kept, out_weights): int64 [requests, heads, keep] places that the rows had, then -1,
     and their weights, then zeros, in `out_weights` or a new tensor of the weights' shape (at least

@@ -481,8 +481,9 @@ def test_refusals(cuda_device):
     assert torch.equal(e.cache, before)
 
 
-@pytest.mark.parametrize("tokens,queries", [((70, 300, 0, 33), None), ((70, 300, 0, 33), (9, 40, 0, 2)),
-                                            ((2000, 1500), (2000, 700)), ((5,) * 40, None)])
+@pytest.mark.parametrize("tokens,queries", [
+    ((70, 300, 0, 33), None), ((70, 300, 0, 33), (9, 40, 0, 2)), ((2000, 1500), (2000, 700)),
+    ((5,) * 40, None)])
 @pytest.mark.parametrize("spare", [1, 63, 20000])
 @pytest.mark.parametrize("bound", ["most", "half", 0, None])
 def test_weights_places_far_past_the_tokens(cuda_device, tokens, queries, spare, bound):
@@ -557,7 +558,7 @@ def test_weights_of_infinite_and_nan_keys(cuda_device, queries, dtype):
     w = Weights(cuda_device, tokens=(70, 300), queries=queries, dtype=dtype)
     want, t = w.run(), 250  # which all rows see
     clean, place = w.cache.clone(), (int(w.tables[1, t // w.bs]), t % w.bs)
-    w.query[:, :4, 7] = w.query[:, :4, 7].abs() + 0.5  # of head 0 all alike, of head 1 of both signs
+    w.query[:, :4, 7] = w.query[:, :4, 7].abs() + 0.5  # of head 1 they stay of both signs
     base = w.run()
     for value in (math.inf, -math.inf, math.nan):
         w.cache.copy_(clean)
