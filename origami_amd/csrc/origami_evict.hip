@@ -969,7 +969,8 @@ constexpr int kMoveThreads = 256, kMoveTokens = 8;
 // has.  Memory bounds it where rows are whole 16 bytes: 33 MB of keys and as much of values go in
 // 22 to 24 us (5.7 TB/s, both ways counted), as 1024 rows of 1024 channels in e4m3 or 4096 of 1024
 // in bfloat16 of each request.  Rows in 4 bits go by dwords, with a quotient, a place and two block
-// ids for each: the same rows, 36 and 18 MB each way, take 21 and 13.5 us (3.4 and 2.6 TB/s).
+// ids for each, and are parts of lines (49 and 47 MB are read): the same rows, 36 and 18 MB each
+// way, take 21 and 13.5 us (3.4 and 2.6 TB/s).
 template <typename V>
 __global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictParams p) {
   const int r = divide(static_cast<int>(blockIdx.x), p.row_tiles);
