@@ -387,8 +387,8 @@ int64_t weigh_parts(int64_t tokens, int64_t query_heads, int64_t heads, int64_t 
 // Zeros, for what a lane reads of rows that are not in the cache and of channels past the last.
 __device__ const U32x4 kZeroRow[33] = {};
 
-// One wave: a range of the tokens of one KV head of one request against its query rows, 16 and
-// fewer as in a decode step, or 16 at a time.  Memory bounds it.  The queries stay in registers;
+// One wave: a range of the tokens of one KV head of one request against its query rows, few as in a
+// decode step.  Memory bounds it.  The queries stay in registers;
 // the keys come 64 tokens at a step (32 past 128 channels) and a step ahead, and their blocks two
 // steps, so that a wave waits for memory as seldom as can be: 16 requests of 2048 to 8192 tokens
 // and 8 heads of 128 take 47 us among other work (39 alone, 4.3 TB/s), in e4m3 24 and in 4 bits 20;
@@ -396,10 +396,11 @@ __device__ const U32x4 kZeroRow[33] = {};
 // heads of the same tokens, and ranges of a request follow each other over the chiplets, as in the
 // attention.
 //
-// Rows past 16 have their queries loaded anew for each step of keys, which is slow (1 us for 16
-// rows and a step), but their request alone is: one of 900 queries and 4 query heads a cache head
-// among 300 of one takes 3.5 ms.  To go over the keys anew for each 16 rows took 10.1, and a
-// rounding each.
+// Drafts of 17 to 32 rows beside shorter ones have two products a key (16 requests of 3 and 5
+// queries with 4 query heads a cache head: 48 us, in 4 bits 25).  Past that the queries are loaded
+// anew for each step of keys, 16 rows at a time, which is slow (1 us each), but their request alone
+// is: one of 900 queries among 300 of one takes 3.4 ms.  To go over the keys anew for each 16 rows
+// took 81, 37 us and 10.1 ms, and a rounding each.
 template <typename T, Cell CELL, int DP, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void weigh_few_kernel(WeighParams p, Divisor beside,
                                                            int chunk) {
@@ -582,21 +583,38 @@ __global__ __launch_bounds__(256, 2) void weigh_few_kernel(WeighParams p, Diviso
     }
   };
 
-  if (rows > MR) {
+  // Over the steps, with the keys of the next on their way.
+  const auto each_step = [&](auto compute) __attribute__((always_inline)) {
+    Step even, other;
+    load_step(even, row_of(t0 + tl, id), t0, weights);
+    __builtin_amdgcn_sched_barrier(0);
+    for (int t = t0; t < t1; t += 2 * STEP) {
+      int mine = row_of(t + STEP + tl, ahead);
+      ahead = block_of(t + 2 * STEP + tl);
+      load_step(other, mine, t + STEP, weights);
+      compute(even, t);
+      if (t + STEP >= t1) break;
+      mine = row_of(t + 2 * STEP + tl, ahead);
+      ahead = block_of(t + 3 * STEP + tl);
+      load_step(even, mine, t + 2 * STEP, weights);
+      compute(other, t + STEP);
+    }
+  };
+
+  constexpr int kHeld = DP <= 128 ? 2 : 1;  // of 16 rows each that there are registers for
+  if (rows > kHeld * MR) {
     // One of the batch's longer requests: each step's keys against all rows that see any of them,
-    // 16 at a time, in sums of binary32 with what they lose.
-    int64_t block = id;
-    for (int t = t0; t < t1; t += STEP) {
-      Step s;
-      load_step(s, row_of(t + tl, block), t, weights);
-      block = block_of(t + STEP + tl);
+    // 16 at a time and the next ones ahead, in sums of binary32 with what they lose.
+    const auto first_row = [&](int t) {
+      return min(max(t - before, 0), q_count) * p.G.d / MR * MR;
+    };
+    Rows16 next;
+    load_rows(next, first_row(t0));
+    const auto compute = [&](const Step& s, int t) __attribute__((always_inline)) {
       float sum[NT] = {}, lost[NT] = {};
-      int from = min(max(t - before, 0), q_count) * p.G.d / MR * MR;
-      Rows16 next;
-      if (from < rows) load_rows(next, from);
-      for (; from < rows; from += MR) {
+      for (int from = first_row(t); from < rows; from += MR) {
         const Rows16 q = next;
-        if (from + MR < rows) load_rows(next, from + MR);
+        load_rows(next, from + MR < rows ? from + MR : first_row(t + STEP));
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const float add = weights_of(q, s, n, t) - lost[n], total = sum[n] + add;
@@ -605,33 +623,42 @@ __global__ __launch_bounds__(256, 2) void weigh_few_kernel(WeighParams p, Diviso
         }
       }
       finish(s, sum, t);
+    };
+    if constexpr (CELL == kWide) {  // there are registers for the keys of one step
+      int64_t block = id;
+      for (int t = t0; t < t1; t += STEP) {
+        Step s;
+        load_step(s, row_of(t + tl, block), t, weights);
+        block = block_of(t + STEP + tl);
+        compute(s, t);
+      }
+    } else {
+      each_step(compute);
     }
     return;
   }
 
-  // with no query row the sums stay what they are
-  Rows16 q;
-  load_rows(q, 0);
-  const auto compute = [&](const Step& s, int t) {
-    float v[NT];
+  const auto held_rows = [&](auto count) __attribute__((always_inline)) {
+    constexpr int N = decltype(count)::value;
+    Rows16 q[N];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) v[n] = weights_of(q, s, n, t);
-    finish(s, v, t);
+    for (int i = 0; i < N; ++i) load_rows(q[i], MR * i);
+    const auto compute = [&](const Step& s, int t) __attribute__((always_inline)) {
+      float v[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        v[n] = weights_of(q[0], s, n, t);
+#pragma unroll
+        for (int i = 1; i < N; ++i) v[n] += weights_of(q[i], s, n, t);
+      }
+      finish(s, v, t);
+    };
+    each_step(compute);
   };
-  Step even, other;
-  load_step(even, row_of(t0 + tl, id), t0, weights);
-  __builtin_amdgcn_sched_barrier(0);
-  for (int t = t0; t < t1; t += 2 * STEP) {
-    int mine = row_of(t + STEP + tl, ahead);
-    ahead = block_of(t + 2 * STEP + tl);
-    load_step(other, mine, t + STEP, weights);
-    compute(even, t);
-    if (t + STEP >= t1) break;
-    mine = row_of(t + 2 * STEP + tl, ahead);
-    ahead = block_of(t + 3 * STEP + tl);
-    load_step(even, mine, t + 2 * STEP, weights);
-    compute(other, t + STEP);
-  }
+  if (kHeld > 1 && rows > MR)
+    held_rows(std::integral_constant<int, kHeld>{});
+  else  // with no query row the sums stay what they are
+    held_rows(std::integral_constant<int, 1>{});
 }
 
 // Whether there are places past max_tokens that are copied: not if they are where they go.

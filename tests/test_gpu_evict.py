@@ -573,3 +573,16 @@ def test_weights_of_infinite_and_nan_keys(cuda_device, queries, dtype):
         else:
             assert got[1, 0, t] == (math.inf if value > 0 else w.weights[1, 0, t])
     assert torch.equal(want[:, 1], base[:, 1])
+
+
+@pytest.mark.parametrize("cache_dtype", [BF16, FP8, U8])
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+@pytest.mark.parametrize("group", [1, 4, 5])
+def test_weights_of_uneven_drafts(cuda_device, cache_dtype, D, group):
+    """16 rows and fewer on average, in requests of 16, of up to 32, and of more."""
+    queries = (3, 5, 1, 7, 0, 4, 2, 8, 9, 1, 1, 1, 1, 1, 1, 1)
+    w = Weights(cuda_device, heads=2, group=group, D=D, cache_dtype=cache_dtype, queries=queries,
+                tokens=[q + 91 * i % 700 for i, q in enumerate(queries)], seed=D + group)
+    w.check(w.run())
+    same = w.weights.clone()
+    assert torch.equal(w.run(weights=same, out=same), w.run())
