@@ -1300,8 +1300,9 @@ struct Parts {
   int64_t first, step;
   int32_t count;
 };
+template <bool SHARES>
 __device__ __forceinline__ Parts parts_of(const AttendParams& p, int64_t row, int most) {
-  if (!p.shares.d) return {row, static_cast<int64_t>(p.tokens) * p.Hq, p.slots};
+  if constexpr (!SHARES) return {row, static_cast<int64_t>(p.tokens) * p.Hq, p.slots};
   const RowParts mine = p.row_parts[row];
   const int step = p.H.d * p.share_rows, last = p.shares.d * step - 1;
   const int first = min(max(mine.first, 0), last);
@@ -1312,7 +1313,7 @@ __device__ __forceinline__ Parts parts_of(const AttendParams& p, int64_t row, in
 // w_s = 2^(m_s - max m).  For few parts: 4 channels a lane, `lanes` lanes a row.  Sums are loaded
 // once it is known which there are: loading them beside the maxima cost 0.3 us of 12.2 for one
 // request, and 30 of 530 for four prompts, whose parts are not all there.
-template <typename T>
+template <typename T, bool SHARES>
 __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams p, int lanes) {
   const int64_t all = static_cast<int64_t>(p.tokens) * p.Hq;
   const int64_t row =
@@ -1321,7 +1322,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams p, 
   if (row >= all || ch >= p.D) return;
   const int64_t n = row / p.Hq, head = row - n * p.Hq;
   if (p.starts && (n < p.starts[0] || n >= p.starts[p.requests.d])) return;
-  const Parts parts = parts_of(p, row, kFewParts);
+  const Parts parts = parts_of<SHARES>(p, row, kFewParts);
   float m[kFewParts], l[kFewParts], best = -INFINITY, total = 0.0f;
 #pragma unroll
   for (int s = 0; s < kFewParts; ++s) {
@@ -1349,7 +1350,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_few_kernel(AttendParams p, 
 // have tokens with their weights, then its lane groups add them up in turn, several loads each on
 // their way: 8 us for 128 rows of 412 parts, where one wave a row after the other took 55.  Waves
 // meet three times; a tree of steps through LDS and maxima by its crossbar cost 0.5 us more.
-template <typename T>
+template <typename T, bool SHARES>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendParams p, int lanes, int blocks) {
   __shared__ float weight[kMaxParts];
   __shared__ int which[kMaxParts];
@@ -1363,7 +1364,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttendParams p, int 
   const int64_t n = row / p.Hq, head = row - n * p.Hq;
   if (p.starts && (n < p.starts[0] || n >= p.starts[p.requests.d])) return;
 
-  const Parts of = parts_of(p, row, kMaxParts);
+  const Parts of = parts_of<SHARES>(p, row, kMaxParts);
   constexpr int kEach = kMaxParts / kJoinThreads;
   float m[kEach], l[kEach], best = -INFINITY;
 #pragma unroll
@@ -1491,27 +1492,31 @@ int launch_units(const AttendParams& p, Way way, hipStream_t stream) {
   return launch_units<T, CELL, DP>(p, stream);
 }
 
-template <typename T, Cell CELL>
-int launch_attend(const AttendParams& p, Way way, hipStream_t stream) {
-  const int rc = p.D <= 64    ? launch_units<T, CELL, 64>(p, way, stream)
-                 : p.D <= 128 ? launch_units<T, CELL, 128>(p, way, stream)
-                              : launch_units<T, CELL, 256>(p, way, stream);
-  if (rc) return rc;
+template <typename T, bool SHARES>
+int launch_join(const AttendParams& p, hipStream_t stream) {
   const dim3 block(kJoinThreads);
-  if (p.slots == 1) return ORIGAMI_OK;
   const int lanes = p.D <= 64 ? 16 : (p.D <= 128 ? 32 : 64);  // of a whole row
   const int64_t rows = static_cast<int64_t>(p.tokens) * p.Hq, per = kJoinThreads / lanes;
   if (p.slots <= kFewParts) {
     const dim3 joins(static_cast<unsigned>((rows + per - 1) / per));
-    hipLaunchKernelGGL(join_few_kernel<T>, joins, block, 0, stream, p, lanes);
+    hipLaunchKernelGGL((join_few_kernel<T, SHARES>), joins, block, 0, stream, p, lanes);
   } else {
     // with few rows, workgroups of 32 channels, so that the GPU has enough of them
     const int some = rows < 2 * kCus ? 8 : lanes;
     const int blocks = (p.D + 4 * some - 1) / (4 * some);
     const dim3 joins(static_cast<unsigned>(rows * blocks));
-    hipLaunchKernelGGL(join_kernel<T>, joins, block, 0, stream, p, some, blocks);
+    hipLaunchKernelGGL((join_kernel<T, SHARES>), joins, block, 0, stream, p, some, blocks);
   }
   return check_launch("join_kernel");
+}
+
+template <typename T, Cell CELL>
+int launch_attend(const AttendParams& p, Way way, hipStream_t stream) {
+  const int rc = p.D <= 64    ? launch_units<T, CELL, 64>(p, way, stream)
+                 : p.D <= 128 ? launch_units<T, CELL, 128>(p, way, stream)
+                              : launch_units<T, CELL, 256>(p, way, stream);
+  if (rc || p.slots == 1) return rc;
+  return way == kFourShares ? launch_join<T, true>(p, stream) : launch_join<T, false>(p, stream);
 }
 
 template <typename T>

@@ -93,9 +93,9 @@ struct __attribute__((aligned(4))) Dwords {
 // where they are; the queries go through LDS, a stage ahead.
 //
 // The exponentials and masks beside the products bound it: two prompts of up to 4096 tokens, 28
-// query heads of 128 channels over 4 heads in 4 bits, take 139 to 145 us (723 to 693 TFLOP/s,
-// matrix units busy in 37% of the CUs' busy cycles); without parts of the rows and stages of 64
-// they took 926.
+// query heads of 128 channels over 4 heads in 4 bits, take 139 to 154 us on different boxes (723 to
+// 653 TFLOP/s, matrix units busy in 37% of the CUs' busy cycles); without parts of the rows and
+// stages of 64 they took 926.
 //
 // The order of the channels in the products is free as long as keys and queries have the same: a
 // lane's 16 bytes of a key are 8, 16 or 32 channels in a row, whole loads of the cache's row.
